@@ -259,6 +259,96 @@ pt_status pt_layernorm_params(const void *input, void *output, int input_dtype, 
                               size_t rows, size_t n, double eps,
                               const void *gamma, const void *beta, int param_dtype, pt_stream_t stream);
 
+/* Gradients of pt_layernorm_params for the upstream gradient `grad` (rows of
+ * n elements of the compute dtype, which is the forward result's): with
+ * x' = (x - mean) / sqrt(var + eps) and h = grad * gamma,
+ *   dinput = (h - mean(h) - x' mean(h x')) / sqrt(var + eps),  input_dtype
+ *   dgamma = sum over rows of grad x',  dbeta = sum over rows of grad,
+ * both [n] of param_dtype.  gamma may be NULL (ones), and each result that is
+ * not wanted; the row statistics are recomputed from the input.  Without
+ * rows dgamma and dbeta are zeros.  Results do not depend on timing. */
+pt_status pt_layernorm_backward(const void *input, const void *grad, int input_dtype, int compute_dtype,
+                                size_t rows, size_t n, double eps, const void *gamma, int param_dtype,
+                                void *dinput, void *dgamma, void *dbeta, pt_stream_t stream);
+
+/* ------------------------------------------------- token probabilities ----
+ * No counterpart in the reference, whose classifier composes its cross
+ * entropy from max, exp, sum and log over whole tensors.
+ *
+ * Per row of `classes` scores (float32, float16 or bfloat16; rows row_stride
+ * elements apart): with p = softmax(row), any of
+ *   logprob [rows]           log p[tokens[row]]; 0 for a negative token (a
+ *                            position without one), NaN for one past the
+ *                            classes, which is not looked up
+ *   entropy [rows]           -sum p log p
+ *   stats [rows][2]          the row's maximum m and log sum exp(row - m), for
+ *                            the backward call
+ *   top_logprob, top_index   the `top` (0 to 64) likeliest classes, their log
+ *     [rows][top]            probabilities in falling order, the lower index
+ *                            first among equals; NaN is never listed, index
+ *                            -1 where fewer classes are left
+ * in float32 and int32, from one read of the scores.  A row of -inf alone has
+ * log probabilities -inf, entropy 0 and no gradient. */
+pt_status pt_logprobs(const void *logits, int dtype, size_t rows, size_t classes, size_t row_stride,
+                      const int32_t *tokens, int top, float *logprob, float *entropy, float *stats,
+                      float *top_logprob, int32_t *top_index, pt_stream_t stream);
+/* dlogits (contiguous rows of the scores' dtype) for upstream gradients of
+ * logprob, entropy and top_logprob, each of which may be NULL; stats, entropy
+ * and top_index are the forward call's. */
+pt_status pt_logprobs_backward(const void *logits, int dtype, size_t rows, size_t classes, size_t row_stride,
+                               const int32_t *tokens, int top, const int32_t *top_index, const float *stats,
+                               const float *entropy, const float *grad_logprob, const float *grad_entropy,
+                               const float *grad_top, void *dlogits, pt_stream_t stream);
+
+/* ------------------------------------------------------------- attention --
+ * No counterpart in the reference.  out = softmax(scale q k^T) v per
+ * sequence and head, query head h reading key head h / (heads / kv_heads).
+ * Operands float32, float16 or bfloat16 (one dtype), products on MFMA with
+ * fp32 sums and softmax; in 16 bits the probabilities are rounded to the
+ * dtype for their product with v.
+ *
+ * A side without starts holds [sequences][queries or keys] tokens, strides
+ * {sequence, token, head} in elements, the head's elements side by side.  A
+ * side with starts is one tensor of token rows: sequence b takes
+ * lengths[b] rows from row starts[b] on (packed prompts, or slots of a
+ * cache).  starts and lengths are device arrays, so a captured graph follows
+ * them; `queries` / `keys` are then upper bounds of the lengths and q_rows /
+ * k_rows the tensor's token rows, and a start or length that leaves either
+ * is cut to it.  Sequences of one call must not share query rows, nor key
+ * rows in the backward call.
+ *
+ * causal: query i of n sees keys 0 .. i + m - n of m (the last query sees
+ * every key).  A query that sees no key gets zeros, lse -inf and no
+ * gradient.  Keys and queries past a sequence's length are never read.
+ * Inside a sequence a value that is NaN or infinite may reach queries that
+ * do not see its key. */
+typedef struct {
+    int dtype;
+    int sequences, heads, kv_heads;
+    int head_size;               /* 1 to 256 */
+    int queries, keys;           /* tokens of each sequence, or the most */
+    size_t q_strides[3], k_strides[3], v_strides[3];
+    const int32_t *q_starts, *q_lengths; /* device int32[sequences], or NULL */
+    const int32_t *k_starts, *k_lengths;
+    int q_rows, k_rows;          /* token rows of a side with starts */
+    int causal;
+    double scale;                /* finite and positive */
+} pt_attention_desc;
+
+/* out: contiguous, q's shape; lse (may be NULL): float32, the log of each
+ * row's sum of exponentials, [sequences][heads][queries], or
+ * [heads][q_rows] where q has starts.  Rows of no sequence are left as they
+ * were. */
+pt_status pt_attention(const pt_attention_desc *desc, const void *q, const void *k, const void *v, void *out,
+                       float *lse, pt_stream_t stream);
+/* Gradients of the operands' dtype, contiguous, of q's and k's shapes, for
+ * the upstream gradient `grad` (contiguous like out, float32 or the operands'
+ * dtype); out and lse are the forward call's.  Rows of no sequence are left
+ * as they were.  Results do not depend on timing. */
+pt_status pt_attention_backward(const pt_attention_desc *desc, const void *q, const void *k, const void *v,
+                                const void *out, const float *lse, const void *grad, int grad_dtype, void *dq,
+                                void *dk, void *dv, pt_stream_t stream);
+
 /* ------------------------------------------------------------------ GEMM --
  * Replaces cuda_matmul_launcher (src/backends/cuda/matmul_kernels.h:40-44),
  * cuda_batched_matmul_nd_launcher (:47-51) and

@@ -1,0 +1,5 @@
+// Attention kernels, bfloat16 (see pt_attention.h).
+#include "../../include/pt_hip.h"
+
+#define PT_ATTN_DT PT_BFLOAT16
+#include "pt_attention_inst.h"

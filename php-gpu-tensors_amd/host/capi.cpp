@@ -308,6 +308,72 @@ phpt_tensor *phpt_scatter_add(phpt_tensor *a, phpt_tensor *indices, phpt_tensor 
     return wrap(cuda_tensor_scatter_add(a->t, indices->t, updates->t, ax));
 }
 
+// ------------------------------------------- operators of language models
+static TensorP tensor_of(phpt_tensor *h) { return h ? h->t : nullptr; }
+static SequencesP sequences_of(phpt_sequences *h) { return h ? h->s : nullptr; }
+
+int phpt_layernorm_backward(phpt_tensor *a, phpt_tensor *grad, const int *axes, int naxes, double eps,
+                            phpt_tensor *scale, phpt_tensor *bias, phpt_tensor **results)
+{
+    clear_error();
+    TensorP out[3];
+    if (!cuda_array_layernorm_backward(a->t, grad->t, axes, naxes, eps, tensor_of(scale), tensor_of(bias), out)) return -1;
+    for (int i = 0; i < 3; i++) results[i] = wrap(out[i]);
+    return 0;
+}
+
+phpt_sequences *phpt_sequences_create(const int *lengths, const int *starts, int count)
+{
+    clear_error();
+    SequencesP s = make_sequences(lengths, starts, count);
+    return s ? new phpt_sequences{s} : nullptr;
+}
+
+void phpt_sequences_release(phpt_sequences *s) { delete s; }
+
+phpt_tensor *phpt_attention(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, int causal, double scale,
+                            phpt_sequences *queries, phpt_sequences *keys, phpt_tensor **lse)
+{
+    clear_error();
+    TensorP out[2];
+    if (!cuda_array_attention(q->t, k->t, v->t, causal != 0, scale, sequences_of(queries), sequences_of(keys),
+                              lse != nullptr, out))
+        return nullptr;
+    if (lse) *lse = wrap(out[1]);
+    return wrap(out[0]);
+}
+
+int phpt_attention_backward(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, phpt_tensor *out, phpt_tensor *lse,
+                            phpt_tensor *grad, int causal, double scale, phpt_sequences *queries,
+                            phpt_sequences *keys, phpt_tensor **results)
+{
+    clear_error();
+    TensorP got[3];
+    if (!cuda_array_attention_backward(q->t, k->t, v->t, out->t, lse->t, grad->t, causal != 0, scale,
+                                       sequences_of(queries), sequences_of(keys), got))
+        return -1;
+    for (int i = 0; i < 3; i++) results[i] = wrap(got[i]);
+    return 0;
+}
+
+int phpt_logprobs(phpt_tensor *a, phpt_tensor *tokens, int top, phpt_tensor **results)
+{
+    clear_error();
+    TensorP out[5];
+    if (!cuda_array_logprobs(a->t, tokens->t, top, out)) return -1;
+    for (int i = 0; i < 5; i++) results[i] = wrap(out[i]);
+    return 0;
+}
+
+phpt_tensor *phpt_logprobs_backward(phpt_tensor *a, phpt_tensor *tokens, phpt_tensor *stats, phpt_tensor *entropy,
+                                    phpt_tensor *top_index, phpt_tensor *grad_logprob, phpt_tensor *grad_entropy,
+                                    phpt_tensor *grad_top)
+{
+    clear_error();
+    return wrap(cuda_array_logprobs_backward(a->t, tokens->t, stats->t, entropy->t, tensor_of(top_index),
+                                             tensor_of(grad_logprob), tensor_of(grad_entropy), tensor_of(grad_top)));
+}
+
 phpt_tensor *phpt_astype(phpt_tensor *a, int dtype)
 {
     clear_error();

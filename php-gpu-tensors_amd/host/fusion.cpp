@@ -259,12 +259,16 @@ static int collect(Plan &p, const TensorP &t, std::map<const Tensor *, int> &ind
         // (fusion_plan.c:462-486); other native steps take a materialized
         // operand
         const NativeSpec &ns = t->node->native;
-        const bool aliasing = ns.kind == NAT_MATMUL || ns.kind == NAT_REDUCE || ns.kind == NAT_ARG_REDUCE;
+        const bool attention = ns.kind == NAT_ATTENTION || ns.kind == NAT_ATTENTION_BACKWARD;
+        const bool aliasing =
+            ns.kind == NAT_MATMUL || ns.kind == NAT_REDUCE || ns.kind == NAT_ARG_REDUCE || attention;
         const bool global = (ns.kind == NAT_REDUCE || ns.kind == NAT_ARG_REDUCE) && ns.axis == kGlobalAxis;
         for (int a : me.args) {
             Item &ai = p.items[a];
             if (ai.kind != IT_ELEM) continue;
             bool view = !ai.cut && ai.t->node->kind == N_VIEW;
+            // attention reads heads and tokens at any stride, a head's elements side by side
+            if (view && attention && ai.t->ndims && ai.t->node->view_strides[ai.t->ndims - 1] != 1) view = false;
             if (view && global) {
                 size_t cs[kMaxDims];
                 contiguous_strides(ai.t->shape, ai.t->ndims, cs);
@@ -1694,6 +1698,8 @@ static bool run_step(Plan &p, const Step &st, std::vector<TensorP> &vals)
 {
     if (!st.native) return launch_kernel(p, p.kernels[st.kernel], vals);
     Item &it = p.items[st.item];
+    const int kind = it.t->node->native.kind;
+    if (kind == NAT_BUFFER || kind == NAT_RESULT) return true;  // placed by prepare_values
     std::vector<TensorP> ins;
     for (int a : it.args) {
         TensorP v = native_arg(p, vals, a);
@@ -1961,8 +1967,12 @@ static bool prepare_values(Plan &p, std::vector<TensorP> &vals)
     for (Kernel &k : p.kernels)
         for (int r : k.roots)
             if (!give(r)) return false;
+    auto result = [&](const Step &st) { return st.native && p.items[st.item].t->node->native.kind == NAT_RESULT; };
     for (Step &st : p.steps)
-        if (st.native && !give(st.item)) return false;
+        if (st.native && !result(st) && !give(st.item)) return false;
+    // a further result of an operator is the buffer it was written to
+    for (Step &st : p.steps)
+        if (result(st)) vals[st.item] = vals[p.items[st.item].args[0]];
     return true;
 }
 
@@ -2646,7 +2656,11 @@ const char *phpt_graph_plan(phpt_graph *g)
         if (st.native) {
             static const char *names[] = {"native-matmul", "native-reduction", "native-reduction",
                                           "native-moments", "native-softmax", "native-layernorm",
-                                          "native-gather", "native-scatter-add"};
+                                          "native-gather", "native-scatter-add",
+                                          "native-buffer", "native-result",
+                                          "native-attention", "native-attention-backward",
+                                          "native-layernorm-backward", "native-logprobs",
+                                          "native-logprobs-backward"};
             const Item &it = p.items[st.item];
             // layout aliases: views passed to this native step without a copy
             for (int a : it.args)

@@ -27,7 +27,7 @@ static void aligned_strides(const Tensor &t, int nd, size_t *out)
     }
 }
 
-static bool guard(const TensorP &t)
+bool guard(const TensorP &t)
 {
     if (!t) {
         if (!error_kind()) set_invalid("Missing tensor operand");
@@ -690,6 +690,11 @@ TensorP native_execute(const NativeSpec &sp, const std::vector<TensorP> &in)
         TensorP bias = sp.has_bias ? in[k++] : nullptr;
         return cuda_array_layernorm(in[0], sp.axes, sp.naxes, sp.eps, scale, bias);
     }
+    case NAT_ATTENTION:
+    case NAT_ATTENTION_BACKWARD:
+    case NAT_LAYERNORM_BACKWARD:
+    case NAT_LOGPROBS:
+    case NAT_LOGPROBS_BACKWARD: return native_execute_model(sp, in);
     default:
         set_runtime("Unknown native step");
         return nullptr;

@@ -81,6 +81,37 @@ phpt_tensor *phpt_where(phpt_tensor *c, phpt_tensor *x, phpt_tensor *y);
  * axis may be negative */
 phpt_tensor *phpt_gather(phpt_tensor *a, phpt_tensor *indices, long long axis);
 phpt_tensor *phpt_scatter_add(phpt_tensor *a, phpt_tensor *indices, phpt_tensor *updates, long long axis);
+/* ---- operators of language models (no counterpart in the reference) ---- */
+/* Gradients of phpt_layernorm: results[3] gets those of the input, the scale
+ * and the bias (NULL where that operand is NULL), each of its operand's
+ * dtype.  Returns 0, or -1 on error, as the calls below. */
+int phpt_layernorm_backward(phpt_tensor *a, phpt_tensor *grad, const int *axes, int naxes, double eps,
+                            phpt_tensor *scale, phpt_tensor *bias, phpt_tensor **results);
+/* Where the sequences of a tensor of token rows lie: lengths[count] rows each
+ * from starts[count] on (starts NULL: one behind the other).  Checked and
+ * copied to the device here; a handle serves any number of calls. */
+typedef struct phpt_sequences phpt_sequences;
+phpt_sequences *phpt_sequences_create(const int *lengths, const int *starts, int count);
+void phpt_sequences_release(phpt_sequences *s);
+/* pt_attention over q, k, v [tokens, heads, size] or [sequences, tokens,
+ * heads, size] (any strides); the first form with sequences of both sides or
+ * with neither.  scale 0: 1 / sqrt(size).  Returns the output, of q's shape
+ * and dtype, zeros in rows of no sequence; lse, where not NULL, gets what the
+ * gradient call takes. */
+phpt_tensor *phpt_attention(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, int causal, double scale,
+                            phpt_sequences *queries, phpt_sequences *keys, phpt_tensor **lse);
+/* results[3]: gradients of q, k and v */
+int phpt_attention_backward(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, phpt_tensor *out, phpt_tensor *lse,
+                            phpt_tensor *grad, int causal, double scale, phpt_sequences *queries,
+                            phpt_sequences *keys, phpt_tensor **results);
+/* pt_logprobs of the rows along a's last axis, tokens int32 of the rows'
+ * shape: results[5] gets the log probability, the entropy, stats, and for
+ * top > 0 the alternatives' log probabilities and indices (else NULL) */
+int phpt_logprobs(phpt_tensor *a, phpt_tensor *tokens, int top, phpt_tensor **results);
+/* top_index and each upstream gradient may be NULL */
+phpt_tensor *phpt_logprobs_backward(phpt_tensor *a, phpt_tensor *tokens, phpt_tensor *stats, phpt_tensor *entropy,
+                                    phpt_tensor *top_index, phpt_tensor *grad_logprob, phpt_tensor *grad_entropy,
+                                    phpt_tensor *grad_top);
 phpt_tensor *phpt_astype(phpt_tensor *a, int dtype);
 phpt_tensor *phpt_copy(phpt_tensor *a);
 

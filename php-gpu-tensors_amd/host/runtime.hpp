@@ -149,6 +149,40 @@ TensorP cuda_tensor_gather(const TensorP &input, const TensorP &indices, int axi
 TensorP cuda_tensor_scatter_add(const TensorP &input, const TensorP &indices, const TensorP &updates, int axis);
 // validation record of the executing Fusion plan (nullptr outside one)
 int32_t *&index_record();
+// Where the sequences of a packed tensor, or of the slots of a cache, lie
+// among its token rows.  Checked on the host when it is made and never
+// changed; the device copy is int32 [2, count], starts then lengths.
+struct Sequences {
+    std::vector<int> starts, lengths;
+    int most = 0;          // longest
+    long long end = 0;     // first row past the last sequence
+    long long total = 0;   // rows of all sequences
+    bool overlap = false;  // some row lies in two of them
+    TensorP device;
+    int count() const { return (int)lengths.size(); }
+    const int32_t *device_starts() const;
+    const int32_t *device_lengths() const;
+    // every row of a tensor of `rows` lies in one sequence
+    bool cover(long long rows) const { return !overlap && total == rows; }
+};
+using SequencesP = std::shared_ptr<Sequences>;
+SequencesP make_sequences(const int *lengths, const int *starts, int count);  // starts null: one behind the other
+
+// Operators with several results: `out` gets one tensor per result (null
+// where it is not wanted).  lse is kept for the gradient.
+bool cuda_array_attention(const TensorP &q, const TensorP &k, const TensorP &v, bool causal, double scale,
+                          const SequencesP &qs, const SequencesP &ks, bool want_lse, TensorP out[2]);
+bool cuda_array_attention_backward(const TensorP &q, const TensorP &k, const TensorP &v, const TensorP &o,
+                                   const TensorP &lse, const TensorP &grad, bool causal, double scale,
+                                   const SequencesP &qs, const SequencesP &ks, TensorP out[3]);
+// gradients of the input, the scale and the bias; scale and bias may be null
+bool cuda_array_layernorm_backward(const TensorP &a, const TensorP &grad, const int *axes, int naxes, double eps,
+                                   const TensorP &scale, const TensorP &bias, TensorP out[3]);
+// log probability, entropy, stats [.., 2], log probabilities and indices of the `top` likeliest
+bool cuda_array_logprobs(const TensorP &a, const TensorP &tokens, int top, TensorP out[5]);
+TensorP cuda_array_logprobs_backward(const TensorP &a, const TensorP &tokens, const TensorP &stats, const TensorP &entropy,
+                                     const TensorP &top_index, const TensorP &g_logprob, const TensorP &g_entropy,
+                                     const TensorP &g_top);
 TensorP tensor_cast(const TensorP &a, int dtype);
 TensorP astype(const TensorP &a, int dtype);  // safe casts only (CudaArray::astype)
 TensorP copy(const TensorP &a);
@@ -169,7 +203,13 @@ enum NodeKind {
 };
 
 enum NativeKind {
-    NAT_MATMUL = 0, NAT_REDUCE, NAT_ARG_REDUCE, NAT_MOMENTS, NAT_SOFTMAX, NAT_LAYERNORM, NAT_GATHER, NAT_SCATTER_ADD
+    NAT_MATMUL = 0, NAT_REDUCE, NAT_ARG_REDUCE, NAT_MOMENTS, NAT_SOFTMAX, NAT_LAYERNORM, NAT_GATHER, NAT_SCATTER_ADD,
+    // A native step has one result.  Further results of an operator are
+    // buffers that the step gets as operands and writes: NAT_BUFFER makes one
+    // (no kernel), and NAT_RESULT is its value once the step in its second
+    // operand has written it.
+    NAT_BUFFER, NAT_RESULT,
+    NAT_ATTENTION, NAT_ATTENTION_BACKWARD, NAT_LAYERNORM_BACKWARD, NAT_LOGPROBS, NAT_LOGPROBS_BACKWARD
 };
 
 struct NativeSpec {
@@ -182,6 +222,9 @@ struct NativeSpec {
     int naxes = 0;
     int axes[kMaxDims] = {0};
     bool has_scale = false, has_bias = false;
+    bool causal = false, has_lse = false;
+    int top = 0, given = 0;  // given: which optional operands follow (a bit each)
+    SequencesP q_seq, k_seq;
 };
 
 struct FusionNode {
@@ -211,9 +254,14 @@ bool fusion_materialize(const TensorP &t);
 
 // Eager implementations of native boundary ops (inputs materialized).
 TensorP native_execute(const NativeSpec &spec, const std::vector<TensorP> &inputs);
+TensorP native_execute_model(const NativeSpec &spec, const std::vector<TensorP> &inputs);  // model_ops.cpp
+bool guard(const TensorP &t);  // materialized, or an error set
 }  // namespace phpt
 
-// Opaque C handle of phpt_host.h: one reference to a tensor.
+// Opaque C handles of phpt_host.h: one reference each.
 struct phpt_tensor {
     phpt::TensorP t;
+};
+struct phpt_sequences {
+    phpt::SequencesP s;
 };

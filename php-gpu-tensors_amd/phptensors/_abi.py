@@ -65,6 +65,15 @@ class PtBackendInfo(ctypes.Structure):
             "staged_copies")]
 
 
+class PtAttentionDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int) for name in ("dtype", "sequences", "heads", "kv_heads", "head_size",
+                                                  "queries", "keys")] + \
+               [(name, ctypes.c_size_t * 3) for name in ("q_strides", "k_strides", "v_strides")] + \
+               [(name, vp) for name in ("q_starts", "q_lengths", "k_starts", "k_lengths")] + \
+               [("q_rows", ctypes.c_int), ("k_rows", ctypes.c_int), ("causal", ctypes.c_int),
+                ("scale", ctypes.c_double)]
+
+
 # name -> (restype, argtypes); every function declared in include/pt_hip.h
 SIGNATURES = {
     "pt_init": (ctypes.c_int, []),
@@ -116,6 +125,15 @@ SIGNATURES = {
                                     ctypes.c_size_t, ctypes.c_double, vp, vp, vp]),
     "pt_layernorm_params": (ctypes.c_int, [vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_size_t,
                                            ctypes.c_size_t, ctypes.c_double, vp, vp, ctypes.c_int, vp]),
+    "pt_layernorm_backward": (ctypes.c_int, [vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_size_t, ctypes.c_size_t,
+                                             ctypes.c_double, vp, ctypes.c_int, vp, vp, vp, vp]),
+    "pt_logprobs": (ctypes.c_int, [vp, ctypes.c_int, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, vp,
+                                   ctypes.c_int, vp, vp, vp, vp, vp, vp]),
+    "pt_logprobs_backward": (ctypes.c_int, [vp, ctypes.c_int, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, vp,
+                                            ctypes.c_int, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "pt_attention": (ctypes.c_int, [ctypes.POINTER(PtAttentionDesc), vp, vp, vp, vp, vp, vp]),
+    "pt_attention_backward": (ctypes.c_int, [ctypes.POINTER(PtAttentionDesc), vp, vp, vp, vp, vp, vp, ctypes.c_int,
+                                             vp, vp, vp, vp]),
     "pt_matmul": (ctypes.c_int, [vp, vp, vp, ctypes.c_int, c_int_p, c_size_p, ctypes.c_int,
                                  c_int_p, c_size_p, ctypes.c_int, c_int_p, ctypes.c_int, vp]),
     "pt_matmul_tune": (ctypes.c_int, [vp, vp, vp, ctypes.c_int, c_int_p, c_size_p, ctypes.c_int,

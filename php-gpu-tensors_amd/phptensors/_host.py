@@ -44,6 +44,14 @@ SIGNATURES = {
     "phpt_variance": (T, [T, ctypes.c_int, ctypes.c_long, ctypes.c_int]),
     "phpt_softmax": (T, [T, ctypes.c_int]),
     "phpt_layernorm": (T, [T, ip, ctypes.c_int, ctypes.c_double, T, T]),
+    "phpt_layernorm_backward": (ctypes.c_int, [T, T, ip, ctypes.c_int, ctypes.c_double, T, T, ctypes.POINTER(T)]),
+    "phpt_sequences_create": (vp, [ip, ip, ctypes.c_int]),
+    "phpt_sequences_release": (None, [vp]),
+    "phpt_attention": (T, [T, T, T, ctypes.c_int, ctypes.c_double, vp, vp, ctypes.POINTER(T)]),
+    "phpt_attention_backward": (ctypes.c_int, [T, T, T, T, T, T, ctypes.c_int, ctypes.c_double, vp, vp,
+                                               ctypes.POINTER(T)]),
+    "phpt_logprobs": (ctypes.c_int, [T, T, ctypes.c_int, ctypes.POINTER(T)]),
+    "phpt_logprobs_backward": (T, [T] * 8),
     "phpt_matmul": (T, [T, T]),
     "phpt_tune_matmul": (T, [T, T, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_float), ctypes.c_int,
                              ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]),

@@ -8,7 +8,9 @@ and accumulates gradients on the leaves.  The gradient formulas follow
 src/autograd.c: matmul (:1539-1585, upstream @ B^T and A^T @ upstream over
 transposed views), broadcast operands reduced back to their shape,
 reductions (:900-1003: sum expands, max shares the upstream gradient equally
-among the maxima), where, exp, log, reshape.  Every gradient is itself a
+among the maxima), where, exp, log, reshape.  layerNorm, attention and
+logProbs, which the reference does not differentiate or does not have, run
+gradient kernels of their own.  Every gradient is itself a
 CudaArray expression, so inside a Fusion scope the backward pass is recorded
 into the plan like the forward pass.
 """
@@ -21,6 +23,33 @@ class Node:
         self.parents = parents
         self.backward = backward
         self.op = op
+
+
+class Parts:
+    """The values that an operation with several differentiable results
+    shares: the parent of each result, and itself an operation of the
+    operands.  Its gradient is a Gradients, so that the operands' gradient is
+    computed once from all of the results' upstream gradients."""
+    __slots__ = ("_rg", "_node", "_grad")
+
+    def __init__(self):
+        self._rg = False
+        self._node = None
+        self._grad = None
+
+    def part(self, out, name):
+        """Make `out` the result that passes its gradient on under `name`."""
+        return record(out, [self], lambda g: [Gradients({name: g})], name)
+
+
+class Gradients(dict):
+    """Upstream gradients of an operation's results, by name."""
+
+    def __add__(self, other):
+        both = Gradients(self)
+        for name, g in other.items():
+            both[name] = both[name] + g if name in both else g
+        return both
 
 
 _recording = [True]

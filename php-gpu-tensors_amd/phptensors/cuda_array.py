@@ -538,9 +538,99 @@ class CudaArray:
 
     def layerNorm(self, axes, epsilon=1e-5, scale=None, bias=None):
         ax, n = _ints(axes)
-        return CudaArray._wrap(_host.load().phpt_layernorm(
+        out = CudaArray._wrap(_host.load().phpt_layernorm(
             self._h, ax, n, float(epsilon), scale._h if scale is not None else None,
             bias._h if bias is not None else None))
+        if AG.active(self, scale, bias):
+            parents = [t for t in (self, scale, bias) if t is not None]
+
+            def back(g):
+                got = (ctypes.c_void_p * 3)()
+                if _host.load().phpt_layernorm_backward(
+                        self._h, g._h, ax, n, float(epsilon), scale._h if scale is not None else None,
+                        bias._h if bias is not None else None, got):
+                    _host.raise_error("layerNorm gradient")
+                grads = [CudaArray._wrap(h) if h else None for h in got]
+                return [gr for gr, t in zip(grads, (self, scale, bias)) if t is not None]
+            AG.record(out, parents, back, "layerNorm")
+        return out
+
+    # ------------------------------------------------- operators of language models
+    def attention(self, key, value, causal=False, scale=None, queries=None, keys=None):
+        """softmax(scale q k^T) v per head, self being the queries: [tokens,
+        heads, size], or [sequences, tokens, heads, size] for sequences of
+        one length, in float32, float16 or bfloat16; key and value likewise,
+        with a divisor of the heads (query head h reads key head h // (heads
+        / key heads)).  Any strides are read in place as long as a head's
+        elements lie side by side.
+
+        queries and keys (Sequences) name the rows of each sequence in a
+        tensor of rank 3, prompts packed behind each other or the slots of a
+        cache; keys defaults to queries.  causal: the last query of a
+        sequence sees all its keys, each earlier one a key less.  scale
+        defaults to 1 / sqrt(size).  Queries that see no key, and rows of no
+        sequence, give zeros.  The gradients have their operands' dtypes."""
+        if not isinstance(key, CudaArray) or not isinstance(value, CudaArray):
+            raise InvalidArgumentException("attention() expects CudaArray keys and values")
+        if scale is not None and not float(scale) > 0.0:
+            raise InvalidArgumentException("attention scale must be finite and positive")
+        keys = queries if keys is None else keys
+        if any(s is not None and not isinstance(s, Sequences) for s in (queries, keys)):
+            raise InvalidArgumentException("attention() expects Sequences")
+        lib = _host.load()
+        c = 0.0 if scale is None else float(scale)
+        at = [s._h if s is not None else None for s in (queries, keys)]
+        active = AG.active(self, key, value)
+        lse_h = ctypes.c_void_p()
+        out = CudaArray._wrap(lib.phpt_attention(self._h, key._h, value._h, int(bool(causal)), c, *at,
+                                                 ctypes.byref(lse_h) if active else None), "attention")
+        if active:
+            lse, result = CudaArray._wrap(lse_h.value), out.detach()
+
+            def back(g):
+                got = (ctypes.c_void_p * 3)()
+                held = (queries, keys)  # the handles behind `at`
+                if lib.phpt_attention_backward(self._h, key._h, value._h, result._h, lse._h, g._h, int(bool(causal)), c,
+                                               *(s._h if s is not None else None for s in held), got):
+                    _host.raise_error("attention gradient")
+                return [CudaArray._wrap(h) for h in got]
+            AG.record(out, [self, key, value], back, "attention")
+        return out
+
+    def logProbs(self, tokens, top=0):
+        """Of each row of scores along the last axis (float32, float16 or
+        bfloat16): "logProbs", the log of the softmax at the row's token
+        (int32, of the rows' shape; 0 for a negative token, a position
+        without one, and NaN for one past the classes), "entropy" and, for
+        top > 0, "topLogProbs" and "topTokens", the `top` likeliest classes,
+        the lower index first among equals; float32 and int32.  The gradients
+        of all of them reach the scores in one pass and in the scores'
+        dtype."""
+        if not isinstance(tokens, CudaArray):
+            raise InvalidArgumentException("logProbs() expects CudaArray tokens")
+        lib = _host.load()
+        got = (ctypes.c_void_p * 5)()
+        if lib.phpt_logprobs(self._h, tokens._h, _int32(top, "top"), got):
+            _host.raise_error("logProbs")
+        logprob, entropy, stats, top_v, top_i = [CudaArray._wrap(h) if h else None for h in got]
+        out = {"logProbs": logprob, "entropy": entropy}
+        if top_v is not None:
+            out.update(topLogProbs=top_v, topTokens=top_i)
+        if AG.active(self):
+            # the gradient reads the entropy's values, not its history
+            values = entropy.detach()
+
+            def back(g):
+                g = {name: x if x.getDtype() == "float32" else x.astype("float32") for name, x in g.items()}
+                grads = [g[n]._h if n in g else None for n in ("logProbs", "entropy", "topLogProbs")]
+                return [CudaArray._wrap(lib.phpt_logprobs_backward(
+                    self._h, tokens._h, stats._h, values._h, top_i._h if grads[2] else None, *grads),
+                    "logProbs gradient")]
+            parts = AG.record(AG.Parts(), [self], back, "logProbs")
+            for name in ("logProbs", "entropy", "topLogProbs"):
+                if name in out:
+                    parts.part(out[name], name)
+        return out
 
     def matmul(self, other):
         if not isinstance(other, CudaArray):
@@ -736,6 +826,35 @@ class CudaArray:
 
     def __repr__(self):
         return f"CudaArray(shape={self.getShape()}, dtype={self.getDtype()})"
+
+
+class Sequences:
+    """Where the sequences of a tensor of token rows lie: `lengths[b]` rows
+    from row `starts[b]` on, by default one sequence behind the other.  Checked
+    and copied to the device once; serves any number of attention() calls."""
+
+    __slots__ = ("_h", "lengths", "starts", "__weakref__")
+
+    def __init__(self, lengths, starts=None):
+        self._h = None
+        n_arr, n = _ints(lengths)
+        s_arr = None
+        if starts is not None:
+            s_arr, m = _ints(starts)
+            if m != n:
+                raise InvalidArgumentException("Sequences need a start for each length")
+        self._h = _host.check_handle(_host.load().phpt_sequences_create(n_arr, s_arr, n), "Sequences")
+        self.lengths = [n_arr[i] for i in range(n)]
+        self.starts = [s_arr[i] if s_arr is not None else sum(self.lengths[:i]) for i in range(n)]
+
+    def __len__(self):
+        return len(self.lengths)
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h and _host._lib is not None:
+            _host._lib.phpt_sequences_release(h)
+            self._h = None
 
 
 def _from_bits(arr, code):
