@@ -24,6 +24,7 @@
 #pragma once
 
 #include <limits.h>
+#include <type_traits>
 
 #include "pt_gemm.h"
 
@@ -41,6 +42,8 @@ struct AttnArgs {
     float scale, scale_log2;
     int splits;               // key ranges computed by workgroups of their own
     float *part_o, *part_ml;  // their results: [split][sequence, key head][row][size], and (m, l)
+    int place, tiles;         // AttnPlace, and the tiles of a head
+    long long part_step;      // backward: parts of dk or dq in part_o, of dv in part_ml, this many elements apart
     // backward
     const void *w;            // upstream gradient in the element type, contiguous like out
     const float *lse2, *delta;  // per (head, token row): lse in base 2 (+inf where nothing is seen), d
@@ -60,6 +63,108 @@ __device__ __forceinline__ AttnSeq attn_seq(const int32_t *starts, const int32_t
     if (!starts) return {0, most};
     const int s = min(max(starts[b], 0), rows);
     return {s, min(max(lengths[b], 0), min(most, rows - s))};
+}
+
+// Which tile, sequence and key head a workgroup takes, the longest work
+// first.  Workgroups go to the 8 XCDs in turn; each XCD has an L2 of 4 MB,
+// which holds the keys and values of a head or two.
+enum AttnPlace {
+    // the tiles of all heads side by side
+    kPlain = 0,
+    // Heads a multiple of 8: a head keeps to an XCD, which takes as many heads
+    // at once as fill its 64 workgroups and the next when those run out.  A
+    // causal head's tiles fall in length, so the next heads' long ones follow
+    // the last's short ones.
+    kGrouped,
+    // Key heads a divisor of 8: the XCDs divide the key heads between them,
+    // and those with one head its tiles, so every sequence loads all of them.
+    kSpread,
+    // Sequences of different lengths: the tiles that exist, numbered through
+    // all sequences by their distance from the short end, the key heads to
+    // the XCDs as above.  Numbering tiles that do not exist too leaves
+    // workgroups empty, which come at a period of the dispatch and leave
+    // whole shader engines idle (225 us instead of 153 for six prompts of
+    // 4096 to 1 tokens).
+    kRagged
+};
+
+// The item-th of the existing tiles, from the highest level down: level t
+// holds the t-th tile of every sequence that has one.  The tiles at level t
+// and above number sum over sequences of max(0, tiles - t).
+__device__ __forceinline__ bool attn_item(const int32_t *starts, const int32_t *lengths, int rows, int most, int batch,
+                                          int group, int levels, int item, int &level, int &b)
+{
+    const int lane = threadIdx.x & 63;
+    auto tiles = [&](int i) { return i < batch ? (int)(((long long)attn_seq(starts, lengths, rows, most, i).n * group + 127) / 128) : 0; };
+    const int first = tiles(lane);
+    auto above = [&](int t) {
+        int n = max(0, first - t);
+        for (int i = lane + 64; i < batch; i += 64) n += max(0, tiles(i) - t);
+        return wave_all(n, FAdd{});
+    };
+    if (item >= above(0)) return false;
+    int low = 0, high = levels;
+    while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (above(mid) > item) low = mid;
+        else high = mid;
+    }
+    int r = item - above(low + 1);
+    for (int c = 0; c < batch; c += 64) {
+        const bool has = (c ? tiles(c + lane) : first) > low;
+        const uint64_t mask = __ballot(has);
+        const int n = (int)__popcll(mask);
+        if (r < n) {
+            const uint64_t it = __ballot(has && (int)__popcll(mask & ((1ull << lane) - 1)) == r);
+            level = low;
+            b = c + (int)__builtin_ctzll(it);
+            return true;
+        }
+        r -= n;
+    }
+    return false;
+}
+
+// `keys`: tiles of the keys, whose first is the longest work (the queries'
+// last is).  false: nothing for this workgroup.
+__device__ __forceinline__ bool attn_place(const AttnArgs &g, bool keys, int &tile, int &bh)
+{
+    const unsigned id = blockIdx.x, nh = (unsigned)(g.batch * g.kv_heads), tiles = (unsigned)g.tiles, kv = (unsigned)g.kv_heads;
+    const unsigned x = id % 8, j = id / 8;
+    if (g.place == kRagged) {
+        unsigned item = id / kv, h = id % kv;
+        if (8 % kv == 0) {
+            item = j * (8 / kv) + x % (8 / kv);
+            h = x / (8 / kv);
+        } else if (kv % 8 == 0) {
+            item = j / (kv / 8);
+            h = x + j % (kv / 8) * 8;
+        }
+        int t, b;
+        const bool some = keys ? attn_item(g.k_starts, g.k_lengths, g.k_rows, g.nk, g.batch, 1, g.tiles, (int)item, t, b)
+                               : attn_item(g.q_starts, g.q_lengths, g.q_rows, g.nq, g.batch, g.group, g.tiles, (int)item, t, b);
+        if (!some) return false;
+        t = __builtin_amdgcn_readfirstlane(t);
+        b = __builtin_amdgcn_readfirstlane(b);
+        if (keys) t = (attn_seq(g.k_starts, g.k_lengths, g.k_rows, g.nk, b).n + 127) / 128 - 1 - t;
+        tile = t;
+        bh = b * g.kv_heads + (int)h;
+        return true;
+    }
+    unsigned t = id / nh, h = id % nh;
+    if (g.place == kGrouped) {
+        const unsigned heads = nh / 8, most = min(heads, max(1u, 64 / tiles));
+        const unsigned first = j / (tiles * most) * most, n = min(most, heads - first), r = j - first * tiles;
+        t = r / n;
+        h = (first + r % n) * 8 + x;
+    } else if (g.place == kSpread) {
+        t = j / (unsigned)g.batch * (8 / kv) + x % (8 / kv);
+        h = j % (unsigned)g.batch * kv + x / (8 / kv);
+    }
+    if (t >= tiles) return false;
+    tile = (int)(keys ? t : tiles - 1 - t);
+    bh = (int)h;
+    return true;
 }
 
 template <int DT> struct AttnT {
@@ -109,16 +214,29 @@ template <int DT, int DP, int ROWS, int NW, bool VEC> struct AttnStage {
             }
         }
     }
+    __device__ __forceinline__ static uint32_t range(const AttnSrc &s, int size, int r0)
+    {
+        return r0 >= s.rows ? 0u : (uint32_t)min((long long)(s.rows - r0 - 1) * s.step + size * T::ES, (long long)0x7fffffff);
+    }
+    // The same chunks to registers; read once.
+    __device__ __forceinline__ void fetch(const AttnSrc &s, int size, int r0, floatx4 (&v)[NI]) const
+    {
+        static_assert(VEC, "whole packs");
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char *>(s.base + (long long)r0 * s.step), (short)0, (int)range(s, size, r0), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+            v[i] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off[i], 0, 2));  // nt
+    }
     // Rows r0 .. r0 + ROWS - 1 into `tile`; rows past the source's last are zeros.
     __device__ __forceinline__ void load(const AttnSrc &s, int size, int r0, S *tile, int wave, int lane) const
     {
         const char *base = s.base + (long long)r0 * s.step;
         if constexpr (VEC) {
-            const long long left = (long long)(s.rows - r0 - 1) * s.step + size * T::ES;
-            const uint32_t range = r0 >= s.rows ? 0u : (uint32_t)min(left, (long long)0x7fffffff);
+            const uint32_t bytes = range(s, size, r0);
 #pragma unroll
             for (int i = 0; i < NI; i++)
-                buffer_load_lds16(base, off[i], (PT_LDS_AS void *)(tile + (wave * NI + i) * 64 * T::PK), range);
+                buffer_load_lds16(base, off[i], (PT_LDS_AS void *)(tile + (wave * NI + i) * 64 * T::PK), bytes);
         } else {
             for (int i = 0; i < NI; i++) {
                 const int at = (wave * NI + i) * 64 + lane, row = at / CPR, c = (at % CPR) ^ attn_swz<CPR>(row);
@@ -197,6 +315,16 @@ template <int DT, int DP> struct AttnLane {
     __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(row), "+v"(col0), "+v"(col1)); }
 };
 
+// Chunk 2 t + lane / 32 of tile row row0 + lane % 32: the left operand's
+// fragment t of the product over the head's size.
+template <int DT, int DP>
+__device__ __forceinline__ typename AttnT<DT>::Frag attn_row_frag(const typename AttnT<DT>::S *tile, int row0, int t,
+                                                                  const AttnLane<DT, DP> &at)
+{
+    const PT_LDS_AS char *base = (const PT_LDS_AS char *)tile + row0 * DP * AttnT<DT>::ES;
+    return __builtin_bit_cast(typename AttnT<DT>::Frag, *(const PT_LDS_AS floatx4 *)(base + (at.row ^ (uint32_t)(t << 5))));
+}
+
 // acc[streamed row][own row] = sum over the head's size, for the 32 tile
 // rows from row0.
 template <int DT, int DP>
@@ -204,16 +332,11 @@ __device__ __forceinline__ floatx16 attn_rows(const typename AttnT<DT>::S *tile,
                                               const typename AttnT<DT>::Frag (&b)[DP * AttnT<DT>::ES / 32],
                                               const AttnLane<DT, DP> &at)
 {
-    using T = AttnT<DT>;
     floatx16 acc;
 #pragma unroll
     for (int e = 0; e < 16; e++) acc[e] = 0.0f;
-    const PT_LDS_AS char *base = (const PT_LDS_AS char *)tile + row0 * DP * T::ES;
 #pragma unroll
-    for (int t = 0; t < DP * T::ES / 32; t++) {
-        const floatx4 a = *(const PT_LDS_AS floatx4 *)(base + (at.row ^ (uint32_t)(t << 5)));
-        attn_mfma<DT>(acc, __builtin_bit_cast(typename T::Frag, a), b[t]);
-    }
+    for (int t = 0; t < DP * AttnT<DT>::ES / 32; t++) attn_mfma<DT>(acc, attn_row_frag<DT, DP>(tile, row0, t, at), b[t]);
     return acc;
 }
 
@@ -241,39 +364,55 @@ __device__ __forceinline__ typename AttnT<DT>::Frag attn_pack(const floatx16 &p,
 // rows; two of them fill the 8 k slots, rows 4 half + 0..3 and 8 + 4 half +
 // 0..3, which are the rows that registers 8 u .. 8 u + 7 hold.  float32: one
 // k slot for each half of the wave, register r's row.
+//
+// Unit u of 2 * DP / 32 (16-bit: rows 16 (u / blocks) .. + 15, element block
+// u % blocks) or of 16 * DP / 32 (float32: register u / blocks).
+template <int DT, int DP> constexpr int attn_col_units() { return (DT == PT_FLOAT32 ? 16 : 2) * DP / 32; }
+template <int DT> using AttnColFrag = std::conditional_t<DT == PT_FLOAT32, float, typename AttnT<DT>::Frag>;
+
+template <int DT, int DP>
+__device__ __forceinline__ AttnColFrag<DT> attn_col_frag(const typename AttnT<DT>::S *tile, int row0, int u,
+                                                         const AttnLane<DT, DP> &at)
+{
+    using T = AttnT<DT>;
+    const PT_LDS_AS char *base = (const PT_LDS_AS char *)tile + row0 * DP * T::ES;
+    const int d = u % (DP / 32), r = u / (DP / 32);
+    if constexpr (DT == PT_FLOAT32) {
+        // row 8 (r / 4) + r % 4 (+ 4 half): the swizzle's bits of r, the half's are in the base
+        const int x = (r % 4) << 2 | ((r / 4) * 2 & 3);
+        return *(const PT_LDS_AS float *)(base + (8 * (r / 4) + r % 4) * DP * 4 + (at.col0 ^ (uint32_t)((8 * d ^ x) << 4)));
+    } else {
+        typedef short v4s __attribute__((ext_vector_type(4)));
+        const PT_LDS_AS char *to = base + r * 16 * DP * T::ES;
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PT_LDS_AS v4s *)(to + (at.col0 ^ (uint32_t)(d << 6))));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PT_LDS_AS v4s *)(to + (at.col1 ^ (uint32_t)(d << 6))));
+        return __builtin_bit_cast(typename T::Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+}
+
+// The right operand of unit u's rows.
+template <int DT, int DP>
+__device__ __forceinline__ AttnColFrag<DT> attn_col_right(const floatx16 &p, int u)
+{
+    if constexpr (DT == PT_FLOAT32) return p[u / (DP / 32)];
+    else return attn_pack<DT>(p, u / (DP / 32));
+}
+
+template <int DT, int DP>
+__device__ __forceinline__ void attn_col_mfma(floatx16 (&acc)[DP / 32], int u, const AttnColFrag<DT> &a, const AttnColFrag<DT> &b)
+{
+    floatx16 &x = acc[u % (DP / 32)];
+    if constexpr (DT == PT_FLOAT32) x = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, x, 0, 0, 0);
+    else attn_mfma<DT>(x, a, b);
+}
+
 template <int DT, int DP>
 __device__ __forceinline__ void attn_cols(floatx16 (&acc)[DP / 32], const typename AttnT<DT>::S *tile, int row0,
                                           const floatx16 &p, const AttnLane<DT, DP> &at)
 {
-    using T = AttnT<DT>;
-    const PT_LDS_AS char *base = (const PT_LDS_AS char *)tile + row0 * DP * T::ES;
-    if constexpr (DT == PT_FLOAT32) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            // rows 8 (r / 4) + r % 4 (+ 4 half): the swizzle's bits of r, the half's are in the base
-            const int x = (r % 4) << 2 | ((r / 4) * 2 & 3);
-#pragma unroll
-            for (int d = 0; d < DP / 32; d++) {
-                const float a = *(const PT_LDS_AS float *)(base + (8 * (r / 4) + r % 4) * DP * 4 +
-                                                           (at.col0 ^ (uint32_t)((8 * d ^ x) << 4)));
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[d], 0, 0, 0);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const typename T::Frag b = attn_pack<DT>(p, u);
-#pragma unroll
-            for (int d = 0; d < DP / 32; d++) {
-                typedef short v4s __attribute__((ext_vector_type(4)));
-                const PT_LDS_AS char *to = base + u * 16 * DP * T::ES;
-                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PT_LDS_AS v4s *)(to + (at.col0 ^ (uint32_t)(d << 6))));
-                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PT_LDS_AS v4s *)(to + (at.col1 ^ (uint32_t)(d << 6))));
-                const auto a = __builtin_bit_cast(typename T::Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                attn_mfma<DT>(acc[d], a, b);
-            }
-        }
-    }
+    for (int u = 0; u < attn_col_units<DT, DP>(); u++)
+        attn_col_mfma<DT, DP>(acc, u, attn_col_frag<DT, DP>(tile, row0, u, at), attn_col_right<DT, DP>(p, u));
 }
 
 // Everything this wave loads or writes to LDS is there, and every wave has
@@ -317,56 +456,115 @@ __device__ __forceinline__ void attn_store4(void *row, int e, int size, float a,
         if (e + i < size) store_c<DT>(p, (size_t)i, v[i]);
 }
 
-// LDS bytes of two tiles in `bufs` buffers, and how many buffers fit.
+// LDS bytes of a tile.
 constexpr int attn_tile_bytes(int rows, int dp, int es) { return rows * dp * es; }
-constexpr int kAttnLds = 131072;
+
+// Joins the waves' results in wave 0 and all others: rescaled to the common
+// maximum, added through `box` (W * 1024 floats that nobody reads any more),
+// 32 elements of the head at a time.
+template <int W, int ND>
+__device__ __forceinline__ void attn_join_waves(float &m, float &l, floatx16 (&o)[ND], float *box, int lane, int wave)
+{
+    __shared__ float ml[2][W][32];
+    if (lane < 32) {
+        ml[0][wave][lane] = m;
+        ml[1][wave][lane] = l;
+    }
+    __syncthreads();
+    float to = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w++) to = fmaxf(to, ml[0][w][lane & 31]);
+    const float ref = to == -INFINITY ? 0.0f : to;
+#pragma unroll
+    for (int w = 0; w < W; w++) sum += ml[1][w][lane & 31] * __builtin_amdgcn_exp2f(ml[0][w][lane & 31] - ref);
+    const float a = __builtin_amdgcn_exp2f(m - ref);
+    m = to;
+    l = sum;
+#pragma unroll
+    for (int d = 0; d < ND; d++) {
+        if (d) __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; e++) box[wave * 1024 + e * 64 + lane] = o[d][e] * a;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            float x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; w++) x += box[w * 1024 + e * 64 + lane];
+            o[d][e] = x;
+        }
+    }
+}
+
+// A wave's rows: the output and lse, or one range's sums.
+template <int DT, int ND>
+__device__ __forceinline__ void attn_result(const AttnArgs &g, float m, float l, const floatx16 (&o)[ND], bool live, int b,
+                                            int bh, int nh, int row, long long token, int qi, int hq, int split, int half)
+{
+    if (!live) return;
+    if (g.splits > 1) {
+        const long long at = ((long long)split * nh + bh) * ((long long)g.nq * g.group) + row;
+        if (half == 0) *(attn_f32x2 *)(g.part_ml + at * 2) = attn_f32x2{m, l};
+        if (l != 0.0f)  // (true of NaN) nothing seen: nothing is read there
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    attn_store4<PT_FLOAT32>(g.part_o + at * g.size, d * 32 + 8 * e + 4 * half, g.size, o[d][4 * e],
+                                            o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]);
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    typename AttnT<DT>::S *to = (typename AttnT<DT>::S *)g.out + b * g.o_bs + token * g.o_ts + hq * g.o_hs;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            attn_store4<DT>(to, d * 32 + 8 * e + 4 * half, g.size, o[d][4 * e] * inv, o[d][4 * e + 1] * inv,
+                            o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv);
+    if (g.lse && half == 0)
+        g.lse[(g.q_starts ? 0 : (long long)b * g.heads * g.nq) + (long long)hq * g.stat_rows + (g.q_starts ? token : qi)] =
+            l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+}
 
 // ------------------------------------------------------------- forward
 // Rows of a key head are its queries times its `group` query heads, row r =
 // query r / group, head r % group, so that the heads that share keys share
 // the staged tiles, and a single token's heads fill a block together.
 //
-// RW = 4: four waves of 32 rows each read every staged key.  RW = 1, for 32
-// rows or fewer: the waves take a quarter of each tile's keys each, with a
-// softmax of their own, and join their results at the end.
-template <int DT, int DP, int RW> struct AttnFwdShape {
-    static constexpr int ES = AttnT<DT>::ES, KW = 4 / RW;
-    static constexpr int BN = RW == 1 ? 128 : (ES == 4 || DP == 256 ? 32 : 64);
-    static constexpr int TILE = attn_tile_bytes(BN, DP, ES);
-    static constexpr int NBUF = 4 * TILE <= kAttnLds ? 2 : 1;
-    static constexpr bool kBuilt = 2 * NBUF * TILE <= kAttnLds;
-    static constexpr int WGS = 2 * NBUF * TILE <= 65536 && DP <= 128 ? 2 : 1;
+// Four waves of 32 rows each read every staged tile of keys and values.  The
+// scores of tile t + 1 are computed beside the exponentials of tile t, and
+// the maximum of those scores beside the product of tile t with its values,
+// so that the matrix and the vector pipe of a SIMD run together also inside
+// one wave: one tile takes 1024 cycles of MFMA and about as many of vector
+// instructions (half of them exponentials, at a quarter of the rate).
+template <int DT, int DP> struct AttnFwdShape {
+    static constexpr int ES = AttnT<DT>::ES;
+    static constexpr int BN = ES == 4 || DP == 256 ? 32 : 64;
+    static constexpr int WGS = 4 * attn_tile_bytes(BN, DP, ES) <= 65536 && DP <= 128 ? 2 : 1;
+    static_assert(4 * attn_tile_bytes(BN, DP, ES) <= 131072, "two buffers of keys and values");
 };
 
-template <int DT, int DP, int RW, bool VEC>
-__global__ __launch_bounds__(256, (AttnFwdShape<DT, DP, RW>::WGS)) void k_attention(AttnArgs g)
+template <int DT, int DP, bool VEC>
+__global__ __launch_bounds__(256, (AttnFwdShape<DT, DP>::WGS)) void k_attention(AttnArgs g)
 {
     using T = AttnT<DT>;
     using S = typename T::S;
-    using Shape = AttnFwdShape<DT, DP, RW>;
-    constexpr int BN = Shape::BN, NBUF = Shape::NBUF, KW = Shape::KW, NKB = BN / 32 / KW, BM = 32 * RW;
+    constexpr int BN = AttnFwdShape<DT, DP>::BN, NKB = BN / 32, BM = 128;
     constexpr int KS = DP * T::ES / 32, ND = DP / 32;
-    __shared__ __attribute__((aligned(1024))) S k0[BN * DP];
-    __shared__ __attribute__((aligned(1024))) S v0[BN * DP];
-    __shared__ __attribute__((aligned(1024))) S k1[NBUF == 2 ? BN * DP : 8];
-    __shared__ __attribute__((aligned(1024))) S v1[NBUF == 2 ? BN * DP : 8];
+    __shared__ __attribute__((aligned(1024))) S k0[BN * DP], v0[BN * DP], k1[BN * DP], v1[BN * DP];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int rw = RW == 4 ? wave : 0, kw = RW == 4 ? 0 : wave;
-    // the longest rows of a causal prompt first, its key heads side by side:
-    // where their number is a multiple of 8 each keeps to one XCD's L2
-    const int nh = g.batch * g.kv_heads, tiles = (int)(gridDim.x / (unsigned)nh);
-    const int tile = tiles - 1 - (int)blockIdx.x / nh, bh = (int)blockIdx.x % nh, b = bh / g.kv_heads, hk = bh % g.kv_heads;
-    const int split = blockIdx.y;
+    const int nh = g.batch * g.kv_heads, split = blockIdx.y;
+    int tile, bh;
+    if (!attn_place(g, false, tile, bh)) return;  // whole workgroup
+    const int b = bh / g.kv_heads, hk = bh % g.kv_heads;
     const AttnSeq sq = attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
     const AttnSeq sk = attn_seq(g.k_starts, g.k_lengths, g.k_rows, g.nk, b);
     const int rows = sq.n * g.group, row0 = tile * BM;
     if (row0 >= rows) return;  // whole workgroup
-    const int row = row0 + rw * 32 + (lane & 31), qi = row / g.group, hq = hk * g.group + row % g.group;
+    const int row = row0 + wave * 32 + (lane & 31), qi = row / g.group, hq = hk * g.group + row % g.group;
     const bool live = row < rows;
-
-    typename T::Frag q[KS];
-    attn_row<DT, DP, VEC>(q, (const S *)g.q + b * g.q_bs + (sq.row + qi) * g.q_ts + hq * g.q_hs, live, g.size, half);
 
     const AttnSrc ks = {(const char *)((const S *)g.k + b * g.k_bs + sk.row * g.k_ts + hk * g.k_hs), g.k_ts * T::ES, sk.n};
     const AttnSrc vs = {(const char *)((const S *)g.v + b * g.v_bs + sk.row * g.v_ts + hk * g.v_hs), g.v_ts * T::ES, sk.n};
@@ -385,40 +583,223 @@ __global__ __launch_bounds__(256, (AttnFwdShape<DT, DP, RW>::WGS)) void k_attent
         t0 = split * per;
         t1 = min(t1, t0 + per);
     }
+    auto load_k = [&](int t, S *to) { kl.load(ks, g.size, t * BN, to, wave, lane); };
+    auto load_v = [&](int t, S *to) { vl.load(vs, g.size, t * BN, to, wave, lane); };
+    if (t0 < t1) load_k(t0, k0);
 
+    typename T::Frag q[KS];
+    attn_row<DT, DP, VEC>(q, (const S *)g.q + b * g.q_bs + (sq.row + qi) * g.q_ts + hq * g.q_hs, live, g.size, half);
+    float m = -INFINITY, l = 0.0f;
+    floatx16 o[ND], sa[NKB], sb[NKB];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+    AttnLane<DT, DP> at;
+    at.init(lane);
+
+    auto scores = [&](const S *kt, floatx16 (&s)[NKB]) {
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++) s[kb] = attn_rows<DT, DP>(kt, kb * 32, q, at);
+    };
+    auto mask = [&](int t, floatx16 (&s)[NKB]) {
+        if ((t + 1) * BN <= lim_first) return;  // uniform: every row sees every key
+        const int key0 = t * BN + 4 * half;
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[kb][r] = key0 + kb * 32 + 8 * (r / 4) + r % 4 < lim ? s[kb][r] : -INFINITY;
+    };
+    auto maximum = [&](const floatx16 (&s)[NKB]) {
+        float top = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) top = fmaxf(top, s[kb][r]);
+        return fmaxf(top, attn_other(top, lane)) * g.scale_log2;
+    };
+    // The reference m of the exponentials follows the maximum only when it is
+    // passed by more than 8 (a factor of 256): sums and products are fp32 and
+    // a probability keeps its relative precision whatever its size, so most
+    // tiles need no rescaling of the sums.
+    auto follow = [&](float top) {
+        if (__all(!(top > m + 8.0f))) return;
+        const float to = fmaxf(m, top), a = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] *= a;
+    };
+    // one exponential of the tile, register e
+    auto exponential = [&](floatx16 (&s)[NKB], int e, float ref) {
+        float x = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16], g.scale_log2, -ref));
+        asm volatile("" : "+v"(x));  // here, beside the products, and not where it is used
+        s[e / 16][e % 16] = x;
+        l += x;
+    };
+    constexpr int NU = NKB * KS, NP = attn_col_units<DT, DP>(), AHEAD = 2;
+    // tile t, whose scores are `now`: the next tile's keys lie in kn, those
+    // after them go to kf, this tile's values lie in vt, the next go to vn
+    auto step = [&](int t, floatx16 (&now)[NKB], floatx16 (&next)[NKB], const S *kn, S *kf, const S *vt, S *vn, auto MORE) {
+        constexpr bool more = decltype(MORE)::value;  // there is a next tile
+        attn_landed();
+        at.fresh();
+        if constexpr (more) {
+            if (t + 2 < t1) load_k(t + 2, kf);
+            load_v(t + 1, vn);
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        // the next scores, beside the first block's exponentials
+        if constexpr (more) {
+            typename T::Frag f[AHEAD + 1];
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) f[u] = attn_row_frag<DT, DP>(kn, u / KS * 32, u % KS, at);
+#pragma unroll
+            for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) next[kb][e] = 0.0f;
+            static_for<0, NU>([&](auto U) {
+                constexpr int u = decltype(U)::value, w = u + AHEAD;
+                if constexpr (w < NU) f[w % (AHEAD + 1)] = attn_row_frag<DT, DP>(kn, w / KS * 32, w % KS, at);
+                attn_mfma<DT>(next[u / KS], f[u % (AHEAD + 1)], q[u % KS]);
+                static_for<u * 16 / NU, (u + 1) * 16 / NU>([&](auto E) { exponential(now, decltype(E)::value, ref); });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        } else {
+            static_for<0, 16>([&](auto E) { exponential(now, decltype(E)::value, ref); });
+        }
+        if constexpr (more) mask(t + 1, next);
+        // the product with the values, beside the second block's
+        // exponentials and, last, the next scores' maximum
+        float top = -INFINITY;
+        static_for<0, NKB>([&](auto KB) {
+            constexpr int kb = decltype(KB)::value;
+            AttnColFrag<DT> f[AHEAD + 1], right;
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) f[u] = attn_col_frag<DT, DP>(vt, kb * 32, u, at);
+            static_for<0, NP>([&](auto U) {
+                constexpr int u = decltype(U)::value, w = u + AHEAD;
+                if constexpr (w < NP) f[w % (AHEAD + 1)] = attn_col_frag<DT, DP>(vt, kb * 32, w, at);
+                if constexpr (u % ND == 0) right = attn_col_right<DT, DP>(now[kb], u);
+                attn_col_mfma<DT, DP>(o, u, f[u % (AHEAD + 1)], right);
+                if constexpr (kb + 1 < NKB) {
+                    static_for<u * 16 / NP, (u + 1) * 16 / NP>([&](auto E) { exponential(now, 16 + decltype(E)::value, ref); });
+                } else if constexpr (more) {
+                    static_for<u * NKB * 16 / NP, (u + 1) * NKB * 16 / NP>([&](auto E) {
+                        constexpr int e = decltype(E)::value;
+                        top = fmaxf(top, next[e / 16][e % 16]);
+                    });
+                    asm volatile("" : "+v"(top));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        });
+        if constexpr (more) follow(fmaxf(top, attn_other(top, lane)) * g.scale_log2);
+    };
+    if (t0 < t1) {
+        attn_landed();
+        if (t0 + 1 < t1) load_k(t0 + 1, k1);
+        load_v(t0, v0);
+        scores(k0, sa);
+        mask(t0, sa);
+        follow(maximum(sa));
+    }
+    int t = t0;
+    for (; t + 2 < t1; t += 2) {
+        step(t, sa, sb, k1, k0, v0, v1, std::true_type{});
+        step(t + 1, sb, sa, k0, k1, v1, v0, std::true_type{});
+    }
+    if (t + 1 < t1) {
+        step(t, sa, sb, k1, k0, v0, v1, std::true_type{});
+        step(t + 1, sb, sa, k0, k1, v1, v0, std::false_type{});
+    } else if (t < t1) {
+        step(t, sa, sb, k1, k0, v0, v1, std::false_type{});
+    }
+    l += attn_other(l, lane);
+    attn_result<DT, ND>(g, m, l, o, live, b, bh, nh, row, sq.row + qi, qi, hq, split, half);
+}
+
+// 32 rows or fewer, rows of whole 16-byte packs: single tokens over a cache,
+// bound by reading keys and values.  Each wave walks key blocks of 32 of its
+// own, every NW-th of the range, through a block of LDS of its own: no
+// barrier, and the waves drift apart, so that loads are on their way at all
+// times.  The next block's loads go to registers while this one is computed.
+template <int DT, int DP> struct AttnTokenShape {
+    static constexpr int TILE = attn_tile_bytes(32, DP, AttnT<DT>::ES);
+    static constexpr int NW = TILE <= 8192 ? 4 : TILE <= 16384 ? 2 : 1;
+    static constexpr int WGS = TILE <= 8192 ? 2 : 1;  // waves per SIMD that the registers are kept for
+};
+
+template <int DT, int DP>
+__global__ __launch_bounds__((64 * AttnTokenShape<DT, DP>::NW), (AttnTokenShape<DT, DP>::WGS))
+void k_attention_token(AttnArgs g)
+{
+    using T = AttnT<DT>;
+    using S = typename T::S;
+    constexpr int NW = AttnTokenShape<DT, DP>::NW, TE = 32 * DP;
+    constexpr int KS = DP * T::ES / 32, ND = DP / 32, NI = TE * T::ES / 1024;
+    __shared__ __attribute__((aligned(1024))) S kt[NW * TE], vt[NW * TE];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int nh = g.batch * g.kv_heads, split = blockIdx.y;
+    const int bh = (int)blockIdx.x, b = bh / g.kv_heads, hk = bh % g.kv_heads;
+    const AttnSeq sq = attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
+    const AttnSeq sk = attn_seq(g.k_starts, g.k_lengths, g.k_rows, g.nk, b);
+    const int rows = sq.n * g.group, row = lane & 31;
+    if (!rows) return;  // whole workgroup
+    const int qi = row / g.group, hq = hk * g.group + row % g.group;
+    const bool live = row < rows;
+
+    const AttnSrc ks = {(const char *)((const S *)g.k + b * g.k_bs + sk.row * g.k_ts + hk * g.k_hs), g.k_ts * T::ES, sk.n};
+    const AttnSrc vs = {(const char *)((const S *)g.v + b * g.v_bs + sk.row * g.v_ts + hk * g.v_hs), g.v_ts * T::ES, sk.n};
+    AttnStage<DT, DP, 32, 1, true> kl, vl;
+    kl.init(ks, g.size, 0, lane);
+    vl.init(vs, g.size, 0, lane);
+    const int shift = sk.n - sq.n + 1, last = g.causal ? min(sk.n, (rows - 1) / g.group + shift) : sk.n;
+    const int lim = g.causal ? min(sk.n, qi + shift) : sk.n, lim_first = g.causal ? min(sk.n, shift) : sk.n;
+    // this range's blocks, every NW-th of them for this wave
+    const int blocks = max(0, (last + 31) / 32), per = (((sk.n + 31) / 32 + g.splits - 1) / g.splits + NW - 1) / NW * NW;
+    const int t1 = min(blocks, per * (split + 1)), t0 = per * split + wave;
+
+    S *const kw = kt + wave * TE, *const vw = vt + wave * TE;
+    floatx4 kr[NI], vr[NI];
+    if (t0 < t1) {
+        kl.fetch(ks, g.size, t0 * 32, kr);
+        vl.fetch(vs, g.size, t0 * 32, vr);
+    }
+    typename T::Frag q[KS];
+    attn_row<DT, DP, true>(q, (const S *)g.q + b * g.q_bs + (sq.row + qi) * g.q_ts + hq * g.q_hs, live, g.size, half);
     float m = -INFINITY, l = 0.0f;
     floatx16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
-
     AttnLane<DT, DP> at;
     at.init(lane);
-    auto step = [&](int t, const S *kt, const S *vt) {
+    for (int t = t0; t < t1; t += NW) {
         at.fresh();
-        floatx16 s[NKB];
 #pragma unroll
-        for (int kb = 0; kb < NKB; kb++) s[kb] = attn_rows<DT, DP>(kt, (kw * NKB + kb) * 32, q, at);
-        const int key0 = t * BN + kw * NKB * 32 + 4 * half;
-        if ((t + 1) * BN > lim_first) {  // uniform: some row does not see some key
+        for (int i = 0; i < NI; i++) *(floatx4 *)(kw + (i * 64 + lane) * T::PK) = kr[i];
 #pragma unroll
-            for (int kb = 0; kb < NKB; kb++)
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    s[kb][r] = key0 + kb * 32 + 8 * (r / 4) + r % 4 < lim ? s[kb][r] : -INFINITY;
+        for (int i = 0; i < NI; i++) *(floatx4 *)(vw + (i * 64 + lane) * T::PK) = vr[i];
+        if (t + NW < t1) {
+            kl.fetch(ks, g.size, (t + NW) * 32, kr);
+            vl.fetch(vs, g.size, (t + NW) * 32, vr);
         }
-        float top = s[0][0];
+        floatx16 s = attn_rows<DT, DP>(kw, 0, q, at);
+        const int key0 = t * 32 + 4 * half;
+        if ((t + 1) * 32 > lim_first) {
 #pragma unroll
-        for (int kb = 0; kb < NKB; kb++)
+            for (int r = 0; r < 16; r++) s[r] = key0 + 8 * (r / 4) + r % 4 < lim ? s[r] : -INFINITY;
+        }
+        float top = s[0];
 #pragma unroll
-            for (int r = 0; r < 16; r++) top = fmaxf(top, s[kb][r]);
+        for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
         top = fmaxf(top, attn_other(top, lane)) * g.scale_log2;
-        // The reference m of the exponentials follows the maximum only when
-        // it is passed by more than 8 (a factor of 256): sums and products
-        // are fp32 and a probability keeps its relative precision whatever
-        // its size, so most tiles need no rescaling of the sums.
-        if (!__all(!(top > m + 8.0f))) {
+        if (!__all(!(top > m + 8.0f))) {  // as in k_attention
             const float to = fmaxf(m, top), a = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
             m = to;
             l *= a;
@@ -429,102 +810,21 @@ __global__ __launch_bounds__(256, (AttnFwdShape<DT, DP, RW>::WGS)) void k_attent
         }
         const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int kb = 0; kb < NKB; kb++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], g.scale_log2, -ref));
-                l += s[kb][r];
-            }
-#pragma unroll
-        for (int kb = 0; kb < NKB; kb++) attn_cols<DT, DP>(o, vt, (kw * NKB + kb) * 32, s[kb], at);
-    };
-    auto load = [&](int t, S *kt, S *vt) {
-        kl.load(ks, g.size, t * BN, kt, wave, lane);
-        vl.load(vs, g.size, t * BN, vt, wave, lane);
-    };
-    if constexpr (NBUF == 2) {
-        if (t0 < t1) load(t0, k0, v0);
-        for (int t = t0; t < t1; t += 2) {
-            attn_landed();  // tile t has landed, and every wave is done with the other buffer
-            if (t + 1 < t1) load(t + 1, k1, v1);
-            step(t, k0, v0);
-            if (t + 1 >= t1) break;
-            attn_landed();
-            if (t + 2 < t1) load(t + 2, k0, v0);
-            step(t + 1, k1, v1);
+        for (int r = 0; r < 16; r++) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], g.scale_log2, -ref));
+            l += s[r];
         }
-    } else {
-        for (int t = t0; t < t1; t++) {
-            attn_landed();
-            load(t, k0, v0);
-            attn_landed();
-            step(t, k0, v0);
-        }
+        attn_cols<DT, DP>(o, vw, 0, s, at);
     }
 
     l += attn_other(l, lane);
-    if constexpr (KW > 1) {
-        // join the waves: rescale to the common maximum, add through LDS
-        __shared__ float ml[2][KW][32];
+    if constexpr (NW > 1) {
         __syncthreads();
-        if (lane < 32) {
-            ml[0][kw][lane] = m;
-            ml[1][kw][lane] = l;
-        }
-        __syncthreads();
-        float to = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < KW; w++) to = fmaxf(to, ml[0][w][lane & 31]);
-        const float ref = to == -INFINITY ? 0.0f : to;
-#pragma unroll
-        for (int w = 0; w < KW; w++) sum += ml[1][w][lane & 31] * __builtin_amdgcn_exp2f(ml[0][w][lane & 31] - ref);
-        const float a = __builtin_amdgcn_exp2f(m - ref);
-        m = to;
-        l = sum;
-        // [wave][element][row] in the first buffer, one wave at a time per 32 elements: KW * 32 * 32 floats fit it
-        float *box = (float *)k0;
-        static_assert(KW * 1024 * 4 <= BN * DP * T::ES, "the joined block fits a tile");
-#pragma unroll
-        for (int d = 0; d < ND; d++) {
-            if (d) __syncthreads();
-#pragma unroll
-            for (int e = 0; e < 16; e++) box[kw * 1024 + e * 64 + lane] = o[d][e] * a;
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                float x = 0.0f;
-#pragma unroll
-                for (int w = 0; w < KW; w++) x += box[w * 1024 + e * 64 + lane];
-                o[d][e] = x;
-            }
-        }
-        if (kw) return;  // wave 0 writes
+        attn_join_waves<NW, ND>(m, l, o, (float *)kt, lane, wave);
+        static_assert(NW * 1024 * 4 <= NW * TE * T::ES, "the joined block fits a tile");
+        if (wave) return;
     }
-    if (!live) return;
-    if (g.splits > 1) {
-        const long long at = ((long long)split * nh + bh) * ((long long)g.nq * g.group) + row;
-        if (half == 0) *(attn_f32x2 *)(g.part_ml + at * 2) = attn_f32x2{m, l};
-        if (l != 0.0f || l != l)  // nothing seen: nothing is read there
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    attn_store4<PT_FLOAT32>(g.part_o + at * g.size, d * 32 + 8 * e + 4 * half, g.size, o[d][4 * e],
-                                            o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]);
-        return;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    S *to = (S *)g.out + b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            attn_store4<DT>(to, d * 32 + 8 * e + 4 * half, g.size, o[d][4 * e] * inv, o[d][4 * e + 1] * inv,
-                            o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv);
-    if (g.lse && half == 0) {
-        const long long stat = (g.q_starts ? sq.row : (long long)b * g.heads * g.nq) + (long long)hq * g.stat_rows + qi;
-        g.lse[stat] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
-    }
+    attn_result<DT, ND>(g, m, l, o, live, b, bh, nh, row, sq.row + qi, qi, hq, split, half);
 }
 
 // ------------------------------------------- gradient of keys and values
@@ -563,9 +863,9 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
     __shared__ __attribute__((aligned(256))) float l0[64], l1[64], e0[64], e1[64];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    // the first keys of a causal sequence, which most queries see, first
-    const int nh = g.batch * g.kv_heads;
-    const int tile = (int)blockIdx.x / nh, bh = (int)blockIdx.x % nh, b = bh / g.kv_heads, hk = bh % g.kv_heads;
+    int tile, bh;
+    if (!attn_place(g, true, tile, bh)) return;  // whole workgroup
+    const int b = bh / g.kv_heads, hk = bh % g.kv_heads;
     const AttnSeq sq = attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
     const AttnSeq sk = attn_seq(g.k_starts, g.k_lengths, g.k_rows, g.nk, b);
     const int first = tile * 128;
@@ -581,7 +881,9 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
     const int shift = sk.n - sq.n;
     const int from = g.causal ? key - shift : INT_MIN;
     const int t0 = g.causal ? max(0, first - shift) / BQ : 0, per = max(0, (sq.n + BQ - 1) / BQ - t0);
-    const int steps = per * g.group;
+    // this workgroup's share of the steps
+    const int share = (per * g.group + g.splits - 1) / g.splits;
+    const int step0 = share * (int)blockIdx.y, steps = min(per * g.group, step0 + share);
 
     floatx16 dk[kK ? ND : 1], dv[kV ? ND : 1];
 #pragma unroll
@@ -640,8 +942,8 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
             }
         }
     };
-    if (steps) load(0, q0, w0, l0, e0);
-    for (int it = 0; it < steps; it += 2) {
+    if (step0 < steps) load(step0, q0, w0, l0, e0);
+    for (int it = step0; it < steps; it += 2) {
         attn_landed();  // this step's tiles are there, and every wave is done with the other buffer
         if (it + 1 < steps) load(it + 1, q1, w1, l1, e1);
         step(it, q0, w0, l0, e0);
@@ -651,18 +953,23 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
         step(it + 1, q1, w1, l1, e1);
     }
     if (!live) return;
-    // gradients are contiguous
+    // gradients are contiguous, and so is each share's part of them
     const long long to = ((g.k_starts ? sk.row + key : (long long)b * g.nk + key) * g.kv_heads + hk) * g.size;
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            if constexpr (kV)
-                attn_store4<DT>((S *)g.dv + to, d * 32 + 8 * e + 4 * half, g.size, dv[d][4 * e], dv[d][4 * e + 1],
-                                dv[d][4 * e + 2], dv[d][4 * e + 3]);
-            if constexpr (kK)
-                attn_store4<DT>((S *)g.dk + to, d * 32 + 8 * e + 4 * half, g.size, dk[d][4 * e] * g.scale,
-                                dk[d][4 * e + 1] * g.scale, dk[d][4 * e + 2] * g.scale, dk[d][4 * e + 3] * g.scale);
+            const int at = d * 32 + 8 * e + 4 * half;
+            auto put = [&](void *whole, float *part, const floatx16 &x, float c) {
+                if (g.splits > 1)
+                    attn_store4<PT_FLOAT32>(part + blockIdx.y * g.part_step + to, at, g.size, x[4 * e] * c, x[4 * e + 1] * c,
+                                            x[4 * e + 2] * c, x[4 * e + 3] * c);
+                else
+                    attn_store4<DT>((S *)whole + to, at, g.size, x[4 * e] * c, x[4 * e + 1] * c, x[4 * e + 2] * c,
+                                    x[4 * e + 3] * c);
+            };
+            if constexpr (kV) put(g.dv, g.part_ml, dv[d], 1.0f);
+            if constexpr (kK) put(g.dk, g.part_o, dk[d], g.scale);
         }
 }
 
@@ -677,8 +984,9 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
     __shared__ __attribute__((aligned(1024))) S k0[BN * DP], v0[BN * DP], k1[BN * DP], v1[BN * DP];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int nh = g.batch * g.kv_heads, tiles = (int)(gridDim.x / (unsigned)nh);
-    const int tile = tiles - 1 - (int)blockIdx.x / nh, bh = (int)blockIdx.x % nh, b = bh / g.kv_heads, hk = bh % g.kv_heads;
+    int tile, bh;
+    if (!attn_place(g, false, tile, bh)) return;  // whole workgroup
+    const int b = bh / g.kv_heads, hk = bh % g.kv_heads;
     const AttnSeq sq = attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
     const AttnSeq sk = attn_seq(g.k_starts, g.k_lengths, g.k_rows, g.nk, b);
     const int rows = sq.n * g.group, row0 = tile * BM;
@@ -701,7 +1009,9 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
     const int lim = g.causal ? min(sk.n, qi + shift) : sk.n;
     const int lim_first = g.causal ? min(sk.n, row0 / g.group + shift) : sk.n;
     const int lim_last = g.causal ? min(sk.n, (min(row0 + BM, rows) - 1) / g.group + shift) : sk.n;
-    const int t1 = max(0, (lim_last + BN - 1) / BN);
+    // this workgroup's share of the sequence's key tiles
+    const int share = ((sk.n + BN - 1) / BN + g.splits - 1) / g.splits, t0 = share * (int)blockIdx.y;
+    const int t1 = min(max(0, (lim_last + BN - 1) / BN), t0 + share);
 
     floatx16 dq[ND];
 #pragma unroll
@@ -733,8 +1043,8 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
         kl.load(ks, g.size, t * BN, kt, wave, lane);
         vl.load(vs, g.size, t * BN, vt, wave, lane);
     };
-    if (t1 > 0) load(0, k0, v0);
-    for (int t = 0; t < t1; t += 2) {
+    if (t0 < t1) load(t0, k0, v0);
+    for (int t = t0; t < t1; t += 2) {
         attn_landed();  // tile t has landed, and every wave is done with the other buffer
         if (t + 1 < t1) load(t + 1, k1, v1);
         step(t, k0, v0);
@@ -744,22 +1054,29 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
         step(t + 1, k1, v1);
     }
     if (!live) return;
-    S *to = (S *)g.dq + b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
+    const long long to = b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            attn_store4<DT>(to, d * 32 + 8 * e + 4 * half, g.size, dq[d][4 * e] * g.scale, dq[d][4 * e + 1] * g.scale,
-                            dq[d][4 * e + 2] * g.scale, dq[d][4 * e + 3] * g.scale);
+        for (int e = 0; e < 4; e++) {
+            const floatx16 &x = dq[d];
+            const int at = d * 32 + 8 * e + 4 * half;
+            const float c = g.scale;
+            if (g.splits > 1)
+                attn_store4<PT_FLOAT32>(g.part_o + blockIdx.y * g.part_step + to, at, g.size, x[4 * e] * c, x[4 * e + 1] * c,
+                                        x[4 * e + 2] * c, x[4 * e + 3] * c);
+            else
+                attn_store4<DT>((S *)g.dq + to, at, g.size, x[4 * e] * c, x[4 * e + 1] * c, x[4 * e + 2] * c, x[4 * e + 3] * c);
+        }
 }
 
 // ------------------------------------------------------------- launches
 // Of one element type (pt_attention_{bf16,f16,f32}.hip).  `vec`: every row
 // of every operand starts on 16 bytes and its size fills whole chunks.
-template <int DT> void launch_attention(const AttnArgs &g, bool narrow, bool vec, unsigned blocks, hipStream_t s);
+template <int DT> void launch_attention(const AttnArgs &g, bool token, bool vec, unsigned blocks, hipStream_t s);
 template <int DT> void launch_attention_dkv(const AttnArgs &g, bool vec, unsigned blocks, hipStream_t s);
 template <int DT> void launch_attention_dq(const AttnArgs &g, bool vec, unsigned blocks, hipStream_t s);
-// whether 32 rows or fewer have a kernel of their own (RW = 1) at this size
-template <int DT> bool attention_narrow_built(int size);
+// streamed rows of a step of the gradient kernels
+template <int DT> int attention_backward_tile(int size);
 
 }  // namespace pt

@@ -5,12 +5,13 @@
 
 #include <algorithm>
 #include <math.h>
+#include <type_traits>
 
 namespace pt {
 
 // Joins the key ranges that workgroups of their own computed: with the
 // common maximum m = max m_s, l = sum l_s 2^(m_s - m) and o = sum o_s
-// 2^(m_s - m) / l.  One wave a row; it reads each part once.
+// 2^(m_s - m) / l.  One wave a row, at most 64 ranges; each part is read once.
 template <int DT>
 __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
 {
@@ -22,58 +23,97 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
     const int qi = row / g.group, hq = bh % g.kv_heads * g.group + row % g.group;
     const AttnSeq sq = attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
     if (qi >= sq.n) return;
+    // lane s holds range s
+    const long long first = at, step = nh * rows;
     float m = -INFINITY, l = 0.0f;
-    for (int s = 0; s < g.splits; s++) m = fmaxf(m, g.part_ml[((long long)s * nh * rows + at) * 2]);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    for (int s = 0; s < g.splits; s++) {
-        const float *ml = g.part_ml + ((long long)s * nh * rows + at) * 2;
-        l += ml[1] * __builtin_amdgcn_exp2f(ml[0] - ref);
+    if (lane < g.splits) {
+        m = g.part_ml[(lane * step + first) * 2];
+        l = g.part_ml[(lane * step + first) * 2 + 1];
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float top = wave_all(m, FMax{}), ref = top == -INFINITY ? 0.0f : top;
+    // a range in which the row sees nothing has written no sums
+    const uint64_t some = __ballot(l != 0.0f);
+    const float weight = __builtin_amdgcn_exp2f(m - ref), sum = wave_all(l * weight, FAdd{});
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     typename AttnT<DT>::S *to = (typename AttnT<DT>::S *)g.out + b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
-    for (int d = lane; d < g.size; d += 64) {
-        float x = 0.0f;
-        for (int s = 0; s < g.splits; s++) {
-            const long long part = (long long)s * nh * rows + at;
-            const float ls = g.part_ml[part * 2 + 1];
-            // a range in which the row sees nothing has written no sums
-            if (ls != 0.0f) x += g.part_o[part * g.size + d] * __builtin_amdgcn_exp2f(g.part_ml[part * 2] - ref);
-        }
-        store_c<DT>(to, (size_t)d, x * inv);
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = 0; s < g.splits; s++) {
+        if (!(some >> s & 1)) continue;
+        const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), s));
+        const float *from = g.part_o + (s * step + first) * g.size;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (k * 64 + lane < g.size) x[k] = fmaf(from[k * 64 + lane], c, x[k]);
     }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (k * 64 + lane < g.size) store_c<DT>(to, (size_t)(k * 64 + lane), x[k] * inv);
     if (g.lse && lane == 0)
         g.lse[(g.q_starts ? sq.row : (long long)b * g.heads * g.nq) + (long long)hq * g.stat_rows + qi] =
-            l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+            sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+}
+
+// Adds the shares of a gradient that workgroups of their own computed, in
+// their order: token rows of the queries (`keys` false: dq) or of the keys
+// (dk, and dv), `heads` heads to a row.  One wave a row and head.
+template <int DT>
+__global__ __launch_bounds__(256) void k_attention_sum(AttnArgs g, bool keys, const float *part, void *out)
+{
+    const int lane = threadIdx.x & 63, heads = keys ? g.kv_heads : g.heads, most = keys ? g.nk : g.nq;
+    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= (long long)g.batch * most * heads) return;
+    const int h = (int)(at % heads), i = (int)(at / heads % most), b = (int)(at / heads / most);
+    const AttnSeq s = keys ? attn_seq(g.k_starts, g.k_lengths, g.k_rows, g.nk, b) : attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
+    if (i >= s.n) return;
+    const bool packed = keys ? g.k_starts != nullptr : g.q_starts != nullptr;
+    const long long to = ((packed ? s.row + i : (long long)b * most + i) * heads + h) * g.size;
+    for (int d = lane; d < g.size; d += 64) {
+        float x = 0.0f;
+        for (int p = 0; p < g.splits; p++) x += part[p * g.part_step + to + d];
+        store_c<DT>(out, (size_t)(to + d), x);
+    }
 }
 
 // Per row and head, before the gradients: d = w . o in fp32, lse in base 2,
 // and the upstream gradient in the element type where it came in float32
 // (the products take 16-bit operands).  A row that sees no key gets lse +inf,
-// so its exponentials are 0.  16 lanes a row; HBM-bound, one read of w and o.
-template <int DT, bool W32>
+// so its exponentials are 0.  16 lanes a row, V elements at a time (V > 1:
+// rows start on 16 bytes and hold whole packs); HBM-bound, one read of w and o.
+template <int DT, bool W32, int V>
 __global__ __launch_bounds__(256) void k_attention_prepare(const void *w, const void *out, const float *lse,
                                                            uint16_t *w16, float *lse2, float *delta, long long rows,
                                                            int heads, int size, int queries, bool packed)
 {
     using S = typename AttnT<DT>::S;
+    typedef S __attribute__((ext_vector_type(V))) SV;
+    typedef uint16_t __attribute__((ext_vector_type(V))) HV;
+    typedef float __attribute__((ext_vector_type(V))) FV;
     const int lane = threadIdx.x & 15;
     const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
     if (at >= rows * heads) return;
     float x = 0.0f;
-    for (int d = lane; d < size; d += 16) {
+    for (int d = lane * V; d < size; d += 16 * V) {
         const long long e = at * size + d;
-        float wv;
+        const SV o = *(const SV *)((const S *)out + e);
         if constexpr (W32) {
-            wv = ((const float *)w)[e];
-            if constexpr (DT != PT_FLOAT32) {
-                const uint16_t h = DT == PT_BFLOAT16 ? float_to_bf16(wv) : float_to_f16(wv);
-                w16[e] = h;
-                wv = DType<DT>::to_c(h);
+            const FV f = *(const FV *)((const float *)w + e);
+            HV h;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                float wv = f[i];
+                if constexpr (DT != PT_FLOAT32) {
+                    h[i] = DT == PT_BFLOAT16 ? float_to_bf16(wv) : float_to_f16(wv);
+                    wv = DT == PT_BFLOAT16 ? bf16_to_float(h[i]) : f16_to_float(h[i]);
+                }
+                x = fmaf(wv, DType<DT>::to_c(o[i]), x);
             }
+            if constexpr (DT != PT_FLOAT32) *(HV *)(w16 + e) = h;
         } else {
-            wv = DType<DT>::to_c(((const S *)w)[e]);
+            const SV f = *(const SV *)((const S *)w + e);
+#pragma unroll
+            for (int i = 0; i < V; i++) x = fmaf(DType<DT>::to_c(f[i]), DType<DT>::to_c(o[i]), x);
         }
-        x = fmaf(wv, DType<DT>::to_c(((const S *)out)[e]), x);
     }
 #pragma unroll
     for (int m = 8; m >= 1; m >>= 1) x += __shfl_xor(x, m, 16);
@@ -109,7 +149,8 @@ static pt_status attention_args(const pt_attention_desc *d, const void *q, const
     const int group = d->heads / d->kv_heads;
     if (!fits_int((long long)d->queries * group) || !fits_int((long long)d->sequences * d->heads) ||
         !fits_int(((long long)d->queries * group / 32 + 1) * d->sequences * d->kv_heads) ||
-        !fits_int(((long long)d->keys / 128 + 1) * d->sequences * d->kv_heads))
+        !fits_int(((long long)d->keys / 128 + 8) * d->sequences * 8 * d->kv_heads) ||
+        !fits_int(((long long)d->queries * group / 128 + 8) * d->sequences * 8 * d->kv_heads))
         return fail(PT_ERR_INVALID, "attention has more rows than 32-bit numbers count");
     g = AttnArgs();
     g.q = q;
@@ -157,16 +198,52 @@ static pt_status attention_args(const pt_attention_desc *d, const void *q, const
     return PT_OK;
 }
 
+// Key ranges of the forward pass.  A prompt's workgroups are split where they
+// are fewer than the CUs; those of single tokens, which only read keys, until
+// there are enough of them to even out caches of different lengths.  256 keys
+// a range at least: a range costs a second kernel's read of its sums.
+static int attention_splits(const AttnArgs &g, bool token, long long blocks)
+{
+    const long long most = std::min<long long>((g.nk + 255) / 256, 64);
+    if (most <= 1) return 1;
+    if (token) return (int)std::min<long long>(std::max<long long>(1, 2048 / blocks), most);
+    // packed prompts have no more tiles than their rows fill
+    if (g.q_starts) blocks = std::min(blocks, ((long long)g.q_rows * g.group / 128 + g.batch) * g.kv_heads);
+    return blocks < 256 ? (int)std::min<long long>((512 + blocks - 1) / blocks, most) : 1;
+}
+
+// Shares of a gradient kernel with `blocks` workgroups of `steps` tiles each:
+// enough to fill the CUs twice, four tiles to a share at least.
+static int backward_splits(long long blocks, long long steps)
+{
+    if (blocks >= 256 || steps < 8) return 1;
+    return (int)std::min<long long>(std::min<long long>((512 + blocks - 1) / blocks, steps / 4), 16);
+}
+
+// Sets the order of the workgroups for `tiles` tiles of 128 rows in the
+// longest sequence and returns their number.  rows: of a packed tensor, which
+// bound the tiles of all its sequences together; 0 for sequences of one length.
+static long long attention_place(AttnArgs &g, long long tiles, long long rows, bool ragged)
+{
+    const long long nh = (long long)g.batch * g.kv_heads;
+    const int share = 8 % g.kv_heads == 0 ? 8 / g.kv_heads : 0;
+    g.tiles = (int)tiles;
+    if (ragged) {
+        g.place = kRagged;
+        const long long items = std::min(tiles * g.batch, rows / 128 + g.batch);
+        return share ? (items + share - 1) / share * 8 : items * g.kv_heads;
+    }
+    g.place = nh % 8 == 0 ? kGrouped : share ? kSpread : kPlain;
+    return g.place == kSpread ? (tiles + share - 1) / share * 8 * g.batch : tiles * nh;
+}
+
 template <int DT> static pt_status attention_typed(AttnArgs &g, bool vec, hipStream_t s)
 {
     const long long nh = (long long)g.batch * g.kv_heads, rows = (long long)g.nq * g.group;
-    const bool narrow = rows <= 32 && attention_narrow_built<DT>(g.size);
-    const long long blocks = (rows + (narrow ? 31 : 127)) / (narrow ? 32 : 128) * nh;
+    const bool token = rows <= 32 && vec;  // k_attention_token
+    const long long blocks = (rows + (token ? 31 : 127)) / (token ? 32 : 128) * nh;
     if (!blocks) return PT_OK;
-    // With fewer workgroups than CUs the keys are split between several, at
-    // least 256 keys each, and joined by a second kernel.
-    const long long most = (g.nk + 255) / 256;
-    if (blocks < 256 && most > 1) g.splits = (int)std::min<long long>(std::min<long long>((512 + blocks - 1) / blocks, most), 64);
+    g.splits = attention_splits(g, token, blocks);
     void *scratch = nullptr;
     if (g.splits > 1) {
         const size_t parts = (size_t)g.splits * nh * rows;
@@ -174,7 +251,7 @@ template <int DT> static pt_status attention_typed(AttnArgs &g, bool vec, hipStr
         g.part_ml = (float *)scratch;
         g.part_o = g.part_ml + parts * 2;
     }
-    launch_attention<DT>(g, narrow, vec, (unsigned)blocks, s);
+    launch_attention<DT>(g, token, vec, (unsigned)(token ? blocks : attention_place(g, blocks / nh, (long long)g.q_rows * g.group, g.q_starts)), s);
     pt_status st = check_hip(hipGetLastError(), "attention");
     if (st == PT_OK && g.splits > 1) {
         k_attention_join<DT><<<(unsigned)((nh * rows + 3) / 4), 256, 0, s>>>(g);
@@ -189,33 +266,65 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
 {
     const long long nh = (long long)g.batch * g.kv_heads, rows = (long long)g.nq * g.group;
     const long long q_rows = g.q_starts ? g.q_rows : (long long)g.batch * g.nq, stats = q_rows * g.heads;
-    const size_t stat_bytes = ((size_t)stats * 4 + 255) & ~(size_t)255;
+    const long long k_elems = (g.k_starts ? g.k_rows : (long long)g.batch * g.nk) * g.kv_heads * g.size;
     const bool round = w32 && DT != PT_FLOAT32;
+    const long long kb = ((long long)g.nk + 127) / 128 * nh, qb = (rows + 127) / 128 * nh;
+    const long long k_live = g.k_starts ? std::min(kb, ((long long)g.k_rows / 128 + g.batch) * g.kv_heads) : kb;
+    const long long q_live = g.q_starts ? std::min(qb, ((long long)g.q_rows * g.group / 128 + g.batch) * g.kv_heads) : qb;
+    const int tile = attention_backward_tile<DT>(g.size);
+    const int k_splits = kb ? backward_splits(std::max(1ll, k_live), ((long long)g.nq + tile - 1) / tile * g.group) : 1;
+    const int q_splits = qb ? backward_splits(std::max(1ll, q_live), ((long long)g.nk + tile - 1) / tile) : 1;
+    // one region: lse2, delta, the rounded upstream gradient, the shares (of
+    // dk and dv, and after them of dq)
+    auto whole = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t stat_bytes = whole((size_t)stats * 4), w_bytes = round ? whole((size_t)stats * g.size * 2) : 0;
+    const size_t k_part = k_splits > 1 ? whole((size_t)k_splits * k_elems * 4) : 0;
+    const size_t q_part = q_splits > 1 ? whole((size_t)q_splits * stats * g.size * 4) : 0;
     void *scratch = nullptr;
-    PT_TRY(scratch_alloc(&scratch, 2 * stat_bytes + (round ? (size_t)stats * g.size * 2 : 0), s));
-    float *lse2 = (float *)scratch, *delta = (float *)((char *)scratch + stat_bytes);
-    uint16_t *w16 = round ? (uint16_t *)((char *)scratch + 2 * stat_bytes) : nullptr;
+    PT_TRY(scratch_alloc(&scratch, 2 * stat_bytes + w_bytes + std::max(2 * k_part, q_part), s));
+    char *base = (char *)scratch;
+    float *lse2 = (float *)base, *delta = (float *)(base + stat_bytes);
+    uint16_t *w16 = round ? (uint16_t *)(base + 2 * stat_bytes) : nullptr;
+    float *part = (float *)(base + 2 * stat_bytes + w_bytes);
     pt_status st = PT_OK;
     if (stats) {
         const unsigned n = (unsigned)((stats + 15) / 16);
         const bool packed = g.q_starts != nullptr;
-        if (w32)
-            k_attention_prepare<DT, true><<<n, 256, 0, s>>>(w, g.out, lse, w16, lse2, delta, q_rows, g.heads, g.size, g.nq, packed);
-        else
-            k_attention_prepare<DT, false><<<n, 256, 0, s>>>(w, g.out, lse, w16, lse2, delta, q_rows, g.heads, g.size, g.nq, packed);
+        const bool packs = g.size % 8 == 0 && !(((uintptr_t)w | (uintptr_t)g.out) & 15);
+        auto go = [&](auto W, auto V) {
+            k_attention_prepare<DT, decltype(W)::value, decltype(V)::value><<<n, 256, 0, s>>>(
+                w, g.out, lse, w16, lse2, delta, q_rows, g.heads, g.size, g.nq, packed);
+        };
+        using P = std::integral_constant<int, AttnT<DT>::PK>;
+        using One = std::integral_constant<int, 1>;
+        if (w32) packs ? go(std::true_type{}, P{}) : go(std::true_type{}, One{});
+        else packs ? go(std::false_type{}, P{}) : go(std::false_type{}, One{});
         st = check_hip(hipGetLastError(), "attention gradient preparation");
     }
     g.w = round ? (const void *)w16 : w;
     g.lse2 = lse2;
     g.delta = delta;
     vec = vec && !((uintptr_t)g.w & 15);
-    const long long kb = ((long long)g.nk + 127) / 128 * nh, qb = (rows + 127) / 128 * nh;
-    if (st == PT_OK && kb && g.dk) {
-        launch_attention_dkv<DT>(g, vec, (unsigned)kb, s);
+    if (st == PT_OK && kb) {
+        g.splits = k_splits;
+        g.part_step = k_elems;
+        g.part_o = part;
+        g.part_ml = (float *)((char *)part + k_part);
+        launch_attention_dkv<DT>(g, vec, (unsigned)attention_place(g, kb / nh, g.k_rows, g.k_starts), s);
+        if (k_splits > 1) {
+            const unsigned n = (unsigned)(((long long)g.batch * g.nk * g.kv_heads + 3) / 4);
+            k_attention_sum<DT><<<n, 256, 0, s>>>(g, true, g.part_o, g.dk);
+            k_attention_sum<DT><<<n, 256, 0, s>>>(g, true, g.part_ml, g.dv);
+        }
         st = check_hip(hipGetLastError(), "attention gradient of keys and values");
     }
-    if (st == PT_OK && qb && g.dq) {
-        launch_attention_dq<DT>(g, vec, (unsigned)qb, s);
+    if (st == PT_OK && qb) {
+        g.splits = q_splits;
+        g.part_step = stats * g.size;
+        g.part_o = part;
+        launch_attention_dq<DT>(g, vec, (unsigned)attention_place(g, qb / nh, (long long)g.q_rows * g.group, g.q_starts), s);
+        if (q_splits > 1)
+            k_attention_sum<DT><<<(unsigned)(((long long)g.batch * g.nq * g.heads + 3) / 4), 256, 0, s>>>(g, false, part, g.dq);
         st = check_hip(hipGetLastError(), "attention gradient of queries");
     }
     scratch_free(scratch, s);

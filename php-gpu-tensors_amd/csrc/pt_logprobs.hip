@@ -35,10 +35,14 @@ template <int DT> struct LpPack {
     using S = typename DType<DT>::S;
     static constexpr int V = 16 / sizeof(S);
     // 16 bytes at any element boundary; read once
-    __device__ __forceinline__ static void load(const S *p, float (&v)[V])
+    __device__ __forceinline__ static lp_u32x4 load(const S *p)
+    {
+        return __builtin_nontemporal_load((const lp_u32x4 *)p);
+    }
+    __device__ __forceinline__ static void widen(const lp_u32x4 &raw, float (&v)[V])
     {
         union { lp_u32x4 raw; S s[V]; } u;
-        u.raw = __builtin_nontemporal_load((const lp_u32x4 *)p);
+        u.raw = raw;
 #pragma unroll
         for (int i = 0; i < V; i++) v[i] = DType<DT>::to_c(u.s[i]);
     }
@@ -83,10 +87,29 @@ struct LpSum {
     }
 };
 
+// The top-th largest of the lanes' values: of elements of which these are
+// some, the top-th largest is no smaller.  A binary search over the bits of
+// an order-preserving key, one ballot a bit, so nothing moves between lanes.
+// NaN counts as -inf.
+__device__ __forceinline__ float lp_bound(float x, int top)
+{
+    const float y = x > -INFINITY ? x : -INFINITY;
+    const uint32_t u = __float_as_uint(y), key = u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
+    uint32_t at = 0;
+#pragma unroll 4
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t to = at | 1u << bit;
+        if (__popcll(__ballot(key >= to)) >= top) at = to;
+    }
+    return __uint_as_float(at >> 31 ? at ^ 0x80000000u : ~at);
+}
+
 // The best `top` elements of a wave, in lanes 0 .. top - 1.
 struct LpTop {
-    float v, worst;
+    float v, worst;  // worst: what an element has to reach
     int i, worst_i;
+    // no element below `x` is wanted (lp_bound; once, while the list is empty)
+    __device__ __forceinline__ void at_least(float x) { worst = x; }
     __device__ __forceinline__ void init()
     {
         v = worst = -INFINITY;
@@ -102,14 +125,19 @@ struct LpTop {
             const float cx = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), from));
             const int ci = __builtin_amdgcn_readlane(at, from);
             const int place = (int)__popcll(__ballot(lane < top && better(v, i, cx, ci)));
-            const float up = __shfl_up(v, 1);
-            const int up_i = __shfl_up(i, 1);
+            // the lane before: one DPP move each (wave_shr:1)
+            const float up = __builtin_bit_cast(
+                float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x138, 0xF, 0xF, false));
+            const int up_i = __builtin_amdgcn_update_dpp(0, i, 0x138, 0xF, 0xF, false);
             if (lane >= place) {
                 v = lane == place ? cx : up;
                 i = lane == place ? ci : up_i;
             }
-            worst = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), top - 1));
-            worst_i = __builtin_amdgcn_readlane(i, top - 1);
+            const int last_i = __builtin_amdgcn_readlane(i, top - 1);
+            if (last_i != INT_MAX) {  // the list is full: its last bounds what follows
+                worst = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), top - 1));
+                worst_i = last_i;
+            }
             want = lane != from && want && better(x, at, worst, worst_i);
         }
     }
@@ -135,9 +163,23 @@ __device__ __forceinline__ LpSum lp_wave(LpSum a)
     return a;
 }
 
-// One wave writes a row's results.
+// The score of the row's token, asked for before the row is read: 0 where
+// there is none, NaN past the classes.
 template <int DT>
-__device__ __forceinline__ void lp_finish(const LpArgs &g, int row, const LpSum &a, const LpTop &top, int lane)
+__device__ __forceinline__ float lp_token(const LpArgs &g, int row, bool &named)
+{
+    named = false;
+    if (!g.logprob) return 0.0f;
+    const int tok = g.tokens[row];
+    if (tok < 0) return 0.0f;
+    named = true;
+    if (tok >= g.classes) return __builtin_nanf("");
+    return DType<DT>::to_c(((const typename DType<DT>::S *)g.x)[(long long)row * g.stride + tok]);
+}
+
+// One wave writes a row's results.
+__device__ __forceinline__ void lp_finish(const LpArgs &g, int row, const LpSum &a, const LpTop &top, float token, bool named,
+                                          int lane)
 {
     // a row of -inf alone: no element has a probability
     const bool none = a.m == -INFINITY && a.s == 0.0f;
@@ -148,16 +190,8 @@ __device__ __forceinline__ void lp_finish(const LpArgs &g, int row, const LpSum 
             g.stats[2 * (long long)row + 1] = log_s;
         }
         if (g.entropy) g.entropy[row] = none ? 0.0f : log_s + a.t / a.s;
-        if (g.logprob) {
-            const int tok = g.tokens[row];
-            float v = 0.0f;  // no token
-            if (tok >= g.classes) v = __builtin_nanf("");
-            else if (tok >= 0) {
-                const float x = DType<DT>::to_c(((const typename DType<DT>::S *)g.x)[(long long)row * g.stride + tok]);
-                v = none ? -INFINITY : x - r - log_s;
-            }
-            g.logprob[row] = v;
-        }
+        // (a NaN token score stays one in a row without probabilities)
+        if (g.logprob) g.logprob[row] = !named ? 0.0f : none && token == token ? -INFINITY : token - r - log_s;
     }
     if (lane < g.top) {
         const long long at = (long long)row * g.top + lane;
@@ -175,30 +209,33 @@ __global__ __launch_bounds__(64 * NW) void k_logprobs(LpArgs g)
     __shared__ float box[NW][3];
     __shared__ float top_v[TOP ? NW : 1][64];
     __shared__ int top_i[TOP ? NW : 1][64];
+    __shared__ float best_v[64];
+    __shared__ int best_i[64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x;
     const typename P::S *x = (const typename P::S *)g.x + (long long)row * g.stride;
     const int per = g.splits > 1 ? ((g.classes + g.splits - 1) / g.splits + V * 64 - 1) / (V * 64) * (V * 64) : g.classes;
     const int begin = min((long long)g.classes, (long long)per * blockIdx.y), end = min((long long)g.classes, (long long)begin + per);
 
+    bool named = false;
+    const float token = g.splits == 1 ? lp_token<DT>(g, row, named) : 0.0f;
     LpSum a;
     a.init();
     LpTop top;
     top.init();
-    // NP packs at once, so that their loads are under way together
-    auto take = [&](int at, auto NP) {
+    bool bounded = false;
+    const int turn = NW * 64 * V;
+    // NP packs at once
+    auto take = [&](int at, const lp_u32x4 *raw, auto NP) {
         constexpr int np = decltype(NP)::value;
         float v[np][V];
 #pragma unroll
-        for (int p = 0; p < np; p++) P::load(x + at + p * NW * 64 * V, v[p]);
-        float hi[np], most = -INFINITY;
+        for (int p = 0; p < np; p++) P::widen(raw[p], v[p]);
+        float most = v[0][0];
 #pragma unroll
-        for (int p = 0; p < np; p++) {
-            hi[p] = v[p][0];
+        for (int p = 0; p < np; p++)
 #pragma unroll
-            for (int k = 1; k < V; k++) hi[p] = fmaxf(hi[p], v[p][k]);
-            most = fmaxf(most, hi[p]);
-        }
+            for (int k = 0; k < V; k++) most = fmaxf(most, v[p][k]);
         a.rise(most);
         const float r = a.ref();
 #pragma unroll
@@ -206,25 +243,54 @@ __global__ __launch_bounds__(64 * NW) void k_logprobs(LpArgs g)
 #pragma unroll
             for (int k = 0; k < V; k++) a.add(v[p][k], r);
         if constexpr (TOP) {
-            if (__any(most >= top.worst)) {
+            if (!bounded) {
+                top.at_least(lp_bound(most, g.top));
+                bounded = true;
+            }
+            // Every lane offers its largest element, and while that is good
+            // enough the next: the first of those equal to the maximum, which
+            // is then put out of the way as a NaN.
+            while (__any(most >= top.worst)) {
+                int from = INT_MAX;
 #pragma unroll
-                for (int p = 0; p < np; p++) {
-                    if (!__any(hi[p] >= top.worst)) continue;
-                    for (int k = 0; k < V; k++) {
-                        float e = v[p][0];
+                for (int p = np - 1; p >= 0; p--)
 #pragma unroll
-                        for (int q = 1; q < V; q++) e = k == q ? v[p][q] : e;
-                        if (__any(e >= top.worst)) top.offer(e, at + p * NW * 64 * V + k, g.top, lane);
-                    }
-                }
+                    for (int k = V - 1; k >= 0; k--) from = v[p][k] == most ? p * turn + k : from;
+                const bool good = most >= top.worst;
+                top.offer(most, from == INT_MAX ? INT_MAX : at + from, g.top, lane);
+#pragma unroll
+                for (int p = 0; p < np; p++)
+#pragma unroll
+                    for (int k = 0; k < V; k++) v[p][k] = from == p * turn + k ? __builtin_nanf("") : v[p][k];
+                most = __builtin_nanf("");
+                if (!__any(good)) break;
+#pragma unroll
+                for (int p = 0; p < np; p++)
+#pragma unroll
+                    for (int k = 0; k < V; k++) most = fmaxf(most, v[p][k]);
             }
         }
     };
     // whole turns of the block first, then whole packs, then single elements
-    const int turn = NW * 64 * V;
     int at = begin;
-    for (; at + UN * turn <= end; at += UN * turn) take(at + (int)threadIdx.x * V, std::integral_constant<int, UN>{});
-    for (; at + turn <= end; at += turn) take(at + (int)threadIdx.x * V, std::integral_constant<int, 1>{});
+    const int mine = (int)threadIdx.x * V;
+    auto load = [&](int from, lp_u32x4 (&raw)[UN]) {
+#pragma unroll
+        for (int p = 0; p < UN; p++) raw[p] = P::load(x + from + mine + p * turn);
+    };
+    lp_u32x4 raw[UN], next[UN];
+    if (at + UN * turn <= end) load(at, raw);
+    for (; at + UN * turn <= end; at += UN * turn) {
+        const bool more = at + 2 * UN * turn <= end;  // the next packs are under way while these are added
+        if (more) load(at + UN * turn, next);
+        take(at + mine, raw, std::integral_constant<int, UN>{});
+#pragma unroll
+        for (int p = 0; p < UN; p++) raw[p] = next[p];
+    }
+    for (; at + turn <= end; at += turn) {
+        const lp_u32x4 one = P::load(x + at + mine);
+        take(at + mine, &one, std::integral_constant<int, 1>{});
+    }
     for (; at < end; at += NW * 64) {
         // one element a thread
         const int i = at + (int)threadIdx.x;
@@ -247,15 +313,42 @@ __global__ __launch_bounds__(64 * NW) void k_logprobs(LpArgs g)
             top_v[wave][lane] = top.v;
             top_i[wave][lane] = top.i;
         }
-        __syncthreads();
-        if (wave) return;
-        for (int w = 1; w < NW; w++) {
-            a.join({box[w][0], box[w][1], box[w][2]});
-            if constexpr (TOP) top.offer(lane < g.top ? top_v[w][lane] : -INFINITY, lane < g.top ? top_i[w][lane] : INT_MAX, g.top, lane);
+        if constexpr (TOP) {
+            if (wave == 0) {
+                best_v[lane] = -INFINITY;
+                best_i[lane] = INT_MAX;
+            }
         }
+        __syncthreads();
+        if constexpr (TOP) {
+            // an element's place among all waves' is its place in its own
+            // list and the number of better ones in each other list, found
+            // by halving
+            int place = lane;
+#pragma unroll
+            for (int o = 1; o < NW; o++) {
+                const int w = (wave + o) % NW;
+                int low = 0, high = g.top;
+                while (low < high) {
+                    const int mid = (low + high) / 2;
+                    if (LpTop::better(top_v[w][mid], top_i[w][mid], top.v, top.i)) low = mid + 1;
+                    else high = mid;
+                }
+                place += low;
+            }
+            if (lane < g.top && place < g.top && top.i != INT_MAX) {
+                best_v[place] = top.v;
+                best_i[place] = top.i;
+            }
+            __syncthreads();
+            top.v = best_v[lane];
+            top.i = best_i[lane];
+        }
+        if (wave) return;
+        for (int w = 1; w < NW; w++) a.join({box[w][0], box[w][1], box[w][2]});
     }
     if (g.splits == 1) {
-        lp_finish<DT>(g, row, a, top, lane);
+        lp_finish(g, row, a, top, token, named, lane);
         return;
     }
     float *part = g.part + ((long long)row * g.splits + blockIdx.y) * (3 + 2 * g.top);
@@ -276,18 +369,41 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LpArgs g)
 {
     const int lane = threadIdx.x, row = blockIdx.x, width = 3 + 2 * g.top;
     const float *part = g.part + (long long)row * g.splits * width;
+    bool named;
+    const float token = lp_token<DT>(g, row, named);
     LpSum a;
     a.init();
-    if (lane < g.splits) a = {part[lane * width], part[lane * width + 1], part[lane * width + 2]};
+    // Each part's list is in order.  With r = top / splits rounded up, j of
+    // the parts' r-th elements have j r elements that are no smaller.
+    const bool in = lane < g.splits;
+    const float *list = part + lane * width + 3;
+    const int r = (g.top + g.splits - 1) / g.splits;
+    if (in) a = {part[lane * width], part[lane * width + 1], part[lane * width + 2]};
+    float bound = -INFINITY, x = -INFINITY;
+    int at = INT_MAX;
+    if (in && g.top) {
+        bound = list[r - 1];
+        x = list[0];
+        at = __builtin_bit_cast(int, list[g.top]);
+    }
     a = lp_wave(a);
     LpTop top;
     top.init();
-    for (int j = lane; j - lane < g.splits * g.top; j += 64) {
-        const bool in = j < g.splits * g.top;
-        const float *from = part + (in ? j / g.top * width + 3 + j % g.top : 0);
-        top.offer(in ? from[0] : -INFINITY, in ? __builtin_bit_cast(int, from[g.top]) : INT_MAX, g.top, lane);
+    if (g.top) top.at_least(lp_bound(bound, (g.top + r - 1) / r));
+    for (int j = 0; j < g.top; j++) {
+        // what follows in any list is no larger than its element j
+        if (!__any(x >= top.worst)) break;
+        float x2 = -INFINITY;
+        int at2 = INT_MAX;
+        if (in && j + 1 < g.top) {
+            x2 = list[j + 1];
+            at2 = __builtin_bit_cast(int, list[g.top + j + 1]);
+        }
+        top.offer(x, at, g.top, lane);
+        x = x2;
+        at = at2;
     }
-    lp_finish<DT>(g, row, a, top, lane);
+    lp_finish(g, row, a, top, token, named, lane);
 }
 
 struct LpBwdArgs {
@@ -331,9 +447,12 @@ __global__ __launch_bounds__(64 * NW) void k_logprobs_backward(LpBwdArgs g)
     };
     auto take = [&](int at, auto NP) {
         constexpr int np = decltype(NP)::value;
+        lp_u32x4 raw[np];
         float v[np][V];
 #pragma unroll
-        for (int p = 0; p < np; p++) P::load(x + at + p * NW * 64 * V, v[p]);
+        for (int p = 0; p < np; p++) raw[p] = P::load(x + at + p * NW * 64 * V);
+#pragma unroll
+        for (int p = 0; p < np; p++) P::widen(raw[p], v[p]);
 #pragma unroll
         for (int p = 0; p < np; p++) {
             union { lp_u32x4 raw; S s[V]; } o;

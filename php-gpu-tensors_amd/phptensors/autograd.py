@@ -17,12 +17,13 @@ into the plan like the forward pass.
 
 
 class Node:
-    __slots__ = ("parents", "backward", "op")
+    __slots__ = ("parents", "backward", "op", "low")
 
-    def __init__(self, parents, backward, op):
+    def __init__(self, parents, backward, op, low=False):
         self.parents = parents
         self.backward = backward
         self.op = op
+        self.low = low  # takes a 16-bit upstream gradient as it is
 
 
 class Parts:
@@ -64,10 +65,10 @@ def active(*ts):
     return _recording[0] and any(needs_grad(t) for t in ts if t is not None and hasattr(t, "_rg"))
 
 
-def record(out, parents, backward, op):
+def record(out, parents, backward, op, low=False):
     """Attach a node to `out` when any parent requires a gradient."""
     if _recording[0] and any(needs_grad(p) for p in parents):
-        out._node = Node(parents, backward, op)
+        out._node = Node(parents, backward, op, low)
     return out
 
 
@@ -124,7 +125,7 @@ def backward(root, gradient=None):
     low = root.getDtype() in ("float16", "bfloat16")
     if gradient is None:
         gradient = CudaArray.ones(root.getShape(), "float32" if low else root.getDtype())
-    elif low:
+    elif low and not (root._node and root._node.low):
         gradient = gradient.astype("float32")
     grads = {id(root): gradient}
     _recording[0] = False  # gradients carry no history of their own

@@ -594,7 +594,7 @@ class CudaArray:
                                                *(s._h if s is not None else None for s in held), got):
                     _host.raise_error("attention gradient")
                 return [CudaArray._wrap(h) for h in got]
-            AG.record(out, [self, key, value], back, "attention")
+            AG.record(out, [self, key, value], back, "attention", low=True)
         return out
 
     def logProbs(self, tokens, top=0):
