@@ -214,16 +214,21 @@ template <int DT, int DP, int ROWS, int NW, bool VEC> struct AttnStage {
             }
         }
     }
+    // bytes from row r0 on that hold rows of the source, for loads of whole
+    // tiles no bound: the compiler's 64-bit product is kept for the last tile
     __device__ __forceinline__ static uint32_t range(const AttnSrc &s, int size, int r0)
     {
-        return r0 >= s.rows ? 0u : (uint32_t)min((long long)(s.rows - r0 - 1) * s.step + size * T::ES, (long long)0x7fffffff);
+        uint32_t bytes = 0x7fffffffu;
+        if (__builtin_expect(r0 + ROWS > s.rows, 0))
+            bytes = r0 >= s.rows ? 0u : (uint32_t)(s.rows - r0 - 1) * (uint32_t)s.step + (uint32_t)(size * T::ES);
+        return bytes;
     }
     // The same chunks to registers; read once.
     __device__ __forceinline__ void fetch(const AttnSrc &s, int size, int r0, floatx4 (&v)[NI]) const
     {
         static_assert(VEC, "whole packs");
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<char *>(s.base + (long long)r0 * s.step), (short)0, (int)range(s, size, r0), 0x00020000);
+            const_cast<char *>(s.base + (unsigned long long)(uint32_t)r0 * (uint32_t)s.step), (short)0, (int)range(s, size, r0), 0x00020000);
 #pragma unroll
         for (int i = 0; i < NI; i++)
             v[i] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off[i], 0, 2));  // nt
@@ -231,7 +236,8 @@ template <int DT, int DP, int ROWS, int NW, bool VEC> struct AttnStage {
     // Rows r0 .. r0 + ROWS - 1 into `tile`; rows past the source's last are zeros.
     __device__ __forceinline__ void load(const AttnSrc &s, int size, int r0, S *tile, int wave, int lane) const
     {
-        const char *base = s.base + (long long)r0 * s.step;
+        // (a step fits 32 bits where rows come in whole packs)
+        const char *base = s.base + (VEC ? (unsigned long long)(uint32_t)r0 * (uint32_t)s.step : (unsigned long long)r0 * s.step);
         if constexpr (VEC) {
             const uint32_t bytes = range(s, size, r0);
 #pragma unroll
@@ -413,6 +419,93 @@ __device__ __forceinline__ void attn_cols(floatx16 (&acc)[DP / 32], const typena
 #pragma unroll
     for (int u = 0; u < attn_col_units<DT, DP>(); u++)
         attn_col_mfma<DT, DP>(acc, u, attn_col_frag<DT, DP>(tile, row0, u, at), attn_col_right<DT, DP>(p, u));
+}
+
+// A fragment of either product, for a queue that reads ahead across both.
+template <int DT>
+__device__ __forceinline__ typename AttnT<DT>::Frag attn_any(const AttnColFrag<DT> &a)
+{
+    if constexpr (DT == PT_FLOAT32) return floatx4{a, 0.0f, 0.0f, 0.0f};
+    else return a;
+}
+template <int DT>
+__device__ __forceinline__ AttnColFrag<DT> attn_of_any(const typename AttnT<DT>::Frag &a)
+{
+    if constexpr (DT == PT_FLOAT32) return a[0];
+    else return a;
+}
+
+// Units 0 .. N - 1 of MFMA work in this order, fragment(unit) read AHEAD units
+// before unit(unit, fragment) uses it; unit() also does what other work runs
+// beside the matrix pipe.  Nothing moves from unit to unit: the order bounds
+// the fragments that are held, and left to itself the compiler reads so far
+// ahead that registers spill, and sinks the work to where it is used.
+template <int DT, int N, int AHEAD, typename F, typename U>
+__device__ __forceinline__ void attn_queue(F &&fragment, U &&unit)
+{
+    typename AttnT<DT>::Frag f[AHEAD + 1];
+    static_for<0, AHEAD>([&](auto I) __attribute__((always_inline)) { f[decltype(I)::value] = fragment(I); });
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<0, N>([&](auto I) __attribute__((always_inline)) {
+        constexpr int u = decltype(I)::value, w = u + AHEAD;
+        if constexpr (w < N) f[w % (AHEAD + 1)] = fragment(IC<w>{});
+        unit(I, f[u % (AHEAD + 1)]);
+        __builtin_amdgcn_sched_barrier(0);
+    });
+}
+
+// The same products with other work beside them: after each unit's MFMA,
+// work(unit) runs while the matrix pipe does, and nothing moves across.  The
+// order also bounds the fragments that are held at once; left to itself the
+// compiler reads so far ahead that the gradient kernels spill.
+template <int DT, int DP, int AHEAD, typename B, typename W>
+__device__ __forceinline__ void attn_rows_beside(floatx16 &acc, const typename AttnT<DT>::S *tile, int row0, B &&right,
+                                                 const AttnLane<DT, DP> &at, W &&work)
+{
+    constexpr int N = DP * AttnT<DT>::ES / 32;
+    typename AttnT<DT>::Frag a[AHEAD + 1], b[AHEAD + 1];
+    static_for<0, AHEAD>([&](auto U) {
+        constexpr int u = decltype(U)::value;
+        a[u] = attn_row_frag<DT, DP>(tile, row0, u, at);
+        b[u] = right(u);
+    });
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] = 0.0f;
+    static_for<0, N>([&](auto U) {
+        constexpr int u = decltype(U)::value, w = u + AHEAD;
+        if constexpr (w < N) {
+            a[w % (AHEAD + 1)] = attn_row_frag<DT, DP>(tile, row0, w, at);
+            b[w % (AHEAD + 1)] = right(w);
+        }
+        attn_mfma<DT>(acc, a[u % (AHEAD + 1)], b[u % (AHEAD + 1)]);
+        work(U, IC<N>{});
+        __builtin_amdgcn_sched_barrier(0);
+    });
+}
+
+template <int DT, int DP, int AHEAD, typename W>
+__device__ __forceinline__ void attn_cols_beside(floatx16 (&acc)[DP / 32], const typename AttnT<DT>::S *tile, int row0,
+                                                 const floatx16 &p, const AttnLane<DT, DP> &at, W &&work)
+{
+    constexpr int N = attn_col_units<DT, DP>(), ND = DP / 32;
+    AttnColFrag<DT> a[AHEAD + 1], b[N / ND];
+#pragma unroll
+    for (int u = 0; u < N; u += ND) b[u / ND] = attn_col_right<DT, DP>(p, u);
+    static_for<0, AHEAD>([&](auto U) { a[decltype(U)::value] = attn_col_frag<DT, DP>(tile, row0, decltype(U)::value, at); });
+    static_for<0, N>([&](auto U) {
+        constexpr int u = decltype(U)::value, w = u + AHEAD;
+        if constexpr (w < N) a[w % (AHEAD + 1)] = attn_col_frag<DT, DP>(tile, row0, w, at);
+        attn_col_mfma<DT, DP>(acc, u, a[u % (AHEAD + 1)], b[u / ND]);
+        work(U, IC<N>{});
+        __builtin_amdgcn_sched_barrier(0);
+    });
+}
+
+// Unit u of n does its share of 16 registers: f(register).
+template <typename U, typename N, typename F>
+__device__ __forceinline__ void attn_share(U, N, F &&f)
+{
+    static_for<U::value * 16 / N::value, (U::value + 1) * 16 / N::value>([&](auto E) { f(decltype(E)::value); });
 }
 
 // Everything this wave loads or writes to LDS is there, and every wave has
@@ -832,16 +925,24 @@ void k_attention_token(AttnArgs g)
 // them, head by head of the group, so the sum over heads that share a key
 // stays in its registers and no order of additions can change.
 //
-// PASS 0 computes both gradients.  float32 heads past 128 elements, whose
-// two rows and two sums together would pass the register file, take PASS 1
-// (values) and PASS 2 (keys).
+// Blocks of 32 queries go through a pipeline of two: the scores and the
+// products with the values of block i + 1 run on the matrix pipe beside the
+// exponentials and differences of block i, then come block i's two products
+// into the sums.  The tiles lie in three buffers, since block i + 1 may be
+// the next tile's: one barrier a tile, and a tile has the time of a whole one
+// to arrive.
+//
+// PASS 0 computes both gradients.  Heads past 128 elements, whose rows and
+// sums together would pass the register file, take PASS 1 (values) and PASS 2
+// (keys).
 template <int DT, int DP> struct AttnBwdShape {
     static constexpr int ES = AttnT<DT>::ES;
-    static constexpr int BQ = ES == 4 || DP == 256 ? 32 : 64;
-    static constexpr int BN = BQ;
-    static constexpr int TILE = attn_tile_bytes(BQ, DP, ES);
-    static constexpr int WGS = 4 * TILE <= 65536 && DP * ES <= 128 ? 2 : 1;
-    static constexpr bool kSplitPasses = DP * ES > 512;
+    static constexpr int BQ = ES == 4 || DP == 256 ? 32 : 64;  // queries of a tile, keys' gradient
+    static constexpr int BN = BQ;                              // keys of a tile, queries' gradient
+    static constexpr int NBUF = 6 * attn_tile_bytes(BQ, DP, ES) <= 131072 ? 3 : 2;
+    static constexpr int KWGS = DP <= 64 ? 2 : 1;              // workgroups a CU
+    static constexpr int QWGS = DP * ES <= 256 ? 2 : 1;
+    static constexpr bool kSplitPasses = DP == 256;
 };
 
 // Four bytes a lane into LDS, zeros past `range`.
@@ -853,14 +954,17 @@ __device__ __forceinline__ void attn_load_lds4(const void *base, uint32_t off, f
 }
 
 template <int DT, int DP, int PASS, bool VEC>
-__global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_dkv(AttnArgs g)
+__global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::KWGS)) void k_attention_dkv(AttnArgs g)
 {
     using T = AttnT<DT>;
     using S = typename T::S;
-    constexpr int BQ = AttnBwdShape<DT, DP>::BQ, NQB = BQ / 32, KS = DP * T::ES / 32, ND = DP / 32;
+    constexpr int BQ = AttnBwdShape<DT, DP>::BQ, NQB = BQ / 32, KS = DP * T::ES / 32, ND = DP / 32, TE = BQ * DP;
+    constexpr int NBUF = AttnBwdShape<DT, DP>::NBUF;
+    constexpr int AHEAD = AttnBwdShape<DT, DP>::KWGS == 1 ? 6 : 3, NCOL = attn_col_units<DT, DP>();
     constexpr bool kV = PASS != 2, kK = PASS != 1;
-    __shared__ __attribute__((aligned(1024))) S q0[BQ * DP], w0[BQ * DP], q1[BQ * DP], w1[BQ * DP];
-    __shared__ __attribute__((aligned(256))) float l0[64], l1[64], e0[64], e1[64];
+    // queries, then upstream gradients; lse, then the rows' sums
+    __shared__ __attribute__((aligned(1024))) S b0[2 * TE], b1[2 * TE], b2[NBUF == 3 ? 2 * TE : 8];
+    __shared__ __attribute__((aligned(256))) float s0[128], s1[128], s2[128];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     int tile, bh;
@@ -872,86 +976,149 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
     if (first >= sk.n) return;  // whole workgroup
     const int key = first + wave * 32 + (lane & 31);
     const bool live = key < sk.n;
-    typename T::Frag k[KS], v[kK ? KS : 1];
-    attn_row<DT, DP, VEC>(k, (const S *)g.k + b * g.k_bs + (sk.row + key) * g.k_ts + hk * g.k_hs, live, g.size, half);
-    if constexpr (kK)
-        attn_row<DT, DP, VEC>(v, (const S *)g.v + b * g.v_bs + (sk.row + key) * g.v_ts + hk * g.v_hs, live, g.size, half);
 
     // query i sees key j where i >= j - shift
     const int shift = sk.n - sq.n;
     const int from = g.causal ? key - shift : INT_MIN;
     const int t0 = g.causal ? max(0, first - shift) / BQ : 0, per = max(0, (sq.n + BQ - 1) / BQ - t0);
-    // this workgroup's share of the steps
+    // this workgroup's share of the tiles of all heads
     const int share = (per * g.group + g.splits - 1) / g.splits;
     const int step0 = share * (int)blockIdx.y, steps = min(per * g.group, step0 + share);
-
-    floatx16 dk[kK ? ND : 1], dv[kV ? ND : 1];
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-#pragma unroll
-        for (int d = 0; d < (kK ? ND : 1); d++) dk[d][e] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < (kV ? ND : 1); d++) dv[d][e] = 0.0f;
-    }
 
     const S *qb = (const S *)g.q + b * g.q_bs + sq.row * g.q_ts, *wb = (const S *)g.w + b * g.o_bs + sq.row * g.o_ts;
     const long long stat = g.q_starts ? sq.row : (long long)b * g.heads * g.nq;
     AttnStage<DT, DP, BQ, 4, VEC> ql, wl;
     ql.init({nullptr, g.q_ts * T::ES, 0}, g.size, wave, lane);
     wl.init({nullptr, g.o_ts * T::ES, 0}, g.size, wave, lane);
-    auto load = [&](int it, S *qt, S *wt, float *lt, float *et) {
+    auto load = [&](int it, S *to, float *st) __attribute__((always_inline)) {
         const int hq = hk * g.group + it / per, r0 = (t0 + it % per) * BQ;
-        ql.load({(const char *)(qb + hq * g.q_hs), g.q_ts * T::ES, sq.n}, g.size, r0, qt, wave, lane);
-        wl.load({(const char *)(wb + hq * g.o_hs), g.o_ts * T::ES, sq.n}, g.size, r0, wt, wave, lane);
+        ql.load({(const char *)(qb + hq * g.q_hs), g.q_ts * T::ES, sq.n}, g.size, r0, to, wave, lane);
+        wl.load({(const char *)(wb + hq * g.o_hs), g.o_ts * T::ES, sq.n}, g.size, r0, to + TE, wave, lane);
         const long long at = stat + (long long)hq * g.stat_rows + r0;
         const uint32_t range = (uint32_t)min(sq.n - r0, BQ) * 4u;
         // rows past the last have zero products; a zero lse keeps their exponentials finite
-        if (wave == 0) attn_load_lds4(g.lse2 + at, lane * 4u, lt, range);
-        if (wave == 1) attn_load_lds4(g.delta + at, lane * 4u, et, range);
+        if (wave == 0) attn_load_lds4(g.lse2 + at, lane * 4u, st, range);
+        if (wave == 1) attn_load_lds4(g.delta + at, lane * 4u, st + 64, range);
     };
+    if (step0 < steps) {
+        load(step0, b0, s0);
+        if (step0 + 1 < steps) load(step0 + 1, b1, s1);
+    }
+    typename T::Frag k[KS], v[kK ? KS : 1];
+    attn_row<DT, DP, VEC>(k, (const S *)g.k + b * g.k_bs + (sk.row + key) * g.k_ts + hk * g.k_hs, live, g.size, half);
+    if constexpr (kK)
+        attn_row<DT, DP, VEC>(v, (const S *)g.v + b * g.v_bs + (sk.row + key) * g.v_ts + hk * g.v_hs, live, g.size, half);
+    floatx16 dk[ND], dv[ND], pa, pb, ta, tb;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) dk[d][e] = dv[d][e] = 0.0f;
+    }
     AttnLane<DT, DP> at;
     at.init(lane);
-    auto step = [&](int it, const S *qt, const S *wt, const float *lt, const float *et) {
+    auto of_key = [&](int f) { return k[f]; };
+    auto of_value = [&](int f) { return v[kK ? f : 0]; };
+    auto nothing = [](auto, auto) {};
+    // block qi of the tile in `now`, step `it`; the next block lies in `next` from row `row`
+    auto block = [&](int it, int qi, floatx16 &p, floatx16 &t, floatx16 &pn, floatx16 &tn, const S *now, const float *st,
+                     const S *next, int row) __attribute__((always_inline)) {
         at.fresh();
-        const int i0 = (t0 + it % per) * BQ + 4 * half;
-        const bool mask = g.causal && (t0 + it % per) * BQ < first + 127 - shift;
+        floatx4 ls[4], es[4];
 #pragma unroll
-        for (int qb2 = 0; qb2 < NQB; qb2++) {
-            floatx16 p = attn_rows<DT, DP>(qt, qb2 * 32, k, at);
+        for (int r = 0; r < 4; r++) {
+            ls[r] = *(const floatx4 *)(st + qi * 32 + 8 * r + 4 * half);
+            if constexpr (kK) es[r] = *(const floatx4 *)(st + 64 + qi * 32 + 8 * r + 4 * half);
+        }
+        // the next block's scores beside this one's exponentials, its products
+        // with the values beside the differences, then this block's sums
+        constexpr int NA = KS, NB = NA + (kK ? KS : 0), NC = NB + (kV ? NCOL : 0), N = NC + (kK ? NCOL : 0);
+        AttnColFrag<DT> right[NCOL / ND];
 #pragma unroll
-            for (int r4 = 0; r4 < 4; r4++) {
-                const floatx4 ls = *(const floatx4 *)(lt + qb2 * 32 + 8 * r4 + 4 * half);
+        for (int e = 0; e < 16; e++) pn[e] = tn[e] = 0.0f;
+        attn_queue<DT, N, AHEAD>(
+            [&](auto I) __attribute__((always_inline)) {
+                constexpr int u = decltype(I)::value;
+                if constexpr (u < NA) return attn_row_frag<DT, DP>(next, row, u, at);
+                else if constexpr (u < NB) return attn_row_frag<DT, DP>(next + TE, row, u - NA, at);
+                else if constexpr (u < NC) return attn_any<DT>(attn_col_frag<DT, DP>(now + TE, qi * 32, u - NB, at));
+                else return attn_any<DT>(attn_col_frag<DT, DP>(now, qi * 32, u - NC, at));
+            },
+            [&](auto I, const typename T::Frag &f) __attribute__((always_inline)) {
+                constexpr int u = decltype(I)::value;
+                // (asm: here, beside the products, and not where they are used)
+                if constexpr (u < NA) {
+                    attn_mfma<DT>(pn, f, k[u]);
+                    attn_share(IC<u>{}, IC<NA>{}, [&](int r) {
+                        float x = __builtin_amdgcn_exp2f(fmaf(p[r], g.scale_log2, -ls[r / 4][r % 4]));
+                        asm volatile("" : "+v"(x));
+                        p[r] = x;
+                    });
+                    if constexpr (u + 1 == NA) {
+                        const int r0 = (t0 + it % per) * BQ;
+                        if (g.causal && r0 < first + 127 - shift) {
+                            const int i0 = r0 + qi * 32 + 4 * half;
 #pragma unroll
-                for (int x = 0; x < 4; x++)
-                    p[4 * r4 + x] = __builtin_amdgcn_exp2f(fmaf(p[4 * r4 + x], g.scale_log2, -ls[x]));
-            }
-            if (mask) {
-#pragma unroll
-                for (int r = 0; r < 16; r++) p[r] = i0 + qb2 * 32 + 8 * (r / 4) + r % 4 >= from ? p[r] : 0.0f;
-            }
-            if constexpr (kV) attn_cols<DT, DP>(dv, wt, qb2 * 32, p, at);
-            if constexpr (kK) {
-                floatx16 t = attn_rows<DT, DP>(wt, qb2 * 32, v, at);
-#pragma unroll
-                for (int r4 = 0; r4 < 4; r4++) {
-                    const floatx4 es = *(const floatx4 *)(et + qb2 * 32 + 8 * r4 + 4 * half);
-#pragma unroll
-                    for (int x = 0; x < 4; x++) t[4 * r4 + x] = p[4 * r4 + x] * (t[4 * r4 + x] - es[x]);
+                            for (int r = 0; r < 16; r++) p[r] = i0 + 8 * (r / 4) + r % 4 >= from ? p[r] : 0.0f;
+                        }
+                    }
+                } else if constexpr (u < NB) {
+                    attn_mfma<DT>(tn, f, v[kK ? u - NA : 0]);
+                    attn_share(IC<u - NA>{}, IC<KS>{}, [&](int r) {
+                        float x = p[r] * (t[r] - es[r / 4][r % 4]);
+                        asm volatile("" : "+v"(x));
+                        t[r] = x;
+                    });
+                } else if constexpr (u < NC) {
+                    if constexpr ((u - NB) % ND == 0) right[(u - NB) / ND] = attn_col_right<DT, DP>(p, u - NB);
+                    attn_col_mfma<DT, DP>(dv, u - NB, attn_of_any<DT>(f), right[(u - NB) / ND]);
+                } else {
+                    if constexpr ((u - NC) % ND == 0) right[(u - NC) / ND] = attn_col_right<DT, DP>(t, u - NC);
+                    attn_col_mfma<DT, DP>(dk, u - NC, attn_of_any<DT>(f), right[(u - NC) / ND]);
                 }
-                attn_cols<DT, DP>(dk, qt, qb2 * 32, t, at);
-            }
+            });
+    };
+    // a step: its tile lies in `now`, the next in `next`, the one after goes to `later`
+    auto step = [&](int it, floatx16 &p, floatx16 &t, floatx16 &pn, floatx16 &tn, S *now, float *st, S *next, S *later, float *sl) __attribute__((always_inline)) {
+        if constexpr (NQB == 2) block(it, 0, p, t, pn, tn, now, st, now, 32);
+        attn_landed();  // the next tile is there, and every wave is done with the one before this
+        if (NBUF == 3 && it + 2 < steps) load(it + 2, later, sl);
+        // (after the last tile the next block is computed from what lies there, and used by nobody)
+        if constexpr (NQB == 2) block(it, 1, pn, tn, p, t, now, st, next, 0);
+        else block(it, 0, p, t, pn, tn, now, st, next, 0);
+        if constexpr (NBUF == 2) {
+            attn_landed();
+            if (it + 2 < steps) load(it + 2, now, st);
         }
     };
-    if (step0 < steps) load(step0, q0, w0, l0, e0);
-    for (int it = step0; it < steps; it += 2) {
-        attn_landed();  // this step's tiles are there, and every wave is done with the other buffer
-        if (it + 1 < steps) load(it + 1, q1, w1, l1, e1);
-        step(it, q0, w0, l0, e0);
-        if (it + 1 >= steps) break;
+    if (step0 < steps) {
         attn_landed();
-        if (it + 2 < steps) load(it + 2, q0, w0, l0, e0);
-        step(it + 1, q1, w1, l1, e1);
+        at.fresh();
+        attn_rows_beside<DT, DP, AHEAD>(pa, b0, 0, of_key, at, nothing);
+        if constexpr (kK) attn_rows_beside<DT, DP, AHEAD>(ta, b0 + TE, 0, of_value, at, nothing);
     }
+    // with one block a tile the two score registers change places from step to step
+    auto steps_of = [&](int it, floatx16 &p, floatx16 &t, floatx16 &pn, floatx16 &tn, auto TURN) __attribute__((always_inline)) {
+        constexpr int n = decltype(TURN)::value % NBUF;
+        if constexpr (NBUF == 2) {
+            if constexpr (n == 0) step(it, p, t, pn, tn, b0, s0, b1, b0, s0);
+            else step(it, p, t, pn, tn, b1, s1, b0, b1, s1);
+        } else if constexpr (n == 0) {
+            step(it, p, t, pn, tn, b0, s0, b1, b2, s2);
+        } else if constexpr (n == 1) {
+            step(it, p, t, pn, tn, b1, s1, b2, b0, s0);
+        } else {
+            step(it, p, t, pn, tn, b2, s2, b0, b1, s1);
+        }
+    };
+    constexpr int TURNS = NQB == 2 ? NBUF : NBUF == 3 ? 6 : 2;
+    for (int it = step0; it < steps; it += TURNS)
+        static_for<0, TURNS>([&](auto TURN) __attribute__((always_inline)) {
+            constexpr int n = decltype(TURN)::value;
+            if (it + n < steps) {
+                if constexpr (NQB == 2 || n % 2 == 0) steps_of(it + n, pa, ta, pb, tb, TURN);
+                else steps_of(it + n, pb, tb, pa, ta, TURN);
+            }
+        });
     if (!live) return;
     // gradients are contiguous, and so is each share's part of them
     const long long to = ((g.k_starts ? sk.row + key : (long long)b * g.nk + key) * g.kv_heads + hk) * g.size;
@@ -976,7 +1143,7 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
 // ------------------------------------------------- gradient of the queries
 // Rows as in the forward pass; the keys and values stream past them.
 template <int DT, int DP, bool VEC>
-__global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_dq(AttnArgs g)
+__global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::QWGS)) void k_attention_dq(AttnArgs g)
 {
     using T = AttnT<DT>;
     using S = typename T::S;
@@ -1026,17 +1193,23 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::WGS)) void k_attention_
         const bool mask = (t + 1) * BN > lim_first;
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++) {
-            floatx16 p = attn_rows<DT, DP>(kt, kb * 32, q, at);
-#pragma unroll
-            for (int r = 0; r < 16; r++) p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], g.scale_log2, -ls));
+            auto nothing = [](auto, auto) {};
+            floatx16 p, x;
+            attn_rows_beside<DT, DP, 2>(p, kt, kb * 32, [&](int f) { return q[f]; }, at, nothing);
+            attn_rows_beside<DT, DP, 2>(x, vt, kb * 32, [&](int f) { return w[f]; }, at, [&](auto U, auto N) {
+                attn_share(U, N, [&](int r) {
+                    float y = __builtin_amdgcn_exp2f(fmaf(p[r], g.scale_log2, -ls));
+                    asm volatile("" : "+v"(y));  // here, beside the products
+                    p[r] = y;
+                });
+            });
             if (mask) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) p[r] = key0 + kb * 32 + 8 * (r / 4) + r % 4 < lim ? p[r] : 0.0f;
             }
-            floatx16 x = attn_rows<DT, DP>(vt, kb * 32, w, at);
 #pragma unroll
             for (int r = 0; r < 16; r++) x[r] = p[r] * (x[r] - es);
-            attn_cols<DT, DP>(dq, kt, kb * 32, x, at);
+            attn_cols_beside<DT, DP, 2>(dq, kt, kb * 32, x, at, nothing);
         }
     };
     auto load = [&](int t, S *kt, S *vt) {

@@ -44,9 +44,9 @@ static void launch_dq(const AttnArgs &g, unsigned blocks, hipStream_t s)
 
 template <> int attention_backward_tile<PT_ATTN_DT>(int size)
 {
-    return size <= 64    ? AttnBwdShape<PT_ATTN_DT, 64>::BQ
-           : size <= 128 ? AttnBwdShape<PT_ATTN_DT, 128>::BQ
-                         : AttnBwdShape<PT_ATTN_DT, 256>::BQ;
+    return size <= 64    ? AttnBwdShape<PT_ATTN_DT, 64>::BN
+           : size <= 128 ? AttnBwdShape<PT_ATTN_DT, 128>::BN
+                         : AttnBwdShape<PT_ATTN_DT, 256>::BN;
 }
 
 template <> void launch_attention<PT_ATTN_DT>(const AttnArgs &g, bool token, bool vec, unsigned blocks, hipStream_t s)
