@@ -163,6 +163,8 @@ def _array(framework, t):
     torch.cuda.synchronize()
     _abi.check(_abi.load().pt_memcpy_d2d(_host.load().phpt_device_pointer(a._h), t.data_ptr(),
                                          t.numel() * t.element_size(), None))
+    # the framework's stream does not wait for torch's, nor torch's for it: the copy ends before t's memory is used again
+    torch.cuda.synchronize()
     return a
 
 
