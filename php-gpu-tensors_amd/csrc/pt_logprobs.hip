@@ -46,6 +46,23 @@ template <int DT> struct LpPack {
 #pragma unroll
         for (int i = 0; i < V; i++) v[i] = DType<DT>::to_c(u.s[i]);
     }
+    // elements that add nothing
+    __device__ __forceinline__ static lp_u32x4 nothing()
+    {
+        const uint32_t low = sizeof(S) == 4 ? 0xff800000u : DT == PT_FLOAT16 ? 0xfc00fc00u : 0xff80ff80u;
+        return lp_u32x4{low, low, low, low};
+    }
+    // element `at`, if it is one of these, becomes a NaN
+    __device__ __forceinline__ static void drop(lp_u32x4 &raw, int at)
+    {
+        if constexpr (sizeof(S) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) raw[i] = at == i ? 0x7fffffffu : raw[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) raw[i] |= (at >> 1) == i ? (at & 1 ? 0x7fff0000u : 0x7fffu) : 0u;
+        }
+    }
 };
 
 // Running maximum, sum and entropy sum.
@@ -88,31 +105,34 @@ struct LpSum {
 };
 
 // The top-th largest of the lanes' values: of elements of which these are
-// some, the top-th largest is no smaller.  A binary search over the bits of
-// an order-preserving key, one ballot a bit, so nothing moves between lanes.
-// NaN counts as -inf.
+// some, the top-th largest is no smaller.  NaN counts as -inf.
 __device__ __forceinline__ float lp_bound(float x, int top)
 {
-    const float y = x > -INFINITY ? x : -INFINITY;
-    const uint32_t u = __float_as_uint(y), key = u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
-    uint32_t at = 0;
-#pragma unroll 4
-    for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t to = at | 1u << bit;
-        if (__popcll(__ballot(key >= to)) >= top) at = to;
+    float y = x > -INFINITY ? x : -INFINITY, m;
+    for (int have = 0;;) {
+        m = wave_all(y, FMax{});
+        have += (int)__popcll(__ballot(y == m));
+        if (have >= top) return m;  // at the latest where all are -inf
+        y = y == m ? -INFINITY : y;
     }
-    return __uint_as_float(at >> 31 ? at ^ 0x80000000u : ~at);
 }
 
 // The best `top` elements of a wave, in lanes 0 .. top - 1.
 struct LpTop {
-    float v, worst;  // worst: what an element has to reach
+    float v, worst, floor;  // worst: what an element has to reach, at least floor
     int i, worst_i;
-    // no element below `x` is wanted (lp_bound; once, while the list is empty)
-    __device__ __forceinline__ void at_least(float x) { worst = x; }
+    // no element below `x` is wanted
+    __device__ __forceinline__ void at_least(float x)
+    {
+        floor = fmaxf(floor, x);
+        if (floor > worst) {
+            worst = floor;
+            worst_i = INT_MAX;
+        }
+    }
     __device__ __forceinline__ void init()
     {
-        v = worst = -INFINITY;
+        v = worst = floor = -INFINITY;
         i = worst_i = INT_MAX;
     }
     __device__ __forceinline__ static bool better(float a, int ai, float b, int bi) { return a > b || (a == b && ai < bi); }
@@ -134,8 +154,9 @@ struct LpTop {
                 i = lane == place ? ci : up_i;
             }
             const int last_i = __builtin_amdgcn_readlane(i, top - 1);
-            if (last_i != INT_MAX) {  // the list is full: its last bounds what follows
-                worst = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), top - 1));
+            const float last = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), top - 1));
+            if (last_i != INT_MAX && last >= floor) {  // the list is full: its last bounds what follows
+                worst = last;
                 worst_i = last_i;
             }
             want = lane != from && want && better(x, at, worst, worst_i);
@@ -202,15 +223,19 @@ __device__ __forceinline__ void lp_finish(const LpArgs &g, int row, const LpSum 
 
 // A row, or the part blockIdx.y of it, by NW waves.
 template <int DT, int NW, bool TOP>
-__global__ __launch_bounds__(64 * NW) void k_logprobs(LpArgs g)
+__global__ __launch_bounds__(64 * NW, 8) void k_logprobs(LpArgs g)
 {
     using P = LpPack<DT>;
-    constexpr int V = P::V, UN = 4;
+    // Packs in flight a lane.  Four of 16 bits and the search need more than
+    // the 64 registers of eight waves a SIMD: 69 us with what spills, 60 with
+    // three (2000 rows of 50021, top 8).
+    constexpr int V = P::V, UN = TOP && V == 8 ? 3 : 4;
     __shared__ float box[NW][3];
     __shared__ float top_v[TOP ? NW : 1][64];
     __shared__ int top_i[TOP ? NW : 1][64];
     __shared__ float best_v[64];
     __shared__ int best_i[64];
+    __shared__ volatile float share[TOP ? NW : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x;
     const typename P::S *x = (const typename P::S *)g.x + (long long)row * g.stride;
@@ -223,19 +248,31 @@ __global__ __launch_bounds__(64 * NW) void k_logprobs(LpArgs g)
     a.init();
     LpTop top;
     top.init();
-    bool bounded = false;
+    // What the waves tell each other: a value that `deep` of a wave's elements
+    // reach; where `wide` waves reach a value, `top` elements do.
+    const int deep = TOP ? (g.top + NW - 1) / NW : 0, wide = TOP ? (g.top + deep - 1) / deep : 0;
+    int calls = 0;
     const int turn = NW * 64 * V;
-    // NP packs at once
-    auto take = [&](int at, const lp_u32x4 *raw, auto NP) {
+    // NP packs at once; `in`: this lane's are inside (all lanes' if NP > 1)
+    auto take = [&](int at, bool in, auto NP) __attribute__((always_inline)) {
         constexpr int np = decltype(NP)::value;
+        lp_u32x4 raw[np];
         float v[np][V];
 #pragma unroll
+        for (int p = 0; p < np; p++) {
+            if (np > 1 || in) raw[p] = P::load(x + at + p * turn);
+            else raw[p] = P::nothing();
+        }
+#pragma unroll
         for (int p = 0; p < np; p++) P::widen(raw[p], v[p]);
-        float most = v[0][0];
+        float each[np], most = __builtin_nanf("");
 #pragma unroll
-        for (int p = 0; p < np; p++)
+        for (int p = 0; p < np; p++) {
+            each[p] = v[p][0];
 #pragma unroll
-            for (int k = 0; k < V; k++) most = fmaxf(most, v[p][k]);
+            for (int k = 1; k < V; k++) each[p] = fmaxf(each[p], v[p][k]);
+            most = fmaxf(most, each[p]);
+        }
         a.rise(most);
         const float r = a.ref();
 #pragma unroll
@@ -243,64 +280,74 @@ __global__ __launch_bounds__(64 * NW) void k_logprobs(LpArgs g)
 #pragma unroll
             for (int k = 0; k < V; k++) a.add(v[p][k], r);
         if constexpr (TOP) {
-            if (!bounded) {
-                top.at_least(lp_bound(most, g.top));
-                bounded = true;
+            asm volatile("" : "+v"(a.s), "+v"(a.t));  // the sums before the search
+            // The bound is looked at after 1, 2, 4, ... calls, which every wave
+            // of the block makes alike; a.m is the largest of a lane so far.
+            if ((calls & (calls + 1)) == 0) {
+                const float own = lp_bound(a.m, deep);
+                if constexpr (NW == 1) top.at_least(own);
+                else {
+                    if (lane == 0) share[wave] = own;
+                    // At the first call only: later values only raise the
+                    // bound, and which of them a wave reads is of no
+                    // consequence for the result.
+                    if (!calls) __syncthreads();
+                    float o[NW], bound = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < NW; w++) o[w] = share[w];
+#pragma unroll
+                    for (int w = 0; w < NW; w++) {
+                        int reach = 0;
+#pragma unroll
+                        for (int z = 0; z < NW; z++) reach += o[z] >= o[w];
+                        bound = fmaxf(bound, reach >= wide ? o[w] : -INFINITY);
+                    }
+                    top.at_least(bound);
+                }
             }
-            // Every lane offers its largest element, and while that is good
-            // enough the next: the first of those equal to the maximum, which
-            // is then put out of the way as a NaN.
-            while (__any(most >= top.worst)) {
-                int from = INT_MAX;
+            calls++;
+            if (np == 1 && !in) {
+                each[0] = __builtin_nanf("");
+                raw[0] = lp_u32x4{~0u, ~0u, ~0u, ~0u};
+            }
+            // Every lane offers a pack's largest element, and while that is
+            // good enough the next: the first of those equal to the maximum,
+            // which is then put out of the way as a NaN.
 #pragma unroll
-                for (int p = np - 1; p >= 0; p--)
+            for (int p = 0; p < np; p++) {
+                while (__any(each[p] >= top.worst)) {
+                    // The pack is widened anew: its elements, kept over the
+                    // search, would halve the waves of a SIMD.
+                    asm volatile("" : "+v"(raw[p]));
+                    float e[V];
+                    int from = INT_MAX;
+                    P::widen(raw[p], e);
 #pragma unroll
-                    for (int k = V - 1; k >= 0; k--) from = v[p][k] == most ? p * turn + k : from;
-                const bool good = most >= top.worst;
-                top.offer(most, from == INT_MAX ? INT_MAX : at + from, g.top, lane);
+                    for (int k = V - 1; k >= 0; k--) from = e[k] == each[p] ? k : from;
+                    top.offer(each[p], from == INT_MAX ? INT_MAX : at + p * turn + from, g.top, lane);
+                    P::drop(raw[p], from);
+                    P::widen(raw[p], e);
+                    each[p] = e[0];
 #pragma unroll
-                for (int p = 0; p < np; p++)
-#pragma unroll
-                    for (int k = 0; k < V; k++) v[p][k] = from == p * turn + k ? __builtin_nanf("") : v[p][k];
-                most = __builtin_nanf("");
-                if (!__any(good)) break;
-#pragma unroll
-                for (int p = 0; p < np; p++)
-#pragma unroll
-                    for (int k = 0; k < V; k++) most = fmaxf(most, v[p][k]);
+                    for (int k = 1; k < V; k++) each[p] = fmaxf(each[p], e[k]);
+                }
             }
         }
     };
-    // whole turns of the block first, then whole packs, then single elements
-    int at = begin;
+    // The elements before the first boundary of 16 bytes and those behind the
+    // last whole pack, one a thread: read first, added last.
+    const int from = min(end, begin + (int)((0 - (uintptr_t)(x + begin)) % 16 / sizeof(typename P::S)));
+    const int packs_end = from + (end - from) / V * V;
+    const int odd = (int)threadIdx.x < from - begin ? begin + (int)threadIdx.x : packs_end - from + begin + (int)threadIdx.x;
+    const float e = odd < end ? DType<DT>::to_c(x[odd]) : -INFINITY;
     const int mine = (int)threadIdx.x * V;
-    auto load = [&](int from, lp_u32x4 (&raw)[UN]) {
-#pragma unroll
-        for (int p = 0; p < UN; p++) raw[p] = P::load(x + from + mine + p * turn);
-    };
-    lp_u32x4 raw[UN], next[UN];
-    if (at + UN * turn <= end) load(at, raw);
-    for (; at + UN * turn <= end; at += UN * turn) {
-        const bool more = at + 2 * UN * turn <= end;  // the next packs are under way while these are added
-        if (more) load(at + UN * turn, next);
-        take(at + mine, raw, std::integral_constant<int, UN>{});
-#pragma unroll
-        for (int p = 0; p < UN; p++) raw[p] = next[p];
-    }
-    for (; at + turn <= end; at += turn) {
-        const lp_u32x4 one = P::load(x + at + mine);
-        take(at + mine, &one, std::integral_constant<int, 1>{});
-    }
-    for (; at < end; at += NW * 64) {
-        // one element a thread
-        const int i = at + (int)threadIdx.x;
-        const bool in = i < end;
-        const float e = in ? DType<DT>::to_c(x[i]) : -INFINITY;
-        a.rise(e);
-        if (in) a.add(e, a.ref());
-        if constexpr (TOP) {
-            if (__any(e >= top.worst)) top.offer(e, in ? i : INT_MAX, g.top, lane);
-        }
+    int at = from;
+    for (; at + UN * turn <= packs_end; at += UN * turn) take(at + mine, true, std::integral_constant<int, UN>{});
+    for (; at < packs_end; at += turn) take(at + mine, at + mine < packs_end, std::integral_constant<int, 1>{});
+    a.rise(e);
+    if (odd < end) a.add(e, a.ref());
+    if constexpr (TOP) {
+        if (__any(e >= top.worst)) top.offer(e, odd < end ? odd : INT_MAX, g.top, lane);
     }
     a = lp_wave(a);
     if constexpr (NW > 1) {
