@@ -90,39 +90,39 @@ __global__ __launch_bounds__(256) void k_attention_prepare(const void *w, const 
     typedef uint16_t __attribute__((ext_vector_type(V))) HV;
     typedef float __attribute__((ext_vector_type(V))) FV;
     const int lane = threadIdx.x & 15;
-    const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (at >= rows * heads) return;
-    float x = 0.0f;
-    for (int d = lane * V; d < size; d += 16 * V) {
-        const long long e = at * size + d;
-        const SV o = *(const SV *)((const S *)out + e);
-        if constexpr (W32) {
-            const FV f = *(const FV *)((const float *)w + e);
-            HV h;
+    for (long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); at < rows * heads; at += (long long)gridDim.x * 16) {
+        float x = 0.0f;
+        for (int d = lane * V; d < size; d += 16 * V) {
+            const long long e = at * size + d;
+            const SV o = *(const SV *)((const S *)out + e);
+            if constexpr (W32) {
+                const FV f = *(const FV *)((const float *)w + e);
+                HV h;
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                float wv = f[i];
-                if constexpr (DT != PT_FLOAT32) {
-                    h[i] = DT == PT_BFLOAT16 ? float_to_bf16(wv) : float_to_f16(wv);
-                    wv = DT == PT_BFLOAT16 ? bf16_to_float(h[i]) : f16_to_float(h[i]);
+                for (int i = 0; i < V; i++) {
+                    float wv = f[i];
+                    if constexpr (DT != PT_FLOAT32) {
+                        h[i] = DT == PT_BFLOAT16 ? float_to_bf16(wv) : float_to_f16(wv);
+                        wv = DT == PT_BFLOAT16 ? bf16_to_float(h[i]) : f16_to_float(h[i]);
+                    }
+                    x = fmaf(wv, DType<DT>::to_c(o[i]), x);
                 }
-                x = fmaf(wv, DType<DT>::to_c(o[i]), x);
+                if constexpr (DT != PT_FLOAT32) *(HV *)(w16 + e) = h;
+            } else {
+                const SV f = *(const SV *)((const S *)w + e);
+#pragma unroll
+                for (int i = 0; i < V; i++) x = fmaf(DType<DT>::to_c(f[i]), DType<DT>::to_c(o[i]), x);
             }
-            if constexpr (DT != PT_FLOAT32) *(HV *)(w16 + e) = h;
-        } else {
-            const SV f = *(const SV *)((const S *)w + e);
-#pragma unroll
-            for (int i = 0; i < V; i++) x = fmaf(DType<DT>::to_c(f[i]), DType<DT>::to_c(o[i]), x);
         }
-    }
 #pragma unroll
-    for (int m = 8; m >= 1; m >>= 1) x += __shfl_xor(x, m, 16);
-    if (lane == 0) {
-        const long long row = at / heads, h = at % heads;
-        const long long stat = packed ? h * rows + row : (row / queries * heads + h) * queries + row % queries;
-        const float l = lse[stat];
-        delta[stat] = x;
-        lse2[stat] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
+        for (int m = 8; m >= 1; m >>= 1) x += __shfl_xor(x, m, 16);
+        if (lane == 0) {
+            const long long row = at / heads, h = at % heads;
+            const long long stat = packed ? h * rows + row : (row / queries * heads + h) * queries + row % queries;
+            const float l = lse[stat];
+            delta[stat] = x;
+            lse2[stat] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
+        }
     }
 }
 
@@ -288,7 +288,7 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
     float *part = (float *)(base + 2 * stat_bytes + w_bytes);
     pt_status st = PT_OK;
     if (stats) {
-        const unsigned n = (unsigned)((stats + 15) / 16);
+        const unsigned n = (unsigned)std::min((stats + 15) / 16, 1ll << 20);
         const bool packed = g.q_starts != nullptr;
         const bool packs = g.size % 8 == 0 && !(((uintptr_t)w | (uintptr_t)g.out) & 15);
         auto go = [&](auto W, auto V) {

@@ -564,6 +564,9 @@ template <int DT> static pt_status logprobs_backward_typed(LpBwdArgs g, hipStrea
     return check_hip(hipGetLastError(), "log probability gradient");
 }
 
+// A launch counts its threads in 32 bits: this many rows at once.
+constexpr size_t kLpRows = 1u << 22;
+
 static pt_status logprobs_check(int dtype, size_t rows, size_t classes, size_t row_stride, int top)
 {
     if (dtype != PT_FLOAT32 && dtype != PT_FLOAT16 && dtype != PT_BFLOAT16)
@@ -592,14 +595,19 @@ pt_status pt_logprobs(const void *logits, int dtype, size_t rows, size_t classes
     PT_TRY(ensure_init());
     if (!rows) return PT_OK;
     counters().fused_row_calls++;
-    const LpArgs g = {logits, (long long)row_stride, (int)rows, (int)classes, 1, top,
-                      tokens, logprob, entropy, stats, top_logprob, top_index, nullptr};
     hipStream_t s = stream_of(stream);
-    switch (dtype) {
-    case PT_FLOAT32: return logprobs_typed<PT_FLOAT32>(g, s);
-    case PT_FLOAT16: return logprobs_typed<PT_FLOAT16>(g, s);
-    default: return logprobs_typed<PT_BFLOAT16>(g, s);
+    for (size_t from = 0; from < rows; from += kLpRows) {
+        auto at = [&](auto *p, size_t width) { return p ? p + from * width : nullptr; };
+        const LpArgs g = {(const char *)logits + from * row_stride * dtype_size(dtype), (long long)row_stride,
+                          (int)std::min(rows - from, kLpRows), (int)classes, 1, top, at(tokens, 1), at(logprob, 1),
+                          at(entropy, 1), at(stats, 2), at(top_logprob, top), at(top_index, top), nullptr};
+        switch (dtype) {
+        case PT_FLOAT32: PT_TRY(logprobs_typed<PT_FLOAT32>(g, s)); break;
+        case PT_FLOAT16: PT_TRY(logprobs_typed<PT_FLOAT16>(g, s)); break;
+        default: PT_TRY(logprobs_typed<PT_BFLOAT16>(g, s));
+        }
     }
+    return PT_OK;
 }
 
 pt_status pt_logprobs_backward(const void *logits, int dtype, size_t rows, size_t classes, size_t row_stride,
@@ -614,14 +622,21 @@ pt_status pt_logprobs_backward(const void *logits, int dtype, size_t rows, size_
     PT_TRY(ensure_init());
     if (!rows) return PT_OK;
     counters().fused_row_calls++;
-    const LpBwdArgs g = {logits, dlogits, (long long)row_stride, (int)rows, (int)classes, 0, top, tokens, top_index,
-                         stats, entropy, grad_logprob, grad_entropy, top ? grad_top : nullptr};
     hipStream_t s = stream_of(stream);
-    switch (dtype) {
-    case PT_FLOAT32: return logprobs_backward_typed<PT_FLOAT32>(g, s);
-    case PT_FLOAT16: return logprobs_backward_typed<PT_FLOAT16>(g, s);
-    default: return logprobs_backward_typed<PT_BFLOAT16>(g, s);
+    const size_t es = dtype_size(dtype);
+    for (size_t from = 0; from < rows; from += kLpRows) {
+        auto at = [&](auto *p, size_t width) { return p ? p + from * width : nullptr; };
+        const LpBwdArgs g = {(const char *)logits + from * row_stride * es, (char *)dlogits + from * classes * es,
+                             (long long)row_stride, (int)std::min(rows - from, kLpRows), (int)classes, 0, top, at(tokens, 1),
+                             at(top_index, top), at(stats, 2), at(entropy, 1), at(grad_logprob, 1), at(grad_entropy, 1),
+                             top ? at(grad_top, top) : nullptr};
+        switch (dtype) {
+        case PT_FLOAT32: PT_TRY(logprobs_backward_typed<PT_FLOAT32>(g, s)); break;
+        case PT_FLOAT16: PT_TRY(logprobs_backward_typed<PT_FLOAT16>(g, s)); break;
+        default: PT_TRY(logprobs_backward_typed<PT_BFLOAT16>(g, s));
+        }
     }
+    return PT_OK;
 }
 
 }  // extern "C"

@@ -266,34 +266,36 @@ __device__ __forceinline__ CT nb_block_sum(CT v, CT *box)
 
 template <int DT, int PDT, typename CT>
 __global__ __launch_bounds__(256) void k_norm_backward_row(const void *x, const CT *g, const void *gamma, void *dx,
-                                                           CT *stats, int n, CT eps)
+                                                           CT *stats, long long rows, int n, CT eps)
 {
     __shared__ CT box[4];
-    const long long base = (long long)blockIdx.x * n;
-    CT s = 0;
-    for (int i = threadIdx.x; i < n; i += 256) s += nb_value<DT, CT>(x, base + i);
-    const CT mean = nb_block_sum(s, box) / (CT)n;
-    CT q = 0, h1 = 0, h2 = 0;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const CT d = nb_value<DT, CT>(x, base + i) - mean;
-        const CT h = gamma ? g[base + i] * nb_value<PDT, CT>(gamma, i) : g[base + i];
-        q += d * d;
-        h1 += h;
-        h2 += h * d;
-    }
-    q = nb_block_sum(q, box);
-    h1 = nb_block_sum(h1, box) / (CT)n;
-    const CT r = (CT)1 / (sizeof(CT) == 8 ? (CT)sqrt((double)(q / (CT)n + eps)) : (CT)sqrtf((float)(q / (CT)n + eps)));
-    h2 = nb_block_sum(h2, box) / (CT)n * r;
-    if (stats && threadIdx.x == 0) {
-        stats[2 * (long long)blockIdx.x] = mean;
-        stats[2 * (long long)blockIdx.x + 1] = r;
-    }
-    if (!dx) return;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const CT u = (nb_value<DT, CT>(x, base + i) - mean) * r;
-        const CT h = gamma ? g[base + i] * nb_value<PDT, CT>(gamma, i) : g[base + i];
-        ((typename DType<DT>::S *)dx)[base + i] = DType<DT>::from_c((typename DType<DT>::C)(r * (h - h1 - u * h2)));
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const long long base = row * n;
+        CT s = 0;
+        for (int i = threadIdx.x; i < n; i += 256) s += nb_value<DT, CT>(x, base + i);
+        const CT mean = nb_block_sum(s, box) / (CT)n;
+        CT q = 0, h1 = 0, h2 = 0;
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const CT d = nb_value<DT, CT>(x, base + i) - mean;
+            const CT h = gamma ? g[base + i] * nb_value<PDT, CT>(gamma, i) : g[base + i];
+            q += d * d;
+            h1 += h;
+            h2 += h * d;
+        }
+        q = nb_block_sum(q, box);
+        h1 = nb_block_sum(h1, box) / (CT)n;
+        const CT r = (CT)1 / (sizeof(CT) == 8 ? (CT)sqrt((double)(q / (CT)n + eps)) : (CT)sqrtf((float)(q / (CT)n + eps)));
+        h2 = nb_block_sum(h2, box) / (CT)n * r;
+        if (stats && threadIdx.x == 0) {
+            stats[2 * row] = mean;
+            stats[2 * row + 1] = r;
+        }
+        if (!dx) continue;
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const CT u = (nb_value<DT, CT>(x, base + i) - mean) * r;
+            const CT h = gamma ? g[base + i] * nb_value<PDT, CT>(gamma, i) : g[base + i];
+            ((typename DType<DT>::S *)dx)[base + i] = DType<DT>::from_c((typename DType<DT>::C)(r * (h - h1 - u * h2)));
+        }
     }
 }
 
@@ -322,7 +324,8 @@ static pt_status norm_backward_general(const void *x, const void *g, const void 
     void *scratch = nullptr;
     if (params) PT_TRY(scratch_alloc(&scratch, ((size_t)rows * 2 + (size_t)parts * 2 * n) * sizeof(CT), s));
     CT *stats = (CT *)scratch, *partial = stats ? stats + rows * 2 : nullptr;
-    k_norm_backward_row<DT, PDT, CT><<<(unsigned)rows, 256, 0, s>>>(x, (const CT *)g, gamma, dx, stats, n, eps);
+    k_norm_backward_row<DT, PDT, CT><<<(unsigned)std::min(rows, 1ll << 20), 256, 0, s>>>(x, (const CT *)g, gamma, dx, stats,
+                                                                                     rows, n, eps);
     if (params) {
         k_norm_backward_columns<DT, CT><<<dim3((n + 255) / 256, parts), 256, 0, s>>>(x, (const CT *)g, stats, partial, rows, n);
         k_norm_params<PDT, CT><<<dim3((n + 63) / 64, 2), 1024, 0, s>>>(partial, parts, n, dgamma, dbeta);

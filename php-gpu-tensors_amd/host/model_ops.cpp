@@ -467,16 +467,17 @@ static TensorP score_rows(const TensorP &a, size_t *rows, size_t *pitch)
     *pitch = classes;
     bool plain = a->shape[nd - 1] == 1 || a->strides[nd - 1] == 1;
     size_t step = 0;  // of the innermost row axis that has several rows
-    for (int d = nd - 2, inner = 1; d >= 0 && plain; d--) {
+    size_t inner = 1;
+    for (int d = nd - 2; d >= 0 && plain; d--) {
         if (a->shape[d] == 1) continue;
         if (!step) {
             step = a->strides[d];
             plain = step >= classes;
-            inner = a->shape[d];
+            inner = (size_t)a->shape[d];
             continue;
         }
-        plain = a->strides[d] == step * (size_t)inner;
-        inner *= a->shape[d];
+        plain = a->strides[d] == step * inner;
+        inner *= (size_t)a->shape[d];
     }
     if (!plain) return materialize(a);
     if (step) *pitch = step;

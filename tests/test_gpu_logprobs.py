@@ -251,3 +251,40 @@ def test_refusals():
                  lambda: a.logProbs(3), lambda: a.logProbs(t, top=2 ** 40)]:
         with pytest.raises(_abi.InvalidArgumentException):
             call()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_alternatives_of_unsplit_rows(dtype):
+    """Many rows of four waves each: rising, falling, equal and nearly all masked scores, the best in one wave's share
+    or at either end, in rows that start at any element of a pack."""
+    rows, n, top = 512, 5005, 30
+    rng = np.random.default_rng(11)
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    x[0], x[1], x[2] = np.arange(n) % 256, -(np.arange(n) % 256.0), 1.0
+    x[3, 40:] = -np.inf
+    x[4, :-40] = -np.inf
+    x[5, 256:320] += 9
+    x[6, :7], x[6, -7:] = 9, 9
+    x[7] = np.arange(n)[::-1] // 64
+    x[8, 1:] = np.float32(-60000)
+    x[9, 2048:4096] = -np.inf
+    a = CudaArray.fromNumpy(x, dtype)
+    check(a, a.toNumpy().astype(np.float64), rng.integers(-1, n, rows), top, dtype)
+
+
+def test_more_rows_than_one_launch_counts():
+    rows, n = (1 << 22) + 3, 3
+    x = np.random.default_rng(1).integers(-3, 4, (rows, n)).astype(np.float32)
+    tokens = (np.arange(rows) % n).astype(np.int32)
+    a = CudaArray.fromNumpy(x).requiresGrad()
+    got = a.logProbs(CudaArray.fromNumpy(tokens), top=1)
+    (got["logProbs"] + got["topLogProbs"].reshape([rows])).sum().backward()
+    r = reference(x.astype(np.float64), tokens)
+    near(got["logProbs"], r["logProbs"], "logProbs")
+    best = listed(x, 1)
+    assert np.array_equal(got["topTokens"].toNumpy(), best)
+    want = -2 * r["p"]
+    want[np.arange(rows), tokens] += 1
+    want[np.arange(rows), best[:, 0]] += 1
+    # as for the view above, for two upstream gradients
+    near(a.grad(), (want, r["p"] * (4 * r["lp"][1] + 32 * U) + 8 * U * (np.abs(want) + 1)), "dx")
