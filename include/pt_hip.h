@@ -337,17 +337,20 @@ typedef struct {
 
 /* out: contiguous, q's shape; lse (may be NULL): float32, the log of each
  * row's sum of exponentials, [sequences][heads][queries], or
- * [heads][q_rows] where q has starts.  Rows of no sequence are left as they
- * were. */
+ * [heads][q_rows] where q has starts; rest (may be NULL; 16 bits only): like
+ * out, what the rounding to the dtype took from it, for the backward call.
+ * Rows of no sequence are left as they were.  Results must not overlap
+ * operands, here and in the backward call. */
 pt_status pt_attention(const pt_attention_desc *desc, const void *q, const void *k, const void *v, void *out,
-                       float *lse, pt_stream_t stream);
+                       float *lse, void *rest, pt_stream_t stream);
 /* Gradients of the operands' dtype, contiguous, of q's and k's shapes, for
  * the upstream gradient `grad` (contiguous like out, float32 or the operands'
- * dtype); out and lse are the forward call's.  Rows of no sequence are left
+ * dtype); out, lse and rest are the forward call's (rest NULL: the row sums of
+ * grad out are then those of the rounded out).  Rows of no sequence are left
  * as they were.  Results do not depend on timing. */
 pt_status pt_attention_backward(const pt_attention_desc *desc, const void *q, const void *k, const void *v,
-                                const void *out, const float *lse, const void *grad, int grad_dtype, void *dq,
-                                void *dk, void *dv, pt_stream_t stream);
+                                const void *out, const float *lse, const void *rest, const void *grad,
+                                int grad_dtype, void *dq, void *dk, void *dv, pt_stream_t stream);
 
 /* ------------------------------------------------------------------ GEMM --
  * Replaces cuda_matmul_launcher (src/backends/cuda/matmul_kernels.h:40-44),

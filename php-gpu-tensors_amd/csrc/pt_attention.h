@@ -32,7 +32,7 @@ namespace pt {
 
 struct AttnArgs {
     const void *q, *k, *v;
-    void *out;
+    void *out, *rest;
     float *lse;
     // strides in elements: sequence (0 where starts are given), token, head
     long long q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, o_bs, o_ts, o_hs;
@@ -46,7 +46,7 @@ struct AttnArgs {
     long long part_step;      // backward: parts of dk or dq in part_o, of dv in part_ml, this many elements apart
     // backward
     const void *w;            // upstream gradient in the element type, contiguous like out
-    const float *lse2, *delta;  // per (head, token row): lse in base 2 (+inf where nothing is seen), d
+    float *lse2, *delta;      // per (head, token row): lse in base 2 (+inf where nothing is seen), d
     void *dq, *dk, *dv;
     long long stat_rows;      // token rows of a head in lse, lse2 and delta
 };
@@ -280,6 +280,25 @@ __device__ __forceinline__ void attn_row(typename AttnT<DT>::Frag (&f)[DP * Attn
         }
         f[t] = __builtin_bit_cast(typename T::Frag, raw);
     }
+}
+
+// The other half's value of the same column.
+__device__ __forceinline__ float attn_other(float v, int lane)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(lane < 32 ? r[1] : r[0]);
+}
+
+// acc + a . b
+template <int DT>
+__device__ __forceinline__ float attn_dot(const typename AttnT<DT>::Frag &a, const typename AttnT<DT>::Frag &b, float acc)
+{
+    using S = typename AttnT<DT>::S;
+    struct E { S s[AttnT<DT>::PK]; };
+    const E x = __builtin_bit_cast(E, a), y = __builtin_bit_cast(E, b);
+#pragma unroll
+    for (int e = 0; e < AttnT<DT>::PK; e++) acc = fmaf(DType<DT>::to_c(x.s[e]), DType<DT>::to_c(y.s[e]), acc);
+    return acc;
 }
 
 template <int DT>
@@ -517,13 +536,6 @@ __device__ __forceinline__ void attn_landed()
     ring_barrier();
 }
 
-// The other half's value of the same column.
-__device__ __forceinline__ float attn_other(float v, int lane)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(lane < 32 ? r[1] : r[0]);
-}
-
 // Four consecutive elements of a contiguous row from e on, where e + 4 may
 // pass the head's size; ALIGNED: the size is a multiple of four.
 template <int DT>
@@ -547,6 +559,42 @@ __device__ __forceinline__ void attn_store4(void *row, int e, int size, float a,
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (e + i < size) store_c<DT>(p, (size_t)i, v[i]);
+}
+
+// A block's column in its contiguous row: register r holds element first +
+// 8 (r / 4) + 4 half + r % 4, value(r) of it.  16 bits: the two lanes of a
+// column change pieces so that each stores whole packs, half the stores and
+// twice the bytes a row in each (all lanes that share a row come here).
+template <int DT, typename F>
+__device__ __forceinline__ void attn_store_block(void *row, int first, int size, int half, F &&value)
+{
+    if constexpr (DT != PT_FLOAT32) {
+        typedef unsigned int u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+        if ((size & 7) == 0) {
+            auto two = [&](int r) {
+                const float x = value(r), y = value(r + 1);
+                return DT == PT_BFLOAT16 ? (uint32_t)float_to_bf16(x) | (uint32_t)float_to_bf16(y) << 16
+                                         : (uint32_t)float_to_f16(x) | (uint32_t)float_to_f16(y) << 16;
+            };
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const auto a = __builtin_amdgcn_permlane32_swap(two(4 * e), two(4 * e + 4), false, false);
+                const auto b = __builtin_amdgcn_permlane32_swap(two(4 * e + 2), two(4 * e + 6), false, false);
+                const int at = first + 8 * (e + half);
+                if (at < size) *(u32x4 *)((typename AttnT<DT>::S *)row + at) = u32x4{a[0], b[0], a[1], b[1]};
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        attn_store4<DT>(row, first + 8 * e + 4 * half, size, value(4 * e), value(4 * e + 1), value(4 * e + 2), value(4 * e + 3));
+}
+
+// What a rounding to the element type takes from x.
+template <int DT> __device__ __forceinline__ float attn_rest(float x)
+{
+    return x - (DT == PT_BFLOAT16 ? bf16_to_float(float_to_bf16(x)) : f16_to_float(float_to_f16(x)));
 }
 
 // LDS bytes of a tile.
@@ -608,13 +656,16 @@ __device__ __forceinline__ void attn_result(const AttnArgs &g, float m, float l,
         return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    typename AttnT<DT>::S *to = (typename AttnT<DT>::S *)g.out + b * g.o_bs + token * g.o_ts + hq * g.o_hs;
+    const long long to = b * g.o_bs + token * g.o_ts + hq * g.o_hs;
 #pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            attn_store4<DT>(to, d * 32 + 8 * e + 4 * half, g.size, o[d][4 * e] * inv, o[d][4 * e + 1] * inv,
-                            o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv);
+    for (int d = 0; d < ND; d++) {
+        attn_store_block<DT>((typename AttnT<DT>::S *)g.out + to, d * 32, g.size, half, [&](int r) { return o[d][r] * inv; });
+        if constexpr (DT != PT_FLOAT32) {
+            if (g.rest)
+                attn_store_block<DT>((typename AttnT<DT>::S *)g.rest + to, d * 32, g.size, half,
+                                     [&](int r) { return attn_rest<DT>(o[d][r] * inv); });
+        }
+    }
     if (g.lse && half == 0)
         g.lse[(g.q_starts ? 0 : (long long)b * g.heads * g.nq) + (long long)hq * g.stat_rows + (g.q_starts ? token : qi)] =
             l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
@@ -1123,25 +1174,20 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::KWGS)) void k_attention
     // gradients are contiguous, and so is each share's part of them
     const long long to = ((g.k_starts ? sk.row + key : (long long)b * g.nk + key) * g.kv_heads + hk) * g.size;
 #pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int at = d * 32 + 8 * e + 4 * half;
-            auto put = [&](void *whole, float *part, const floatx16 &x, float c) {
-                if (g.splits > 1)
-                    attn_store4<PT_FLOAT32>(part + blockIdx.y * g.part_step + to, at, g.size, x[4 * e] * c, x[4 * e + 1] * c,
-                                            x[4 * e + 2] * c, x[4 * e + 3] * c);
-                else
-                    attn_store4<DT>((S *)whole + to, at, g.size, x[4 * e] * c, x[4 * e + 1] * c, x[4 * e + 2] * c,
-                                    x[4 * e + 3] * c);
-            };
-            if constexpr (kV) put(g.dv, g.part_ml, dv[d], 1.0f);
-            if constexpr (kK) put(g.dk, g.part_o, dk[d], g.scale);
-        }
+    for (int d = 0; d < ND; d++) {
+        auto put = [&](void *whole, float *part, const floatx16 &x, float c) {
+            auto value = [&](int r) { return x[r] * c; };
+            if (g.splits > 1) attn_store_block<PT_FLOAT32>(part + blockIdx.y * g.part_step + to, d * 32, g.size, half, value);
+            else attn_store_block<DT>((S *)whole + to, d * 32, g.size, half, value);
+        };
+        if constexpr (kV) put(g.dv, g.part_ml, dv[d], 1.0f);
+        if constexpr (kK) put(g.dk, g.part_o, dk[d], g.scale);
+    }
 }
 
 // ------------------------------------------------- gradient of the queries
-// Rows as in the forward pass; the keys and values stream past them.
+// Rows as in the forward pass; the keys and values stream past them.  This
+// pass runs first and leaves lse2 and d for the other: it holds w anyway.
 template <int DT, int DP, bool VEC>
 __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::QWGS)) void k_attention_dq(AttnArgs g)
 {
@@ -1165,7 +1211,30 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::QWGS)) void k_attention
     attn_row<DT, DP, VEC>(q, (const S *)g.q + b * g.q_bs + (sq.row + qi) * g.q_ts + hq * g.q_hs, live, g.size, half);
     attn_row<DT, DP, VEC>(w, (const S *)g.w + b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs, live, g.size, half);
     const long long stat = (g.q_starts ? sq.row : (long long)b * g.heads * g.nq) + (long long)hq * g.stat_rows + qi;
-    const float ls = live ? g.lse2[stat] : INFINITY, es = live ? g.delta[stat] : 0.0f;
+    // d in fp32, of the output as it was before its rounding where that is
+    // known; a row that sees no key gets lse +inf, so its exponentials are 0
+    float es = 0.0f, ls = INFINITY;
+    {
+        typename T::Frag o[KS];
+        const long long from = b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
+        attn_row<DT, DP, VEC>(o, (const S *)g.out + from, live, g.size, half);
+#pragma unroll
+        for (int f = 0; f < KS; f++) es = attn_dot<DT>(w[f], o[f], es);
+        if (DT != PT_FLOAT32 && g.rest) {
+            attn_row<DT, DP, VEC>(o, (const S *)g.rest + from, live, g.size, half);
+#pragma unroll
+            for (int f = 0; f < KS; f++) es = attn_dot<DT>(w[f], o[f], es);
+        }
+        es += attn_other(es, lane);
+        if (live) {
+            const float l = g.lse[stat];
+            if (l != -INFINITY) ls = l * 1.4426950408889634f;
+            if (blockIdx.y == 0 && half == 0) {
+                g.lse2[stat] = ls;
+                g.delta[stat] = es;
+            }
+        }
+    }
 
     const AttnSrc ks = {(const char *)((const S *)g.k + b * g.k_bs + sk.row * g.k_ts + hk * g.k_hs), g.k_ts * T::ES, sk.n};
     const AttnSrc vs = {(const char *)((const S *)g.v + b * g.v_bs + sk.row * g.v_ts + hk * g.v_hs), g.v_ts * T::ES, sk.n};
@@ -1229,18 +1298,11 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::QWGS)) void k_attention
     if (!live) return;
     const long long to = b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
 #pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const floatx16 &x = dq[d];
-            const int at = d * 32 + 8 * e + 4 * half;
-            const float c = g.scale;
-            if (g.splits > 1)
-                attn_store4<PT_FLOAT32>(g.part_o + blockIdx.y * g.part_step + to, at, g.size, x[4 * e] * c, x[4 * e + 1] * c,
-                                        x[4 * e + 2] * c, x[4 * e + 3] * c);
-            else
-                attn_store4<DT>((S *)g.dq + to, at, g.size, x[4 * e] * c, x[4 * e + 1] * c, x[4 * e + 2] * c, x[4 * e + 3] * c);
-        }
+    for (int d = 0; d < ND; d++) {
+        auto value = [&](int r) { return dq[d][r] * g.scale; };
+        if (g.splits > 1) attn_store_block<PT_FLOAT32>(g.part_o + blockIdx.y * g.part_step + to, d * 32, g.size, half, value);
+        else attn_store_block<DT>((S *)g.dq + to, d * 32, g.size, half, value);
+    }
 }
 
 // ------------------------------------------------------------- launches

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
     const uint64_t some = __ballot(l != 0.0f);
     const float weight = __builtin_amdgcn_exp2f(m - ref), sum = wave_all(l * weight, FAdd{});
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    typename AttnT<DT>::S *to = (typename AttnT<DT>::S *)g.out + b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
+    const long long to = b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int s = 0; s < g.splits; s++) {
@@ -48,7 +48,13 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
     }
 #pragma unroll
     for (int k = 0; k < 4; k++)
-        if (k * 64 + lane < g.size) store_c<DT>(to, (size_t)(k * 64 + lane), x[k] * inv);
+        if (k * 64 + lane < g.size) {
+            store_c<DT>((typename AttnT<DT>::S *)g.out + to, (size_t)(k * 64 + lane), x[k] * inv);
+            if constexpr (DT != PT_FLOAT32) {
+                if (g.rest)
+                    store_c<DT>((typename AttnT<DT>::S *)g.rest + to, (size_t)(k * 64 + lane), attn_rest<DT>(x[k] * inv));
+            }
+        }
     if (g.lse && lane == 0)
         g.lse[(g.q_starts ? sq.row : (long long)b * g.heads * g.nq) + (long long)hq * g.stat_rows + qi] =
             sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
@@ -72,57 +78,6 @@ __global__ __launch_bounds__(256) void k_attention_sum(AttnArgs g, bool keys, co
         float x = 0.0f;
         for (int p = 0; p < g.splits; p++) x += part[p * g.part_step + to + d];
         store_c<DT>(out, (size_t)(to + d), x);
-    }
-}
-
-// Per row and head, before the gradients: d = w . o in fp32, lse in base 2,
-// and the upstream gradient in the element type where it came in float32
-// (the products take 16-bit operands).  A row that sees no key gets lse +inf,
-// so its exponentials are 0.  16 lanes a row, V elements at a time (V > 1:
-// rows start on 16 bytes and hold whole packs); HBM-bound, one read of w and o.
-template <int DT, bool W32, int V>
-__global__ __launch_bounds__(256) void k_attention_prepare(const void *w, const void *out, const float *lse,
-                                                           uint16_t *w16, float *lse2, float *delta, long long rows,
-                                                           int heads, int size, int queries, bool packed)
-{
-    using S = typename AttnT<DT>::S;
-    typedef S __attribute__((ext_vector_type(V))) SV;
-    typedef uint16_t __attribute__((ext_vector_type(V))) HV;
-    typedef float __attribute__((ext_vector_type(V))) FV;
-    const int lane = threadIdx.x & 15;
-    for (long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); at < rows * heads; at += (long long)gridDim.x * 16) {
-        float x = 0.0f;
-        for (int d = lane * V; d < size; d += 16 * V) {
-            const long long e = at * size + d;
-            const SV o = *(const SV *)((const S *)out + e);
-            if constexpr (W32) {
-                const FV f = *(const FV *)((const float *)w + e);
-                HV h;
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    float wv = f[i];
-                    if constexpr (DT != PT_FLOAT32) {
-                        h[i] = DT == PT_BFLOAT16 ? float_to_bf16(wv) : float_to_f16(wv);
-                        wv = DT == PT_BFLOAT16 ? bf16_to_float(h[i]) : f16_to_float(h[i]);
-                    }
-                    x = fmaf(wv, DType<DT>::to_c(o[i]), x);
-                }
-                if constexpr (DT != PT_FLOAT32) *(HV *)(w16 + e) = h;
-            } else {
-                const SV f = *(const SV *)((const S *)w + e);
-#pragma unroll
-                for (int i = 0; i < V; i++) x = fmaf(DType<DT>::to_c(f[i]), DType<DT>::to_c(o[i]), x);
-            }
-        }
-#pragma unroll
-        for (int m = 8; m >= 1; m >>= 1) x += __shfl_xor(x, m, 16);
-        if (lane == 0) {
-            const long long row = at / heads, h = at % heads;
-            const long long stat = packed ? h * rows + row : (row / queries * heads + h) * queries + row % queries;
-            const float l = lse[stat];
-            delta[stat] = x;
-            lse2[stat] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
-        }
     }
 }
 
@@ -262,7 +217,7 @@ template <int DT> static pt_status attention_typed(AttnArgs &g, bool vec, hipStr
 }
 
 template <int DT>
-static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, bool w32, const float *lse, hipStream_t s)
+static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, bool w32, hipStream_t s)
 {
     const long long nh = (long long)g.batch * g.kv_heads, rows = (long long)g.nq * g.group;
     const long long q_rows = g.q_starts ? g.q_rows : (long long)g.batch * g.nq, stats = q_rows * g.heads;
@@ -275,7 +230,7 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
     const int k_splits = kb ? backward_splits(std::max(1ll, k_live), ((long long)g.nq + tile - 1) / tile * g.group) : 1;
     const int q_splits = qb ? backward_splits(std::max(1ll, q_live), ((long long)g.nk + tile - 1) / tile) : 1;
     // one region: lse2, delta, the rounded upstream gradient, the shares (of
-    // dk and dv, and after them of dq)
+    // dq, and after them of dk and dv)
     auto whole = [](size_t n) { return (n + 255) & ~(size_t)255; };
     const size_t stat_bytes = whole((size_t)stats * 4), w_bytes = round ? whole((size_t)stats * g.size * 2) : 0;
     const size_t k_part = k_splits > 1 ? whole((size_t)k_splits * k_elems * 4) : 0;
@@ -283,28 +238,29 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
     void *scratch = nullptr;
     PT_TRY(scratch_alloc(&scratch, 2 * stat_bytes + w_bytes + std::max(2 * k_part, q_part), s));
     char *base = (char *)scratch;
-    float *lse2 = (float *)base, *delta = (float *)(base + stat_bytes);
-    uint16_t *w16 = round ? (uint16_t *)(base + 2 * stat_bytes) : nullptr;
+    g.lse2 = (float *)base;
+    g.delta = (float *)(base + stat_bytes);
+    void *w16 = base + 2 * stat_bytes;
     float *part = (float *)(base + 2 * stat_bytes + w_bytes);
     pt_status st = PT_OK;
-    if (stats) {
-        const unsigned n = (unsigned)std::min((stats + 15) / 16, 1ll << 20);
-        const bool packed = g.q_starts != nullptr;
-        const bool packs = g.size % 8 == 0 && !(((uintptr_t)w | (uintptr_t)g.out) & 15);
-        auto go = [&](auto W, auto V) {
-            k_attention_prepare<DT, decltype(W)::value, decltype(V)::value><<<n, 256, 0, s>>>(
-                w, g.out, lse, w16, lse2, delta, q_rows, g.heads, g.size, g.nq, packed);
-        };
-        using P = std::integral_constant<int, AttnT<DT>::PK>;
-        using One = std::integral_constant<int, 1>;
-        if (w32) packs ? go(std::true_type{}, P{}) : go(std::true_type{}, One{});
-        else packs ? go(std::false_type{}, P{}) : go(std::false_type{}, One{});
-        st = check_hip(hipGetLastError(), "attention gradient preparation");
+    if (round && stats) {
+        // the products take 16-bit operands
+        const int shape[4] = {g.q_starts ? 1 : g.batch, g.q_starts ? g.q_rows : g.nq, g.heads, g.size};
+        const size_t strides[4] = {(size_t)g.o_ts * shape[1], (size_t)g.o_ts, (size_t)g.o_hs, 1};
+        st = pt_cast(w, PT_FLOAT32, strides, 0, w16, DT, shape, 4, (pt_stream_t)s);
     }
-    g.w = round ? (const void *)w16 : w;
-    g.lse2 = lse2;
-    g.delta = delta;
-    vec = vec && !((uintptr_t)g.w & 15);
+    g.w = round ? w16 : w;
+    vec = vec && !(((uintptr_t)g.w | (uintptr_t)g.out | (uintptr_t)g.rest) & 15);
+    // the queries' pass leaves lse2 and d to the keys'
+    if (st == PT_OK && qb) {
+        g.splits = q_splits;
+        g.part_step = stats * g.size;
+        g.part_o = part;
+        launch_attention_dq<DT>(g, vec, (unsigned)attention_place(g, qb / nh, (long long)g.q_rows * g.group, g.q_starts), s);
+        if (q_splits > 1)
+            k_attention_sum<DT><<<(unsigned)(((long long)g.batch * g.nq * g.heads + 3) / 4), 256, 0, s>>>(g, false, part, g.dq);
+        st = check_hip(hipGetLastError(), "attention gradient of queries");
+    }
     if (st == PT_OK && kb) {
         g.splits = k_splits;
         g.part_step = k_elems;
@@ -318,15 +274,6 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
         }
         st = check_hip(hipGetLastError(), "attention gradient of keys and values");
     }
-    if (st == PT_OK && qb) {
-        g.splits = q_splits;
-        g.part_step = stats * g.size;
-        g.part_o = part;
-        launch_attention_dq<DT>(g, vec, (unsigned)attention_place(g, qb / nh, (long long)g.q_rows * g.group, g.q_starts), s);
-        if (q_splits > 1)
-            k_attention_sum<DT><<<(unsigned)(((long long)g.batch * g.nq * g.heads + 3) / 4), 256, 0, s>>>(g, false, part, g.dq);
-        st = check_hip(hipGetLastError(), "attention gradient of queries");
-    }
     scratch_free(scratch, s);
     return st;
 }
@@ -338,7 +285,7 @@ using namespace pt;
 extern "C" {
 
 pt_status pt_attention(const pt_attention_desc *desc, const void *q, const void *k, const void *v, void *out, float *lse,
-                       pt_stream_t stream)
+                       void *rest, pt_stream_t stream)
 {
     AttnArgs g;
     bool vec;
@@ -347,6 +294,7 @@ pt_status pt_attention(const pt_attention_desc *desc, const void *q, const void 
     PT_TRY(ensure_init());
     g.out = out;
     g.lse = lse;
+    g.rest = rest;
     hipStream_t s = stream_of(stream);
     switch (desc->dtype) {
     case PT_FLOAT32: return attention_typed<PT_FLOAT32>(g, vec, s);
@@ -356,8 +304,8 @@ pt_status pt_attention(const pt_attention_desc *desc, const void *q, const void 
 }
 
 pt_status pt_attention_backward(const pt_attention_desc *desc, const void *q, const void *k, const void *v,
-                                const void *out, const float *lse, const void *grad, int grad_dtype, void *dq, void *dk,
-                                void *dv, pt_stream_t stream)
+                                const void *out, const float *lse, const void *rest, const void *grad, int grad_dtype,
+                                void *dq, void *dk, void *dv, pt_stream_t stream)
 {
     AttnArgs g;
     bool vec;
@@ -370,15 +318,17 @@ pt_status pt_attention_backward(const pt_attention_desc *desc, const void *q, co
         return fail(PT_ERR_INVALID, "attention backward misses the gradient of keys or values");
     PT_TRY(ensure_init());
     g.out = const_cast<void *>(out);
+    g.rest = const_cast<void *>(rest);
+    g.lse = const_cast<float *>(lse);
     g.dq = dq;
     g.dk = dk;
     g.dv = dv;
     hipStream_t s = stream_of(stream);
     const bool w32 = grad_dtype == PT_FLOAT32;
     switch (desc->dtype) {
-    case PT_FLOAT32: return attention_backward_typed<PT_FLOAT32>(g, vec, grad, w32, lse, s);
-    case PT_FLOAT16: return attention_backward_typed<PT_FLOAT16>(g, vec, grad, w32, lse, s);
-    default: return attention_backward_typed<PT_BFLOAT16>(g, vec, grad, w32, lse, s);
+    case PT_FLOAT32: return attention_backward_typed<PT_FLOAT32>(g, vec, grad, w32, s);
+    case PT_FLOAT16: return attention_backward_typed<PT_FLOAT16>(g, vec, grad, w32, s);
+    default: return attention_backward_typed<PT_BFLOAT16>(g, vec, grad, w32, s);
     }
 }
 

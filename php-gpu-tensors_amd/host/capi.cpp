@@ -332,24 +332,24 @@ phpt_sequences *phpt_sequences_create(const int *lengths, const int *starts, int
 void phpt_sequences_release(phpt_sequences *s) { delete s; }
 
 phpt_tensor *phpt_attention(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, int causal, double scale,
-                            phpt_sequences *queries, phpt_sequences *keys, phpt_tensor **lse)
+                            phpt_sequences *queries, phpt_sequences *keys, phpt_tensor **kept)
 {
     clear_error();
-    TensorP out[2];
+    TensorP out[3];
     if (!cuda_array_attention(q->t, k->t, v->t, causal != 0, scale, sequences_of(queries), sequences_of(keys),
-                              lse != nullptr, out))
+                              kept != nullptr, out))
         return nullptr;
-    if (lse) *lse = wrap(out[1]);
+    for (int i = 0; kept && i < 2; i++) kept[i] = wrap(out[1 + i]);
     return wrap(out[0]);
 }
 
 int phpt_attention_backward(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, phpt_tensor *out, phpt_tensor *lse,
-                            phpt_tensor *grad, int causal, double scale, phpt_sequences *queries,
+                            phpt_tensor *rest, phpt_tensor *grad, int causal, double scale, phpt_sequences *queries,
                             phpt_sequences *keys, phpt_tensor **results)
 {
     clear_error();
     TensorP got[3];
-    if (!cuda_array_attention_backward(q->t, k->t, v->t, out->t, lse->t, grad->t, causal != 0, scale,
+    if (!cuda_array_attention_backward(q->t, k->t, v->t, out->t, lse->t, rest ? rest->t : nullptr, grad->t, causal != 0, scale,
                                        sequences_of(queries), sequences_of(keys), got))
         return -1;
     for (int i = 0; i < 3; i++) results[i] = wrap(got[i]);

@@ -187,7 +187,8 @@ static int lse_shape(const Tensor &q, int *shape)
 }
 
 static bool attention_run(const TensorP &q, const TensorP &k, const TensorP &v, bool causal, double scale,
-                          const SequencesP &qs, const SequencesP &ks, const TensorP &out, const TensorP &lse)
+                          const SequencesP &qs, const SequencesP &ks, const TensorP &out, const TensorP &lse,
+                          const TensorP &rest)
 {
     pt_attention_desc d;
     if (!attention_desc(q, k, v, causal, scale, qs, ks, d)) return false;
@@ -196,18 +197,19 @@ static bool attention_run(const TensorP &q, const TensorP &k, const TensorP &v, 
     // rows of no sequence are zeros
     if (qs && !qs->cover(q->shape[0]) && !clear(out)) return false;
     return check_status(pt_attention(&d, a->data(), b->data(), c->data(), out->data(), lse ? (float *)lse->data() : nullptr,
-                                     nullptr),
+                                     rest ? rest->data() : nullptr, nullptr),
                         "Attention kernel failed");
 }
 
 bool cuda_array_attention(const TensorP &q, const TensorP &k, const TensorP &v, bool causal, double scale,
-                          const SequencesP &qs, const SequencesP &ks, bool want_lse, TensorP out[2])
+                          const SequencesP &qs, const SequencesP &ks, bool keep, TensorP out[3])
 {
     pt_attention_desc d;
     if (!attention_desc(q, k, v, causal, scale, qs, ks, d)) return false;
     int ls[kMaxDims];
     const int ln = lse_shape(*q, ls);
-    out[1] = nullptr;
+    out[1] = out[2] = nullptr;
+    const bool rest = keep && q->dtype != PT_FLOAT32;
     if (fusion_active()) {
         NativeSpec sp;
         sp.kind = NAT_ATTENTION;
@@ -215,22 +217,25 @@ bool cuda_array_attention(const TensorP &q, const TensorP &k, const TensorP &v, 
         sp.eps = scale;
         sp.q_seq = qs;
         sp.k_seq = ks;
-        sp.has_lse = want_lse;
         std::vector<TensorP> ins = {q, k, v};
-        TensorP box = want_lse ? record_buffer(ls, ln, PT_FLOAT32) : nullptr;
-        if (want_lse && !box) return false;
-        if (box) ins.push_back(box);
+        for (int i = 0; i < keep + rest; i++) {
+            ins.push_back(i ? record_buffer(q->shape, q->ndims, q->dtype) : record_buffer(ls, ln, PT_FLOAT32));
+            if (!ins.back()) return false;
+        }
         out[0] = fusion_record_native(sp, ins, q->shape, q->ndims, q->dtype);
-        if (out[0] && box) out[1] = record_result(box, out[0]);
-        return out[0] && (!box || out[1]);
+        for (int i = 0; out[0] && i < keep + rest; i++)
+            if (!(out[1 + i] = record_result(ins[3 + i], out[0]))) return false;
+        return out[0] != nullptr;
     }
     if (!guard(q) || !guard(k) || !guard(v)) return false;
     out[0] = output_tensor(q->shape, q->ndims, q->dtype);
-    if (out[0] && want_lse) out[1] = make_empty(ls, ln, PT_FLOAT32);
-    if (!out[0] || (want_lse && !out[1])) return false;
-    return attention_run(q, k, v, causal, scale, qs, ks, out[0], out[1]);
+    if (out[0] && keep) out[1] = make_empty(ls, ln, PT_FLOAT32);
+    if (out[0] && rest) out[2] = make_empty(q->shape, q->ndims, q->dtype);
+    if (!out[0] || (keep && !out[1]) || (rest && !out[2])) return false;
+    return attention_run(q, k, v, causal, scale, qs, ks, out[0], out[1], out[2]);
 }
 
+// in: q, k, v, the output, lse, the upstream gradient, rest (or null)
 static bool attention_backward_run(const TensorP *in, bool causal, double scale, const SequencesP &qs, const SequencesP &ks,
                                    const TensorP *out)
 {
@@ -239,17 +244,18 @@ static bool attention_backward_run(const TensorP *in, bool causal, double scale,
     if (!attention_desc(q, k, v, causal, scale, qs, ks, d)) return false;
     TensorP a = attention_operand(q, d.q_strides), b = attention_operand(k, d.k_strides), c = attention_operand(v, d.v_strides);
     TensorP o = materialize(in[3]), lse = materialize(in[4]), g = materialize(in[5]);
-    if (!a || !b || !c || !o || !lse || !g) return false;
+    TensorP rest = in[6] ? materialize(in[6]) : nullptr;
+    if (!a || !b || !c || !o || !lse || !g || (in[6] && !rest)) return false;
     if (qs && !qs->cover(q->shape[0]) && !clear(out[0])) return false;
     if (ks && !ks->cover(k->shape[0]) && (!clear(out[1]) || !clear(out[2]))) return false;
     return check_status(pt_attention_backward(&d, a->data(), b->data(), c->data(), o->data(), (const float *)lse->data(),
-                                              g->data(), g->dtype, out[0]->data(), out[1]->data(), out[2]->data(), nullptr),
+                                              rest ? rest->data() : nullptr, g->data(), g->dtype, out[0]->data(), out[1]->data(), out[2]->data(), nullptr),
                         "Attention gradient kernel failed");
 }
 
 bool cuda_array_attention_backward(const TensorP &q, const TensorP &k, const TensorP &v, const TensorP &o,
-                                   const TensorP &lse, const TensorP &grad, bool causal, double scale,
-                                   const SequencesP &qs, const SequencesP &ks, TensorP out[3])
+                                   const TensorP &lse, const TensorP &rest, const TensorP &grad, bool causal,
+                                   double scale, const SequencesP &qs, const SequencesP &ks, TensorP out[3])
 {
     pt_attention_desc d;
     if (!attention_desc(q, k, v, causal, scale, qs, ks, d)) return false;
@@ -260,7 +266,8 @@ bool cuda_array_attention_backward(const TensorP &q, const TensorP &k, const Ten
     int ls[kMaxDims];
     const int ln = lse_shape(*q, ls);
     if (!o || !lse || !grad || !same_shape(*o, *q) || o->dtype != q->dtype || lse->dtype != PT_FLOAT32 || lse->ndims != ln ||
-        !std::equal(ls, ls + ln, lse->shape)) {
+        !std::equal(ls, ls + ln, lse->shape) ||
+        (rest && (q->dtype == PT_FLOAT32 || !same_shape(*rest, *q) || rest->dtype != q->dtype))) {
         set_invalid("attention gradients need the forward pass's results");
         return false;
     }
@@ -277,15 +284,17 @@ bool cuda_array_attention_backward(const TensorP &q, const TensorP &k, const Ten
         sp.k_seq = ks;
         TensorP dk = record_buffer(k->shape, k->ndims, k->dtype), dv = dk ? record_buffer(v->shape, v->ndims, v->dtype) : nullptr;
         if (!dv) return false;
-        out[0] = fusion_record_native(sp, {q, k, v, o, lse, grad, dk, dv}, q->shape, q->ndims, q->dtype);
+        std::vector<TensorP> ins = {q, k, v, o, lse, grad, dk, dv};
+        if (rest) ins.push_back(rest);
+        out[0] = fusion_record_native(sp, ins, q->shape, q->ndims, q->dtype);
         if (!out[0]) return false;
         out[1] = record_result(dk, out[0]);
         out[2] = record_result(dv, out[0]);
         return out[1] && out[2];
     }
-    const TensorP in[6] = {q, k, v, o, lse, grad};
+    const TensorP in[7] = {q, k, v, o, lse, grad, rest};
     for (const TensorP &t : in)
-        if (!guard(t)) return false;
+        if (t && !guard(t)) return false;
     out[0] = output_tensor(q->shape, q->ndims, q->dtype);
     out[1] = make_empty(k->shape, k->ndims, k->dtype);
     out[2] = make_empty(v->shape, v->ndims, v->dtype);
@@ -603,12 +612,13 @@ TensorP native_execute_model(const NativeSpec &sp, const std::vector<TensorP> &i
     case NAT_ATTENTION:
         out = output_tensor(in[0]->shape, in[0]->ndims, in[0]->dtype);
         ok = out && attention_run(in[0], in[1], in[2], sp.causal, sp.eps, sp.q_seq, sp.k_seq, out,
-                                  sp.has_lse ? in[3] : nullptr);
+                                  in.size() > 3 ? in[3] : nullptr, in.size() > 4 ? in[4] : nullptr);
         break;
     case NAT_ATTENTION_BACKWARD: {
         const TensorP to[3] = {output_tensor(in[0]->shape, in[0]->ndims, in[0]->dtype), in[6], in[7]};
         out = to[0];
-        ok = out && attention_backward_run(in.data(), sp.causal, sp.eps, sp.q_seq, sp.k_seq, to);
+        const TensorP ops[7] = {in[0], in[1], in[2], in[3], in[4], in[5], in.size() > 8 ? in[8] : nullptr};
+        ok = out && attention_backward_run(ops, sp.causal, sp.eps, sp.q_seq, sp.k_seq, to);
         break;
     }
     case NAT_LAYERNORM_BACKWARD: {

@@ -96,13 +96,13 @@ void phpt_sequences_release(phpt_sequences *s);
 /* pt_attention over q, k, v [tokens, heads, size] or [sequences, tokens,
  * heads, size] (any strides); the first form with sequences of both sides or
  * with neither.  scale 0: 1 / sqrt(size).  Returns the output, of q's shape
- * and dtype, zeros in rows of no sequence; lse, where not NULL, gets what the
- * gradient call takes. */
+ * and dtype, zeros in rows of no sequence; kept[2], where not NULL, gets the
+ * lse and the rest (NULL for float32) that the gradient call takes. */
 phpt_tensor *phpt_attention(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, int causal, double scale,
-                            phpt_sequences *queries, phpt_sequences *keys, phpt_tensor **lse);
+                            phpt_sequences *queries, phpt_sequences *keys, phpt_tensor **kept);
 /* results[3]: gradients of q, k and v */
 int phpt_attention_backward(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, phpt_tensor *out, phpt_tensor *lse,
-                            phpt_tensor *grad, int causal, double scale, phpt_sequences *queries,
+                            phpt_tensor *rest, phpt_tensor *grad, int causal, double scale, phpt_sequences *queries,
                             phpt_sequences *keys, phpt_tensor **results);
 /* pt_logprobs of the rows along a's last axis, tokens int32 of the rows'
  * shape: results[5] gets the log probability, the entropy, stats, and for

@@ -169,12 +169,13 @@ using SequencesP = std::shared_ptr<Sequences>;
 SequencesP make_sequences(const int *lengths, const int *starts, int count);  // starts null: one behind the other
 
 // Operators with several results: `out` gets one tensor per result (null
-// where it is not wanted).  lse is kept for the gradient.
+// where it is not wanted).  lse and, for 16-bit operands, rest are kept for
+// the gradient.
 bool cuda_array_attention(const TensorP &q, const TensorP &k, const TensorP &v, bool causal, double scale,
-                          const SequencesP &qs, const SequencesP &ks, bool want_lse, TensorP out[2]);
+                          const SequencesP &qs, const SequencesP &ks, bool keep, TensorP out[3]);
 bool cuda_array_attention_backward(const TensorP &q, const TensorP &k, const TensorP &v, const TensorP &o,
-                                   const TensorP &lse, const TensorP &grad, bool causal, double scale,
-                                   const SequencesP &qs, const SequencesP &ks, TensorP out[3]);
+                                   const TensorP &lse, const TensorP &rest, const TensorP &grad, bool causal,
+                                   double scale, const SequencesP &qs, const SequencesP &ks, TensorP out[3]);
 // gradients of the input, the scale and the bias; scale and bias may be null
 bool cuda_array_layernorm_backward(const TensorP &a, const TensorP &grad, const int *axes, int naxes, double eps,
                                    const TensorP &scale, const TensorP &bias, TensorP out[3]);
@@ -222,7 +223,7 @@ struct NativeSpec {
     int naxes = 0;
     int axes[kMaxDims] = {0};
     bool has_scale = false, has_bias = false;
-    bool causal = false, has_lse = false;
+    bool causal = false;
     int top = 0, given = 0;  // given: which optional operands follow (a bit each)
     SequencesP q_seq, k_seq;
 };

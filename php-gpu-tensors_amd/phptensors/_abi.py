@@ -131,8 +131,8 @@ SIGNATURES = {
                                    ctypes.c_int, vp, vp, vp, vp, vp, vp]),
     "pt_logprobs_backward": (ctypes.c_int, [vp, ctypes.c_int, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, vp,
                                             ctypes.c_int, vp, vp, vp, vp, vp, vp, vp, vp]),
-    "pt_attention": (ctypes.c_int, [ctypes.POINTER(PtAttentionDesc), vp, vp, vp, vp, vp, vp]),
-    "pt_attention_backward": (ctypes.c_int, [ctypes.POINTER(PtAttentionDesc), vp, vp, vp, vp, vp, vp, ctypes.c_int,
+    "pt_attention": (ctypes.c_int, [ctypes.POINTER(PtAttentionDesc), vp, vp, vp, vp, vp, vp, vp]),
+    "pt_attention_backward": (ctypes.c_int, [ctypes.POINTER(PtAttentionDesc), vp, vp, vp, vp, vp, vp, vp, ctypes.c_int,
                                              vp, vp, vp, vp]),
     "pt_matmul": (ctypes.c_int, [vp, vp, vp, ctypes.c_int, c_int_p, c_size_p, ctypes.c_int,
                                  c_int_p, c_size_p, ctypes.c_int, c_int_p, ctypes.c_int, vp]),

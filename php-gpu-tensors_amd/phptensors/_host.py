@@ -48,7 +48,7 @@ SIGNATURES = {
     "phpt_sequences_create": (vp, [ip, ip, ctypes.c_int]),
     "phpt_sequences_release": (None, [vp]),
     "phpt_attention": (T, [T, T, T, ctypes.c_int, ctypes.c_double, vp, vp, ctypes.POINTER(T)]),
-    "phpt_attention_backward": (ctypes.c_int, [T, T, T, T, T, T, ctypes.c_int, ctypes.c_double, vp, vp,
+    "phpt_attention_backward": (ctypes.c_int, [T, T, T, T, T, T, T, ctypes.c_int, ctypes.c_double, vp, vp,
                                                ctypes.POINTER(T)]),
     "phpt_logprobs": (ctypes.c_int, [T, T, ctypes.c_int, ctypes.POINTER(T)]),
     "phpt_logprobs_backward": (T, [T] * 8),

@@ -581,16 +581,18 @@ class CudaArray:
         c = 0.0 if scale is None else float(scale)
         at = [s._h if s is not None else None for s in (queries, keys)]
         active = AG.active(self, key, value)
-        lse_h = ctypes.c_void_p()
+        kept = (ctypes.c_void_p * 2)()
         out = CudaArray._wrap(lib.phpt_attention(self._h, key._h, value._h, int(bool(causal)), c, *at,
-                                                 ctypes.byref(lse_h) if active else None), "attention")
+                                                 kept if active else None), "attention")
         if active:
-            lse, result = CudaArray._wrap(lse_h.value), out.detach()
+            result = out.detach()
+            lse, rest = [CudaArray._wrap(h) if h else None for h in kept]
 
             def back(g):
                 got = (ctypes.c_void_p * 3)()
                 held = (queries, keys)  # the handles behind `at`
-                if lib.phpt_attention_backward(self._h, key._h, value._h, result._h, lse._h, g._h, int(bool(causal)), c,
+                if lib.phpt_attention_backward(self._h, key._h, value._h, result._h, lse._h,
+                                               rest._h if rest is not None else None, g._h, int(bool(causal)), c,
                                                *(s._h if s is not None else None for s in held), got):
                     _host.raise_error("attention gradient")
                 return [CudaArray._wrap(h) for h in got]

@@ -185,7 +185,7 @@ def test_captured_graphs_share_a_workspace():
     heads, kv, size, slot, count = 4, 2, 64, 3000, 2
     f = lambda *s: rng.standard_normal(s).astype(np.float16)
     b = Buffers(q=f(count, heads, size), k=f(count * slot, kv, size), v=f(count * slot, kv, size), w=f(count, heads, size),
-                out=f(count, heads, size), lse=np.zeros((heads, count), np.float32), dq=f(count, heads, size),
+                out=f(count, heads, size), lse=np.zeros((heads, count), np.float32), dq=f(count, heads, size), rest=f(count, heads, size),
                 dk=f(count * slot, kv, size), dv=f(count * slot, kv, size),
                 qs=np.arange(count, dtype=np.int32), qn=np.ones(count, np.int32),
                 ks=(np.arange(count) * slot).astype(np.int32), kn=np.array([slot, 1700], np.int32),
@@ -203,15 +203,15 @@ def test_captured_graphs_share_a_workspace():
         setattr(d, n, x)
 
     def attend(stream):
-        _abi.check(lib.pt_attention(ctypes.byref(d), b.q, b.k, b.v, b.out, b.lse, stream))
-        _abi.check(lib.pt_attention_backward(ctypes.byref(d), b.q, b.k, b.v, b.out, b.lse, b.w, _abi.FLOAT16, b.dq, b.dk,
+        _abi.check(lib.pt_attention(ctypes.byref(d), b.q, b.k, b.v, b.out, b.lse, b.rest, stream))
+        _abi.check(lib.pt_attention_backward(ctypes.byref(d), b.q, b.k, b.v, b.out, b.lse, b.rest, b.w, _abi.FLOAT16, b.dq, b.dk,
                                              b.dv, stream))
 
     def score(stream):
         _abi.check(lib.pt_logprobs(b.x, _abi.FLOAT32, 3, 40000, 40000, b.tokens, 8, b.lp, b.ent, b.stats, b.tv, b.ti, stream))
         _abi.check(lib.pt_logprobs_backward(b.x, _abi.FLOAT32, 3, 40000, 40000, b.tokens, 8, b.ti, b.stats, b.ent, b.g, b.g,
                                             b.gt, b.dx, stream))
-    results = {attend: ("out", "lse", "dq", "dk", "dv"), score: ("lp", "ent", "stats", "tv", "ti", "dx")}
+    results = {attend: ("out", "lse", "rest", "dq", "dk", "dv"), score: ("lp", "ent", "stats", "tv", "ti", "dx")}
 
     def eager(call):
         b.blank(*results[call])
@@ -262,7 +262,7 @@ def test_captured_graphs_share_a_workspace():
         replay()
     # a workspace too small is refused, nothing written past it
     _abi.check(lib.pt_workspace_begin(space.ptr, 256))
-    assert lib.pt_attention(ctypes.byref(d), b.q, b.k, b.v, b.out, b.lse, None) != _abi.PT_OK
+    assert lib.pt_attention(ctypes.byref(d), b.q, b.k, b.v, b.out, b.lse, b.rest, None) != _abi.PT_OK
     _abi.check(lib.pt_workspace_end(None))
     for g in graphs.values():
         _abi.check(lib.pt_graph_destroy(g))

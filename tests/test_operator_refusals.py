@@ -34,22 +34,22 @@ BAD = [dict(dtype=_abi.FLOAT64), dict(dtype=_abi.INT32), dict(sequences=-1), dic
 @pytest.mark.parametrize("change", BAD, ids=str)
 def test_attention_descriptions(change):
     d = ctypes.byref(desc(**change))
-    refused(LIB.pt_attention(d, P, P, P, P, P, None))
-    refused(LIB.pt_attention_backward(d, P, P, P, P, P, P, _abi.BFLOAT16, P, P, P, None))
+    refused(LIB.pt_attention(d, P, P, P, P, P, P, None))
+    refused(LIB.pt_attention_backward(d, P, P, P, P, P, P, P, _abi.BFLOAT16, P, P, P, None))
 
 
 def test_attention_operands():
     d = ctypes.byref(desc())
-    refused(LIB.pt_attention(None, P, P, P, P, P, None))
-    refused(LIB.pt_attention(ctypes.byref(desc(head_size=257)), P, P, P, P, P, None), _abi.PT_ERR_UNSUPPORTED)
+    refused(LIB.pt_attention(None, P, P, P, P, P, P, None))
+    refused(LIB.pt_attention(ctypes.byref(desc(head_size=257)), P, P, P, P, P, None, None), _abi.PT_ERR_UNSUPPORTED)
     for missing in range(4):
         args = [None if i == missing else P for i in range(4)]
-        refused(LIB.pt_attention(d, *args, None, None))
+        refused(LIB.pt_attention(d, *args, None, None, None))
     for missing in range(9):  # q, k, v, out, lse, grad, dq, dk, dv
         a = [None if i == missing else P for i in range(9)]
-        refused(LIB.pt_attention_backward(d, *a[:6], _abi.BFLOAT16, *a[6:], None))
-    refused(LIB.pt_attention_backward(d, P, P, P, P, P, P, _abi.FLOAT16, P, P, P, None))
-    refused(LIB.pt_attention_backward(d, P, P, P, P, P, P, _abi.FLOAT64, P, P, P, None))
+        refused(LIB.pt_attention_backward(d, *a[:5], None, a[5], _abi.BFLOAT16, *a[6:], None))
+    refused(LIB.pt_attention_backward(d, P, P, P, P, P, None, P, _abi.FLOAT16, P, P, P, None))
+    refused(LIB.pt_attention_backward(d, P, P, P, P, P, None, P, _abi.FLOAT64, P, P, P, None))
 
 
 def test_layernorm_gradients():
