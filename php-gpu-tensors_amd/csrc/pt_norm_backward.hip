@@ -63,17 +63,17 @@ struct NormBwdArgs {
 };
 
 // fp32 statistics, rows of up to 64 * WPR * V * NCH elements, WPR waves a
-// row and 8 / WPR rows at a time in a block of 8 waves.  V is 8 elements: one
+// row and 8 / WPR rows at a time in a block of 8 waves (WPR 16: of 16).  V is 8 elements: one
 // 16-byte load of x in 16 bits, two in 32.  A row that ends inside a chunk
 // reads its last chunk V elements before the end; the elements that another
 // lane owns count for nothing in the sums and get the same dx twice.
 template <int DT, int PDT, int NCH, int WPR>
-__global__ __launch_bounds__(512) void k_norm_backward(NormBwdArgs a)
+__global__ __launch_bounds__(64 * (WPR > 8 ? WPR : 8)) void k_norm_backward(NormBwdArgs a)
 {
     using S = typename DType<DT>::S;
     using PS = typename DType<PDT>::S;
-    constexpr int V = 8, RPB = 8 / WPR, TPR = 64 * WPR;
-    __shared__ float lds[2][8][3];
+    constexpr int V = 8, W = WPR > 8 ? WPR : 8, RPB = W / WPR, TPR = 64 * WPR;
+    __shared__ float lds[2][W][3];
     __shared__ float sums[WPR < 8 ? 2 * TPR * V * NCH : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = threadIdx.x % TPR, first = wave - wave % WPR;
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(NormBwdArgs a)
         q = wave_all(q, FAdd{});
         r = wave_all(r, FAdd{});
         if constexpr (WPR > 1) {
-            float(&box)[8][3] = lds[turn];  // two in turn: one barrier a call keeps reads and writes apart
+            float(&box)[W][3] = lds[turn];  // two in turn: one barrier a call keeps reads and writes apart
             turn ^= 1;
             if (lane == 0) {
                 box[wave][0] = p;
@@ -175,14 +175,22 @@ __global__ __launch_bounds__(512) void k_norm_backward(NormBwdArgs a)
         }
     };
     // rows blockIdx.x * RPB + wave / WPR and so on; the next row's loads are
-    // issued before this row's reductions.  Every row group of a block runs
-    // the same number of turns, for the barriers.
+    // issued before this row's reductions where registers hold two rows.
+    // Every row group of a block runs the same number of turns, for the
+    // barriers.
     const long long step = (long long)gridDim.x * RPB, row0 = (long long)blockIdx.x * RPB;
     const long long mine = wave / WPR;
-    float x[NCH][V], g[NCH][V], xn[NCH][V], gn[NCH][V];
+    float x[NCH][V], g[NCH][V];
     auto clamp_row = [&](long long r) { return min(r, a.rows - 1); };
-    if (row0 < a.rows) load(clamp_row(row0 + mine), x, g);
-    for (long long r = row0; r < a.rows; r += step) {
+    if constexpr (NCH > 1) {
+        for (long long r = row0; r < a.rows; r += step) {
+            load(clamp_row(r + mine), x, g);
+            process(r + mine, x, g, r + mine < a.rows);
+        }
+    }
+    float xn[NCH][V], gn[NCH][V];
+    if (NCH == 1 && row0 < a.rows) load(clamp_row(row0 + mine), x, g);
+    for (long long r = row0; NCH == 1 && r < a.rows; r += step) {
         if (r + step < a.rows) load(clamp_row(r + step + mine), xn, gn);
         process(r + mine, x, g, r + mine < a.rows);
 #pragma unroll
@@ -341,8 +349,8 @@ static pt_status norm_backward_f32(NormBwdArgs a, void *dgamma, void *dbeta, hip
     if (a.n < 8 || a.n > 16384)
         return norm_backward_general<DT, PDT, float>(a.x, a.g, a.gamma, a.dx, dgamma, dbeta, a.rows, a.n, a.eps, s);
     const int wpr = a.n <= 512 ? 1 : a.n <= 1024 ? 2 : a.n <= 2048 ? 4 : 8, rpb = 8 / wpr;
-    // two blocks a CU hide each other's reductions
-    const int blocks = (int)std::min<long long>((a.rows + rpb - 1) / rpb, 512);
+    // two blocks a CU hide each other's reductions (one of 16 waves fills it)
+    const int blocks = (int)std::min<long long>((a.rows + rpb - 1) / rpb, a.n <= 4096 ? 512 : 256);
     void *scratch = nullptr;
     if (dgamma || dbeta) PT_TRY(scratch_alloc(&scratch, (size_t)blocks * 2 * a.n * sizeof(float), s));
     a.partial = (float *)scratch;
@@ -352,8 +360,8 @@ static pt_status norm_backward_f32(NormBwdArgs a, void *dgamma, void *dbeta, hip
     case 4: k_norm_backward<DT, PDT, 1, 4><<<blocks, 512, 0, s>>>(a); break;
     default:
         if (a.n <= 4096) k_norm_backward<DT, PDT, 1, 8><<<blocks, 512, 0, s>>>(a);
-        else if (a.n <= 8192) k_norm_backward<DT, PDT, 2, 8><<<blocks, 512, 0, s>>>(a);
-        else k_norm_backward<DT, PDT, 4, 8><<<blocks, 512, 0, s>>>(a);
+        else if (a.n <= 8192) k_norm_backward<DT, PDT, 1, 16><<<blocks, 1024, 0, s>>>(a);
+        else k_norm_backward<DT, PDT, 2, 16><<<blocks, 1024, 0, s>>>(a);
     }
     if (scratch)
         k_norm_params<PDT, float><<<dim3((a.n + 63) / 64, 2), 1024, 0, s>>>(a.partial, blocks, a.n, dgamma, dbeta);
