@@ -8,18 +8,24 @@
 // (t' = (t + d s) e^-d and s' = s e^-d for m' = m + d); every term of H is
 // positive, so nothing cancels.  m and log s are kept apart for the gradient:
 // their sum would lose log s in a row masked by the type's lowest value.
-// HBM-bound; an element takes about 9 vector instructions and one exponential.
+// HBM-bound; an element takes about 9 vector instructions and one exponential:
+// 4096 rows of 32768 float32 scores 82 us (6.5 TB/s), 2000 rows of 50021 in
+// bfloat16 36 us (5.6 TB/s).
 //
 // The likeliest `top` elements come from the same read.  A wave holds the
 // best it has seen in order, one a lane; a pack of elements is compared with
 // the worst of them by its maximum, which the running maximum needs anyway,
 // so on a row without order almost no pack is looked at again (about k (1 +
-// ln(n / k)) insertions of n elements).  Equal values: the lower index first.
+// ln(n / k)) insertions of n elements).  The waves tell each other how large
+// their best are, so that each lists its share only.  Equal values: the lower
+// index first.  With 8 alternatives the bfloat16 rows above take 59 us, bound
+// by the search's instructions; the float32 rows of that width 73 against 67.
 //
 // Gradient, for upstream a of log p_token, h of H and u_i of the log
 // probability of alternative i:
 //   dx_j = [j = token] a + sum_i [j = i] u_i
 //          - p_j (a + sum u_i) - h p_j (log p_j + H)
+// One read and one write: 200 us for the float32 scores above (5.4 TB/s).
 #include "pt_common.h"
 
 #include <algorithm>

@@ -9,7 +9,10 @@
 // registers and adds its columns' part of dgamma and dbeta there over all
 // the rows it takes; each block then writes one partial row of both, and a
 // second kernel adds the partial rows in a fixed order, so results do not
-// depend on timing.
+// depend on timing.  8192 rows of 4096 float32: 80 us (5.0 TB/s) and 5 us;
+// 6000 rows of 1001 bfloat16: 16 and 4 us.  Rows past 4096 elements take 16
+// waves: chunks of two or four a thread, with the next row's beside them,
+// spilled (4096 rows of 10001 bfloat16 256 us, 129 with 16 waves).
 #include "pt_common.h"
 
 #include <algorithm>

@@ -52,7 +52,7 @@ def close(got, want, what):
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("rows,n", [(1, 1), (3, 7), (1, 8), (5, 9), (37, 64), (700, 100), (4, 511), (9, 512), (130, 513),
                                     (64, 1024), (33, 1025), (20, 2048), (11, 2049), (600, 4096), (7, 4097), (5, 8192),
-                                    (3, 8193), (2, 16384), (2, 16385), (1, 40001), (5000, 16)])
+                                    (3, 8193), (2, 16384), (2, 16385), (1, 40001), (5000, 16), (600, 5003), (300, 16000)])
 def test_gradients(rows, n, dtype):
     x, xv = values((rows, n), dtype, 1, 2.0, 0.5)
     scale, sv = values((n,), dtype, 2, 0.2, 1.0)
