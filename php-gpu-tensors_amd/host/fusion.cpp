@@ -1587,6 +1587,14 @@ static Plan *build_plan(const std::vector<TensorP> &roots, const std::vector<Ten
         if (!st.native) continue;
         const int kind = p->items[st.item].t->node->native.kind;
         if (kind == NAT_GATHER || kind == NAT_SCATTER_ADD) p->indexed = true;
+        // Operators with several results run step by step: the capture of
+        // such a plan over several streams ended in a host segmentation
+        // fault (attention with its gradients in float16, whose first kernel
+        // falls on a side stream), of which no cause is known.
+        if (kind == NAT_BUFFER) {
+            p->graph_compatible = false;
+            p->incompatibility = "several-results";
+        }
     }
     // (fusion_plan.c:505-509: an indexed step makes the plan neither stream-
     // nor graph-compatible, with the incompatibility "indexed-operation")

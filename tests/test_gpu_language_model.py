@@ -6,7 +6,6 @@ import math
 
 import numpy as np
 import pytest
-import torch
 
 import attention_ref as R
 from phptensors import CudaArray, Fusion, Sequences, _abi
@@ -41,33 +40,66 @@ def loss_of(x, w, tokens, seqs):
     return got["logProbs"].sum() * -0.1 + got["entropy"].sum() * 0.01 + got["topLogProbs"].sum() * 0.02
 
 
-def reference(x, w, tokens):
-    """The loss and the gradients in float64 by torch's differentiation on the CPU."""
-    x = torch.tensor(x, dtype=torch.float64, requires_grad=True)
-    w = {n: torch.tensor(t, dtype=torch.float64, requires_grad=True) for n, t in w.items()}
+def norm(t, scale, bias):
+    c = t - t.mean(1, keepdims=True)
+    r = 1 / np.sqrt((c * c).mean(1, keepdims=True) + 1e-5)
+    return c * r * scale + bias, c * r, r
 
-    def norm(t, s, b):
-        c = t - t.mean(1, keepdim=True)
-        return c / torch.sqrt((c * c).mean(1, keepdim=True) + 1e-5) * s + b
-    h = norm(x, w["s1"], w["b1"])
+
+def norm_back(g, unit, r, scale):
+    h = g * scale
+    return r * (h - h.mean(1, keepdims=True) - unit * (h * unit).mean(1, keepdims=True)), (g * unit).sum(0), g.sum(0)
+
+
+def reference(x, w, tokens, gradients=True):
+    """The loss and, by hand, its gradients in float64."""
+    x, w = x.astype(np.float64), {n: t.astype(np.float64) for n, t in w.items()}
+    h, unit1, r1 = norm(x, w["s1"], w["b1"])
     q, k, v = ((h @ w[n]).reshape(ROWS, heads, SIZE) for n, heads in (("wq", HEADS), ("wk", KV), ("wv", KV)))
-    rows, at = [], 0
+    c, o, probs, at = 1 / math.sqrt(SIZE), np.zeros((ROWS, HEADS, SIZE)), {}, 0
     for n in LENGTHS:
-        hidden = torch.triu(torch.ones(n, n, dtype=torch.bool), 1)
-        heads = []
+        rows = slice(at, at + n)
         for i in range(HEADS):
             j = i // (HEADS // KV)
-            s = q[at:at + n, i] @ k[at:at + n, j].T / math.sqrt(SIZE)
-            heads.append(torch.softmax(s.masked_fill(hidden, -math.inf), 1) @ v[at:at + n, j])
-        rows.append(torch.stack(heads, 1))
+            e = np.where(np.tri(n) > 0, np.exp(c * q[rows, i] @ k[rows, j].T), 0.0)
+            probs[at, i] = p = e / e.sum(1, keepdims=True)
+            o[rows, i] = p @ v[rows, j]
         at += n
-    y = x + torch.cat(rows).reshape(ROWS, -1) @ w["wo"]
-    lp = torch.log_softmax(norm(y, w["s2"], w["b2"]) @ w["head"], 1)
-    named = torch.tensor(tokens >= 0)
-    picked = lp[torch.arange(ROWS), torch.tensor(np.maximum(tokens, 0), dtype=torch.int64)]
-    loss = -0.1 * picked[named].sum() + 0.01 * -(lp.exp() * lp).sum() + 0.02 * lp.topk(2, 1).values.sum()
-    loss.backward()
-    return {"loss": loss.item(), "x": x.grad.numpy(), **{n: t.grad.numpy() for n, t in w.items()}}
+    y = x + o.reshape(ROWS, -1) @ w["wo"]
+    z, unit2, r2 = norm(y, w["s2"], w["b2"])
+    logits = z @ w["head"]
+    lp = logits - np.log(np.exp(logits).sum(1, keepdims=True))
+    p, one, named = np.exp(lp), np.arange(ROWS), tokens >= 0
+    entropy, best = -(p * lp).sum(1, keepdims=True), np.argsort(-lp, 1, kind="stable")[:, :2]
+    loss = -0.1 * lp[one, tokens][named].sum() + 0.01 * entropy.sum() + 0.02 * np.take_along_axis(lp, best, 1).sum()
+    if not gradients:
+        return loss
+    d = p * (0.1 * named[:, None] - 0.04) - 0.01 * p * (lp + entropy)
+    d[one[named], tokens[named]] -= 0.1
+    for i in range(2):
+        d[one, best[:, i]] += 0.02
+    out = {"loss": loss, "head": z.T @ d}
+    dy, out["s2"], out["b2"] = norm_back(d @ w["head"].T, unit2, r2, w["s2"])
+    out["wo"] = o.reshape(ROWS, -1).T @ dy
+    do = (dy @ w["wo"].T).reshape(o.shape)
+    dq, dk, dv = np.zeros_like(q), np.zeros_like(k), np.zeros_like(v)
+    for at, n in zip(np.cumsum([0] + LENGTHS), LENGTHS):
+        rows = slice(at, at + n)
+        for i in range(HEADS):
+            j, p = i // (HEADS // KV), probs[at, i]
+            dp = do[rows, i] @ v[rows, j].T
+            ds = c * p * (dp - (dp * p).sum(1, keepdims=True))
+            dv[rows, j] += p.T @ do[rows, i]
+            dq[rows, i] = ds @ k[rows, j]
+            dk[rows, j] += ds.T @ q[rows, i]
+    dh = 0
+    for n, g in (("wq", dq), ("wk", dk), ("wv", dv)):
+        g = g.reshape(ROWS, -1)
+        out[n] = h.T @ g
+        dh = dh + g @ w[n].T
+    dx, out["s1"], out["b1"] = norm_back(dh, unit1, r1, w["s1"])
+    out["x"] = dy + dx
+    return out
 
 
 def leaves(x, w):
@@ -81,6 +113,15 @@ def test_training_step():
     on: 20 * 128 * 8 * 2^-24 = 1.2e-3 of a gradient's largest element."""
     (x, tokens), w = inputs(1), weights(2)
     want = reference(x, w, tokens)
+    # the reference itself, against differences along a direction of every operand (step 1e-5: off by 1e-10 times
+    # third derivatives and 1e-16 / 1e-5 of the loss)
+    rng = np.random.default_rng(3)
+    for n in ("x", *w):
+        step = 1e-5 * rng.standard_normal(want[n].shape)
+        sides = [reference(x + s if n == "x" else x, {m: t + s if m == n else t for m, t in w.items()}, tokens, False)
+                 for s in (step, -step)]
+        slope = (want[n] * step).sum()
+        assert abs((sides[0] - sides[1]) / 2 - slope) < 1e-10, n   # slopes are of order 1e-5
     a, p = leaves(x, w)
     loss = loss_of(a, p, CudaArray.fromNumpy(tokens), Sequences(LENGTHS))
     loss.backward()
@@ -114,6 +155,9 @@ def test_compiled_training_step(graph):
         ins = arrays(seed)
         want = [t.toBits() for t in step(*ins)]
         assert all(np.array_equal(a, b.toBits()) for a, b in zip(want, plan.run(*ins)))
+    # operators with several results are not captured, also where a graph is asked for
+    assert plan.getStats()["backend"] == "stream" and plan.getStats()["graphLaunches"] == 0
+    assert not graph or plan.getStats()["cudaGraphIncompatibility"] == "several-results"
     alive.backward()
     want = step(held.detach(), *(t.detach() for t in p.values()))
     assert all(np.array_equal(a.toBits(), b.toBits()) for a, b in zip([held.grad(), *(t.grad() for t in p.values())], want[1:]))
@@ -297,3 +341,49 @@ def test_many_ragged_sequences(count, heads, kv, size, dtype):
         want, off = ref[name]
         got = t.toNumpy().astype(np.float64).reshape(want.shape)
         assert (np.abs(got - want) <= off).all(), name
+
+
+def test_operand_in_several_places_and_sequences_of_a_plan():
+    """One tensor as queries, keys and values gets the sum of the three gradients; Sequences made while a plan is
+    recorded belong to it."""
+    x = CudaArray.fromNumpy(np.random.default_rng(1).standard_normal((40, 3, 16)).astype(np.float32))
+    w = CudaArray.fromNumpy(np.random.default_rng(2).standard_normal((40, 3, 16)).astype(np.float32))
+
+    def step(x, w):
+        a, b, c = (x.detach().requiresGrad() for _ in range(3))
+        a.attention(b, c, causal=True, queries=Sequences([30, 10])).backward(w)
+        return [a.grad(), b.grad(), c.grad()]
+    each = step(x, w)
+    one = x.detach().requiresGrad()
+    one.attention(one, one, causal=True, queries=Sequences([30, 10])).backward(w)
+    total, size = sum(t.toNumpy().astype(np.float64) for t in each), sum(np.abs(t.toNumpy()) for t in each)
+    assert (np.abs(one.grad().toNumpy() - total) <= 2 * R.U * size).all()   # two additions
+    for graph in (True, False):
+        plan = Fusion.compile(step, [x, w], cudaGraph=graph)
+        for _ in range(3):
+            assert all(np.array_equal(a.toBits(), b.toBits()) for a, b in zip(each, plan.run(x, w)))
+
+
+def test_gradient_calls_of_the_host_refuse_what_the_forward_calls_refuse():
+    from phptensors import _host
+    lib = _host.load()
+    x, g, s = CudaArray.zeros([4, 6]), CudaArray.zeros([4, 6]), CudaArray.zeros([6])
+    got = (ctypes.c_void_p * 3)()
+
+    def call(axes, eps=1e-5, x=x, g=g, scale=s):
+        a = (ctypes.c_int * len(axes))(*axes)
+        return lib.phpt_layernorm_backward(x._h, g._h, a, len(axes), eps, scale._h if scale is not None else None, None, got)
+    for args in [dict(axes=[2]), dict(axes=[-3]), dict(axes=[1, 1], scale=None), dict(axes=[0]), dict(axes=[1], eps=0.0),
+                 dict(axes=[1], g=CudaArray.zeros([4, 5])), dict(axes=[1], g=CudaArray.zeros([4, 6], "int32")),
+                 dict(axes=[1], scale=CudaArray.zeros([6], "int32")), dict(axes=[0, 1, 2], scale=None)]:
+        assert call(**args) != 0, args
+    q = CudaArray.zeros([4, 2, 8])
+    kept = (ctypes.c_void_p * 2)()
+    o = CudaArray._wrap(lib.phpt_attention(q._h, q._h, q._h, 0, 0.0, None, None, kept))
+    lse = CudaArray._wrap(kept[0])
+    assert not kept[1]   # float32 keeps no rest
+    for bad in [dict(o=CudaArray.zeros([4, 2, 4])), dict(lse=CudaArray.zeros([4, 2])), dict(g=CudaArray.zeros([3, 2, 8])),
+                dict(g=CudaArray.zeros([4, 2, 8], "bfloat16")), dict(rest=q)]:
+        a = {"o": o, "lse": lse, "rest": None, "g": q, **bad}
+        assert lib.phpt_attention_backward(q._h, q._h, q._h, a["o"]._h, a["lse"]._h, a["rest"]._h if a["rest"] is not None else None,
+                                           a["g"]._h, 0, 0.0, None, None, got) != 0, bad
