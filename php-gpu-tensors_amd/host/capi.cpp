@@ -5,8 +5,9 @@
 #include "runtime.hpp"
 
 #include <limits.h>
-
 #include <string.h>
+
+#include <exception>
 
 using namespace phpt;
 
@@ -30,6 +31,18 @@ static Scalar make_scalar(double value, int64_t ivalue, int kind)
 static phpt_tensor *lazy_view(const TensorP &t, const int *shape, const size_t *strides, int nd, size_t off)
 {
     return wrap(fusion_record_view(t, shape, strides, nd, off));
+}
+
+// An exception (host memory running out) ends at the boundary as an error.
+template <typename R, typename F> static R bounded(R failed, F &&call)
+{
+    clear_error();
+    try {
+        return call();
+    } catch (const std::exception &e) {
+        set_runtime("%s", e.what());
+        return failed;
+    }
 }
 
 extern "C" {
@@ -315,18 +328,20 @@ static SequencesP sequences_of(phpt_sequences *h) { return h ? h->s : nullptr; }
 int phpt_layernorm_backward(phpt_tensor *a, phpt_tensor *grad, const int *axes, int naxes, double eps,
                             phpt_tensor *scale, phpt_tensor *bias, phpt_tensor **results)
 {
-    clear_error();
-    TensorP out[3];
-    if (!cuda_array_layernorm_backward(a->t, grad->t, axes, naxes, eps, tensor_of(scale), tensor_of(bias), out)) return -1;
-    for (int i = 0; i < 3; i++) results[i] = wrap(out[i]);
-    return 0;
+    return bounded(-1, [&]() -> int {
+        TensorP out[3];
+        if (!cuda_array_layernorm_backward(a->t, grad->t, axes, naxes, eps, tensor_of(scale), tensor_of(bias), out)) return -1;
+        for (int i = 0; i < 3; i++) results[i] = wrap(out[i]);
+        return 0;
+    });
 }
 
 phpt_sequences *phpt_sequences_create(const int *lengths, const int *starts, int count)
 {
-    clear_error();
-    SequencesP s = make_sequences(lengths, starts, count);
-    return s ? new phpt_sequences{s} : nullptr;
+    return bounded((phpt_sequences *)nullptr, [&]() -> phpt_sequences * {
+        SequencesP s = make_sequences(lengths, starts, count);
+        return s ? new phpt_sequences{s} : nullptr;
+    });
 }
 
 void phpt_sequences_release(phpt_sequences *s) { delete s; }
@@ -334,44 +349,48 @@ void phpt_sequences_release(phpt_sequences *s) { delete s; }
 phpt_tensor *phpt_attention(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, int causal, double scale,
                             phpt_sequences *queries, phpt_sequences *keys, phpt_tensor **kept)
 {
-    clear_error();
-    TensorP out[3];
-    if (!cuda_array_attention(q->t, k->t, v->t, causal != 0, scale, sequences_of(queries), sequences_of(keys),
-                              kept != nullptr, out))
-        return nullptr;
-    for (int i = 0; kept && i < 2; i++) kept[i] = wrap(out[1 + i]);
-    return wrap(out[0]);
+    return bounded((phpt_tensor *)nullptr, [&]() -> phpt_tensor * {
+        TensorP out[3];
+        if (!cuda_array_attention(q->t, k->t, v->t, causal != 0, scale, sequences_of(queries), sequences_of(keys),
+                                  kept != nullptr, out))
+            return nullptr;
+        for (int i = 0; kept && i < 2; i++) kept[i] = wrap(out[1 + i]);
+        return wrap(out[0]);
+    });
 }
 
 int phpt_attention_backward(phpt_tensor *q, phpt_tensor *k, phpt_tensor *v, phpt_tensor *out, phpt_tensor *lse,
                             phpt_tensor *rest, phpt_tensor *grad, int causal, double scale, phpt_sequences *queries,
                             phpt_sequences *keys, phpt_tensor **results)
 {
-    clear_error();
-    TensorP got[3];
-    if (!cuda_array_attention_backward(q->t, k->t, v->t, out->t, lse->t, rest ? rest->t : nullptr, grad->t, causal != 0, scale,
-                                       sequences_of(queries), sequences_of(keys), got))
-        return -1;
-    for (int i = 0; i < 3; i++) results[i] = wrap(got[i]);
-    return 0;
+    return bounded(-1, [&]() -> int {
+        TensorP got[3];
+        if (!cuda_array_attention_backward(q->t, k->t, v->t, out->t, lse->t, rest ? rest->t : nullptr, grad->t, causal != 0, scale,
+                                           sequences_of(queries), sequences_of(keys), got))
+            return -1;
+        for (int i = 0; i < 3; i++) results[i] = wrap(got[i]);
+        return 0;
+    });
 }
 
 int phpt_logprobs(phpt_tensor *a, phpt_tensor *tokens, int top, phpt_tensor **results)
 {
-    clear_error();
-    TensorP out[5];
-    if (!cuda_array_logprobs(a->t, tokens->t, top, out)) return -1;
-    for (int i = 0; i < 5; i++) results[i] = wrap(out[i]);
-    return 0;
+    return bounded(-1, [&]() -> int {
+        TensorP out[5];
+        if (!cuda_array_logprobs(a->t, tokens->t, top, out)) return -1;
+        for (int i = 0; i < 5; i++) results[i] = wrap(out[i]);
+        return 0;
+    });
 }
 
 phpt_tensor *phpt_logprobs_backward(phpt_tensor *a, phpt_tensor *tokens, phpt_tensor *stats, phpt_tensor *entropy,
                                     phpt_tensor *top_index, phpt_tensor *grad_logprob, phpt_tensor *grad_entropy,
                                     phpt_tensor *grad_top)
 {
-    clear_error();
-    return wrap(cuda_array_logprobs_backward(a->t, tokens->t, stats->t, entropy->t, tensor_of(top_index),
-                                             tensor_of(grad_logprob), tensor_of(grad_entropy), tensor_of(grad_top)));
+    return bounded((phpt_tensor *)nullptr, [&]() -> phpt_tensor * {
+        return wrap(cuda_array_logprobs_backward(a->t, tokens->t, stats->t, entropy->t, tensor_of(top_index),
+                                                 tensor_of(grad_logprob), tensor_of(grad_entropy), tensor_of(grad_top)));
+    });
 }
 
 phpt_tensor *phpt_astype(phpt_tensor *a, int dtype)

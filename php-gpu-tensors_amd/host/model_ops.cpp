@@ -394,11 +394,12 @@ bool cuda_array_layernorm_backward(const TensorP &a, const TensorP &grad, const 
         out[0] = nullptr;
         return true;
     }
-    if (!a || !grad || !same_shape(*a, *grad) || !is_floating(grad->dtype) || naxes < 1 ||
-        naxes > a->ndims) {
+    if (!a || !grad || !same_shape(*a, *grad) || !is_floating(grad->dtype)) {
         set_invalid("LayerNorm gradients need a floating input and an upstream gradient of its shape");
         return false;
     }
+    int checked[kMaxDims];
+    if (!layernorm_axes(a, axes, naxes, eps, scale, bias, checked)) return false;
     if (fusion_active()) {
         NativeSpec sp;
         sp.kind = NAT_LAYERNORM_BACKWARD;

@@ -468,37 +468,36 @@ TensorP cuda_array_softmax(const TensorP &a, int axis)
 
 // cuda_array_layernorm (cuda_array_ce.c:2215-2339) with validation
 // (:2037-2087 axes, :2131-2155 parameters, :2219-2247 eps / dtype).
-TensorP cuda_array_layernorm(const TensorP &a, const int *axes_in, int naxes, double eps,
-                             const TensorP &scale, const TensorP &bias)
+bool layernorm_axes(const TensorP &a, const int *axes_in, int naxes, double eps, const TensorP &scale, const TensorP &bias,
+                    int *axes)
 {
-    if (!a) return nullptr;
+    if (!a) return false;
     if (naxes <= 0 || naxes > a->ndims) {
         set_invalid("LayerNorm requires a non-empty list of distinct axes");
-        return nullptr;
+        return false;
     }
-    int axes[kMaxDims];
     int seen[kMaxDims] = {0};
     for (int i = 0; i < naxes; i++) {
         int ax = axes_in[i] < 0 ? axes_in[i] + a->ndims : axes_in[i];
         if (ax < 0 || ax >= a->ndims) {
             set_invalid("LayerNorm axis is out of range for tensor rank %d", a->ndims);
-            return nullptr;
+            return false;
         }
         if (seen[ax]) {
             set_invalid("LayerNorm axes must not contain duplicates");
-            return nullptr;
+            return false;
         }
         seen[ax] = 1;
         axes[i] = ax;
     }
     if (!isfinite(eps) || eps <= 0.0) {
         set_invalid("LayerNorm epsilon must be finite and greater than zero");
-        return nullptr;
+        return false;
     }
     for (int i = 0; i < naxes; i++)
         if (!a->shape[axes[i]]) {
             set_invalid("LayerNorm cannot normalize an empty dimension");
-            return nullptr;
+            return false;
         }
     const TensorP *params[2] = {&scale, &bias};
     const char *pname[2] = {"scale", "bias"};
@@ -507,24 +506,34 @@ TensorP cuda_array_layernorm(const TensorP &a, const int *axes_in, int naxes, do
         if (!t) continue;
         if (!is_floating(t->dtype)) {
             set_invalid("LayerNorm %s must have a floating-point dtype", pname[p]);
-            return nullptr;
+            return false;
         }
         if (t->ndims != naxes) {
             set_invalid("LayerNorm %s rank must match the number of normalized axes", pname[p]);
-            return nullptr;
+            return false;
         }
         for (int i = 0; i < naxes; i++)
             if (t->shape[i] != a->shape[axes[i]]) {
                 set_invalid("LayerNorm %s shape does not match the normalized dimensions", pname[p]);
-                return nullptr;
+                return false;
             }
     }
     int cdt = (a->dtype == PT_FLOAT64 || !is_floating(a->dtype)) ? PT_FLOAT64 : PT_FLOAT32;
     if ((scale && scale->dtype == PT_FLOAT64) || (bias && bias->dtype == PT_FLOAT64)) cdt = PT_FLOAT64;
     if (cdt == PT_FLOAT32 && (!isfinite((float)eps) || (float)eps <= 0.0f)) {
         set_invalid("LayerNorm epsilon is not representable as float32");
-        return nullptr;
+        return false;
     }
+    return true;
+}
+
+TensorP cuda_array_layernorm(const TensorP &a, const int *axes_in, int naxes, double eps,
+                             const TensorP &scale, const TensorP &bias)
+{
+    int axes[kMaxDims];
+    if (!layernorm_axes(a, axes_in, naxes, eps, scale, bias, axes)) return nullptr;
+    int cdt = (a->dtype == PT_FLOAT64 || !is_floating(a->dtype)) ? PT_FLOAT64 : PT_FLOAT32;
+    if ((scale && scale->dtype == PT_FLOAT64) || (bias && bias->dtype == PT_FLOAT64)) cdt = PT_FLOAT64;
     if (fusion_active()) {
         NativeSpec sp;
         sp.kind = NAT_LAYERNORM;
@@ -546,7 +555,7 @@ TensorP cuda_array_layernorm(const TensorP &a, const int *axes_in, int naxes, do
     std::sort(sorted, sorted + naxes);
     int perm[kMaxDims], k = 0;
     for (int d = 0; d < a->ndims; d++)
-        if (!seen[d]) perm[k++] = d;
+        if (std::find(axes, axes + naxes, d) == axes + naxes) perm[k++] = d;
     for (int i = 0; i < naxes; i++) perm[k++] = sorted[i];
     bool identity = true;
     for (int d = 0; d < a->ndims; d++) identity = identity && perm[d] == d;

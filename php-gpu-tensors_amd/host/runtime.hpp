@@ -176,6 +176,9 @@ bool cuda_array_attention(const TensorP &q, const TensorP &k, const TensorP &v, 
 bool cuda_array_attention_backward(const TensorP &q, const TensorP &k, const TensorP &v, const TensorP &o,
                                    const TensorP &lse, const TensorP &rest, const TensorP &grad, bool causal,
                                    double scale, const SequencesP &qs, const SequencesP &ks, TensorP out[3]);
+// layerNorm's checks; axes (at most kMaxDims) without negative ones
+bool layernorm_axes(const TensorP &a, const int *axes_in, int naxes, double eps, const TensorP &scale, const TensorP &bias,
+                    int *axes);
 // gradients of the input, the scale and the bias; scale and bias may be null
 bool cuda_array_layernorm_backward(const TensorP &a, const TensorP &grad, const int *axes, int naxes, double eps,
                                    const TensorP &scale, const TensorP &bias, TensorP out[3]);

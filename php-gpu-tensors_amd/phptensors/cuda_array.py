@@ -7,6 +7,7 @@ against the PHP class reads the same here.  Every operation runs on the GPU;
 when the HIP libraries are not built, the first call raises RuntimeException.
 """
 import ctypes
+import itertools
 import numbers
 
 import numpy as np
@@ -847,7 +848,8 @@ class Sequences:
                 raise InvalidArgumentException("Sequences need a start for each length")
         self._h = _host.check_handle(_host.load().phpt_sequences_create(n_arr, s_arr, n), "Sequences")
         self.lengths = [n_arr[i] for i in range(n)]
-        self.starts = [s_arr[i] if s_arr is not None else sum(self.lengths[:i]) for i in range(n)]
+        self.starts = ([s_arr[i] for i in range(n)] if s_arr is not None else
+                       list(itertools.accumulate(self.lengths, initial=0))[:n])
 
     def __len__(self):
         return len(self.lengths)
