@@ -16,15 +16,16 @@ template <int DT>
 __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
 {
     const int lane = threadIdx.x & 63;
-    const long long rows = (long long)g.nq * g.group, nh = (long long)g.batch * g.kv_heads;
-    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    // (split work is small: its rows fit 32 bits)
+    const unsigned rows = (unsigned)(g.nq * g.group), nh = (unsigned)(g.batch * g.kv_heads);
+    const unsigned at = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (at >= nh * rows) return;
-    const int bh = (int)(at / rows), row = (int)(at % rows), b = bh / g.kv_heads;
+    const int bh = (int)(at / rows), row = (int)(at - bh * rows), b = bh / g.kv_heads;
     const int qi = row / g.group, hq = bh % g.kv_heads * g.group + row % g.group;
     const AttnSeq sq = attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
     if (qi >= sq.n) return;
     // lane s holds range s
-    const long long first = at, step = nh * rows;
+    const long long first = at, step = (long long)nh * rows;
     float m = -INFINITY, l = 0.0f;
     if (lane < g.splits) {
         m = g.part_ml[(lane * step + first) * 2];
@@ -64,18 +65,23 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
 // their order: token rows of the queries (`keys` false: dq) or of the keys
 // (dk, and dv), `heads` heads to a row.  One wave a row and head.
 template <int DT>
-__global__ __launch_bounds__(256) void k_attention_sum(AttnArgs g, bool keys, const float *part, void *out)
+__global__ __launch_bounds__(256) void k_attention_sum(AttnArgs g, bool keys)
 {
+    const float *part = blockIdx.y ? g.part_ml : g.part_o;
+    void *out = !keys ? g.dq : blockIdx.y ? g.dv : g.dk;
     const int lane = threadIdx.x & 63, heads = keys ? g.kv_heads : g.heads, most = keys ? g.nk : g.nq;
-    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= (long long)g.batch * most * heads) return;
-    const int h = (int)(at % heads), i = (int)(at / heads % most), b = (int)(at / heads / most);
+    // (split work is small: its rows fit 32 bits)
+    const unsigned at = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= (unsigned)(g.batch * most * heads)) return;
+    const unsigned row = at / heads;
+    const int h = (int)(at - row * heads), b = (int)(row / most), i = (int)(row - b * (unsigned)most);
     const AttnSeq s = keys ? attn_seq(g.k_starts, g.k_lengths, g.k_rows, g.nk, b) : attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
     if (i >= s.n) return;
     const bool packed = keys ? g.k_starts != nullptr : g.q_starts != nullptr;
     const long long to = ((packed ? s.row + i : (long long)b * most + i) * heads + h) * g.size;
     for (int d = lane; d < g.size; d += 64) {
         float x = 0.0f;
+#pragma unroll 4
         for (int p = 0; p < g.splits; p++) x += part[p * g.part_step + to + d];
         store_c<DT>(out, (size_t)(to + d), x);
     }
@@ -129,10 +135,11 @@ static pt_status attention_args(const pt_attention_desc *d, const void *q, const
     g.kv_heads = d->kv_heads;
     g.group = group;
     g.size = d->head_size;
-    g.nq = d->queries;
-    g.nk = d->keys;
     g.q_rows = d->q_rows;
     g.k_rows = d->k_rows;
+    // no sequence is longer than its tensor
+    g.nq = d->q_starts ? std::min(d->queries, d->q_rows) : d->queries;
+    g.nk = d->k_starts ? std::min(d->keys, d->k_rows) : d->keys;
     g.o_hs = g.size;
     g.o_ts = (long long)g.size * g.heads;
     g.o_bs = g.q_starts ? 0 : g.o_ts * g.nq;
@@ -159,7 +166,7 @@ static pt_status attention_args(const pt_attention_desc *d, const void *q, const
 // a range at least: a range costs a second kernel's read of its sums.
 static int attention_splits(const AttnArgs &g, bool token, long long blocks)
 {
-    const long long most = std::min<long long>((g.nk + 255) / 256, 64);
+    const long long most = std::min<long long>((g.nk + 255ll) / 256, 64);
     if (most <= 1) return 1;
     if (token) return (int)std::min<long long>(std::max<long long>(1, 2048 / blocks), most);
     // packed prompts have no more tiles than their rows fill
@@ -258,7 +265,7 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
         g.part_o = part;
         launch_attention_dq<DT>(g, vec, (unsigned)attention_place(g, qb / nh, (long long)g.q_rows * g.group, g.q_starts), s);
         if (q_splits > 1)
-            k_attention_sum<DT><<<(unsigned)(((long long)g.batch * g.nq * g.heads + 3) / 4), 256, 0, s>>>(g, false, part, g.dq);
+            k_attention_sum<DT><<<(unsigned)(((long long)g.batch * g.nq * g.heads + 3) / 4), 256, 0, s>>>(g, false);
         st = check_hip(hipGetLastError(), "attention gradient of queries");
     }
     if (st == PT_OK && kb) {
@@ -269,8 +276,7 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
         launch_attention_dkv<DT>(g, vec, (unsigned)attention_place(g, kb / nh, g.k_rows, g.k_starts), s);
         if (k_splits > 1) {
             const unsigned n = (unsigned)(((long long)g.batch * g.nk * g.kv_heads + 3) / 4);
-            k_attention_sum<DT><<<n, 256, 0, s>>>(g, true, g.part_o, g.dk);
-            k_attention_sum<DT><<<n, 256, 0, s>>>(g, true, g.part_ml, g.dv);
+            k_attention_sum<DT><<<dim3(n, 2), 256, 0, s>>>(g, true);
         }
         st = check_hip(hipGetLastError(), "attention gradient of keys and values");
     }
