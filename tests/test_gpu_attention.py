@@ -1,5 +1,6 @@
 """CudaArray.attention and its gradients against float64, within bounds that
 count the roundings (attention_ref)."""
+import ctypes
 import math
 
 import numpy as np
@@ -7,7 +8,7 @@ import pytest
 
 import attention_ref as R
 import oracle_lib as O
-from phptensors import CudaArray, Fusion, Sequences, _abi
+from phptensors import CudaArray, Fusion, Sequences, _abi, _host
 
 pytestmark = pytest.mark.gpu
 DTYPES = ["float32", "float16", "bfloat16"]
@@ -280,3 +281,61 @@ def test_refusals():
     four = CudaArray.zeros([1, 4, 4, 16])
     with pytest.raises(bad):
         four.attention(four, four, queries=Sequences([4]))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("size", [64, 20])
+def test_float32_upstream_gradient(dtype, size):
+    """16-bit operands, the upstream gradient in float32: rounded once to the operands' type.  Also without what the
+    forward pass kept of the output's rounding, which the bounds allow for."""
+    lengths, starts, rows, heads, kv = [40, 0, 33], [2, 45, 50], 90, 4, 2
+    q, qv = values((rows, heads, size), dtype, 1)
+    k, kvv = values((rows, kv, size), dtype, 2)
+    v, vv = values((rows, kv, size), dtype, 3)
+    w, w32 = values((rows, heads, size), "float32", 4)
+    wv = CudaArray.fromNumpy(w32.astype(np.float32), dtype).toNumpy().astype(np.float64).reshape(w32.shape)
+    seqs = Sequences(lengths, starts)
+    spans = [(a, n, a, n) for a, n in zip(starts, lengths)]
+    lib = _host.load()
+    kept = (ctypes.c_void_p * 2)()
+    out = CudaArray._wrap(lib.phpt_attention(q._h, k._h, v._h, 1, 0.0, seqs._h, seqs._h, kept))
+    lse, rest = (CudaArray._wrap(h) for h in kept)
+    assert rest.getDtype() == dtype
+    for given in (rest._h, None):
+        got = (ctypes.c_void_p * 3)()
+        assert not lib.phpt_attention_backward(q._h, k._h, v._h, out._h, lse._h, given, w._h, 1, 0.0, seqs._h, seqs._h, got)
+        check(qv, kvv, vv, True, dtype, spans, out, wv, grads=[CudaArray._wrap(h) for h in got])
+
+
+def test_bounds_past_the_tensors():
+    """pt_attention's `queries` and `keys` are bounds: larger ones than the tensors hold give the same results."""
+    lib = _abi.load()
+    heads, kv, size, rows = 4, 2, 64, 300
+    arrays = [np.random.default_rng(i).standard_normal((rows, n, size)).astype(np.float32) for i, n in enumerate((heads, kv, kv, heads))]
+    dev = [_abi.to_device(a) for a in arrays]
+    seq = [_abi.to_device(np.array(a, np.int32)) for a in ([0, 130], [130, 170])]
+    names = [("out", arrays[0]), ("lse", np.zeros((heads, rows), np.float32)), ("dq", arrays[0]), ("dk", arrays[1]), ("dv", arrays[1])]
+    bits = []
+    for most in (170, 300, 100000):
+        d = _abi.PtAttentionDesc()
+        for n, h in (("q", heads), ("k", kv), ("v", kv)):
+            setattr(d, n + "_strides", (ctypes.c_size_t * 3)(0, h * size, size))
+        for n, x in dict(dtype=_abi.FLOAT32, sequences=2, heads=heads, kv_heads=kv, head_size=size, queries=most, keys=most,
+                         q_starts=seq[0].ptr, q_lengths=seq[1].ptr, k_starts=seq[0].ptr, k_lengths=seq[1].ptr, q_rows=rows,
+                         k_rows=rows, causal=1, scale=0.125).items():
+            setattr(d, n, x)
+        to = {n: _abi.to_device(np.zeros_like(a)) for n, a in names}
+        p = {n: t.ptr for n, t in to.items()}
+        _abi.check(lib.pt_attention(ctypes.byref(d), *(a.ptr for a in dev[:3]), p["out"], p["lse"], None, None))
+        _abi.check(lib.pt_attention_backward(ctypes.byref(d), *(a.ptr for a in dev[:3]), p["out"], p["lse"], None, dev[3].ptr,
+                                             _abi.FLOAT32, p["dq"], p["dk"], p["dv"], None))
+        _abi.synchronize()
+        bits.append([to[n].download(np.uint32, a.shape) for n, a in names])
+    spans = [(0, 130, 0, 130), (130, 170, 130, 170)]
+    x = [a.astype(np.float64) for a in arrays]
+    ref = R.attention(*x[:3], True, 0.125, "float32", spans, x[3])
+    for got in bits:   # (another bound may split the work otherwise: the same within the bounds, not always bit for bit)
+        for (n, a), b in zip(names, got):
+            want, off = (x.reshape(a.shape) if n != "lse" else x.T for x in ref["o" if n == "out" else n])
+            assert (np.abs(b.view(np.float32).astype(np.float64) - want) <= off).all(), n
+    assert all(np.array_equal(a, b) for a, b in zip(bits[1], bits[2]))
