@@ -2280,6 +2280,41 @@ static bool compile_plan(Plan &p)
     return true;
 }
 
+// Operators of several results that a plan runs once (Fusion::run, a read
+// inside its callback): the first result and the buffers of the others become
+// concrete together, whichever of them was asked for.  A plan that is made
+// later then takes a further result from the buffer that this run wrote, and
+// does not run the operator again.  Added to the plan's outputs.
+static std::vector<TensorP> operator_results(Plan &p)
+{
+    auto kind_of = [&](int id) {
+        const Item &it = p.items[id];
+        return it.kind == IT_NATIVE ? it.t->node->native.kind : -1;
+    };
+    std::vector<TensorP> more;
+    for (size_t i = 0; i < p.items.size(); i++) {
+        const int kind = kind_of((int)i);
+        if (kind < 0 || kind == NAT_BUFFER || kind == NAT_RESULT) continue;
+        std::vector<int> ids;
+        for (int a : p.items[i].args)
+            if (kind_of(a) == NAT_BUFFER) ids.push_back(a);
+        if (ids.empty()) continue;
+        ids.push_back((int)i);
+        for (int id : ids) {
+            p.outputs.push_back(id);
+            more.push_back(p.items[id].t);
+        }
+    }
+    return more;
+}
+
+static void take_value(const TensorP &t, const TensorP &value)
+{
+    t->storage = value->storage;
+    t->offset = value->offset;
+    for (int d = 0; d < t->ndims; d++) t->strides[d] = value->strides[d];
+}
+
 bool fusion_materialize(const TensorP &t)
 {
     if (t->fusion_failed) {
@@ -2298,14 +2333,14 @@ bool fusion_materialize(const TensorP &t)
             set_runtime("Fusion::compile cannot read tensor data during capture; use FusionGraph::run");
             return false;
         }
+    const std::vector<TensorP> more = operator_results(*p);
     bool ok = compile_plan(*p);
     std::vector<TensorP> outs;
     if (ok) ok = execute(*p, {}, outs, false);
     t_scope = saved;
     if (!ok) return false;
-    t->storage = outs[0]->storage;
-    t->offset = outs[0]->offset;
-    for (int d = 0; d < t->ndims; d++) t->strides[d] = outs[0]->strides[d];
+    take_value(t, outs[0]);
+    for (size_t i = 0; i < more.size(); i++) take_value(more[i], outs[1 + i]);
     return true;
 }
 
@@ -2418,20 +2453,20 @@ int phpt_fusion_run_once(phpt_tensor **outputs, int count)
     for (int i = 0; i < count; i++)
         if (outputs[i]->t->lazy()) roots.push_back(outputs[i]->t);
     for (const TensorP &t : scope->recorded)
-        if (t->lazy() && t.use_count() > 2 &&
+        // (a buffer for a further result is nobody's value without its operator)
+        if (t->lazy() && t.use_count() > 2 && !(t->node->kind == N_NATIVE && t->node->native.kind == NAT_BUFFER) &&
             std::find(roots.begin(), roots.end(), t) == roots.end())
             roots.push_back(t);
     int rc = 0;
     if (!roots.empty()) {
         std::unique_ptr<Plan> p(build_plan(roots, {}));
+        for (const TensorP &t : operator_results(*p)) roots.push_back(t);
         std::vector<TensorP> outs;
         if (!compile_plan(*p) || !execute(*p, {}, outs, true)) {
             rc = -1;
         } else {
             for (size_t i = 0; i < roots.size(); i++) {
-                roots[i]->storage = outs[i]->storage;
-                roots[i]->offset = outs[i]->offset;
-                for (int d = 0; d < roots[i]->ndims; d++) roots[i]->strides[d] = outs[i]->strides[d];
+                take_value(roots[i], outs[i]);
                 roots[i]->node.reset();
             }
         }

@@ -1,0 +1,117 @@
+"""What the host runtime does with operators of several results in Fusion scopes and plans, shown on a double of the
+device library: no GPU."""
+import pytest
+
+import device_double
+
+
+@pytest.fixture(scope="module")
+def double(tmp_path_factory):
+    folder = str(tmp_path_factory.mktemp("double"))
+    device_double.build(folder)
+    return lambda code: device_double.run(folder, code)
+
+
+OPERATORS = """
+import itertools
+
+def logprobs(read):
+    x, t = CudaArray.zeros([5, 30]), CudaArray.zeros([5], "int32")
+    got = x.logProbs(t, top=2)
+    return read([(got["logProbs"], 1.5), (got["entropy"], 2.5), (got["topLogProbs"], 4.5), (got["topTokens"], 7)])
+
+def norm(read):
+    x, s, b = (CudaArray.zeros(n).requiresGrad() for n in ([4, 6], [6], [6]))
+    x.layerNorm([1], 1e-5, s, b).backward(CudaArray.zeros([4, 6]))
+    return read([(x.grad(), 5.0), (s.grad(), 6.0), (b.grad(), 7.0)])
+
+def attention(read):
+    q, k, v = (CudaArray.zeros([6, n, 8]).requiresGrad() for n in (4, 2, 2))
+    o = q.attention(k, v, causal=True)
+    o.backward(CudaArray.zeros([6, 4, 8]))
+    return read([(o, 1.5), (q.grad(), 5.0), (k.grad(), 6.0), (v.grad(), 7.0)])
+
+KERNELS = {logprobs: ["pt_logprobs"], norm: ["pt_layernorm_backward"], attention: ["pt_attention", "pt_attention_backward"]}
+
+def holds(t, x):
+    got = t.toNumpy()
+    assert (got == x).all(), (got.ravel()[:3], x)
+"""
+
+
+def test_results_read_one_by_one_inside_a_scope(double):
+    """In every order; each operator runs once."""
+    double(OPERATORS + """
+for op, kernels in KERNELS.items():
+    for order in itertools.permutations(range({logprobs: 4, norm: 3, attention: 4}[op])):
+        before = [count(k) for k in kernels]
+        def read(results):
+            for i in order:
+                holds(*results[i])
+            return [t for t, _ in results]
+        Fusion.run(lambda: op(read))
+        assert [count(k) - n for k, n in zip(kernels, before)] == [1] * len(kernels), (op.__name__, order)
+""")
+
+
+def test_results_read_after_their_scope(double):
+    """One result is returned, the others are kept by the program and read later."""
+    double(OPERATORS + """
+for op, kernels in KERNELS.items():
+    n = {logprobs: 4, norm: 3, attention: 4}[op]
+    for first in range(n):
+        before, kept = [count(k) for k in kernels], []
+        def read(results):
+            kept[:] = results
+            return results[first][0]
+        Fusion.run(lambda: op(read))
+        for i in range(n):
+            holds(*kept[(first + 1 + i) % n])
+        assert [count(k) - m for k, m in zip(kernels, before)] == [1] * len(kernels), (op.__name__, first)
+""")
+
+
+def test_results_of_an_operator_whose_first_was_dropped(double):
+    double(OPERATORS + """
+for n in (1, 2, 3):
+    kept, before = [], count("pt_logprobs")
+    def read(results):
+        kept[:] = results[1:1 + n]
+        return CudaArray.zeros([3]) + 1.0
+    Fusion.run(lambda: logprobs(read))
+    for t, x in kept:
+        holds(t, x)
+    assert count("pt_logprobs") == before + 1
+""")
+
+
+def test_gradients_after_the_scope_of_their_forward_pass(double):
+    """What the forward pass leaves for the gradients is there when the gradients are asked for outside the scope."""
+    double(OPERATORS + """
+q, k, v = (CudaArray.zeros([6, n, 8]).requiresGrad() for n in (4, 2, 2))
+o = Fusion.run(lambda: q.attention(k, v))
+o.backward(CudaArray.zeros([6, 4, 8]))
+holds(o, 1.5), holds(q.grad(), 5.0), holds(k.grad(), 6.0), holds(v.grad(), 7.0)
+assert count("pt_attention") == count("pt_attention_backward") == 1
+x, t, kept = CudaArray.zeros([5, 30]).requiresGrad(), CudaArray.zeros([5], "int32"), []
+def read():
+    kept.append(x.logProbs(t))
+    return kept[0]["entropy"]
+Fusion.run(read)
+kept[0]["logProbs"].backward(CudaArray.zeros([5]))
+holds(x.grad(), 6.0)   # stats and entropy
+""")
+
+
+def test_results_read_while_a_plan_is_recorded(double):
+    """Of an operator that depends on no input of the plan, which may be read then."""
+    double(OPERATORS + """
+def read(results):
+    for r in results[::turn]:
+        holds(*r)
+    return [t for t, _ in results]
+for op, turn in itertools.product(KERNELS, (1, -1)):
+    plan = Fusion.compile(lambda y: [y + 1.0] + [t.detach() for t in op(read)], [CudaArray.zeros([3])])
+    for t, x in zip(plan.run(CudaArray.zeros([3]))[1:], {logprobs: (1.5, 2.5, 4.5, 7), norm: (5, 6, 7), attention: (1.5, 5, 6, 7)}[op]):
+        holds(t, x)
+""")
