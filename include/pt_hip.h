@@ -305,7 +305,8 @@ pt_status pt_logprobs_backward(const void *logits, int dtype, size_t rows, size_
  * sequence and head, query head h reading key head h / (heads / kv_heads).
  * Operands float32, float16 or bfloat16 (one dtype), products on MFMA with
  * fp32 sums and softmax; in 16 bits the probabilities are rounded to the
- * dtype for their product with v.
+ * dtype for their product with v.  Scores may be as large as float32 holds:
+ * weights go by their differences, and their gradients too.
  *
  * A side without starts holds [sequences][queries or keys] tokens, strides
  * {sequence, token, head} in elements, the head's elements side by side.  A

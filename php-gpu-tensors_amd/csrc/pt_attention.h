@@ -41,12 +41,13 @@ struct AttnArgs {
     int causal;
     float scale, scale_log2;
     int splits;               // key ranges computed by workgroups of their own
-    float *part_o, *part_ml;  // their results: [split][sequence, key head][row][size], and (m, l)
+    float *part_o, *part_ml;  // their results: [split][sequence, key head][row][size], and (m, l), as attn_far_part says
     int place, tiles;         // AttnPlace, and the tiles of a head
     long long part_step;      // backward: parts of dk or dq in part_o, of dv in part_ml, this many elements apart
     // backward
     const void *w;            // upstream gradient in the element type, contiguous like out
-    float *lse2, *delta;      // per (head, token row): lse in base 2 (+inf where nothing is seen), d
+    // per (head, token row): lse in base 2 (+inf where nothing is seen), d, and what scores lose first (kExactLse)
+    float *lse2, *delta, *tops;
     void *dq, *dk, *dv;
     long long stat_rows;      // token rows of a head in lse, lse2 and delta
 };
@@ -600,14 +601,83 @@ template <int DT> __device__ __forceinline__ float attn_rest(float x)
     return x - (DT == PT_BFLOAT16 ? bf16_to_float(float_to_bf16(x)) : f16_to_float(float_to_f16(x)));
 }
 
+// The reference of a row's exponentials is m = round(c s_max), c = scale
+// log2(e), and the exponent fma(c, s, -m).  It is off by the rounding of m in
+// every element of the row alike: a factor that the sum cancels, 2^0.5 at most
+// while |m| <= 2^24.  Beyond, the factor itself would leave float16, and from
+// 2^32 on float32 (float16 operands of some thousands give scores of 1e9).
+// Rows with such a reference are far: their workgroup computes its rows once
+// more by (s - s_max) c, in a plain loop behind the fast one.
+constexpr float kFarScore = 16777216.0f;
+__device__ __forceinline__ bool attn_far(float m) { return fabsf(m) > kFarScore && m != -INFINITY; }
+
+// Is x (uniform in a wave) true in any of the W waves?  One barrier.
+template <int W> __device__ __forceinline__ bool attn_any_wave(bool x, int lane, int wave)
+{
+    __shared__ int box[W];
+    if (lane == 0) box[wave] = x;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) any |= box[w];
+    return __builtin_amdgcn_readfirstlane(any) != 0;
+}
+
+// One block's scores (masked) into sums that are kept by (s - m) c, m the
+// largest score so far.
+template <int DT, int DP>
+__device__ __forceinline__ void attn_far_block(floatx16 &s, float &m, float &l, floatx16 (&o)[DP / 32], float c,
+                                               const typename AttnT<DT>::S *vt, int row0, const AttnLane<DT, DP> &at, int lane)
+{
+    float top = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+    top = fmaxf(m, fmaxf(top, attn_other(top, lane)));
+    const float ref = top == -INFINITY ? 0.0f : top, a = __builtin_amdgcn_exp2f((m - ref) * c);
+    m = top;
+    l *= a;
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[d][e] *= a;
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        s[r] = __builtin_amdgcn_exp2f((s[r] - ref) * c);
+        l += s[r];
+    }
+    attn_cols<DT, DP>(o, vt, row0, s, at);
+}
+
+// What these sums hand on.  m becomes round(c m) where that is the row's
+// result.  A range's part of a far row keeps m as it is and says so by a
+// negative l; of other rows it is as the fast loop leaves it.
+template <int ND>
+__device__ __forceinline__ void attn_far_part(float &m, float &l, floatx16 (&o)[ND], float c, bool part)
+{
+    const float mc = m * c;
+    if (!part || m == -INFINITY) {
+        m = mc;
+    } else if (attn_far(mc)) {
+        l = -l;
+    } else {
+        const float f = __builtin_amdgcn_exp2f(fmaf(m, c, -mc));
+        m = mc;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] *= f;
+    }
+}
+
 // LDS bytes of a tile.
 constexpr int attn_tile_bytes(int rows, int dp, int es) { return rows * dp * es; }
 
 // Joins the waves' results in wave 0 and all others: rescaled to the common
 // maximum, added through `box` (W * 1024 floats that nobody reads any more),
-// 32 elements of the head at a time.
+// 32 elements of the head at a time.  c: by what differences of m count.
 template <int W, int ND>
-__device__ __forceinline__ void attn_join_waves(float &m, float &l, floatx16 (&o)[ND], float *box, int lane, int wave)
+__device__ __forceinline__ void attn_join_waves(float &m, float &l, floatx16 (&o)[ND], float c, float *box, int lane, int wave)
 {
     __shared__ float ml[2][W][32];
     if (lane < 32) {
@@ -620,8 +690,8 @@ __device__ __forceinline__ void attn_join_waves(float &m, float &l, floatx16 (&o
     for (int w = 0; w < W; w++) to = fmaxf(to, ml[0][w][lane & 31]);
     const float ref = to == -INFINITY ? 0.0f : to;
 #pragma unroll
-    for (int w = 0; w < W; w++) sum += ml[1][w][lane & 31] * __builtin_amdgcn_exp2f(ml[0][w][lane & 31] - ref);
-    const float a = __builtin_amdgcn_exp2f(m - ref);
+    for (int w = 0; w < W; w++) sum += ml[1][w][lane & 31] * __builtin_amdgcn_exp2f((ml[0][w][lane & 31] - ref) * c);
+    const float a = __builtin_amdgcn_exp2f((m - ref) * c);
     m = to;
     l = sum;
 #pragma unroll
@@ -772,9 +842,11 @@ __global__ __launch_bounds__(256, (AttnFwdShape<DT, DP>::WGS)) void k_attention(
     // passed by more than 8 (a factor of 256): sums and products are fp32 and
     // a probability keeps its relative precision whatever its size, so most
     // tiles need no rescaling of the sums.
+    bool far = false;
     auto follow = [&](float top) {
         if (__all(!(top > m + 8.0f))) return;
         const float to = fmaxf(m, top), a = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        far = far || __any(attn_far(to));
         m = to;
         l *= a;
 #pragma unroll
@@ -867,8 +939,35 @@ __global__ __launch_bounds__(256, (AttnFwdShape<DT, DP>::WGS)) void k_attention(
     } else if (t < t1) {
         step(t, sa, sb, k1, k0, v0, v1, std::false_type{});
     }
+    if (__builtin_expect(attn_any_wave<4>(far, lane, wave), 0)) {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+        for (t = t0; t < t1; t++) {
+            __syncthreads();
+            load_k(t, k0);
+            load_v(t, v0);
+            attn_landed();
+#pragma unroll 1
+            for (int kb = 0; kb < NKB; kb++) {
+                at.fresh();
+                floatx16 s = attn_rows<DT, DP>(k0, kb * 32, q, at);
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = t * BN + kb * 32 + 4 * half + 8 * (r / 4) + r % 4 < lim ? s[r] : -INFINITY;
+                attn_far_block<DT, DP>(s, m, l, o, g.scale_log2, v0, kb * 32, at, lane);
+            }
+        }
+        attn_far_part<ND>(m, l, o, g.scale_log2, g.splits > 1);
+    }
     l += attn_other(l, lane);
-    attn_result<DT, ND>(g, m, l, o, live, b, bh, nh, row, sq.row + qi, qi, hq, split, half);
+    // the row's numbers once more, so that no register holds them in the loops
+    int at_row = row0 + wave * 32 + (lane & 31);
+    asm volatile("" : "+v"(at_row));
+    const int token = at_row / g.group;
+    attn_result<DT, ND>(g, m, l, o, at_row < rows, b, bh, nh, at_row, sq.row + token, token, hk * g.group + at_row % g.group, split, half);
 }
 
 // 32 rows or fewer, rows of whole 16-byte packs: single tokens over a cache,
@@ -931,6 +1030,7 @@ void k_attention_token(AttnArgs g)
         for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
     AttnLane<DT, DP> at;
     at.init(lane);
+    bool far = false;
     for (int t = t0; t < t1; t += NW) {
         at.fresh();
 #pragma unroll
@@ -953,6 +1053,7 @@ void k_attention_token(AttnArgs g)
         top = fmaxf(top, attn_other(top, lane)) * g.scale_log2;
         if (!__all(!(top > m + 8.0f))) {  // as in k_attention
             const float to = fmaxf(m, top), a = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+            far = far || __any(attn_far(to));
             m = to;
             l *= a;
 #pragma unroll
@@ -968,15 +1069,42 @@ void k_attention_token(AttnArgs g)
         }
         attn_cols<DT, DP>(o, vw, 0, s, at);
     }
+    const bool again = NW > 1 ? attn_any_wave<NW>(far, lane, wave) : far;
+    if (__builtin_expect(again, 0)) {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+        for (int t = t0; t < t1; t += NW) {
+            kl.fetch(ks, g.size, t * 32, kr);
+            vl.fetch(vs, g.size, t * 32, vr);
+#pragma unroll
+            for (int i = 0; i < NI; i++) *(floatx4 *)(kw + (i * 64 + lane) * T::PK) = kr[i];
+#pragma unroll
+            for (int i = 0; i < NI; i++) *(floatx4 *)(vw + (i * 64 + lane) * T::PK) = vr[i];
+            at.fresh();
+            floatx16 s = attn_rows<DT, DP>(kw, 0, q, at);
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = t * 32 + 4 * half + 8 * (r / 4) + r % 4 < lim ? s[r] : -INFINITY;
+            attn_far_block<DT, DP>(s, m, l, o, g.scale_log2, vw, 0, at, lane);
+        }
+        if (NW > 1) __syncthreads();
+    }
 
     l += attn_other(l, lane);
     if constexpr (NW > 1) {
-        __syncthreads();
-        attn_join_waves<NW, ND>(m, l, o, (float *)kt, lane, wave);
+        attn_join_waves<NW, ND>(m, l, o, again ? g.scale_log2 : 1.0f, (float *)kt, lane, wave);
         static_assert(NW * 1024 * 4 <= NW * TE * T::ES, "the joined block fits a tile");
         if (wave) return;
     }
-    attn_result<DT, ND>(g, m, l, o, live, b, bh, nh, row, sq.row + qi, qi, hq, split, half);
+    if (again) attn_far_part<ND>(m, l, o, g.scale_log2, g.splits > 1);
+    // the row's numbers once more, as in k_attention
+    int at_row = lane & 31;
+    asm volatile("" : "+v"(at_row));
+    const int token = at_row / g.group;
+    attn_result<DT, ND>(g, m, l, o, at_row < rows, b, bh, nh, at_row, sq.row + token, token, hk * g.group + at_row % g.group, split, half);
 }
 
 // ------------------------------------------- gradient of keys and values
@@ -1024,9 +1152,9 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::KWGS)) void k_attention
     constexpr int NBUF = AttnBwdShape<DT, DP>::NBUF;
     constexpr int AHEAD = AttnBwdShape<DT, DP>::KWGS == 1 ? 6 : 3, NCOL = attn_col_units<DT, DP>();
     constexpr bool kV = PASS != 2, kK = PASS != 1;
-    // queries, then upstream gradients; lse, then the rows' sums
+    // queries, then upstream gradients; lse, the rows' sums, what their scores lose
     __shared__ __attribute__((aligned(1024))) S b0[2 * TE], b1[2 * TE], b2[NBUF == 3 ? 2 * TE : 8];
-    __shared__ __attribute__((aligned(256))) float s0[128], s1[128], s2[128];
+    __shared__ __attribute__((aligned(256))) float s0[192], s1[192], s2[192];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     int tile, bh;
@@ -1061,6 +1189,7 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::KWGS)) void k_attention
         // rows past the last have zero products; a zero lse keeps their exponentials finite
         if (wave == 0) attn_load_lds4(g.lse2 + at, lane * 4u, st, range);
         if (wave == 1) attn_load_lds4(g.delta + at, lane * 4u, st + 64, range);
+        if (wave == 2) attn_load_lds4(g.tops + at, lane * 4u, st + 128, range);
     };
     if (step0 < steps) {
         load(step0, b0, s0);
@@ -1090,6 +1219,10 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::KWGS)) void k_attention
         for (int r = 0; r < 4; r++) {
             ls[r] = *(const floatx4 *)(st + qi * 32 + 8 * r + 4 * half);
             if constexpr (kK) es[r] = *(const floatx4 *)(st + 64 + qi * 32 + 8 * r + 4 * half);
+        }
+        if (__builtin_expect(__any(st[128 + qi * 32 + (lane & 31)] != 0.0f), 0)) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) p[r] -= st[128 + qi * 32 + 8 * (r / 4) + 4 * half + r % 4];
         }
         // the next block's scores beside this one's exponentials, its products
         // with the values beside the differences, then this block's sums
@@ -1196,6 +1329,12 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::KWGS)) void k_attention
     }
 }
 
+// Rows whose lse is farther from 0 than this have it computed anew by the
+// queries' gradient, as the largest score and the sum of exponentials beside
+// it: p = 2^(c s - lse2) is off by the rounding of lse, 2^-24 of it, in every
+// element of the row (6e-5 at 512, everything at 1e9).
+constexpr float kExactLse = 512.0f;
+
 // ------------------------------------------------- gradient of the queries
 // Rows as in the forward pass; the keys and values stream past them.  This
 // pass runs first and leaves lse2 and d for the other: it holds w anyway.  Two
@@ -1224,10 +1363,11 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::QWGS)) void k_attention
     typename T::Frag q[KS], w[KS];
     attn_row<DT, DP, VEC>(q, (const S *)g.q + b * g.q_bs + (sq.row + qi) * g.q_ts + hq * g.q_hs, live, g.size, half);
     attn_row<DT, DP, VEC>(w, (const S *)g.w + b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs, live, g.size, half);
-    const long long stat = (g.q_starts ? sq.row : (long long)b * g.heads * g.nq) + (long long)hq * g.stat_rows + qi;
+    const long long stat0 = g.q_starts ? sq.row : (long long)b * g.heads * g.nq, stat = stat0 + (long long)hq * g.stat_rows + qi;
     // d in fp32, of the output as it was before its rounding where that is
     // known; a row that sees no key gets lse +inf, so its exponentials are 0
-    float es = 0.0f, ls = INFINITY;
+    float es = 0.0f, ls = INFINITY, lost = 0.0f;
+    bool far = false;
     {
         typename T::Frag o[KS];
         const long long from = b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
@@ -1243,10 +1383,7 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::QWGS)) void k_attention
         if (live) {
             const float l = g.lse[stat];
             if (l != -INFINITY) ls = l * 1.4426950408889634f;
-            if (blockIdx.y == 0 && half == 0) {
-                g.lse2[stat] = ls;
-                g.delta[stat] = es;
-            }
+            far = l != -INFINITY && fabsf(l) > kExactLse;
         }
     }
 
@@ -1261,15 +1398,82 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::QWGS)) void k_attention
     const int lim_last = g.causal ? min(sk.n, (min(row0 + BM, rows) - 1) / g.group + shift) : sk.n;
     // this workgroup's share of the sequence's key tiles
     const int share = ((sk.n + BN - 1) / BN + g.splits - 1) / g.splits, t0 = share * (int)blockIdx.y;
-    const int t1 = min(max(0, (lim_last + BN - 1) / BN), t0 + share);
+    const int tiles = max(0, (lim_last + BN - 1) / BN);
+    int t1 = min(tiles, t0 + share);
+    AttnLane<DT, DP> at;
+    at.init(lane);
+
+    // every wave looks at the rows of all four, for the barriers
+    bool some = false;
+    for (int r = row0 + lane; r < min(row0 + BM, rows); r += 64) {
+        const float l = g.lse[stat0 + (long long)(hk * g.group + r % g.group) * g.stat_rows + r / g.group];
+        some = some || (l != -INFINITY && fabsf(l) > kExactLse);
+    }
+    const bool exact = __any(some);
+    if (__builtin_expect(exact, 0)) {
+        float m = -INFINITY, l = 0.0f;
+        for (int t = 0; t < tiles; t++) {
+            __syncthreads();
+            kl.load(ks, g.size, t * BN, k0, wave, lane);
+            attn_landed();
+            at.fresh();
+#pragma unroll 1
+            for (int kb = 0; kb < NKB; kb++) {
+                floatx16 s = attn_rows<DT, DP>(k0, kb * 32, q, at);
+                float top = m;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[r] = t * BN + kb * 32 + 4 * half + 8 * (r / 4) + r % 4 < lim ? s[r] : -INFINITY;
+                    top = fmaxf(top, s[r]);
+                }
+                const float from = top == -INFINITY ? 0.0f : top;
+                l *= __builtin_amdgcn_exp2f((m - from) * g.scale_log2);
+                m = top;
+#pragma unroll
+                for (int r = 0; r < 16; r++) l += __builtin_amdgcn_exp2f((s[r] - from) * g.scale_log2);
+            }
+        }
+        // the two lanes of a row
+        const float m2 = attn_other(m, lane), l2 = attn_other(l, lane), top = fmaxf(m, m2);
+        l = l * __builtin_amdgcn_exp2f((m - top) * g.scale_log2) + l2 * __builtin_amdgcn_exp2f((m2 - top) * g.scale_log2);
+        if (far) {
+            lost = top;
+            ls = __builtin_amdgcn_logf(l);
+        }
+    }
+    if (live && blockIdx.y == 0 && half == 0) {
+        g.lse2[stat] = ls;
+        g.delta[stat] = es;
+        g.tops[stat] = lost;
+    }
 
     floatx16 dq[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int e = 0; e < 16; e++) dq[d][e] = 0.0f;
-    AttnLane<DT, DP> at;
-    at.init(lane);
+    // These workgroups go through their tiles here, without the loop below.  (In that loop the difference would be a
+    // branch behind the scores' product, and for such a branch the compiler left out the waits for the product.)
+    if (__builtin_expect(exact, 0)) {
+        for (int t = t0; t < t1; t++) {
+            __syncthreads();
+            kl.load(ks, g.size, t * BN, k0, wave, lane);
+            vl.load(vs, g.size, t * BN, v0, wave, lane);
+            attn_landed();
+#pragma unroll 1
+            for (int kb = 0; kb < NKB; kb++) {
+                at.fresh();
+                floatx16 p = attn_rows<DT, DP>(k0, kb * 32, q, at), x = attn_rows<DT, DP>(v0, kb * 32, w, at);
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(p[r] - lost, g.scale_log2, -ls));
+                    x[r] = t * BN + kb * 32 + 4 * half + 8 * (r / 4) + r % 4 < lim ? e * (x[r] - es) : 0.0f;
+                }
+                attn_cols<DT, DP>(dq, k0, kb * 32, x, at);
+            }
+        }
+        t1 = t0;
+    }
     auto step = [&](int t, const S *kt, const S *vt) {
         at.fresh();
         const int key0 = t * BN + 4 * half;

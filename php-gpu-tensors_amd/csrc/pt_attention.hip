@@ -31,10 +31,20 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
         m = g.part_ml[(lane * step + first) * 2];
         l = g.part_ml[(lane * step + first) * 2 + 1];
     }
-    const float top = wave_all(m, FMax{}), ref = top == -INFINITY ? 0.0f : top;
+    // (attn_far_part: of a far row m is unscaled, and its parts are told apart by the exact difference)
+    const float c = g.scale_log2;
+    const bool far = l < 0.0f;
+    l = fabsf(l);
+    const float mc = far ? m * c : m, top = wave_all(mc, FMax{}), ref = top == -INFINITY ? 0.0f : top;
+    float up = mc - ref;
+    if (__any(far)) {
+        const bool farthest = attn_far(top);  // then every part at the top is far
+        const float most = wave_all(far && mc == top ? m : -INFINITY, FMax{});
+        up = farthest ? (far ? (m - most) * c : -fmaf(most, c, -m)) : far ? fmaf(m, c, -ref) : up;
+    }
     // a range in which the row sees nothing has written no sums
     const uint64_t some = __ballot(l != 0.0f);
-    const float weight = __builtin_amdgcn_exp2f(m - ref), sum = wave_all(l * weight, FAdd{});
+    const float weight = __builtin_amdgcn_exp2f(up), sum = wave_all(l * weight, FAdd{});
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const long long to = b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -236,19 +246,20 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
     const int tile = attention_backward_tile<DT>(g.size);
     const int k_splits = kb ? backward_splits(std::max(1ll, k_live), ((long long)g.nq + tile - 1) / tile * g.group) : 1;
     const int q_splits = qb ? backward_splits(std::max(1ll, q_live), ((long long)g.nk + tile - 1) / tile) : 1;
-    // one region: lse2, delta, the rounded upstream gradient, the shares (of
+    // one region: lse2, delta, tops, the rounded upstream gradient, the shares (of
     // dq, and after them of dk and dv)
     auto whole = [](size_t n) { return (n + 255) & ~(size_t)255; };
     const size_t stat_bytes = whole((size_t)stats * 4), w_bytes = round ? whole((size_t)stats * g.size * 2) : 0;
     const size_t k_part = k_splits > 1 ? whole((size_t)k_splits * k_elems * 4) : 0;
     const size_t q_part = q_splits > 1 ? whole((size_t)q_splits * stats * g.size * 4) : 0;
     void *scratch = nullptr;
-    PT_TRY(scratch_alloc(&scratch, 2 * stat_bytes + w_bytes + std::max(2 * k_part, q_part), s));
+    PT_TRY(scratch_alloc(&scratch, 3 * stat_bytes + w_bytes + std::max(2 * k_part, q_part), s));
     char *base = (char *)scratch;
     g.lse2 = (float *)base;
     g.delta = (float *)(base + stat_bytes);
-    void *w16 = base + 2 * stat_bytes;
-    float *part = (float *)(base + 2 * stat_bytes + w_bytes);
+    g.tops = (float *)(base + 2 * stat_bytes);
+    void *w16 = base + 3 * stat_bytes;
+    float *part = (float *)(base + 3 * stat_bytes + w_bytes);
     pt_status st = PT_OK;
     if (round && stats) {
         // the products take 16-bit operands
