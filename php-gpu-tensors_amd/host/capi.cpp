@@ -393,6 +393,16 @@ phpt_tensor *phpt_logprobs_backward(phpt_tensor *a, phpt_tensor *tokens, phpt_te
     });
 }
 
+phpt_tensor *phpt_cast(phpt_tensor *a, int dtype)
+{
+    clear_error();
+    if (!is_valid_dtype(dtype)) {
+        set_invalid("Cannot cast to dtype %d", dtype);
+        return nullptr;
+    }
+    return wrap(tensor_cast(a->t, dtype));
+}
+
 phpt_tensor *phpt_astype(phpt_tensor *a, int dtype)
 {
     clear_error();

@@ -113,6 +113,9 @@ phpt_tensor *phpt_logprobs_backward(phpt_tensor *a, phpt_tensor *tokens, phpt_te
                                     phpt_tensor *top_index, phpt_tensor *grad_logprob, phpt_tensor *grad_entropy,
                                     phpt_tensor *grad_top);
 phpt_tensor *phpt_astype(phpt_tensor *a, int dtype);
+/* to any dtype, rounding to the nearest (phpt_astype refuses casts that may
+ * lose values): gradients of several uses, added up in float32, round once */
+phpt_tensor *phpt_cast(phpt_tensor *a, int dtype);
 phpt_tensor *phpt_copy(phpt_tensor *a);
 
 /* ---- Fusion (fusion.c, fusion_capture.c, fusion_plan.c, fusion_execute.c) ---- */

@@ -59,6 +59,7 @@ SIGNATURES = {
     "phpt_gather": (T, [T, T, ctypes.c_longlong]),
     "phpt_scatter_add": (T, [T, T, T, ctypes.c_longlong]),
     "phpt_astype": (T, [T, ctypes.c_int]),
+    "phpt_cast": (T, [T, ctypes.c_int]),
     "phpt_copy": (T, [T]),
     "phpt_fusion_begin": (ctypes.c_int, [ctypes.c_int]),
     "phpt_fusion_active": (ctypes.c_int, []),

@@ -53,6 +53,42 @@ class Gradients(dict):
         return both
 
 
+def cast(t, dtype):
+    """t in `dtype`, rounded to the nearest where that is narrower."""
+    from . import _host
+    from .cuda_array import CudaArray, dtype_code
+    return t if t.getDtype() == dtype else CudaArray._wrap(_host.load().phpt_cast(t._h, dtype_code(dtype)), "cast")
+
+
+class Sum:
+    """Gradients of one 16-bit type added up in float32: rounded once, when
+    an operation or the program takes the sum."""
+    __slots__ = ("total", "dtype", "_rounded")
+
+    def __init__(self, total, dtype):
+        self.total, self.dtype, self._rounded = total, dtype, None
+
+    def rounded(self):
+        if self._rounded is None:
+            self._rounded = cast(self.total, self.dtype)
+        return self._rounded
+
+
+def add(a, b):
+    """The sum of two gradients of one tensor."""
+    if isinstance(a, Gradients):
+        return a + b
+    kinds = [g.dtype if isinstance(g, Sum) else g.getDtype() for g in (a, b)]
+    x, y = (g.total if isinstance(g, Sum) else g for g in (a, b))
+    if kinds[0] == kinds[1] and kinds[0] in ("float16", "bfloat16"):
+        return Sum(cast(x, "float32") + y, kinds[0])
+    return x + y
+
+
+def rounded(g):
+    return g.rounded() if isinstance(g, Sum) else g
+
+
 _recording = [True]
 
 
@@ -142,10 +178,10 @@ def _walk(order, grads):
             continue
         if t._node is None:
             if t._rg:
-                t._grad = g if t._grad is None else t._grad + g
+                t._grad = g if t._grad is None else add(t._grad, g)
             continue
-        pg = t._node.backward(g)
+        pg = t._node.backward(rounded(g))
         for p, gp in zip(t._node.parents, pg):
             if gp is None or not needs_grad(p):
                 continue
-            grads[id(p)] = gp if id(p) not in grads else grads[id(p)] + gp
+            grads[id(p)] = gp if id(p) not in grads else add(grads[id(p)], gp)

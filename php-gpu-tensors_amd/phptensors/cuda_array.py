@@ -818,7 +818,7 @@ class CudaArray:
             self._node = None
 
     def grad(self):
-        return self._grad
+        return AG.rounded(self._grad)
 
     def zeroGrad(self):
         self._grad = None

@@ -37,13 +37,33 @@ static void say(const char *what, void *a, void *b)
 }
 const char *double_record(void) { return text; }
 static void floats(void *p, size_t n, float x) { for (size_t i = 0; p && i < n; i++) ((float *)p)[i] = x; }
+static void values(void *p, size_t n, float x, int dtype)
+{
+    unsigned bits;
+    memcpy(&bits, &x, 4);
+    if (dtype == PT_FLOAT32) floats(p, n, x);
+    else if (dtype == PT_FLOAT64) for (size_t i = 0; p && i < n; i++) ((double *)p)[i] = x;
+    else for (size_t i = 0; p && i < n; i++)  // (small numbers, exact in 16 bits)
+        ((unsigned short *)p)[i] = dtype == PT_BFLOAT16 ? bits >> 16 : (bits >> 13 & 0x3FF) | ((bits >> 23 & 0xFF) - 112) << 10;
+}
+static float value(const void *p, int dtype)
+{
+    unsigned short h;
+    unsigned bits;
+    float x;
+    if (dtype == PT_FLOAT32) return *(const float *)p;
+    memcpy(&h, p, 2);
+    bits = dtype == PT_BFLOAT16 ? (unsigned)h << 16 : (unsigned)(h & 0x3FF) << 13 | ((unsigned)(h >> 10) + 112) << 23;
+    memcpy(&x, &bits, 4);
+    return x;
+}
 static size_t tokens(const pt_attention_desc *d, int keys)
 {
     return keys ? (d->k_starts ? d->k_rows : d->sequences * d->keys) : d->q_starts ? d->q_rows : d->sequences * d->queries;
 }
 """
 
-# what a function does besides being counted; operators are written for float32
+# what a function does besides being counted
 BODY = {
     "pt_alloc": "*ptr = malloc(bytes + 64); memset(*ptr, 0xFF, bytes + 64);",
     "pt_free": "free(ptr);",
@@ -62,19 +82,21 @@ BODY = {
     "pt_launch": 'say("launch", current, 0);', "pt_matmul": 'say("launch", current, 0);',
     "pt_reduce": 'say("launch", current, 0);',
     "pt_attention": 'say("launch", current, 0);'
-                    "floats(out, tokens(desc, 0) * desc->heads * desc->head_size, 1.5f); floats(lse, tokens(desc, 0) * desc->heads, 2.5f);",
+                    "values(out, tokens(desc, 0) * desc->heads * desc->head_size, 1.5f, desc->dtype);"
+                    "values(rest, tokens(desc, 0) * desc->heads * desc->head_size, 0.5f, desc->dtype);"
+                    " floats(lse, tokens(desc, 0) * desc->heads, 2.5f);",
     # (what the forward pass left is read back, so that a gradient of unwritten results shows)
     "pt_attention_backward": 'say("launch", current, 0);'
-                             "const float x = *(const float *)out + *lse;"
-                             "floats(dq, tokens(desc, 0) * desc->heads * desc->head_size, x + 1.0f);"
-                             "floats(dk, tokens(desc, 1) * desc->kv_heads * desc->head_size, x + 2.0f);"
-                             "floats(dv, tokens(desc, 1) * desc->kv_heads * desc->head_size, x + 3.0f);",
+                             "const float x = value(out, desc->dtype) + *lse;"
+                             "values(dq, tokens(desc, 0) * desc->heads * desc->head_size, x + 1.0f, desc->dtype);"
+                             "values(dk, tokens(desc, 1) * desc->kv_heads * desc->head_size, x + 2.0f, desc->dtype);"
+                             "values(dv, tokens(desc, 1) * desc->kv_heads * desc->head_size, x + 3.0f, desc->dtype);",
     "pt_layernorm_backward": 'say("launch", current, 0);'
-                             "floats(dinput, rows * n, 5.0f); floats(dgamma, n, 6.0f); floats(dbeta, n, 7.0f);",
+                             "values(dinput, rows * n, 5.0f, input_dtype); values(dgamma, n, 6.0f, param_dtype); values(dbeta, n, 7.0f, param_dtype);",
     "pt_logprobs": 'say("launch", current, 0);'
                    "floats(logprob, rows, 1.5f); floats(entropy, rows, 2.5f); floats(stats, 2 * rows, 3.5f);"
                    "floats(top_logprob, rows * top, 4.5f); for (size_t i = 0; i < rows * top; i++) top_index[i] = 7;",
-    "pt_logprobs_backward": 'say("launch", current, 0); floats(dlogits, rows * classes, stats[1] + (entropy ? entropy[0] : 0.0f));',
+    "pt_logprobs_backward": 'say("launch", current, 0); values(dlogits, rows * classes, stats[1] + (entropy ? entropy[0] : 0.0f), dtype);',
 }
 
 SCRIPT = """

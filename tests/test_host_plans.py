@@ -115,3 +115,29 @@ for op, turn in itertools.product(KERNELS, (1, -1)):
     for t, x in zip(plan.run(CudaArray.zeros([3]))[1:], {logprobs: (1.5, 2.5, 4.5, 7), norm: (5, 6, 7), attention: (1.5, 5, 6, 7)}[op]):
         holds(t, x)
 """)
+
+
+def test_types_of_gradients_that_add_up(double):
+    """16-bit gradients of several uses, and of several backward calls, add up in float32 and are handed out in the
+    operand's type; an operation in front gets its operand's type too."""
+    double("""
+from phptensors import autograd
+for dtype in ("float16", "bfloat16"):
+    q = CudaArray.zeros([6, 2, 8], dtype).requiresGrad()
+    for n in range(3):
+        before = count("pt_cast")
+        o = q.attention(q, q)
+        o.backward(o.detach())
+        assert isinstance(q._grad, autograd.Sum) and q._grad.total.getDtype() == "float32"
+        assert q.grad().getDtype() == dtype and q.grad() is q.grad()
+        # the first of the walk's gradients is widened, and what is handed out rounded once
+        assert count("pt_cast") - before == 2, count("pt_cast") - before
+    w = CudaArray.zeros([16, 16], dtype).requiresGrad()
+    y = CudaArray.zeros([6, 16], dtype).matmul(w).reshape([6, 2, 8])
+    o = y.attention(y, y)
+    o.backward(o.detach())
+    assert w.grad().getDtype() == dtype
+    plan = Fusion.compile(lambda a, g: (lambda b: (b.attention(b, b).backward(g), b.grad())[1])(a.detach().requiresGrad()),
+                          [q.detach(), o.detach()])
+    assert plan.run(q.detach(), o.detach()).getDtype() == dtype
+""")
