@@ -590,6 +590,9 @@ class CudaArray:
             lse, rest = [CudaArray._wrap(h) if h else None for h in kept]
 
             def back(g):
+                given = g.getDtype()
+                if given != "float32" and given != result.getDtype():
+                    g = AG.cast(g, "float32")   # of an operation with a float64 tensor
                 got = (ctypes.c_void_p * 3)()
                 held = (queries, keys)  # the handles behind `at`
                 if lib.phpt_attention_backward(self._h, key._h, value._h, result._h, lse._h,
@@ -624,7 +627,7 @@ class CudaArray:
             values = entropy.detach()
 
             def back(g):
-                g = {name: x if x.getDtype() == "float32" else x.astype("float32") for name, x in g.items()}
+                g = {name: AG.cast(x, "float32") for name, x in g.items()}
                 grads = [g[n]._h if n in g else None for n in ("logProbs", "entropy", "topLogProbs")]
                 return [CudaArray._wrap(lib.phpt_logprobs_backward(
                     self._h, tokens._h, stats._h, values._h, top_i._h if grads[2] else None, *grads),

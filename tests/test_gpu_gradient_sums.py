@@ -72,3 +72,18 @@ def test_a_sum_of_both_types(dtype):
     assert got.getDtype() == "float32"
     # (the three uses' sum was rounded above, and is not here)
     assert (np.abs(got.toNumpy().astype(np.float64) - (low + 3.0)) <= R.H[dtype] * np.abs(low) * 1.01 + 4 * R.U * (np.abs(low) + 3.0) + R.TINY[dtype]).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_results_that_meet_float64(dtype):
+    """An upstream gradient in float64, of a factor that float32 holds: the bits of the same factor in float32."""
+    factor = np.random.default_rng(5).standard_normal((20, 2, 16)).astype(np.float32)
+    tokens = CudaArray.fromNumpy(np.arange(20, dtype=np.int32))
+    bits = []
+    for up in ("float32", "float64"):
+        q, x = made((20, 2, 16), 1, dtype).requiresGrad(), made((20, 40), 2, dtype).requiresGrad()
+        (q.attention(q, q) * CudaArray.fromNumpy(factor.astype(up), up)).sum().backward()
+        (x.logProbs(tokens)["entropy"] * CudaArray.fromNumpy(factor[:, 0, 0].astype(up), up)).sum().backward()
+        assert q.grad().getDtype() == x.grad().getDtype() == dtype
+        bits.append((q.grad().toBits(), x.grad().toBits()))
+    assert all(np.array_equal(a, b) for a, b in zip(*bits))

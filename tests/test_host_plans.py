@@ -141,3 +141,26 @@ for dtype in ("float16", "bfloat16"):
                           [q.detach(), o.detach()])
     assert plan.run(q.detach(), o.detach()).getDtype() == dtype
 """)
+
+
+def test_upstream_gradients_of_every_floating_type(double):
+    """Results that meet a float64 or a 16-bit tensor on the way to the loss."""
+    double("""
+def attention(dtype, up):
+    q = CudaArray.zeros([6, 2, 8], dtype).requiresGrad()
+    (q.attention(q, q) * CudaArray.ones([6, 2, 8], up)).sum().backward()
+    return q
+def logprobs(dtype, up):
+    x = CudaArray.zeros([6, 9], dtype).requiresGrad()
+    got = x.logProbs(CudaArray.zeros([6], "int32"), top=2)
+    (got["entropy"] * CudaArray.ones([6], up) + got["topLogProbs"].sum(1) * CudaArray.ones([6], up)).sum().backward()
+    return x
+def norm(dtype, up):
+    x = CudaArray.zeros([6, 9], dtype).requiresGrad()
+    (x.layerNorm([1]) * CudaArray.ones([6, 9], up)).sum().backward()
+    return x
+for op in (attention, logprobs, norm):
+    for dtype in ("float32", "float16", "bfloat16"):
+        for up in ("float32", "float64", "float16", "bfloat16"):
+            assert op(dtype, up).grad().getDtype() == dtype, (op.__name__, dtype, up)
+""")
