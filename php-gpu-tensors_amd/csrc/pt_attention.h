@@ -41,7 +41,10 @@ struct AttnArgs {
     int causal;
     float scale, scale_log2;
     int splits;               // key ranges computed by workgroups of their own
-    float *part_o, *part_ml;  // their results: [split][sequence, key head][row][size], and (m, l), as attn_far_part says
+    // their results: [split][part_step rows][size], and (m, l), as attn_far_part says; a row is one of a sequence and
+    // key head, or (part_packed) a token row's head
+    float *part_o, *part_ml;
+    int part_packed;
     int place, tiles;         // AttnPlace, and the tiles of a head
     long long part_step;      // backward: parts of dk or dq in part_o, of dv in part_ml, this many elements apart
     // backward
@@ -710,14 +713,21 @@ __device__ __forceinline__ void attn_join_waves(float &m, float &l, floatx16 (&o
     }
 }
 
+// The row among part_step that query qi of sequence b, query head hq has;
+// row: the same among the sequence's and key head's.
+__device__ __forceinline__ long long attn_part_row(const AttnArgs &g, int bh, int row, long long token, int hq)
+{
+    return g.part_packed ? token * g.heads + hq : bh * ((long long)g.nq * g.group) + row;
+}
+
 // A wave's rows: the output and lse, or one range's sums.
 template <int DT, int ND>
 __device__ __forceinline__ void attn_result(const AttnArgs &g, float m, float l, const floatx16 (&o)[ND], bool live, int b,
-                                            int bh, int nh, int row, long long token, int qi, int hq, int split, int half)
+                                            int bh, int row, long long token, int qi, int hq, int split, int half)
 {
     if (!live) return;
     if (g.splits > 1) {
-        const long long at = ((long long)split * nh + bh) * ((long long)g.nq * g.group) + row;
+        const long long at = split * g.part_step + attn_part_row(g, bh, row, token, hq);
         if (half == 0) *(attn_f32x2 *)(g.part_ml + at * 2) = attn_f32x2{m, l};
         if (l != 0.0f)  // (true of NaN) nothing seen: nothing is read there
 #pragma unroll
@@ -775,7 +785,7 @@ __global__ __launch_bounds__(256, (AttnFwdShape<DT, DP>::WGS)) void k_attention(
     __shared__ __attribute__((aligned(1024))) S k0[BN * DP], v0[BN * DP], k1[BN * DP], v1[BN * DP];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int nh = g.batch * g.kv_heads, split = blockIdx.y;
+    const int split = blockIdx.y;
     int tile, bh;
     if (!attn_place(g, false, tile, bh)) return;  // whole workgroup
     const int b = bh / g.kv_heads, hk = bh % g.kv_heads;
@@ -967,7 +977,7 @@ __global__ __launch_bounds__(256, (AttnFwdShape<DT, DP>::WGS)) void k_attention(
     int at_row = row0 + wave * 32 + (lane & 31);
     asm volatile("" : "+v"(at_row));
     const int token = at_row / g.group;
-    attn_result<DT, ND>(g, m, l, o, at_row < rows, b, bh, nh, at_row, sq.row + token, token, hk * g.group + at_row % g.group, split, half);
+    attn_result<DT, ND>(g, m, l, o, at_row < rows, b, bh, at_row, sq.row + token, token, hk * g.group + at_row % g.group, split, half);
 }
 
 // 32 rows or fewer, rows of whole 16-byte packs: single tokens over a cache,
@@ -994,7 +1004,7 @@ void k_attention_token(AttnArgs g)
     __shared__ __attribute__((aligned(1024))) S kt[NW * TE], vt[NW * TE];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int nh = g.batch * g.kv_heads, split = blockIdx.y;
+    const int split = blockIdx.y;
     const int bh = (int)blockIdx.x, b = bh / g.kv_heads, hk = bh % g.kv_heads;
     const AttnSeq sq = attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
     const AttnSeq sk = attn_seq(g.k_starts, g.k_lengths, g.k_rows, g.nk, b);
@@ -1104,7 +1114,7 @@ void k_attention_token(AttnArgs g)
     int at_row = lane & 31;
     asm volatile("" : "+v"(at_row));
     const int token = at_row / g.group;
-    attn_result<DT, ND>(g, m, l, o, at_row < rows, b, bh, nh, at_row, sq.row + token, token, hk * g.group + at_row % g.group, split, half);
+    attn_result<DT, ND>(g, m, l, o, at_row < rows, b, bh, at_row, sq.row + token, token, hk * g.group + at_row % g.group, split, half);
 }
 
 // ------------------------------------------- gradient of keys and values

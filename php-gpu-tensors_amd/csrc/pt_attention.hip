@@ -9,6 +9,57 @@
 
 namespace pt {
 
+// A token of a sequence, and a head.
+struct AttnToken {
+    int b, i, h;
+    long long row;  // in a packed tensor
+};
+
+// The token and head that this wave of a block of four takes.  Of a packed
+// tensor with fewer rows than all sequences would have at the longest's
+// length (`packed`), a token row, whose sequence the lanes look for; else one
+// of that many.  Either fits 32 bits: split work is small.
+__device__ __forceinline__ bool attn_wave_token(const AttnArgs &g, bool keys, bool packed, AttnToken &t)
+{
+    const int32_t *starts = keys ? g.k_starts : g.q_starts, *lengths = keys ? g.k_lengths : g.q_lengths;
+    const int rows = keys ? g.k_rows : g.q_rows, most = keys ? g.nk : g.nq, heads = keys ? g.kv_heads : g.heads;
+    const unsigned at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = at / (unsigned)heads;
+    t.h = (int)(at - x * heads);
+    if (!packed) {
+        t.b = (int)(x / (unsigned)most);
+        t.i = (int)(x - (unsigned)t.b * most);
+        if (t.b >= g.batch) return false;
+        const AttnSeq s = attn_seq(starts, lengths, rows, most, t.b);
+        t.row = s.row + t.i;
+        return t.i < s.n;
+    }
+    if (x >= (unsigned)rows) return false;
+    for (int c = 0; c < g.batch; c += 64) {
+        const int b = c + (int)(threadIdx.x & 63);
+        AttnSeq s = {0, 0};
+        if (b < g.batch) s = attn_seq(starts, lengths, rows, most, b);
+        const uint64_t in = __ballot(s.n && (long long)x >= s.row && (long long)x < s.row + s.n);
+        if (!in) continue;
+        const int lane = (int)__builtin_ctzll(in);
+        t.b = c + lane;
+        t.row = x;
+        t.i = (int)x - __builtin_amdgcn_readlane((int)s.row, lane);
+        return true;
+    }
+    return false;
+}
+
+// Is it, and blocks for it.
+static bool attention_packed(const AttnArgs &g, bool keys)
+{
+    return keys ? g.k_starts && g.k_rows < (long long)g.batch * g.nk : g.q_starts && g.q_rows < (long long)g.batch * g.nq;
+}
+static dim3 attention_wave_tokens(const AttnArgs &g, bool keys, bool packed)
+{
+    const long long tokens = packed ? (keys ? g.k_rows : g.q_rows) : (long long)g.batch * (keys ? g.nk : g.nq);
+    return dim3((unsigned)((tokens * (keys ? g.kv_heads : g.heads) + 3) / 4), keys ? 2 : 1);
+}
+
 // Joins the key ranges that workgroups of their own computed: with the
 // common maximum m = max m_s, l = sum l_s 2^(m_s - m) and o = sum o_s
 // 2^(m_s - m) / l.  One wave a row, at most 64 ranges; each part is read once.
@@ -16,16 +67,11 @@ template <int DT>
 __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
 {
     const int lane = threadIdx.x & 63;
-    // (split work is small: its rows fit 32 bits)
-    const unsigned rows = (unsigned)(g.nq * g.group), nh = (unsigned)(g.batch * g.kv_heads);
-    const unsigned at = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= nh * rows) return;
-    const int bh = (int)(at / rows), row = (int)(at - bh * rows), b = bh / g.kv_heads;
-    const int qi = row / g.group, hq = bh % g.kv_heads * g.group + row % g.group;
-    const AttnSeq sq = attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
-    if (qi >= sq.n) return;
+    AttnToken at;
+    if (!attn_wave_token(g, false, g.part_packed, at)) return;
+    const int b = at.b, qi = at.i, hq = at.h, hk = hq / g.group;
     // lane s holds range s
-    const long long first = at, step = (long long)nh * rows;
+    const long long first = attn_part_row(g, b * g.kv_heads + hk, qi * g.group + hq % g.group, at.row, hq), step = g.part_step;
     float m = -INFINITY, l = 0.0f;
     if (lane < g.splits) {
         m = g.part_ml[(lane * step + first) * 2];
@@ -46,7 +92,7 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
     const uint64_t some = __ballot(l != 0.0f);
     const float weight = __builtin_amdgcn_exp2f(up), sum = wave_all(l * weight, FAdd{});
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const long long to = b * g.o_bs + (sq.row + qi) * g.o_ts + hq * g.o_hs;
+    const long long to = b * g.o_bs + at.row * g.o_ts + hq * g.o_hs;
     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int s = 0; s < g.splits; s++) {
@@ -67,7 +113,7 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
             }
         }
     if (g.lse && lane == 0)
-        g.lse[(g.q_starts ? sq.row : (long long)b * g.heads * g.nq) + (long long)hq * g.stat_rows + qi] =
+        g.lse[(g.q_starts ? at.row : (long long)b * g.heads * g.nq + qi) + (long long)hq * g.stat_rows] =
             sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
 }
 
@@ -75,20 +121,15 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs g)
 // their order: token rows of the queries (`keys` false: dq) or of the keys
 // (dk, and dv), `heads` heads to a row.  One wave a row and head.
 template <int DT>
-__global__ __launch_bounds__(256) void k_attention_sum(AttnArgs g, bool keys)
+__global__ __launch_bounds__(256) void k_attention_sum(AttnArgs g, bool keys, bool packed)
 {
     const float *part = blockIdx.y ? g.part_ml : g.part_o;
     void *out = !keys ? g.dq : blockIdx.y ? g.dv : g.dk;
-    const int lane = threadIdx.x & 63, heads = keys ? g.kv_heads : g.heads, most = keys ? g.nk : g.nq;
-    // (split work is small: its rows fit 32 bits)
-    const unsigned at = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= (unsigned)(g.batch * most * heads)) return;
-    const unsigned row = at / heads;
-    const int h = (int)(at - row * heads), b = (int)(row / most), i = (int)(row - b * (unsigned)most);
-    const AttnSeq s = keys ? attn_seq(g.k_starts, g.k_lengths, g.k_rows, g.nk, b) : attn_seq(g.q_starts, g.q_lengths, g.q_rows, g.nq, b);
-    if (i >= s.n) return;
-    const bool packed = keys ? g.k_starts != nullptr : g.q_starts != nullptr;
-    const long long to = ((packed ? s.row + i : (long long)b * most + i) * heads + h) * g.size;
+    const int lane = threadIdx.x & 63;
+    AttnToken t;
+    if (!attn_wave_token(g, keys, packed, t)) return;
+    const long long row = (keys ? g.k_starts : g.q_starts) ? t.row : (long long)t.b * (keys ? g.nk : g.nq) + t.i;
+    const long long to = (row * (keys ? g.kv_heads : g.heads) + t.h) * g.size;
     for (int d = lane; d < g.size; d += 64) {
         float x = 0.0f;
 #pragma unroll 4
@@ -218,7 +259,10 @@ template <int DT> static pt_status attention_typed(AttnArgs &g, bool vec, hipStr
     g.splits = attention_splits(g, token, blocks);
     void *scratch = nullptr;
     if (g.splits > 1) {
-        const size_t parts = (size_t)g.splits * nh * rows;
+        // the longest of packed prompts may be much longer than most of them
+        g.part_packed = attention_packed(g, false);
+        g.part_step = g.part_packed ? (long long)g.q_rows * g.heads : nh * rows;
+        const size_t parts = (size_t)g.splits * g.part_step;
         PT_TRY(scratch_alloc(&scratch, parts * (g.size + 2) * sizeof(float), s));
         g.part_ml = (float *)scratch;
         g.part_o = g.part_ml + parts * 2;
@@ -226,7 +270,7 @@ template <int DT> static pt_status attention_typed(AttnArgs &g, bool vec, hipStr
     launch_attention<DT>(g, token, vec, (unsigned)(token ? blocks : attention_place(g, blocks / nh, (long long)g.q_rows * g.group, g.q_starts)), s);
     pt_status st = check_hip(hipGetLastError(), "attention");
     if (st == PT_OK && g.splits > 1) {
-        k_attention_join<DT><<<(unsigned)((nh * rows + 3) / 4), 256, 0, s>>>(g);
+        k_attention_join<DT><<<attention_wave_tokens(g, false, g.part_packed), 256, 0, s>>>(g);
         st = check_hip(hipGetLastError(), "attention join");
     }
     if (scratch) scratch_free(scratch, s);
@@ -275,8 +319,10 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
         g.part_step = stats * g.size;
         g.part_o = part;
         launch_attention_dq<DT>(g, vec, (unsigned)attention_place(g, qb / nh, (long long)g.q_rows * g.group, g.q_starts), s);
-        if (q_splits > 1)
-            k_attention_sum<DT><<<(unsigned)(((long long)g.batch * g.nq * g.heads + 3) / 4), 256, 0, s>>>(g, false);
+        if (q_splits > 1) {
+            const bool packed = attention_packed(g, false);
+            k_attention_sum<DT><<<attention_wave_tokens(g, false, packed), 256, 0, s>>>(g, false, packed);
+        }
         st = check_hip(hipGetLastError(), "attention gradient of queries");
     }
     if (st == PT_OK && kb) {
@@ -286,8 +332,8 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
         g.part_ml = (float *)((char *)part + k_part);
         launch_attention_dkv<DT>(g, vec, (unsigned)attention_place(g, kb / nh, g.k_rows, g.k_starts), s);
         if (k_splits > 1) {
-            const unsigned n = (unsigned)(((long long)g.batch * g.nk * g.kv_heads + 3) / 4);
-            k_attention_sum<DT><<<dim3(n, 2), 256, 0, s>>>(g, true);
+            const bool packed = attention_packed(g, true);
+            k_attention_sum<DT><<<attention_wave_tokens(g, true, packed), 256, 0, s>>>(g, true, packed);
         }
         st = check_hip(hipGetLastError(), "attention gradient of keys and values");
     }
