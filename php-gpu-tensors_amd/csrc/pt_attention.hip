@@ -159,10 +159,13 @@ static pt_status attention_args(const pt_attention_desc *d, const void *q, const
     if ((d->q_starts && d->q_rows < 0) || (d->k_starts && d->k_rows < 0))
         return fail(PT_ERR_INVALID, "attention row counts must not be negative");
     const int group = d->heads / d->kv_heads;
-    if (!fits_int((long long)d->queries * group) || !fits_int((long long)d->sequences * d->heads) ||
-        !fits_int(((long long)d->queries * group / 32 + 1) * d->sequences * d->kv_heads) ||
-        !fits_int(((long long)d->keys / 128 + 8) * d->sequences * 8 * d->kv_heads) ||
-        !fits_int(((long long)d->queries * group / 128 + 8) * d->sequences * 8 * d->kv_heads))
+    // no sequence is longer than its tensor
+    const int nq = d->q_starts ? std::min(d->queries, d->q_rows) : d->queries, nk = d->k_starts ? std::min(d->keys, d->k_rows) : d->keys;
+    // (the last tile's rows are numbered past the last row)
+    if (!fits_int((long long)nq * group + 255) || !fits_int(nk + 255ll) || !fits_int((long long)d->sequences * d->heads) ||
+        !fits_int(((long long)nq * group / 32 + 1) * d->sequences * d->kv_heads) ||
+        !fits_int(((long long)nk / 128 + 8) * d->sequences * 8 * d->kv_heads) ||
+        !fits_int(((long long)nq * group / 128 + 8) * d->sequences * 8 * d->kv_heads))
         return fail(PT_ERR_INVALID, "attention has more rows than 32-bit numbers count");
     g = AttnArgs();
     g.q = q;
@@ -188,9 +191,8 @@ static pt_status attention_args(const pt_attention_desc *d, const void *q, const
     g.size = d->head_size;
     g.q_rows = d->q_rows;
     g.k_rows = d->k_rows;
-    // no sequence is longer than its tensor
-    g.nq = d->q_starts ? std::min(d->queries, d->q_rows) : d->queries;
-    g.nk = d->k_starts ? std::min(d->keys, d->k_rows) : d->keys;
+    g.nq = nq;
+    g.nk = nk;
     g.o_hs = g.size;
     g.o_ts = (long long)g.size * g.heads;
     g.o_bs = g.q_starts ? 0 : g.o_ts * g.nq;
@@ -250,10 +252,34 @@ static long long attention_place(AttnArgs &g, long long tiles, long long rows, b
     return g.place == kSpread ? (tiles + share - 1) / share * 8 * g.batch : tiles * nh;
 }
 
+// Is it work for k_attention_token?
+static bool attention_token(const AttnArgs &g, bool vec) { return (long long)g.nq * g.group <= 32 && vec; }
+
+// Workgroups of the forward pass, of the queries' gradient and of the keys';
+// each sets the order of the kernel that is launched next.
+static long long forward_grid(AttnArgs &g, bool token, long long tiles)
+{
+    return token ? (long long)g.batch * g.kv_heads : attention_place(g, tiles, (long long)g.q_rows * g.group, g.q_starts);
+}
+static long long queries_grid(AttnArgs &g) { return forward_grid(g, false, ((long long)g.nq * g.group + 127) / 128); }
+static long long keys_grid(AttnArgs &g) { return attention_place(g, ((long long)g.nk + 127) / 128, g.k_rows, g.k_starts); }
+
+// A launch counts its threads, 256 a workgroup, in 32 bits.
+static pt_status attention_launches(AttnArgs g, bool vec, bool backward)
+{
+    const long long most = 0xffffffffll / 256;
+    const bool token = !backward && attention_token(g, vec);
+    if (g.batch && g.nq && (token ? forward_grid(g, true, 1) : queries_grid(g)) > most)
+        return fail(PT_ERR_INVALID, "attention has more tiles of queries than a launch holds");
+    if (backward && g.batch && g.nk && keys_grid(g) > most)
+        return fail(PT_ERR_INVALID, "attention has more tiles of keys than a launch holds");
+    return PT_OK;
+}
+
 template <int DT> static pt_status attention_typed(AttnArgs &g, bool vec, hipStream_t s)
 {
     const long long nh = (long long)g.batch * g.kv_heads, rows = (long long)g.nq * g.group;
-    const bool token = rows <= 32 && vec;  // k_attention_token
+    const bool token = attention_token(g, vec);
     const long long blocks = (rows + (token ? 31 : 127)) / (token ? 32 : 128) * nh;
     if (!blocks) return PT_OK;
     g.splits = attention_splits(g, token, blocks);
@@ -267,7 +293,7 @@ template <int DT> static pt_status attention_typed(AttnArgs &g, bool vec, hipStr
         g.part_ml = (float *)scratch;
         g.part_o = g.part_ml + parts * 2;
     }
-    launch_attention<DT>(g, token, vec, (unsigned)(token ? blocks : attention_place(g, blocks / nh, (long long)g.q_rows * g.group, g.q_starts)), s);
+    launch_attention<DT>(g, token, vec, (unsigned)forward_grid(g, token, blocks / nh), s);
     pt_status st = check_hip(hipGetLastError(), "attention");
     if (st == PT_OK && g.splits > 1) {
         k_attention_join<DT><<<attention_wave_tokens(g, false, g.part_packed), 256, 0, s>>>(g);
@@ -318,7 +344,7 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
         g.splits = q_splits;
         g.part_step = stats * g.size;
         g.part_o = part;
-        launch_attention_dq<DT>(g, vec, (unsigned)attention_place(g, qb / nh, (long long)g.q_rows * g.group, g.q_starts), s);
+        launch_attention_dq<DT>(g, vec, (unsigned)queries_grid(g), s);
         if (q_splits > 1) {
             const bool packed = attention_packed(g, false);
             k_attention_sum<DT><<<attention_wave_tokens(g, false, packed), 256, 0, s>>>(g, false, packed);
@@ -330,7 +356,7 @@ static pt_status attention_backward_typed(AttnArgs &g, bool vec, const void *w, 
         g.part_step = k_elems;
         g.part_o = part;
         g.part_ml = (float *)((char *)part + k_part);
-        launch_attention_dkv<DT>(g, vec, (unsigned)attention_place(g, kb / nh, g.k_rows, g.k_starts), s);
+        launch_attention_dkv<DT>(g, vec, (unsigned)keys_grid(g), s);
         if (k_splits > 1) {
             const bool packed = attention_packed(g, true);
             k_attention_sum<DT><<<attention_wave_tokens(g, true, packed), 256, 0, s>>>(g, true, packed);
@@ -354,6 +380,7 @@ pt_status pt_attention(const pt_attention_desc *desc, const void *q, const void 
     bool vec;
     PT_TRY(attention_args(desc, q, k, v, g, vec));
     if (!out && g.batch && g.nq && g.stat_rows) return fail(PT_ERR_INVALID, "attention output is missing");
+    PT_TRY(attention_launches(g, vec, false));
     PT_TRY(ensure_init());
     g.out = out;
     g.lse = lse;
@@ -379,6 +406,7 @@ pt_status pt_attention_backward(const pt_attention_desc *desc, const void *q, co
     if (any_q && (!out || !lse || !grad || !dq)) return fail(PT_ERR_INVALID, "attention backward misses an operand");
     if ((dk == nullptr) != (dv == nullptr) || (any_k && !dk))
         return fail(PT_ERR_INVALID, "attention backward misses the gradient of keys or values");
+    PT_TRY(attention_launches(g, vec, true));
     PT_TRY(ensure_init());
     g.out = const_cast<void *>(out);
     g.rest = const_cast<void *>(rest);
