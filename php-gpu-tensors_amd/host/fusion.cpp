@@ -1829,6 +1829,20 @@ static double step_cost_us(const Plan &p, const Step &st, bool &heavy)
     return 3.0 + b / 6e6;
 }
 
+// Does a step launch anything?  Buffers and further results of an operator do
+// not, nor do steps whose value is empty.
+static bool step_launches(const Plan &p, const Step &st)
+{
+    if (!st.native) return p.kernels[st.kernel].total > 0;
+    const Item &it = p.items[st.item];
+    const int kind = it.t->node->native.kind;
+    if (kind == NAT_BUFFER || kind == NAT_RESULT) return false;
+    if (it.t->numel()) return true;
+    for (int a : it.args)  // (an operator may have other results than its first)
+        if (p.items[a].kind == IT_NATIVE && p.items[a].t->node->native.kind == NAT_BUFFER && p.items[a].t->numel()) return true;
+    return false;
+}
+
 // The side streams of the branches (this thread's), created outside any
 // graph capture.
 static bool branch_streams(std::vector<pt_stream_t> &streams)
@@ -1848,11 +1862,17 @@ static bool run_steps_branched(Plan &p, std::vector<TensorP> &vals, std::vector<
 {
     const int ns = (int)p.steps.size();
     // a chain member's values are produced where the chain runs: at its
-    // last member
+    // last member; a further result of an operator, by the operator; and
+    // what launches nothing is waited for by nobody
     std::vector<int> producer(p.items.size(), -1);
     for (int i = 0; i < ns; i++) {
         const Step &st = p.steps[i];
         const int c = chain_of(p, i);
+        if (c < 0 && !step_launches(p, st)) {
+            if (st.native && p.items[st.item].t->node->native.kind == NAT_RESULT)
+                producer[st.item] = producer[p.items[st.item].args[1]];
+            continue;
+        }
         const int at = c >= 0 ? p.chains[c].members.back() : i;
         if (st.native) producer[st.item] = at;
         else
@@ -1886,6 +1906,15 @@ static bool run_steps_branched(Plan &p, std::vector<TensorP> &vals, std::vector<
         const Step &st = p.steps[i];
         const int chain = chain_of(p, i);
         if (chain >= 0 && i != p.chains[chain].members.back()) continue;
+        // A step without a launch takes no branch: on one, its event would
+        // stand for no captured work, and on the capture's own stream it would
+        // push the plan's first kernel to a side stream.
+        if (chain < 0 && !step_launches(p, st)) {
+            pt_stream_set_current(streams[0]);
+            ok = run_step(p, st, vals);
+            pt_stream_set_current(nullptr);
+            continue;
+        }
         std::vector<int> deps;
         auto step_deps = [&](const Step &s) {
             if (s.native) {

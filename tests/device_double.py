@@ -79,7 +79,7 @@ BODY = {
     "pt_graph_end_capture": "capturing = 0; *graph = (pt_graph_t)1;",
     "pt_graph_end_capture_update": "capturing = 0;",
     "pt_workspace_end": "if (peak_bytes) *peak_bytes = 4096;",
-    "pt_launch": 'say("launch", current, 0);', "pt_matmul": 'say("launch", current, 0);',
+    "pt_launch": 'say("launch", current, 0);', "pt_matmul": 'int full = 1; for (int i = 0; i < nd_c; i++) full = full && shape_c[i]; if (full) say("launch", current, 0);',
     "pt_reduce": 'say("launch", current, 0);',
     "pt_attention": 'say("launch", current, 0);'
                     "values(out, tokens(desc, 0) * desc->heads * desc->head_size, 1.5f, desc->dtype);"

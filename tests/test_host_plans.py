@@ -164,3 +164,67 @@ for op in (attention, logprobs, norm):
         for up in ("float32", "float64", "float16", "bfloat16"):
             assert op(dtype, up).grad().getDtype() == dtype, (op.__name__, dtype, up)
 """)
+
+
+CAPTURES = """
+def captured(step, inputs):
+    plan = Fusion.compile(step, inputs, cudaGraph=True)
+    for _ in range(2):   # the first run sizes the workspace, the second captures
+        plan.run(*inputs)
+    assert plan.getStats()["graphLaunches"] == 1, plan.getStats()
+    return record()
+
+def rules(calls, kernels):
+    # every event stands for work on its stream (the first for the capture itself), waits are for recorded events, and
+    # the plan's first kernel is on the capture's own stream
+    assert sum(w == "launch" for w, _, _ in calls) == kernels, calls
+    worked, events = set(), {}
+    for n, (what, a, b) in enumerate(calls):
+        if what == "launch":
+            assert worked or a == 0, calls
+            worked.add(a)
+        elif what == "record":
+            assert a not in events and (n == 0 or b in worked), (n, calls)
+            events[a] = b
+        else:
+            assert b in events, calls
+    # the capture's own stream ends behind all others
+    waited = {events[b] for w, a, b in calls if w == "wait" and a == 0}
+    assert worked - {0} <= waited, calls
+"""
+
+
+def test_branches_of_a_capture(double):
+    """Steps that launch nothing (empty values) take no branch, wherever they stand."""
+    double(CAPTURES + """
+a, b, none = CudaArray.zeros([40, 40]), CudaArray.zeros([40, 40]), CudaArray.zeros([0, 40])
+rules(captured(lambda x, y, e: [e * 2.0, x.matmul(y), y.matmul(x), x.sum(0)], [a, b, none]), 3)
+rules(captured(lambda x, y, e: [e * 2.0, e.matmul(x), x.matmul(y), e.matmul(y), y.matmul(x).matmul(x)], [a, b, none]), 3)
+rules(captured(lambda x, y, e: [x.matmul(y).matmul(x.matmul(x)), e + 1.0, y.matmul(x)], [a, b, none]), 4)
+""")
+
+
+def test_captured_attention_without_gradients(double):
+    """Projections on several branches, attention behind them, and attention alone."""
+    double(CAPTURES + """
+for dtype in ("float32", "float16", "bfloat16"):
+    x, w = CudaArray.zeros([24, 32], dtype), [CudaArray.zeros([32, n], dtype) for n in (32, 16, 16, 32)]
+    at = Sequences([10, 14])
+    def layer(x, wq, wk, wv, wo):
+        q, k, v = (x.matmul(p).reshape([24, -1, 8]) for p in (wq, wk, wv))
+        return q.attention(k, v, causal=True, queries=at).reshape([24, 32]).matmul(wo)
+    rules(captured(layer, [x, *w]), 5)
+    q, k = CudaArray.zeros([24, 4, 8], dtype), CudaArray.zeros([24, 2, 8], dtype)
+    rules(captured(lambda q, k: [q.attention(k, k), k.attention(k, k)], [q, k]), 2)
+""")
+
+
+def test_plans_of_several_results_are_not_captured(double):
+    double("""
+x, t = CudaArray.zeros([5, 30]), CudaArray.zeros([5], "int32")
+plan = Fusion.compile(lambda x: list(x.logProbs(t).values()), [x], cudaGraph=True)
+for _ in range(3):
+    plan.run(x)
+stats = plan.getStats()
+assert stats["graphLaunches"] == 0 and stats["cudaGraphIncompatibility"] == "several-results" and count("pt_graph_begin_capture") == 0
+""")
