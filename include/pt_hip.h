@@ -294,7 +294,7 @@ pt_status pt_logprobs(const void *logits, int dtype, size_t rows, size_t classes
                       float *top_logprob, int32_t *top_index, pt_stream_t stream);
 /* dlogits (contiguous rows of the scores' dtype) for upstream gradients of
  * logprob, entropy and top_logprob, each of which may be NULL; stats, entropy
- * and top_index are the forward call's. */
+ * and top_index are the forward call's.  dlogits must not overlap logits. */
 pt_status pt_logprobs_backward(const void *logits, int dtype, size_t rows, size_t classes, size_t row_stride,
                                const int32_t *tokens, int top, const int32_t *top_index, const float *stats,
                                const float *entropy, const float *grad_logprob, const float *grad_entropy,

@@ -767,7 +767,8 @@ __device__ __forceinline__ void attn_result(const AttnArgs &g, float m, float l,
 // instructions (half of them exponentials, at a quarter of the rate).  Issue
 // of both pipes and the clock under this load bound it (MFMA busy 50 %; taking
 // any one part away saves 4 to 17 %): six causal prompts of 1 to 4096 tokens,
-// 16 heads of 128 in bfloat16, 142 us, 960 TFLOP/s.
+// 16 heads of 128 in bfloat16, 140 to 149 us on different cards, 910 to 975
+// TFLOP/s.
 template <int DT, int DP> struct AttnFwdShape {
     static constexpr int ES = AttnT<DT>::ES;
     static constexpr int BN = ES == 4 || DP == 256 ? 32 : 64;
@@ -986,7 +987,7 @@ __global__ __launch_bounds__(256, (AttnFwdShape<DT, DP>::WGS)) void k_attention(
 // barrier, and the waves drift apart, so that loads are on their way at all
 // times.  The next block's loads go to registers while this one is computed.
 // 32 caches of 977 to 8076 tokens, 8 key heads of 128 in bfloat16, 594 MB:
-// 115 us (5.2 TB/s) and 5.5 us for the join of the ranges.
+// 107 to 112 us (5.3 to 5.5 TB/s) and 5.4 us for the join of the ranges.
 template <int DT, int DP> struct AttnTokenShape {
     static constexpr int TILE = attn_tile_bytes(32, DP, AttnT<DT>::ES);
     static constexpr int NW = TILE <= 8192 ? 4 : TILE <= 16384 ? 2 : 1;
@@ -1128,9 +1129,10 @@ void k_attention_token(AttnArgs g)
 // into the sums.  The tiles lie in three buffers, since block i + 1 may be
 // the next tile's: one barrier a tile, and a tile has the time of a whole one
 // to arrive.  4 x 2048 causal tokens, 16 heads of 128 over 8 key heads in
-// bfloat16: 181 us against 232 without the pipeline (MFMA busy 40 %, 760
-// TFLOP/s of the four products); one wave a SIMD, since the two sums and the
-// two rows take 320 registers.
+// bfloat16: 180 us at the highest clock, where it took 232 without the
+// pipeline (MFMA busy 40 %, 760 TFLOP/s of the four products; up to 199 on
+// cards that clock lower under it); one wave a SIMD, since the two sums and
+// the two rows take 320 registers.
 //
 // PASS 0 computes both gradients.  Heads past 128 elements, whose rows and
 // sums together would pass the register file, take PASS 1 (values) and PASS 2
@@ -1230,6 +1232,8 @@ __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::KWGS)) void k_attention
             ls[r] = *(const floatx4 *)(st + qi * 32 + 8 * r + 4 * half);
             if constexpr (kK) es[r] = *(const floatx4 *)(st + 64 + qi * 32 + 8 * r + 4 * half);
         }
+        // (looked at here and not once for all queries: 2 us of 180 instead of 6; these scores' product ended a block
+        // ago, so nothing has to wait for it behind the branch)
         if (__builtin_expect(__any(st[128 + qi * 32 + (lane & 31)] != 0.0f), 0)) {
 #pragma unroll
             for (int r = 0; r < 16; r++) p[r] -= st[128 + qi * 32 + 8 * (r / 4) + 4 * half + r % 4];
@@ -1348,9 +1352,9 @@ constexpr float kExactLse = 512.0f;
 // ------------------------------------------------- gradient of the queries
 // Rows as in the forward pass; the keys and values stream past them.  This
 // pass runs first and leaves lse2 and d for the other: it holds w anyway.  Two
-// workgroups a CU run beside each other's waits where the registers allow it
-// (heads of 128 in 16 bits just spill): 145 us for the tokens above, 160 with
-// one; reading further ahead spilled more (158 and 173 us).
+// workgroups a CU run beside each other's waits where the registers allow it:
+// 134 us for the tokens above at the highest clock, 147 in the middle, against
+// 160 with one; reading further ahead spilled (158 and 173 us).
 template <int DT, int DP, bool VEC>
 __global__ __launch_bounds__(256, (AttnBwdShape<DT, DP>::QWGS)) void k_attention_dq(AttnArgs g)
 {
