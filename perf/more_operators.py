@@ -127,7 +127,7 @@ def _shapes(c):
 
 
 def _places(shapes):
-    """Where each tensor's moments begin in the one array that holds them all, at whole blocks, and the array's size."""
+    """Where each tensor's moments begin in the one array of blocks that holds them all, and the array's size."""
     at = [0]
     for s in shapes:
         at.append(at[-1] + -(-math.prod(s) // BLOCK) * BLOCK)
@@ -187,10 +187,10 @@ def _make(c, seed):
     shapes = _shapes(c)
     made = {"p": [r.normal(s, std=0.02) for s in shapes], "g": [r.normal(s, c["grad"], 1e-3) for s in shapes]}
     if c["master"]:
-        made["master"] = _joined(shapes, made["p"])
+        made["master"] = _joined(shapes, made["p"]).reshape(-1, BLOCK)
     made["p"] = [p.to(TORCH[dt]) for p in made["p"]]
-    made["m"] = _joined(shapes, [r.normal(t, std=3e-4) for t in shapes])
-    made["v"] = _joined(shapes, [r.normal(t, std=1e-3) ** 2 * 0.02 for t in shapes])
+    made["m"] = _joined(shapes, [r.normal(t, std=3e-4) for t in shapes]).reshape(-1, BLOCK)
+    made["v"] = _joined(shapes, [r.normal(t, std=1e-3) ** 2 * 0.02 for t in shapes]).reshape(-1, BLOCK)
     if c["bits"] == 8:
         made["m"], made["me"] = _encode(made["m"], False, None)
         made["v"], made["ve"] = _encode(made["v"], True, None)
@@ -379,17 +379,16 @@ def _plain_gated(s):
 # 8-bit moments: 256 elements in a row share the power of two 2^e that takes the largest of them into [128, 256).  A first
 # moment is held as a sign, 4 bits of exponent and 3 of mantissa, the root of a second one as 4 and 4 bits.
 def _decode(code, exponent, root):
-    bits = code.reshape(-1, BLOCK).int()
+    bits = code.int()
     size = ((bits << 19) if root else ((bits & 127) << 20)).view(torch.float32) * 2.0 ** 120
     scale = ((exponent.int() + 127) << 23).view(torch.float32)[:, None]
     x = size * scale
-    x = x * x if root else torch.where(bits >= 128, -x, x)
-    return x.reshape(-1)
+    return x * x if root else torch.where(bits >= 128, -x, x)
 
 
 def _encode(x, root, rounding):
     """(codes, exponents); rounding: a number of 16 bits an element, None to round to the nearest."""
-    blocks = (torch.sqrt(x) if root else x).reshape(-1, BLOCK)
+    blocks = torch.sqrt(x) if root else x
     top = blocks.abs().amax(1).view(torch.int32) >> 23
     exponent = (top - 127 - 7).clamp_min(-126)
     scale = ((127 - exponent) << 23).view(torch.float32)[:, None]
@@ -398,10 +397,10 @@ def _encode(x, root, rounding):
     if rounding is None:
         code = (size + (1 << (low - 1))) >> low
     else:
-        code = (size + (rounding.reshape(-1, BLOCK) << (low - 16)) + (1 << (low - 17))) >> low
+        code = (size + (rounding << (low - 16)) + (1 << (low - 17))) >> low
     if not root:
         code = code | torch.where(blocks < 0.0, 128, 0)
-    return code.reshape(-1).to(torch.uint8), exponent.to(torch.int8)
+    return code.to(torch.uint8), exponent.to(torch.int8)
 
 
 def _mix(h):
@@ -413,9 +412,9 @@ def _mix(h):
     return h ^ (h >> 16)
 
 
-def _rounding(draws, size):
+def _rounding(draws, like):
     """Numbers of 16 bits for the first and for the second moment of each element."""
-    h = _mix((torch.arange(size, device="cuda") + _mix(draws.long())) & 0xFFFFFFFF)
+    h = _mix((torch.arange(like.numel(), device="cuda") + _mix(draws.long())) & 0xFFFFFFFF).reshape(like.shape)
     return (h & 0xFFFF).int(), (h >> 16).int()
 
 
@@ -423,23 +422,24 @@ def _plain_adamw(s):
     c, small = s["case"], s["case"]["bits"] == 8
     c1, c2 = ((p * b - 1.0) * -1.0 for p, b in zip(s["powers"], (BETA1, BETA2)))
     m0, v0 = (_decode(s["m"], s["me"], False), _decode(s["v"], s["ve"], True)) if small else (s["m"], s["v"])
-    m1, v1, params = torch.zeros_like(m0), torch.zeros_like(v0), []
+    first, second, params = torch.zeros_like(m0), torch.zeros_like(v0), []
     masters = torch.zeros_like(m0) if c["master"] else None
+    m0, v0, m1, v1 = (t.reshape(-1) for t in (m0, v0, first, second))
     for i, (at, given) in enumerate(zip(_places(_shapes(c))[0], s["p"])):
         here = slice(at, at + given.numel())
         g = s["g"][i].float().reshape(-1)
-        p = s["master"][here] if c["master"] else given.float().reshape(-1)
+        p = s["master"].reshape(-1)[here] if c["master"] else given.float().reshape(-1)
         m1[here] = m = m0[here] * BETA1 + g * (1.0 - BETA1)
         v1[here] = v = v0[here] * BETA2 + (g * g) * (1.0 - BETA2)
         step = (m / c1) / (torch.sqrt(v / c2) + ADAM_EPSILON) * RATE
         new = p * (1.0 - RATE * DECAY) - step if s["decays"][i] else p - step
         params.append(new.to(given.dtype).reshape(given.shape))
         if c["master"]:
-            masters[here] = new
+            masters.reshape(-1)[here] = new
     if small:
-        r = _rounding(s["draws"], m1.numel())
-        m1, v1 = _decode(*_encode(m1, False, r[0]), False), _decode(*_encode(v1, True, r[1]), True)
-    return params + ([masters] if c["master"] else []) + [m1, v1]
+        r = _rounding(s["draws"], first)
+        first, second = _decode(*_encode(first, False, r[0]), False), _decode(*_encode(second, True, r[1]), True)
+    return params + ([masters] if c["master"] else []) + [first, second]
 
 
 # ------------------------------------------------------------------ what a pass cannot do without
@@ -511,11 +511,11 @@ def _exact_adamw(c, d):
     p1, p2 = (p.double() for p in _powers())
     shapes, small = _shapes(c), c["bits"] == 8
     m0, v0 = (_decode(d["m"], d["me"], False), _decode(d["v"], d["ve"], True)) if small else (d["m"], d["v"])
-    grads = _joined(shapes, d["g"]).double()
+    grads = _joined(shapes, d["g"]).double().reshape(-1, BLOCK)
     m, v = torch.lerp(grads, m0.double(), BETA1), torch.lerp(grads.square(), v0.double(), BETA2)
     rate = v.div(1.0 - p2 * BETA2).sqrt().add(ADAM_EPSILON).reciprocal().mul(RATE / (1.0 - p1 * BETA1))
-    old = (d["master"] if c["master"] else _joined(shapes, d["p"])).double()
-    keep = _joined(shapes, [torch.full(t, float(y), device="cuda") for t, y in zip(shapes, _decays(shapes))]).double()
-    new = old - m * rate - RATE * DECAY * keep * old
-    params = [new[a:a + math.prod(t)].reshape(t) for a, t in zip(_places(shapes)[0], shapes)]
+    old = (d["master"] if c["master"] else _joined(shapes, d["p"]).reshape(-1, BLOCK)).double()
+    keep = _joined(shapes, [torch.full(t, float(y), device="cuda") for t, y in zip(shapes, _decays(shapes))])
+    new = old - m * rate - RATE * DECAY * keep.double().reshape(-1, BLOCK) * old
+    params = [new.reshape(-1)[a:a + math.prod(t)].reshape(t) for a, t in zip(_places(shapes)[0], shapes)]
     return params + ([new] if c["master"] else []) + [None if small else m, None if small else v]
