@@ -353,6 +353,95 @@ pt_status pt_attention_backward(const pt_attention_desc *desc, const void *q, co
                                 const void *out, const float *lse, const void *rest, const void *grad,
                                 int grad_dtype, void *dq, void *dk, void *dv, pt_stream_t stream);
 
+/* ---------------------------------------------------------------- rotary --
+ * No counterpart in the reference.  Turns the first `part` elements of every
+ * head by angles position * frequency, in pairs (i, i + part / 2), or
+ * (2i, 2i + 1) where interleaved, and scales them by `magnitude`; the other
+ * elements pass.  With a scale the head is normalised first: x / sqrt(mean(
+ * x^2) + epsilon) * scale.  Two sets of heads (queries and keys) go in one
+ * launch; heads[1] = 0: one.  Angles are taken in double and statistics in
+ * fp32; positions are device values (any int32), so a captured graph follows
+ * them. */
+typedef struct {
+    int dtype;                   /* float32, float16, bfloat16 */
+    int sequences, tokens;       /* of each sequence */
+    int heads[2];
+    size_t strides[2][3];        /* sequence, token, head in elements; a head's elements side by side */
+    int size;                    /* 1 to 256 */
+    int part;                    /* even, 2 to size */
+    int interleaved;
+    double magnitude, epsilon;
+    const double *turns;         /* device double[part / 2]: turns a position (frequency / 2 pi) */
+    const int32_t *positions;    /* device, or NULL: 0, 1, .. in each sequence */
+    size_t position_strides[2];  /* sequence, token */
+} pt_rotary_desc;
+
+/* x, scale, y: an address for each set of heads; scale (may be NULL, or hold
+ * NULLs): [size] of the heads' dtype; y: contiguous [sequences, tokens,
+ * heads, size], not overlapping x. */
+pt_status pt_rotary(const pt_rotary_desc *desc, const void *const *x, const void *const *scale, void *const *y,
+                    pt_stream_t stream);
+/* Gradients for the upstream gradients `grad` (contiguous like y, float32 or
+ * the heads' dtype): dx (a NULL in it: not wanted where the scale's is)
+ * contiguous, and dscale (may be NULL, or hold NULLs) [size], both of the
+ * heads' dtype.  x may hold NULL where there is no scale.  Results do not
+ * depend on timing. */
+pt_status pt_rotary_backward(const pt_rotary_desc *desc, const void *const *x, const void *const *scale,
+                             const void *const *grad, int grad_dtype, void *const *dx, void *const *dscale,
+                             pt_stream_t stream);
+
+/* ----------------------------------------------------------------- AdamW --
+ * No counterpart in the reference, whose step is composed of tensor
+ * operations (src/optimizer.c:471-607).  One step over many tensors.  The
+ * float32 form rounds operation by operation as those do:
+ *   m = m0 b1 + g (1 - b1),  v = v0 b2 + (g g) (1 - b2)
+ *   p = p0 (1 - rate decay) - (m / c1) / (sqrt(v / c2) + eps) rate
+ * c = 1 - power, power the betas' t-th.  An element whose gradient is NaN
+ * stays as it was.  16-bit parameters are rounded once, from float32
+ * arithmetic, and step from a float32 master where there is one (their own
+ * address is then not read).
+ *
+ * The moments and masters of all tensors lie in one array each, a tensor's
+ * `at` elements on, a multiple of 256; the elements from a tensor's end to
+ * the next multiple of 256 are written as zeros.  8-bit moments are
+ * bytes, each 256 with a power of two in the exponent arrays: the first
+ * moment as sign, 4 bits of exponent, 3 of mantissa, the second moment's root
+ * as 4 and 4; both rounded up or down by numbers drawn from `draws`, which
+ * every step advances.  An element one of whose new moments is NaN or 2^126
+ * and more then stays as it was.
+ *
+ * Any new_ address may be the one it is made from, except the powers' and
+ * `draws`'; the results must not overlap the operands in another way. */
+typedef struct {
+    const void *param, *grad;    /* contiguous */
+    void *new_param;
+    size_t n, at;
+    int param_dtype, grad_dtype; /* float32, float16, bfloat16 */
+    int decay;                   /* the weight decay applies */
+} pt_adamw_tensor;
+typedef struct {
+    int bits;                    /* of the moments: 32 or 8 */
+    double beta1, beta2, epsilon, weight_decay;
+    const float *rate;           /* device float32, or NULL: rate_value */
+    double rate_value;
+    const void *first, *second;  /* moments: float32, or bytes */
+    void *new_first, *new_second;
+    const float *master;         /* or NULL, both */
+    float *new_master;
+    const float *power1, *power2; /* device float32: the betas' powers before this step */
+    float *new_power1, *new_power2;
+    /* 8-bit moments only */
+    const int8_t *first_exponent, *second_exponent;
+    int8_t *new_first_exponent, *new_second_exponent;
+    const int32_t *draws;
+    int32_t *new_draws;
+} pt_adamw_desc;
+pt_status pt_adamw(const pt_adamw_desc *desc, const pt_adamw_tensor *tensors, int count, pt_stream_t stream);
+/* The float32 values of n 8-bit moments, n a multiple of 256. */
+pt_status pt_adamw_moments(const void *first, const int8_t *first_exponent, const void *second,
+                           const int8_t *second_exponent, float *first_values, float *second_values, size_t n,
+                           pt_stream_t stream);
+
 /* ------------------------------------------------------------------ GEMM --
  * Replaces cuda_matmul_launcher (src/backends/cuda/matmul_kernels.h:40-44),
  * cuda_batched_matmul_nd_launcher (:47-51) and

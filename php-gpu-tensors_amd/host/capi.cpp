@@ -393,6 +393,99 @@ phpt_tensor *phpt_logprobs_backward(phpt_tensor *a, phpt_tensor *tokens, phpt_te
     });
 }
 
+phpt_rotary_plan *phpt_rotary_create(int part, double base, int interleaved, double factor, double context, double low,
+                                     double high, double magnitude, const double *frequencies)
+{
+    return bounded((phpt_rotary_plan *)nullptr, [&]() -> phpt_rotary_plan * {
+        RotaryP p = make_rotary(part, base, interleaved != 0, factor, context, low, high, magnitude, frequencies);
+        return p ? new phpt_rotary_plan{p} : nullptr;
+    });
+}
+
+void phpt_rotary_release(phpt_rotary_plan *plan) { delete plan; }
+
+int phpt_rotary(phpt_tensor *q, phpt_tensor *k, phpt_tensor *positions, phpt_rotary_plan *plan, phpt_tensor *qs,
+                phpt_tensor *ks, double eps, phpt_tensor **results)
+{
+    return bounded(-1, [&]() -> int {
+        TensorP out[2];
+        if (!cuda_array_rotary(q->t, tensor_of(k), tensor_of(positions), plan ? plan->p : nullptr, tensor_of(qs), tensor_of(ks),
+                               eps, out))
+            return -1;
+        for (int i = 0; i < 2; i++) results[i] = wrap(out[i]);
+        return 0;
+    });
+}
+
+int phpt_rotary_backward(phpt_tensor *q, phpt_tensor *k, phpt_tensor *positions, phpt_rotary_plan *plan, phpt_tensor *qs,
+                         phpt_tensor *ks, double eps, phpt_tensor *gq, phpt_tensor *gk, phpt_tensor **results)
+{
+    return bounded(-1, [&]() -> int {
+        TensorP out[4];
+        if (!cuda_array_rotary_backward(q->t, tensor_of(k), tensor_of(positions), plan ? plan->p : nullptr, tensor_of(qs),
+                                        tensor_of(ks), eps, tensor_of(gq), tensor_of(gk), out))
+            return -1;
+        for (int i = 0; i < 4; i++) results[i] = wrap(out[i]);
+        return 0;
+    });
+}
+
+static std::vector<TensorP> tensors_of(phpt_tensor **h, int count)
+{
+    std::vector<TensorP> out;
+    for (int i = 0; i < count; i++) out.push_back(tensor_of(h[i]));
+    return out;
+}
+
+int phpt_adamw(phpt_tensor **params, phpt_tensor **grads, const unsigned char *decay, int count, phpt_tensor **states,
+               int bits, int master, double beta1, double beta2, double epsilon, double weight_decay, phpt_tensor *rate,
+               double rate_value, phpt_tensor **results)
+{
+    return bounded(-1, [&]() -> int {
+        if (count < 1 || (bits != 32 && bits != 8)) {
+            set_invalid("AdamW needs parameters, and moments of 32 or 8 bits");
+            return -1;
+        }
+        auto step = std::make_shared<AdamwStep>();
+        step->bits = bits;
+        step->master = master != 0;
+        step->has_rate = rate != nullptr;
+        step->beta1 = beta1;
+        step->beta2 = beta2;
+        step->epsilon = epsilon;
+        step->weight_decay = weight_decay;
+        step->rate = rate_value;
+        step->decay.assign(decay, decay + count);
+        std::vector<TensorP> out;
+        if (!cuda_array_adamw(step, tensors_of(params, count), tensors_of(grads, count), tensors_of(states, step->states()),
+                              tensor_of(rate), out))
+            return -1;
+        for (size_t i = 0; i < out.size(); i++) results[i] = wrap(out[i]);
+        return 0;
+    });
+}
+
+long long phpt_adamw_blocks(phpt_tensor **params, int count)
+{
+    return bounded(-1ll, [&]() { return adamw_blocks(tensors_of(params, count)); });
+}
+
+phpt_tensor *phpt_adamw_masters(phpt_tensor **params, int count)
+{
+    return bounded((phpt_tensor *)nullptr, [&]() { return wrap(cuda_array_adamw_masters(tensors_of(params, count))); });
+}
+
+int phpt_adamw_moments(phpt_tensor *first, phpt_tensor *first_exponent, phpt_tensor *second, phpt_tensor *second_exponent,
+                       phpt_tensor **results)
+{
+    return bounded(-1, [&]() -> int {
+        TensorP out[2];
+        if (!cuda_array_adamw_moments(first->t, first_exponent->t, second->t, second_exponent->t, out)) return -1;
+        for (int i = 0; i < 2; i++) results[i] = wrap(out[i]);
+        return 0;
+    });
+}
+
 phpt_tensor *phpt_cast(phpt_tensor *a, int dtype)
 {
     clear_error();

@@ -259,7 +259,8 @@ static int collect(Plan &p, const TensorP &t, std::map<const Tensor *, int> &ind
         // (fusion_plan.c:462-486); other native steps take a materialized
         // operand
         const NativeSpec &ns = t->node->native;
-        const bool attention = ns.kind == NAT_ATTENTION || ns.kind == NAT_ATTENTION_BACKWARD;
+        const bool attention = ns.kind == NAT_ATTENTION || ns.kind == NAT_ATTENTION_BACKWARD ||
+                               ns.kind == NAT_ROTARY || ns.kind == NAT_ROTARY_BACKWARD;
         const bool aliasing =
             ns.kind == NAT_MATMUL || ns.kind == NAT_REDUCE || ns.kind == NAT_ARG_REDUCE || attention;
         const bool global = (ns.kind == NAT_REDUCE || ns.kind == NAT_ARG_REDUCE) && ns.axis == kGlobalAxis;
@@ -267,7 +268,7 @@ static int collect(Plan &p, const TensorP &t, std::map<const Tensor *, int> &ind
             Item &ai = p.items[a];
             if (ai.kind != IT_ELEM) continue;
             bool view = !ai.cut && ai.t->node->kind == N_VIEW;
-            // attention reads heads and tokens at any stride, a head's elements side by side
+            // attention and rotary read heads and tokens at any stride, a head's elements side by side
             if (view && attention && ai.t->ndims && ai.t->node->view_strides[ai.t->ndims - 1] != 1) view = false;
             if (view && global) {
                 size_t cs[kMaxDims];

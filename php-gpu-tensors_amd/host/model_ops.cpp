@@ -13,9 +13,9 @@
 
 namespace phpt {
 
-static bool low_or_f32(int dt) { return dt == PT_FLOAT32 || dt == PT_FLOAT16 || dt == PT_BFLOAT16; }
+bool low_or_f32(int dt) { return dt == PT_FLOAT32 || dt == PT_FLOAT16 || dt == PT_BFLOAT16; }
 
-static bool same_shape(const Tensor &a, const Tensor &b)
+bool same_shape(const Tensor &a, const Tensor &b)
 {
     return a.ndims == b.ndims && std::equal(a.shape, a.shape + a.ndims, b.shape);
 }
@@ -28,16 +28,14 @@ static bool clear(const TensorP &t)
     return check_status(pt_fill(t->data(), t->dtype, t->numel(), &zero, nullptr), "fill");
 }
 
-// A further result of the native step `main` (see NativeKind), its buffer
-// recorded before the step.
-static TensorP record_buffer(const int *shape, int nd, int dtype)
+TensorP record_buffer(const int *shape, int nd, int dtype)
 {
     NativeSpec sp;
     sp.kind = NAT_BUFFER;
     return fusion_record_native(sp, {}, shape, nd, dtype);
 }
 
-static TensorP record_result(const TensorP &buffer, const TensorP &main)
+TensorP record_result(const TensorP &buffer, const TensorP &main)
 {
     NativeSpec sp;
     sp.kind = NAT_RESULT;
@@ -163,7 +161,7 @@ static bool attention_desc(const TensorP &q, const TensorP &k, const TensorP &v,
 }
 
 // The operand itself where a head's elements lie side by side, else packed.
-static TensorP attention_operand(const TensorP &t, size_t strides[3])
+TensorP head_operand(const TensorP &t, size_t strides[3])
 {
     TensorP u = t;
     const int nd = t->ndims;
@@ -192,7 +190,7 @@ static bool attention_run(const TensorP &q, const TensorP &k, const TensorP &v, 
 {
     pt_attention_desc d;
     if (!attention_desc(q, k, v, causal, scale, qs, ks, d)) return false;
-    TensorP a = attention_operand(q, d.q_strides), b = attention_operand(k, d.k_strides), c = attention_operand(v, d.v_strides);
+    TensorP a = head_operand(q, d.q_strides), b = head_operand(k, d.k_strides), c = head_operand(v, d.v_strides);
     if (!a || !b || !c) return false;
     // rows of no sequence are zeros
     if (qs && !qs->cover(q->shape[0]) && !clear(out)) return false;
@@ -242,7 +240,7 @@ static bool attention_backward_run(const TensorP *in, bool causal, double scale,
     const TensorP &q = in[0], &k = in[1], &v = in[2];
     pt_attention_desc d;
     if (!attention_desc(q, k, v, causal, scale, qs, ks, d)) return false;
-    TensorP a = attention_operand(q, d.q_strides), b = attention_operand(k, d.k_strides), c = attention_operand(v, d.v_strides);
+    TensorP a = head_operand(q, d.q_strides), b = head_operand(k, d.k_strides), c = head_operand(v, d.v_strides);
     TensorP o = materialize(in[3]), lse = materialize(in[4]), g = materialize(in[5]);
     TensorP rest = in[6] ? materialize(in[6]) : nullptr;
     if (!a || !b || !c || !o || !lse || !g || (in[6] && !rest)) return false;

@@ -704,6 +704,10 @@ TensorP native_execute(const NativeSpec &sp, const std::vector<TensorP> &in)
     case NAT_LAYERNORM_BACKWARD:
     case NAT_LOGPROBS:
     case NAT_LOGPROBS_BACKWARD: return native_execute_model(sp, in);
+    case NAT_ROTARY:
+    case NAT_ROTARY_BACKWARD:
+    case NAT_ADAMW:
+    case NAT_ADAMW_MOMENTS: return native_execute_block(sp, in);
     default:
         set_runtime("Unknown native step");
         return nullptr;

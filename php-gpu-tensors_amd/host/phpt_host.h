@@ -112,6 +112,42 @@ int phpt_logprobs(phpt_tensor *a, phpt_tensor *tokens, int top, phpt_tensor **re
 phpt_tensor *phpt_logprobs_backward(phpt_tensor *a, phpt_tensor *tokens, phpt_tensor *stats, phpt_tensor *entropy,
                                     phpt_tensor *top_index, phpt_tensor *grad_logprob, phpt_tensor *grad_entropy,
                                     phpt_tensor *grad_top);
+/* A rotation by position of `part` elements of a head: frequencies base^(-2i
+ * / part), or the given part / 2.  factor: the stretch of the context; with
+ * context 0 every frequency is divided by it, else those that turn at most
+ * `low` times within the context, none of at least `high`, and linearly
+ * between.  Checked and copied to the device here; a handle serves any number
+ * of calls. */
+typedef struct phpt_rotary_plan phpt_rotary_plan;
+phpt_rotary_plan *phpt_rotary_create(int part, double base, int interleaved, double factor, double context, double low,
+                                     double high, double magnitude, const double *frequencies);
+void phpt_rotary_release(phpt_rotary_plan *plan);
+/* pt_rotary over q and k (NULL: none) [tokens, heads, size] or [sequences,
+ * tokens, heads, size] at any strides; positions int32 [tokens] or
+ * [sequences, tokens] (NULL: a sequence's tokens from 0 on); qs and ks (NULL:
+ * no norm) [size] of the heads' dtype.  results[2]: q, and k or NULL. */
+int phpt_rotary(phpt_tensor *q, phpt_tensor *k, phpt_tensor *positions, phpt_rotary_plan *plan, phpt_tensor *qs,
+                phpt_tensor *ks, double eps, phpt_tensor **results);
+/* gq or gk may be NULL: that side's results are too.  results[4]: gradients
+ * of q, k, qs and ks */
+int phpt_rotary_backward(phpt_tensor *q, phpt_tensor *k, phpt_tensor *positions, phpt_rotary_plan *plan, phpt_tensor *qs,
+                         phpt_tensor *ks, double eps, phpt_tensor *gq, phpt_tensor *gk, phpt_tensor **results);
+/* pt_adamw over `count` parameters.  states: the moments [blocks, 256] that
+ * phpt_adamw_blocks counts, the betas' powers float32 [1] each, with masters
+ * (master not 0) float32 [blocks, 256], and with 8 bits int8 [blocks] twice
+ * and int32 [1].  rate: float32 [1], or NULL for rate_value.  results gets
+ * the parameters, then the states, all new. */
+int phpt_adamw(phpt_tensor **params, phpt_tensor **grads, const unsigned char *decay, int count, phpt_tensor **states,
+               int bits, int master, double beta1, double beta2, double epsilon, double weight_decay, phpt_tensor *rate,
+               double rate_value, phpt_tensor **results);
+/* blocks of 256 elements that hold the parameters' moments; -1: too many */
+long long phpt_adamw_blocks(phpt_tensor **params, int count);
+/* float32 [blocks, 256]: masters of the parameters' values (not inside a
+ * Fusion scope) */
+phpt_tensor *phpt_adamw_masters(phpt_tensor **params, int count);
+/* results[2]: the float32 values of 8-bit moments */
+int phpt_adamw_moments(phpt_tensor *first, phpt_tensor *first_exponent, phpt_tensor *second, phpt_tensor *second_exponent,
+                       phpt_tensor **results);
 phpt_tensor *phpt_astype(phpt_tensor *a, int dtype);
 /* to any dtype, rounding to the nearest (phpt_astype refuses casts that may
  * lose values): gradients of several uses, added up in float32, round once */

@@ -187,6 +187,43 @@ bool cuda_array_logprobs(const TensorP &a, const TensorP &tokens, int top, Tenso
 TensorP cuda_array_logprobs_backward(const TensorP &a, const TensorP &tokens, const TensorP &stats, const TensorP &entropy,
                                      const TensorP &top_index, const TensorP &g_logprob, const TensorP &g_entropy,
                                      const TensorP &g_top);
+// Frequencies of a rotation by position: part / 2 of them on the device, in
+// turns a position.  Checked when it is made and never changed.
+struct Rotary {
+    int part = 0;
+    bool interleaved = false;
+    double magnitude = 1.0;
+    TensorP turns;
+};
+using RotaryP = std::shared_ptr<Rotary>;
+RotaryP make_rotary(int part, double base, bool interleaved, double factor, double context, double low, double high,
+                    double magnitude, const double *frequencies);
+// k, positions, qs and ks may be null; out: the turned q and, with k, k
+bool cuda_array_rotary(const TensorP &q, const TensorP &k, const TensorP &positions, const RotaryP &plan, const TensorP &qs,
+                       const TensorP &ks, double eps, TensorP out[2]);
+// gq or gk null: that side has no gradient; out: of q, k, qs, ks
+bool cuda_array_rotary_backward(const TensorP &q, const TensorP &k, const TensorP &positions, const RotaryP &plan,
+                                const TensorP &qs, const TensorP &ks, double eps, const TensorP &gq, const TensorP &gk,
+                                TensorP out[4]);
+// One AdamW step over many tensors; the state's arrays in the order
+// first, second, power1, power2, then with masters master, then with 8-bit
+// moments first's and second's exponents and draws.
+struct AdamwStep {
+    int bits = 32;
+    bool master = false, has_rate = false;
+    double beta1 = 0, beta2 = 0, epsilon = 0, weight_decay = 0, rate = 0;
+    std::vector<uint8_t> decay;
+    int count() const { return (int)decay.size(); }
+    int states() const { return 4 + master + (bits == 8 ? 3 : 0); }
+};
+using AdamwStepP = std::shared_ptr<const AdamwStep>;
+// out: the parameters, then the states
+bool cuda_array_adamw(const AdamwStepP &step, const std::vector<TensorP> &params, const std::vector<TensorP> &grads,
+                      const std::vector<TensorP> &states, const TensorP &rate, std::vector<TensorP> &out);
+long long adamw_blocks(const std::vector<TensorP> &params);  // -1: too many
+TensorP cuda_array_adamw_masters(const std::vector<TensorP> &params);
+bool cuda_array_adamw_moments(const TensorP &first, const TensorP &first_exponent, const TensorP &second,
+                              const TensorP &second_exponent, TensorP out[2]);
 TensorP tensor_cast(const TensorP &a, int dtype);
 TensorP astype(const TensorP &a, int dtype);  // safe casts only (CudaArray::astype)
 TensorP copy(const TensorP &a);
@@ -213,7 +250,8 @@ enum NativeKind {
     // (no kernel), and NAT_RESULT is its value once the step in its second
     // operand has written it.
     NAT_BUFFER, NAT_RESULT,
-    NAT_ATTENTION, NAT_ATTENTION_BACKWARD, NAT_LAYERNORM_BACKWARD, NAT_LOGPROBS, NAT_LOGPROBS_BACKWARD
+    NAT_ATTENTION, NAT_ATTENTION_BACKWARD, NAT_LAYERNORM_BACKWARD, NAT_LOGPROBS, NAT_LOGPROBS_BACKWARD,
+    NAT_ROTARY, NAT_ROTARY_BACKWARD, NAT_ADAMW, NAT_ADAMW_MOMENTS
 };
 
 struct NativeSpec {
@@ -229,6 +267,8 @@ struct NativeSpec {
     bool causal = false;
     int top = 0, given = 0;  // given: which optional operands follow (a bit each)
     SequencesP q_seq, k_seq;
+    RotaryP rotary;
+    AdamwStepP adamw;
 };
 
 struct FusionNode {
@@ -259,6 +299,16 @@ bool fusion_materialize(const TensorP &t);
 // Eager implementations of native boundary ops (inputs materialized).
 TensorP native_execute(const NativeSpec &spec, const std::vector<TensorP> &inputs);
 TensorP native_execute_model(const NativeSpec &spec, const std::vector<TensorP> &inputs);  // model_ops.cpp
+TensorP native_execute_block(const NativeSpec &spec, const std::vector<TensorP> &inputs);  // block_ops.cpp
+// A further result of the native step `main` (see NativeKind), its buffer
+// recorded before the step.
+TensorP record_buffer(const int *shape, int nd, int dtype);
+TensorP record_result(const TensorP &buffer, const TensorP &main);
+bool low_or_f32(int dt);
+bool same_shape(const Tensor &a, const Tensor &b);
+// A tensor whose last axis is read with its elements side by side: itself
+// where they lie so, else packed.  strides (of rank 3 or 4): sequence, token, head.
+TensorP head_operand(const TensorP &t, size_t strides[3]);
 bool guard(const TensorP &t);  // materialized, or an error set
 }  // namespace phpt
 
@@ -268,4 +318,7 @@ struct phpt_tensor {
 };
 struct phpt_sequences {
     phpt::SequencesP s;
+};
+struct phpt_rotary_plan {
+    phpt::RotaryP p;
 };

@@ -74,6 +74,27 @@ class PtAttentionDesc(ctypes.Structure):
                 ("scale", ctypes.c_double)]
 
 
+class PtRotaryDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("sequences", ctypes.c_int), ("tokens", ctypes.c_int),
+                ("heads", ctypes.c_int * 2), ("strides", ctypes.c_size_t * 3 * 2), ("size", ctypes.c_int),
+                ("part", ctypes.c_int), ("interleaved", ctypes.c_int), ("magnitude", ctypes.c_double),
+                ("epsilon", ctypes.c_double), ("turns", vp), ("positions", vp), ("position_strides", ctypes.c_size_t * 2)]
+
+
+class PtAdamwTensor(ctypes.Structure):
+    _fields_ = [("param", vp), ("grad", vp), ("new_param", vp), ("n", ctypes.c_size_t), ("at", ctypes.c_size_t),
+                ("param_dtype", ctypes.c_int), ("grad_dtype", ctypes.c_int), ("decay", ctypes.c_int)]
+
+
+class PtAdamwDesc(ctypes.Structure):
+    _fields_ = [("bits", ctypes.c_int)] + \
+               [(name, ctypes.c_double) for name in ("beta1", "beta2", "epsilon", "weight_decay")] + \
+               [("rate", vp), ("rate_value", ctypes.c_double)] + \
+               [(name, vp) for name in ("first", "second", "new_first", "new_second", "master", "new_master", "power1",
+                                        "power2", "new_power1", "new_power2", "first_exponent", "second_exponent",
+                                        "new_first_exponent", "new_second_exponent", "draws", "new_draws")]
+
+
 # name -> (restype, argtypes); every function declared in include/pt_hip.h
 SIGNATURES = {
     "pt_init": (ctypes.c_int, []),
@@ -134,6 +155,11 @@ SIGNATURES = {
     "pt_attention": (ctypes.c_int, [ctypes.POINTER(PtAttentionDesc), vp, vp, vp, vp, vp, vp, vp]),
     "pt_attention_backward": (ctypes.c_int, [ctypes.POINTER(PtAttentionDesc), vp, vp, vp, vp, vp, vp, vp, ctypes.c_int,
                                              vp, vp, vp, vp]),
+    "pt_rotary": (ctypes.c_int, [ctypes.POINTER(PtRotaryDesc)] + [ctypes.POINTER(vp)] * 3 + [vp]),
+    "pt_rotary_backward": (ctypes.c_int, [ctypes.POINTER(PtRotaryDesc)] + [ctypes.POINTER(vp)] * 3 + [ctypes.c_int]
+                           + [ctypes.POINTER(vp)] * 2 + [vp]),
+    "pt_adamw": (ctypes.c_int, [ctypes.POINTER(PtAdamwDesc), ctypes.POINTER(PtAdamwTensor), ctypes.c_int, vp]),
+    "pt_adamw_moments": (ctypes.c_int, [vp] * 6 + [ctypes.c_size_t, vp]),
     "pt_matmul": (ctypes.c_int, [vp, vp, vp, ctypes.c_int, c_int_p, c_size_p, ctypes.c_int,
                                  c_int_p, c_size_p, ctypes.c_int, c_int_p, ctypes.c_int, vp]),
     "pt_matmul_tune": (ctypes.c_int, [vp, vp, vp, ctypes.c_int, c_int_p, c_size_p, ctypes.c_int,

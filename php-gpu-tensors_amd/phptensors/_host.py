@@ -52,6 +52,17 @@ SIGNATURES = {
                                                ctypes.POINTER(T)]),
     "phpt_logprobs": (ctypes.c_int, [T, T, ctypes.c_int, ctypes.POINTER(T)]),
     "phpt_logprobs_backward": (T, [T] * 8),
+    "phpt_rotary_create": (vp, [ctypes.c_int, ctypes.c_double, ctypes.c_int] + [ctypes.c_double] * 5
+                           + [ctypes.POINTER(ctypes.c_double)]),
+    "phpt_rotary_release": (None, [vp]),
+    "phpt_rotary": (ctypes.c_int, [T, T, T, vp, T, T, ctypes.c_double, ctypes.POINTER(T)]),
+    "phpt_rotary_backward": (ctypes.c_int, [T, T, T, vp, T, T, ctypes.c_double, T, T, ctypes.POINTER(T)]),
+    "phpt_adamw": (ctypes.c_int, [ctypes.POINTER(T), ctypes.POINTER(T), ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(T),
+                                  ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 4 + [T, ctypes.c_double,
+                                                                                      ctypes.POINTER(T)]),
+    "phpt_adamw_blocks": (ctypes.c_longlong, [ctypes.POINTER(T), ctypes.c_int]),
+    "phpt_adamw_masters": (T, [ctypes.POINTER(T), ctypes.c_int]),
+    "phpt_adamw_moments": (ctypes.c_int, [T, T, T, T, ctypes.POINTER(T)]),
     "phpt_matmul": (T, [T, T]),
     "phpt_tune_matmul": (T, [T, T, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_float), ctypes.c_int,
                              ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]),

@@ -38,9 +38,9 @@ class Parts:
         self._node = None
         self._grad = None
 
-    def part(self, out, name):
+    def part(self, out, name, low=False):
         """Make `out` the result that passes its gradient on under `name`."""
-        return record(out, [self], lambda g: [Gradients({name: g})], name)
+        return record(out, [self], lambda g: [Gradients({name: g})], name, low)
 
 
 class Gradients(dict):

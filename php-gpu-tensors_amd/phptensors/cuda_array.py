@@ -603,6 +603,50 @@ class CudaArray:
             AG.record(out, [self, key, value], back, "attention", low=True)
         return out
 
+    def rotary(self, plan, positions=None, key=None, scale=None, keyScale=None, epsilon=1e-6):
+        """self, the queries, turned by their positions: [tokens, heads,
+        size], or [sequences, tokens, heads, size], in float32, float16 or
+        bfloat16, heads of at most 256 elements at any strides.  With key,
+        keys of the same tokens and size with heads of their own go along and
+        the pair (queries, keys) is returned.
+
+        plan (Rotary) holds the angles; positions is int32 [tokens] or
+        [sequences, tokens], by default a sequence's tokens from 0 on.  scale
+        and keyScale ([size], the heads' dtype) normalise each head first: x /
+        sqrt(mean(x^2) + epsilon) * scale.  The gradients of queries, keys and
+        scales have their operands' dtypes."""
+        if not isinstance(plan, Rotary):
+            raise InvalidArgumentException("rotary() expects a Rotary plan")
+        given = (positions, key, scale, keyScale)
+        if any(t is not None and not isinstance(t, CudaArray) for t in given):
+            raise InvalidArgumentException("rotary() expects CudaArray positions, keys and scales")
+        lib, eps = _host.load(), float(epsilon)
+        p, k, qs, ks = (t._h if t is not None else None for t in given)
+        got = (ctypes.c_void_p * 2)()
+        if lib.phpt_rotary(self._h, k, p, plan._h, qs, ks, eps, got):
+            _host.raise_error("rotary")
+        out = [CudaArray._wrap(h) if h else None for h in got]
+        leaves = (self, key, scale, keyScale)
+        if AG.active(*leaves):
+            held = (plan, positions)  # the handles behind the call
+
+            def back(g):
+                dtypes = {t.getDtype() for t in g.values()}
+                if len(dtypes) > 1 or not dtypes <= {"float32", self.getDtype()}:
+                    g = {name: AG.cast(t, "float32") for name, t in g.items()}
+                grads = (ctypes.c_void_p * 4)()
+                if lib.phpt_rotary_backward(self._h, *(t._h if t is not None else None for t in (key, held[1])),
+                                            held[0]._h, *(t._h if t is not None else None for t in (scale, keyScale)), eps,
+                                            *(g[n]._h if n in g else None for n in ("queries", "keys")), grads):
+                    _host.raise_error("rotary gradient")
+                wrapped = [CudaArray._wrap(h) if h else None for h in grads]
+                return [gr for gr, t in zip(wrapped, leaves) if t is not None]
+            parts = AG.record(AG.Parts(), [t for t in leaves if t is not None], back, "rotary")
+            for t, name in zip(out, ("queries", "keys")):
+                if t is not None:
+                    parts.part(t, name, low=True)
+        return out[0] if key is None else (out[0], out[1])
+
     def logProbs(self, tokens, top=0):
         """Of each row of scores along the last axis (float32, float16 or
         bfloat16): "logProbs", the log of the softmax at the row's token
@@ -861,6 +905,43 @@ class Sequences:
         h = getattr(self, "_h", None)
         if h and _host._lib is not None:
             _host._lib.phpt_sequences_release(h)
+            self._h = None
+
+
+class Rotary:
+    """The angles of a rotation by position: `size` elements of a head
+    (even, 2 to 256) turn in pairs (i, i + size / 2), or (2i, 2i + 1) where
+    interleaved, by position * base^(-2i / size), or by position *
+    frequencies[i], and are scaled by `magnitude`.
+
+    factor stretches the context: without `context` every frequency is
+    divided by it; with the context that a model was trained on, those that
+    turn at most `low` times within it are, those that turn at least `high`
+    times stay, and those between go over linearly.  Checked and copied to the
+    device once; serves any number of rotary() calls."""
+
+    __slots__ = ("_h", "size", "__weakref__")
+
+    def __init__(self, size, base=10000.0, interleaved=False, factor=1.0, context=None, low=1.0, high=32.0, magnitude=1.0,
+                 frequencies=None):
+        self._h = None
+        self.size = _int32(size, "size")
+        given = None
+        if frequencies is not None:
+            frequencies = [float(f) for f in frequencies]
+            if 2 * len(frequencies) != self.size:
+                raise InvalidArgumentException("Rotary needs a frequency for each pair")
+            given = (ctypes.c_double * max(1, len(frequencies)))(*frequencies)
+        if context is not None and not float(context) > 0.0:
+            raise InvalidArgumentException("Rotary context must be finite and positive")
+        self._h = _host.check_handle(_host.load().phpt_rotary_create(
+            self.size, float(base), int(bool(interleaved)), float(factor), 0.0 if context is None else float(context),
+            float(low), float(high), float(magnitude), given), "Rotary")
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h and _host._lib is not None:
+            _host._lib.phpt_rotary_release(h)
             self._h = None
 
 

@@ -6,10 +6,13 @@ reference evaluates them (optimizer_adamw_step, optimizer.c:471-607), so a
 step inside Fusion.compile is recorded and fused like any other code, and the
 per-operation float32 rounding matches the reference's eager kernels.
 """
+import ctypes
 import math
+import numbers
 
+from . import _host
 from ._abi import InvalidArgumentException
-from .cuda_array import CudaArray
+from .cuda_array import CudaArray, _int32
 
 
 class Optimizer:
@@ -115,6 +118,93 @@ class Optimizer:
             out_v.append(self._selected(g, v, v0, False))
         return {"parameters": out_p,
                 "state": {"firstMoment": out_m, "secondMoment": out_v, "beta1Power": b1p, "beta2Power": b2p}}
+
+    # ------------------------------------------------ many tensors at once
+    _STATE = ["firstMoment", "secondMoment", "beta1Power", "beta2Power"]
+    _SMALL = ["firstExponent", "secondExponent", "draws"]
+
+    @staticmethod
+    def _handles(tensors, what):
+        tensors = list(tensors)
+        if not all(isinstance(t, CudaArray) for t in tensors):
+            raise InvalidArgumentException(f"{what} must be CudaArrays")
+        return (ctypes.c_void_p * max(1, len(tensors)))(*(t._h for t in tensors))
+
+    def initFusedState(self, parameters, bits=32, master=False, seed=0):
+        """A state for fusedStep(): the moments of all parameters in one
+        array each, [blocks, 256], a tensor's from a whole block on.  bits 32:
+        float32 moments; 8: bytes with an exponent a block (firstExponent,
+        secondExponent), rounded by numbers drawn from `seed` on (draws).
+        master: float32 masters of the parameters' values, as 16-bit
+        parameters need them for steps smaller than their rounding."""
+        if self.kind != "adamW":
+            raise InvalidArgumentException("A state over many tensors is AdamW's")
+        if bits not in (32, 8):
+            raise InvalidArgumentException("AdamW moments have 32 or 8 bits")
+        parameters = list(parameters)
+        handles, lib = self._handles(parameters, "parameters"), _host.load()
+        blocks = lib.phpt_adamw_blocks(handles, len(parameters))
+        if not parameters or blocks < 0:
+            raise InvalidArgumentException("AdamW needs parameters, and not too many elements")
+        dtype = "uint8" if bits == 8 else "float32"
+        state = {"bits": bits, "firstMoment": CudaArray.zeros([blocks, 256], dtype),
+                 "secondMoment": CudaArray.zeros([blocks, 256], dtype),
+                 "beta1Power": CudaArray.ones([1]), "beta2Power": CudaArray.ones([1])}
+        if master:
+            state["master"] = CudaArray._wrap(lib.phpt_adamw_masters(handles, len(parameters)), "masters")
+        if bits == 8:
+            state.update(firstExponent=CudaArray.full([blocks], -126, "int8"),
+                         secondExponent=CudaArray.full([blocks], -126, "int8"),
+                         draws=CudaArray.full([1], _int32(seed, "seed"), "int32"))
+        return state
+
+    def fusedStep(self, parameters, gradients, state, learningRate=None, weightDecayMask=None):
+        """step() of AdamW over all tensors in one launch, with a state of
+        initFusedState(): the new parameters and the new state.  Parameters
+        and gradients are float32, float16 or bfloat16, each tensor of its
+        own; float32 parameters with 32-bit moments get step()'s values bit for
+        bit.  16-bit parameters are rounded once from float32 arithmetic, and
+        from their masters where the state has them.  learningRate: a number,
+        or float32 [1].  An element whose gradient is NaN stays as it was."""
+        if self.kind != "adamW":
+            raise InvalidArgumentException("A step over many tensors is AdamW's")
+        parameters, gradients = list(parameters), list(gradients)
+        if not parameters or len(parameters) != len(gradients):
+            raise InvalidArgumentException("parameters and gradients must be equally sized CudaArray lists")
+        mask = [True] * len(parameters) if weightDecayMask is None else list(weightDecayMask)
+        if len(mask) != len(parameters) or not all(isinstance(m, bool) for m in mask):
+            raise InvalidArgumentException("weightDecayMask must hold a boolean for each parameter")
+        rate = self.learningRate if learningRate is None else learningRate
+        on_device = isinstance(rate, CudaArray)
+        if not on_device:
+            if isinstance(rate, bool) or not isinstance(rate, numbers.Real):
+                raise InvalidArgumentException("learningRate must be a number or a CudaArray")
+            self._nonneg(rate, "learningRate")
+        bits = state.get("bits", 32)
+        names = self._STATE + (["master"] if state.get("master") is not None else []) + (self._SMALL if bits == 8 else [])
+        if bits not in (32, 8) or any(not isinstance(state.get(n), CudaArray) for n in names):
+            raise InvalidArgumentException("fusedStep() expects a state of initFusedState()")
+        got = (ctypes.c_void_p * (len(parameters) + len(names)))()
+        if _host.load().phpt_adamw(
+                self._handles(parameters, "parameters"), self._handles(gradients, "gradients"), bytes(mask),
+                len(parameters), self._handles([state[n] for n in names], "state"), bits, int("master" in names),
+                self.beta1, self.beta2, self.epsilon, self.weightDecay, rate._h if on_device else None,
+                0.0 if on_device else float(rate), got):
+            _host.raise_error("AdamW")
+        out = [CudaArray._wrap(h) for h in got]
+        return {"parameters": out[:len(parameters)], "state": {"bits": bits, **dict(zip(names, out[len(parameters):]))}}
+
+    @staticmethod
+    def moments(state):
+        """The moments of a state of initFusedState() as float32 values,
+        [blocks, 256]: {"firstMoment", "secondMoment"}."""
+        if state.get("bits", 32) == 32:
+            return {n: state[n] for n in ("firstMoment", "secondMoment")}
+        got = (ctypes.c_void_p * 2)()
+        if _host.load().phpt_adamw_moments(*(state[n]._h for n in ("firstMoment", "firstExponent", "secondMoment",
+                                                                   "secondExponent")), got):
+            _host.raise_error("moments")
+        return dict(zip(("firstMoment", "secondMoment"), map(CudaArray._wrap, got)))
 
     def _sgd(self, parameters, gradients, state, lr, mask):
         """optimizer_sgd_step (optimizer.c:609-676): the velocity g + v·momentum
