@@ -390,6 +390,32 @@ pt_status pt_rotary_backward(const pt_rotary_desc *desc, const void *const *x, c
                              const void *const *grad, int grad_dtype, void *const *dx, void *const *dscale,
                              pt_stream_t stream);
 
+/* ------------------------------------------------------ gated projection --
+ * No counterpart in the reference.  h = act(x gate) * (x up), x [rows][inner],
+ * gate and up [inner][outer], all contiguous and of one dtype (float32,
+ * float16, bfloat16); both products are summed and taken through the
+ * activation in fp32 and h is rounded once. */
+#define PT_GATE_SILU 0     /* g / (1 + exp(-g)) */
+#define PT_GATE_GELU 1     /* g (1 + erf(g / sqrt 2)) / 2 */
+#define PT_GATE_RELU 2
+#define PT_GATE_SIGMOID 3
+typedef struct {
+    int dtype, activation;
+    int rows, inner, outer;   /* each at most 2^21 */
+} pt_gated_desc;
+/* kept (may be NULL): [2][rows][outer], both products rounded to the dtype,
+ * for the backward call.  Results must not overlap operands, here and in
+ * the backward call. */
+pt_status pt_gated(const pt_gated_desc *desc, const void *x, const void *gate, const void *up, void *h, void *kept,
+                   pt_stream_t stream);
+/* Gradients, contiguous and of the dtype, for the upstream gradient `grad`
+ * (contiguous like h, float32 or the dtype): dx, and dgate with dup; dx may
+ * be NULL, or dgate and dup both.  In 16 bits the products' gradients are
+ * rounded to the dtype for the products that follow.  Results do not depend
+ * on timing. */
+pt_status pt_gated_backward(const pt_gated_desc *desc, const void *x, const void *gate, const void *up, const void *kept,
+                            const void *grad, int grad_dtype, void *dx, void *dgate, void *dup, pt_stream_t stream);
+
 /* ----------------------------------------------------------------- AdamW --
  * No counterpart in the reference, whose step is composed of tensor
  * operations (src/optimizer.c:471-607).  One step over many tensors.  The

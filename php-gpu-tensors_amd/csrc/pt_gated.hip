@@ -1,0 +1,570 @@
+// Gated projection h = act(x gate) * (x up) and its gradients for gfx950:
+//   dg = dh u act'(g),  du = dh act(g)   (g, u: the two products)
+//   dx = dg gate^T + du up^T,  dgate = x^T dg,  dup = x^T du.
+// Forms, by the rows and the type:
+//   16 bits, more than 32 rows: products over a pair of matrices in one
+//     kernel (pt_gated_ring.hip), bound by the matrix cores.
+//   32 rows or fewer: k_gated_few, bound by the weights' bytes.
+//   float32, more rows: the framework's fp32 products (94 % of the matrix
+//     cores' rate) and a pass over both results; fusing would save that
+//     pass, 2 % of the time at 4096 inner elements.
+#include "pt_gated.h"
+
+#include <algorithm>
+
+namespace pt {
+
+// ------------------------------------------------------------- few rows
+// The weights stream once, in place and at any alignment.  A wave owns a
+// strip of columns of both matrices (a 16-byte pack in each of 16 lanes: 128
+// columns in 16 bits, 64 in 32) and takes steps of 32 k: lane l loads 8 rows,
+// k = 8 (l / 16) .. + 7, of both.  16 bits: those are an 8 x 8 block, whose
+// columns, brought side by side by byte permutations (half an instruction
+// per element), are the B operands of 8 16x16x32 MFMAs, the c-th of which
+// yields each lane's column c; x, 16 rows of it, is the A operand as it
+// lies.  32 bits: each loaded row is the B operand of 4 16x16x4 MFMAs.  So no
+// weight passes through LDS, and the next step's 16 loads are in flight over
+// this step's MFMAs.  The k-steps go to the 8 waves of a block and to S
+// blocks in turn; the waves' sums meet in LDS, in a fixed order, and the
+// blocks' in a second kernel.
+constexpr int kFewWaves = 8;
+typedef unsigned gd_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
+
+template <int DT, int MT>
+__global__ __launch_bounds__(64 * kFewWaves) void k_gated_few(PairArgs g)
+{
+    using S = typename GE<DT>::S;
+    constexpr int NC = 16 / sizeof(S);  // columns of a lane
+    constexpr bool LOW = DT != PT_FLOAT32;
+    __shared__ float box[kFewWaves / 2][2 * NC * 4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = lane >> 4, n0 = blockIdx.x * 16 * NC + (lane & 15) * NC, at = min(n0, g.N - NC);
+    const S *B[2] = {(const S *)g.b0 + at, (const S *)g.b1 + at};
+    const S *x[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) x[m] = (const S *)g.a0 + (long long)min(m * 16 + (lane & 15), g.M - 1) * g.lda;
+
+    floatx4 acc[MT][2][NC];
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) acc[m][j][c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // rows past K: the last one again, taken as zeros below
+    gd_u32x4 w[2][8], xv[MT][LOW ? 1 : 2];
+    auto load = [&](int k0, gd_u32x4 (&w)[2][8], gd_u32x4 (&xv)[MT][LOW ? 1 : 2]) {
+        const int k = k0 + kg * 8;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                w[j][i] = __builtin_nontemporal_load((const gd_u32x4 *)(B[j] + (long long)min(k + i, g.K - 1) * g.ldb));
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int q = 0; q < (LOW ? 1 : 2); q++) {
+                const int kx = k + q * NC;
+                if (kx + NC <= g.K) xv[m][q] = *(const gd_u32x4 *)(x[m] + kx);
+                else {
+                    union { gd_u32x4 raw; S s[NC]; } u;
+#pragma unroll
+                    for (int c = 0; c < NC; c++) u.s[c] = kx + c < g.K ? x[m][kx + c] : (S)0;
+                    xv[m][q] = u.raw;
+                }
+            }
+    };
+    auto multiply = [&](int k0, gd_u32x4 (&w)[2][8], gd_u32x4 (&xv)[MT][LOW ? 1 : 2]) {
+        if (k0 + 32 > g.K) {  // uniform: what the last step has past K is zeros
+            const int k = k0 + kg * 8;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int d = 0; d < 4; d++) w[j][i][d] = k + i < g.K ? w[j][i][d] : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if constexpr (LOW) {
+                using Frag = typename FragT<DT>::type;
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        gd_u32x4 col;
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            col[i] = __builtin_amdgcn_perm(w[j][2 * i + 1][d], w[j][2 * i][d], h ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                        for (int m = 0; m < MT; m++) {
+                            floatx4 &to = acc[m][j][2 * d + h];
+                            const Frag fx = __builtin_bit_cast(Frag, xv[m][0]), fw = __builtin_bit_cast(Frag, col);
+                            if constexpr (DT == PT_BFLOAT16) to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fw, to, 0, 0, 0);
+                            else to = __builtin_amdgcn_mfma_f32_16x16x32_f16(fx, fw, to, 0, 0, 0);
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+#pragma unroll
+                        for (int c = 0; c < NC; c++)
+                            acc[m][j][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(xv[m][i / 4][i % 4]),
+                                                                                __uint_as_float(w[j][i][c]), acc[m][j][c], 0, 0, 0);
+            }
+        }
+    };
+    const int step = 32 * kFewWaves * g.split;
+    int k0 = 32 * ((int)blockIdx.y * kFewWaves + wave);
+    if (k0 < g.K) {
+        load(k0, w, xv);
+        for (;;) {
+            gd_u32x4 wn[2][8], xn[MT][LOW ? 1 : 2];
+            const bool more = k0 + step < g.K;
+            if (more) load(k0 + step, wn, xn);
+            multiply(k0, w, xv);
+            if (!more) break;
+            k0 += step;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[j][i] = wn[j][i];
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int q = 0; q < (LOW ? 1 : 2); q++) xv[m][q] = xn[m][q];
+        }
+    }
+    // waves w + half add to waves w, half = 4, 2, 1
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+        for (int half = kFewWaves / 2; half; half >>= 1) {
+            __syncthreads();
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int c = 0; c < NC; c++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) box[wave - half][(j * NC + c) * 4 + e][lane] = acc[m][j][c][e];
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int c = 0; c < NC; c++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[m][j][c][e] += box[wave][(j * NC + c) * 4 + e][lane];
+            }
+        }
+    if (wave || n0 >= g.n_out) return;
+    // lane: rows 4 (l / 16) + e, columns at .. at + NC - 1.  The lane whose
+    // pack was moved back from the end stores what its neighbour stores too.
+    const long long plane = (long long)g.M * g.n_out;
+    const int live = min(NC, g.n_out - at);
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int row = m * 16 + kg * 4 + e;
+            if (row >= g.M) continue;
+            const long long to = (long long)row * g.n_out + at;
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                if (c >= live) continue;
+                const float p = acc[m][0][c][e], q = acc[m][1][c][e];
+                if (g.split > 1) {
+                    float *part = g.parts + (long long)blockIdx.y * 2 * plane + to + c;
+                    part[0] = p;
+                    part[plane] = q;
+                    continue;
+                }
+                if (g.c1) {
+                    store_c<DT>(g.c1, (size_t)(to + c), p);
+                    store_c<DT>(g.c2, (size_t)(to + c), q);
+                }
+                store_c<DT>(g.c0, (size_t)(to + c), gated_act<LOW>(g.act, p) * q);
+            }
+        }
+}
+
+// ------------------------------------------------- passes over elements
+// h of fp32 products that lie behind each other.
+__global__ __launch_bounds__(256) void k_gated_product(const float *p, float *h, long long n, int act)
+{
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (i + k < n) h[i + k] = gated_act<false>(act, p[i + k]) * p[n + i + k];
+}
+
+// V elements from p at any element boundary
+template <int DT, int V>
+__device__ __forceinline__ void gd_load(const typename GE<DT>::S *p, int live, float (&v)[V])
+{
+    using S = typename GE<DT>::S;
+    if (live >= V) {
+#pragma unroll
+        for (int q = 0; q < V / GE<DT>::PK; q++) {
+            union { gd_u32x4 raw; S s[GE<DT>::PK]; } u;
+            u.raw = *(const gd_u32x4 *)(p + q * GE<DT>::PK);
+#pragma unroll
+            for (int k = 0; k < GE<DT>::PK; k++) v[q * GE<DT>::PK + k] = DType<DT>::to_c(u.s[k]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < V; k++) v[k] = k < live ? DType<DT>::to_c(p[k]) : 0.0f;
+}
+
+// dg and du from the upstream gradient and both products, into rows `pitch`
+// elements apart from d and d + second on, zeros in columns `cols` to
+// `padded` - 1.  A thread takes 8 columns.
+template <int DT, int GDT>
+__global__ __launch_bounds__(256) void k_gated_slope(const void *kept, const void *grad, void *d, long long second, int rows,
+                                                     int cols, int padded, int pitch, int act)
+{
+    using S = typename GE<DT>::S;
+    const int packs = (cols + 7) / 8;
+    const long long total = (long long)rows * packs, plane = (long long)rows * cols;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long row = i / packs;
+        const int c = (int)(i - row * packs) * 8, live = min(8, cols - c);
+        const long long from = row * cols + c;
+        float g[8], u[8], dh[8];
+        gd_load<DT, 8>((const S *)kept + from, live, g);
+        gd_load<DT, 8>((const S *)kept + plane + from, live, u);
+        gd_load<GDT, 8>((const typename GE<GDT>::S *)grad + from, live, dh);
+        S dg[8], du[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            float value, slope;
+            gated_slope<DT != PT_FLOAT32>(act, g[k], value, slope);
+            dg[k] = DType<DT>::from_c(k < live ? dh[k] * u[k] * slope : 0.0f);
+            du[k] = DType<DT>::from_c(k < live ? dh[k] * value : 0.0f);
+        }
+        S *to = (S *)d + row * pitch + c;
+        const int room = min(8, padded - c);
+        if (room == 8) {
+#pragma unroll
+            for (int q = 0; q < 8 / GE<DT>::PK; q++) {
+                *(gd_u32x4 *)(to + q * GE<DT>::PK) = *(gd_u32x4 *)(dg + q * GE<DT>::PK);
+                *(gd_u32x4 *)(to + second + q * GE<DT>::PK) = *(gd_u32x4 *)(du + q * GE<DT>::PK);
+            }
+        } else {
+            for (int k = 0; k < room; k++) {
+                to[k] = dg[k];
+                to[second + k] = du[k];
+            }
+        }
+    }
+}
+
+// two fp32 matrices side by side
+__global__ __launch_bounds__(256) void k_gated_beside(const float *a, const float *b, float *to, int rows, int cols)
+{
+    const long long n = (long long)rows * cols;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long row = i / cols, at = i + row * cols;
+        to[at] = a[i];
+        to[at + cols] = b[i];
+    }
+}
+
+// rows x cols of 16-bit elements into rows of `pitch`, zeros past the end
+__global__ __launch_bounds__(256) void k_gated_pack(const uint16_t *from, uint16_t *to, long long rows, int cols, int pitch)
+{
+    const int packs = pitch / 8;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * packs; i += (long long)gridDim.x * 256) {
+        const long long row = i / packs;
+        const int c = (int)(i - row * packs) * 8, live = cols - c;
+        union { gd_u32x4 raw; uint16_t s[8]; } u;
+        if (live >= 8) u.raw = *(const gd_u32x4 *)(from + row * cols + c);
+        else
+#pragma unroll
+            for (int k = 0; k < 8; k++) u.s[k] = k < live ? from[row * cols + c + k] : (uint16_t)0;
+        *(gd_u32x4 *)(to + row * pitch + c) = u.raw;
+    }
+}
+
+// The transpose of rows x cols 16-bit elements, in rows of `pitch` (a
+// multiple of 8, zeros past `rows`): 64 x 64 tiles through LDS.
+__global__ __launch_bounds__(256) void k_gated_transpose(const uint16_t *from, uint16_t *to, int rows, int cols, int pitch)
+{
+    __shared__ uint16_t tile[64][66];
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, a = threadIdx.x & 7, b = threadIdx.x >> 3;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int r = r0 + b + 32 * h, c = c0 + a * 8;
+        union { gd_u32x4 raw; uint16_t s[8]; } u;
+        if (r < rows && c + 8 <= cols) u.raw = *(const gd_u32x4 *)(from + (long long)r * cols + c);
+        else
+#pragma unroll
+            for (int k = 0; k < 8; k++) u.s[k] = r < rows && c + k < cols ? from[(long long)r * cols + c + k] : (uint16_t)0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) tile[a * 8 + k][b + 32 * h] = u.s[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int c = c0 + b + 32 * h, r = r0 + a * 8;
+        if (c >= cols || r >= pitch) continue;  // (pitch and r are multiples of 8)
+        union { gd_u32x4 raw; uint16_t s[8]; } u;
+#pragma unroll
+        for (int k = 0; k < 8; k++) u.s[k] = tile[b + 32 * h][a * 8 + k];
+        *(gd_u32x4 *)(to + (long long)c * pitch + r) = u.raw;
+    }
+}
+
+// ------------------------------------------------------------- the calls
+static int round8(int n) { return (n + 7) / 8 * 8; }
+static unsigned grid_for(long long items) { return (unsigned)std::min<long long>((items + 255) / 256, 1 << 20); }
+
+// Scratch of one call, given back in the stream's order.
+struct GatedScratch {
+    hipStream_t s;
+    void *held[8];
+    int count = 0;
+    explicit GatedScratch(hipStream_t stream) : s(stream) {}
+    ~GatedScratch()
+    {
+        while (count) scratch_free(held[--count], s);
+    }
+    pt_status take(void **p, size_t bytes)
+    {
+        PT_TRY(scratch_alloc(p, bytes, s));
+        held[count++] = *p;
+        return PT_OK;
+    }
+    // a 16-bit matrix whose rows start at 16-byte boundaries: itself, or a copy
+    pt_status rows16(const void *from, long long rows, int cols, const void **to, long long *pitch)
+    {
+        *pitch = round8(cols);
+        *to = from;
+        if (cols % 8 == 0 && ((uintptr_t)from & 15) == 0) return PT_OK;
+        void *p = nullptr;
+        PT_TRY(take(&p, (size_t)rows * *pitch * 2));
+        k_gated_pack<<<grid_for(rows * (*pitch / 8)), 256, 0, s>>>((const uint16_t *)from, (uint16_t *)p, rows, cols, (int)*pitch);
+        *to = p;
+        return PT_OK;
+    }
+};
+
+static pt_status gated_check(const pt_gated_desc *d)
+{
+    if (!d) return fail(PT_ERR_INVALID, "gated projection description missing");
+    if (d->dtype != PT_FLOAT32 && d->dtype != PT_FLOAT16 && d->dtype != PT_BFLOAT16)
+        return fail(PT_ERR_INVALID, "gated projection takes float32, float16 or bfloat16");
+    if (d->activation < PT_GATE_SILU || d->activation > PT_GATE_SIGMOID)
+        return fail(PT_ERR_INVALID, "gated projection activation %d is not known", d->activation);
+    if (d->rows < 0 || d->inner < 0 || d->outer < 0) return fail(PT_ERR_INVALID, "gated projection sizes must not be negative");
+    if (d->rows > kPairPitch || d->inner > kPairPitch || d->outer > kPairPitch)
+        return fail(PT_ERR_UNSUPPORTED, "gated projection takes at most %lld rows, and elements in each", kPairPitch);
+    return PT_OK;
+}
+
+static pt_status zeros(void *p, int dtype, size_t n, pt_stream_t stream)
+{
+    const pt_scalar_t zero = {{0.0}, dtype};
+    return p && n ? pt_fill(p, dtype, n, &zero, stream) : PT_OK;
+}
+
+// C = A B, fp32, strides in elements
+static pt_status product_f32(const float *a, size_t am, size_t ak, const float *b, size_t bk, size_t bn, float *c, int m, int n,
+                             int k, pt_stream_t stream)
+{
+    const int sa[2] = {m, k}, sb[2] = {k, n}, sc[2] = {m, n};
+    const size_t ta[2] = {am, ak}, tb[2] = {bk, bn};
+    return pt_matmul(a, b, c, PT_FLOAT32, sa, ta, 2, sb, tb, 2, sc, 2, stream);
+}
+
+// Blocks that a strip's k-steps are split over: up to a block for every CU.
+template <int DT>
+static pt_status launch_few(PairArgs &g, GatedScratch &scratch, hipStream_t s)
+{
+    constexpr int COLS = 16 * GE<DT>::PK;
+    const int strips = (g.n_out + COLS - 1) / COLS, steps = (g.K + 31) / 32;
+    g.split = std::max(1, std::min({256 / strips, steps / kFewWaves, 16}));
+    if (g.split > 1) PT_TRY(scratch.take((void **)&g.parts, (size_t)g.split * 2 * g.M * g.n_out * sizeof(float)));
+    const dim3 grid(strips, g.split);
+    if (g.M <= 16) k_gated_few<DT, 1><<<grid, 64 * kFewWaves, 0, s>>>(g);
+    else k_gated_few<DT, 2><<<grid, 64 * kFewWaves, 0, s>>>(g);
+    if (g.split > 1) launch_pair_join(g, DT, g.c1 ? GATED_KEPT : GATED_PRODUCT, s);
+    return PT_OK;
+}
+
+static pt_status gated_run(const pt_gated_desc *d, const void *x, const void *gate, const void *up, void *h, void *kept,
+                           pt_stream_t stream)
+{
+    hipStream_t s = stream_of(stream);
+    GatedScratch scratch(s);
+    const int M = d->rows, K = d->inner, F = d->outer;
+    const size_t size = dtype_size(d->dtype), n = (size_t)M * F;
+    void *second = kept ? (char *)kept + n * size : nullptr;
+    PairArgs g = {};
+    g.M = M;
+    g.act = d->activation;
+    g.n_out = F;
+    g.c0 = h;
+    g.c1 = kept;
+    g.c2 = second;
+    g.a0 = x;
+    g.b0 = gate;
+    g.b1 = up;
+    g.lda = K;
+    g.ldb = g.N = F;
+    g.K = g.kb = K;
+    const int pack = (int)(16 / size);
+    if (M <= 32 && F >= pack) {
+        if (d->dtype == PT_FLOAT32) return launch_few<PT_FLOAT32>(g, scratch, s);
+        return d->dtype == PT_FLOAT16 ? launch_few<PT_FLOAT16>(g, scratch, s) : launch_few<PT_BFLOAT16>(g, scratch, s);
+    }
+    if (d->dtype == PT_FLOAT32) {
+        float *p = (float *)kept;
+        if (!p) PT_TRY(scratch.take((void **)&p, 2 * n * sizeof(float)));
+        PT_TRY(product_f32((const float *)x, K, 1, (const float *)gate, F, 1, p, M, F, K, stream));
+        PT_TRY(product_f32((const float *)x, K, 1, (const float *)up, F, 1, p + n, M, F, K, stream));
+        k_gated_product<<<grid_for((long long)(n + 3) / 4), 256, 0, s>>>(p, (float *)h, (long long)n, d->activation);
+        return PT_OK;
+    }
+    PT_TRY(scratch.rows16(x, M, K, &g.a0, &g.lda));
+    PT_TRY(scratch.rows16(gate, K, F, &g.b0, &g.ldb));
+    PT_TRY(scratch.rows16(up, K, F, &g.b1, &g.ldb));
+    // (of K rounded to 8, A's elements past K are zeros or B's rows past it are out of range)
+    g.K = round8(K);
+    g.N = (int)g.ldb;
+    int tm;
+    pair_plan(g, true, tm);
+    if (g.split > 1) PT_TRY(scratch.take((void **)&g.parts, (size_t)g.split * 2 * n * sizeof(float)));
+    launch_pair_columns(g, d->dtype, tm, kept ? GATED_KEPT : GATED_PRODUCT, s);
+    return PT_OK;
+}
+
+static pt_status gated_backward_f32(const pt_gated_desc *d, const float *x, const float *gate, const float *up, const void *kept,
+                                    const void *grad, float *dx, float *dgate, float *dup, GatedScratch &scratch, pt_stream_t stream)
+{
+    hipStream_t s = stream_of(stream);
+    const int M = d->rows, K = d->inner, F = d->outer;
+    // dg and du side by side: one product takes both contractions of dx
+    float *both = nullptr, *weights = nullptr;
+    PT_TRY(scratch.take((void **)&both, (size_t)M * 2 * F * sizeof(float)));
+    k_gated_slope<PT_FLOAT32, PT_FLOAT32><<<grid_for((long long)M * ((F + 7) / 8)), 256, 0, s>>>(kept, grad, both, F, M, F, F, 2 * F,
+                                                                                              d->activation);
+    if (dx) {
+        PT_TRY(scratch.take((void **)&weights, (size_t)K * 2 * F * sizeof(float)));
+        k_gated_beside<<<grid_for((long long)K * F), 256, 0, s>>>(gate, up, weights, K, F);
+        PT_TRY(product_f32(both, 2 * F, 1, weights, 1, 2 * F, dx, M, K, 2 * F, stream));
+    }
+    if (dgate) {
+        PT_TRY(product_f32(x, 1, K, both, 2 * F, 1, dgate, K, F, M, stream));
+        PT_TRY(product_f32(x, 1, K, both + F, 2 * F, 1, dup, K, F, M, stream));
+    }
+    return PT_OK;
+}
+
+static pt_status gated_backward_run(const pt_gated_desc *d, const void *x, const void *gate, const void *up, const void *kept,
+                                    const void *grad, int grad_dtype, void *dx, void *dgate, void *dup, pt_stream_t stream)
+{
+    hipStream_t s = stream_of(stream);
+    GatedScratch scratch(s);
+    const int M = d->rows, K = d->inner, F = d->outer, pitch = round8(F);
+    if (d->dtype == PT_FLOAT32)
+        return gated_backward_f32(d, (const float *)x, (const float *)gate, (const float *)up, kept, grad, (float *)dx,
+                                  (float *)dgate, (float *)dup, scratch, stream);
+    uint16_t *dg = nullptr;
+    const long long second = (long long)M * pitch;
+    PT_TRY(scratch.take((void **)&dg, (size_t)second * 2 * 2));
+    const unsigned blocks = grid_for((long long)M * (pitch / 8));
+    const bool same = grad_dtype == d->dtype;
+    if (d->dtype == PT_BFLOAT16) {
+        if (same) k_gated_slope<PT_BFLOAT16, PT_BFLOAT16><<<blocks, 256, 0, s>>>(kept, grad, dg, second, M, F, pitch, pitch, d->activation);
+        else k_gated_slope<PT_BFLOAT16, PT_FLOAT32><<<blocks, 256, 0, s>>>(kept, grad, dg, second, M, F, pitch, pitch, d->activation);
+    } else {
+        if (same) k_gated_slope<PT_FLOAT16, PT_FLOAT16><<<blocks, 256, 0, s>>>(kept, grad, dg, second, M, F, pitch, pitch, d->activation);
+        else k_gated_slope<PT_FLOAT16, PT_FLOAT32><<<blocks, 256, 0, s>>>(kept, grad, dg, second, M, F, pitch, pitch, d->activation);
+    }
+    int tm;
+    if (dx) {
+        PairArgs g = {};
+        g.a0 = dg;
+        g.a1 = dg + second;
+        g.lda = pitch;
+        PT_TRY(scratch.rows16(gate, K, F, &g.b0, &g.ldb));
+        PT_TRY(scratch.rows16(up, K, F, &g.b1, &g.ldb));
+        g.M = M;
+        g.N = g.n_out = K;
+        g.K = pitch;
+        g.c0 = dx;
+        pair_plan(g, false, tm);
+        if (g.split > 1) PT_TRY(scratch.take((void **)&g.parts, (size_t)g.split * M * K * sizeof(float)));
+        launch_pair_sum(g, d->dtype, tm, s);
+    }
+    if (dgate) {
+        PairArgs g = {};
+        const int across = round8(M);
+        uint16_t *xt = nullptr;
+        PT_TRY(scratch.take((void **)&xt, (size_t)K * across * 2));
+        k_gated_transpose<<<dim3((K + 63) / 64, (across + 63) / 64), 256, 0, s>>>((const uint16_t *)x, xt, M, K, across);
+        g.a0 = xt;
+        g.lda = g.K = across;
+        g.kb = M;
+        g.b0 = dg;
+        g.b1 = dg + second;
+        g.ldb = g.N = pitch;
+        g.n_out = F;
+        g.M = K;
+        g.c1 = dgate;
+        g.c2 = dup;
+        pair_plan(g, true, tm);
+        if (g.split > 1) PT_TRY(scratch.take((void **)&g.parts, (size_t)g.split * 2 * K * F * sizeof(float)));
+        launch_pair_columns(g, d->dtype, tm, GATED_BOTH, s);
+    }
+    return PT_OK;
+}
+
+}  // namespace pt
+
+using namespace pt;
+
+extern "C" {
+
+pt_status pt_gated(const pt_gated_desc *d, const void *x, const void *gate, const void *up, void *h, void *kept,
+                   pt_stream_t stream)
+{
+    PT_TRY(gated_check(d));
+    const size_t n = (size_t)d->rows * d->outer;
+    if (n && (!h || (d->inner && (!x || !gate || !up)))) return fail(PT_ERR_INVALID, "gated projection misses an operand");
+    PT_TRY(ensure_init());
+    if (!n) return PT_OK;
+    if (!d->inner) {  // empty sums: act(0) 0
+        PT_TRY(zeros(kept, d->dtype, 2 * n, stream));
+        return zeros(h, d->dtype, n, stream);
+    }
+    PT_TRY(gated_run(d, x, gate, up, h, kept, stream));
+    return check_hip(hipGetLastError(), "gated projection");
+}
+
+pt_status pt_gated_backward(const pt_gated_desc *d, const void *x, const void *gate, const void *up, const void *kept,
+                            const void *grad, int grad_dtype, void *dx, void *dgate, void *dup, pt_stream_t stream)
+{
+    PT_TRY(gated_check(d));
+    if (grad_dtype != d->dtype && grad_dtype != PT_FLOAT32)
+        return fail(PT_ERR_INVALID, "the gated projection's upstream gradient must be float32 or of its dtype");
+    if (!dgate != !dup || (!dx && !dgate)) return fail(PT_ERR_INVALID, "gated projection gradient misses a result");
+    const bool some = d->rows && d->inner && d->outer;
+    if (some && (!x || !gate || !up || !kept || !grad)) return fail(PT_ERR_INVALID, "gated projection gradient misses an operand");
+    PT_TRY(ensure_init());
+    if (!some) {  // empty sums
+        PT_TRY(zeros(dx, d->dtype, (size_t)d->rows * d->inner, stream));
+        PT_TRY(zeros(dgate, d->dtype, (size_t)d->inner * d->outer, stream));
+        return zeros(dup, d->dtype, (size_t)d->inner * d->outer, stream);
+    }
+    PT_TRY(gated_backward_run(d, x, gate, up, kept, grad, grad_dtype, dx, dgate, dup, stream));
+    return check_hip(hipGetLastError(), "gated projection gradient");
+}
+
+}  // extern "C"

@@ -1,5 +1,6 @@
 // Dispatch of the operators around a block's matrix products: the rotation
-// of queries and keys, and the AdamW step over many tensors.  As in
+// of queries and keys, the gated projection, and the AdamW step over many
+// tensors.  As in
 // model_ops.cpp, each checks its operands, allocates its results and
 // launches through the C-ABI, or records one native step in a Fusion scope.
 #include "runtime.hpp"
@@ -258,6 +259,157 @@ bool cuda_array_rotary_backward(const TensorP &q, const TensorP &k, const Tensor
             if (!out[i]) return false;
         }
     return rotary_backward_run(q, k, positions, plan, qs, ks, eps, gq, gk, out);
+}
+
+// -------------------------------------------------------- gated projection
+static bool gated_desc(const TensorP &x, const TensorP &gate, const TensorP &up, int activation, pt_gated_desc &d)
+{
+    if (!x || !gate || !up) {
+        set_invalid("Missing tensor operand");
+        return false;
+    }
+    if (!low_or_f32(x->dtype) || gate->dtype != x->dtype || up->dtype != x->dtype) {
+        set_invalid("gatedProjection requires matching float32, float16 or bfloat16 operands");
+        return false;
+    }
+    if (x->ndims < 1 || gate->ndims != 2 || !same_shape(*gate, *up) || gate->shape[0] != x->shape[x->ndims - 1]) {
+        set_invalid("gatedProjection requires [.., inner] and two matrices [inner, outer] of one shape");
+        return false;
+    }
+    if (activation < PT_GATE_SILU || activation > PT_GATE_SIGMOID) {
+        set_invalid("gatedProjection activations are silu, gelu, relu and sigmoid");
+        return false;
+    }
+    long long rows = 1;
+    bool none = false;
+    for (int i = 0; i + 1 < x->ndims; i++) none = none || !x->shape[i];
+    for (int i = 0; !none && i + 1 < x->ndims && rows <= 1 << 21; i++) rows *= x->shape[i];
+    if (none) rows = 0;
+    if (rows > 1 << 21 || gate->shape[0] > 1 << 21 || gate->shape[1] > 1 << 21) {
+        set_invalid("gatedProjection takes at most %d rows, and elements in each", 1 << 21);
+        return false;
+    }
+    memset(&d, 0, sizeof(d));
+    d.dtype = x->dtype;
+    d.activation = activation;
+    d.rows = (int)rows;
+    d.inner = gate->shape[0];
+    d.outer = gate->shape[1];
+    return true;
+}
+
+static int gated_shape(const Tensor &x, const Tensor &gate, int *shape)
+{
+    std::copy(x.shape, x.shape + x.ndims, shape);
+    shape[x.ndims - 1] = gate.shape[1];
+    return x.ndims;
+}
+
+static bool gated_run(const TensorP &x, const TensorP &gate, const TensorP &up, int activation, const TensorP &h,
+                      const TensorP &kept)
+{
+    pt_gated_desc d;
+    if (!gated_desc(x, gate, up, activation, d)) return false;
+    TensorP a = materialize(x), b = materialize(gate), c = materialize(up);
+    if (!a || !b || !c) return false;
+    return check_status(pt_gated(&d, a->data(), b->data(), c->data(), h->data(), kept ? kept->data() : nullptr, nullptr),
+                        "Gated projection kernel failed");
+}
+
+bool cuda_array_gated(const TensorP &x, const TensorP &gate, const TensorP &up, int activation, bool keep, TensorP out[2])
+{
+    pt_gated_desc d;
+    if (!gated_desc(x, gate, up, activation, d)) return false;
+    int shape[kMaxDims];
+    const int nd = gated_shape(*x, *gate, shape), both[3] = {2, d.rows, d.outer};
+    out[1] = nullptr;
+    if (fusion_active()) {
+        NativeSpec sp;
+        sp.kind = NAT_GATED;
+        sp.activation = activation;
+        std::vector<TensorP> ins = {x, gate, up};
+        TensorP box = keep ? record_buffer(both, 3, x->dtype) : nullptr;
+        if (keep && !box) return false;
+        if (box) ins.push_back(box);
+        out[0] = fusion_record_native(sp, ins, shape, nd, x->dtype);
+        if (out[0] && box) out[1] = record_result(box, out[0]);
+        return out[0] && (!keep || out[1]);
+    }
+    if (!guard(x) || !guard(gate) || !guard(up)) return false;
+    out[0] = output_tensor(shape, nd, x->dtype);
+    if (out[0] && keep) out[1] = make_empty(both, 3, x->dtype);
+    if (!out[0] || (keep && !out[1])) return false;
+    return gated_run(x, gate, up, activation, out[0], out[1]);
+}
+
+static bool gated_backward_run(const TensorP &x, const TensorP &gate, const TensorP &up, const TensorP &kept,
+                               const TensorP &grad, int activation, const TensorP *out)
+{
+    pt_gated_desc d;
+    if (!gated_desc(x, gate, up, activation, d)) return false;
+    TensorP a = materialize(x), b = materialize(gate), c = materialize(up), k = materialize(kept), g = materialize(grad);
+    if (!a || !b || !c || !k || !g) return false;
+    auto at = [](const TensorP &t) -> void * { return t ? t->data() : nullptr; };
+    return check_status(pt_gated_backward(&d, a->data(), b->data(), c->data(), k->data(), g->data(), g->dtype, at(out[0]),
+                                          at(out[1]), at(out[2]), nullptr),
+                        "Gated projection gradient kernel failed");
+}
+
+// Results in order; the first of those wanted is the native step's own.
+enum { GATED_X = 1, GATED_WEIGHTS = 2 };
+
+bool cuda_array_gated_backward(const TensorP &x, const TensorP &gate, const TensorP &up, const TensorP &kept,
+                               const TensorP &grad, int activation, bool want_x, bool want_weights, TensorP out[3])
+{
+    pt_gated_desc d;
+    if (!gated_desc(x, gate, up, activation, d)) return false;
+    int shape[kMaxDims];
+    const int nd = gated_shape(*x, *gate, shape);
+    if (!kept || kept->dtype != x->dtype || kept->ndims != 3 || kept->shape[0] != 2 || kept->shape[1] != d.rows ||
+        kept->shape[2] != d.outer) {
+        set_invalid("gatedProjection gradients need the forward pass's products");
+        return false;
+    }
+    if (!grad || grad->ndims != nd || !std::equal(shape, shape + nd, grad->shape) ||
+        (grad->dtype != x->dtype && grad->dtype != PT_FLOAT32)) {
+        set_invalid("gatedProjection's upstream gradient must have the output's shape, in float32 or its dtype");
+        return false;
+    }
+    if (!want_x && !want_weights) {
+        set_invalid("gatedProjection gradients: none is wanted");
+        return false;
+    }
+    const TensorP want[3] = {want_x ? x : nullptr, want_weights ? gate : nullptr, want_weights ? up : nullptr};
+    const int first = want_x ? 0 : 1;
+    for (int i = 0; i < 3; i++) out[i] = nullptr;
+    if (fusion_active()) {
+        NativeSpec sp;
+        sp.kind = NAT_GATED_BACKWARD;
+        sp.activation = activation;
+        sp.given = (want_x ? GATED_X : 0) | (want_weights ? GATED_WEIGHTS : 0);
+        std::vector<TensorP> ins = {x, gate, up, kept, grad};
+        TensorP box[3];
+        for (int i = first + 1; i < 3; i++)
+            if (want[i]) {
+                box[i] = record_buffer(want[i]->shape, want[i]->ndims, want[i]->dtype);
+                if (!box[i]) return false;
+                ins.push_back(box[i]);
+            }
+        out[first] = fusion_record_native(sp, ins, want[first]->shape, want[first]->ndims, x->dtype);
+        if (!out[first]) return false;
+        for (int i = first + 1; i < 3; i++)
+            if (box[i] && !(out[i] = record_result(box[i], out[first]))) return false;
+        return true;
+    }
+    for (const TensorP *t : {&x, &gate, &up, &kept, &grad})
+        if (!guard(*t)) return false;
+    for (int i = first; i < 3; i++)
+        if (want[i]) {
+            out[i] = i == first ? output_tensor(want[i]->shape, want[i]->ndims, want[i]->dtype)
+                                : make_empty(want[i]->shape, want[i]->ndims, want[i]->dtype);
+            if (!out[i]) return false;
+        }
+    return gated_backward_run(x, gate, up, kept, grad, activation, out);
 }
 
 // ------------------------------------------------------------------ AdamW
@@ -535,6 +687,24 @@ TensorP native_execute_block(const NativeSpec &sp, const std::vector<TensorP> &i
         if (gq && qs) to[2] = in[at++];
         if (gk && ks) to[3] = in[at++];
         ok = out && rotary_backward_run(in[0], k, positions, sp.rotary, qs, ks, sp.eps, gq, gk, to);
+        break;
+    }
+    case NAT_GATED: {
+        int shape[kMaxDims];
+        const int nd = gated_shape(*in[0], *in[1], shape);
+        out = output_tensor(shape, nd, in[0]->dtype);
+        ok = out && gated_run(in[0], in[1], in[2], sp.activation, out, in.size() > 3 ? in[3] : nullptr);
+        break;
+    }
+    case NAT_GATED_BACKWARD: {
+        const TensorP &first = sp.given & GATED_X ? in[0] : in[1];
+        out = output_tensor(first->shape, first->ndims, first->dtype);
+        TensorP to[3];
+        at = 5;
+        to[sp.given & GATED_X ? 0 : 1] = out;
+        if ((sp.given & GATED_X) && (sp.given & GATED_WEIGHTS)) to[1] = in[at++];
+        if (sp.given & GATED_WEIGHTS) to[2] = in[at++];
+        ok = out && gated_backward_run(in[0], in[1], in[2], in[3], in[4], sp.activation, to);
         break;
     }
     case NAT_ADAMW: {

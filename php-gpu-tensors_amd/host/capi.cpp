@@ -430,6 +430,28 @@ int phpt_rotary_backward(phpt_tensor *q, phpt_tensor *k, phpt_tensor *positions,
     });
 }
 
+phpt_tensor *phpt_gated(phpt_tensor *x, phpt_tensor *gate, phpt_tensor *up, int activation, phpt_tensor **kept)
+{
+    return bounded((phpt_tensor *)nullptr, [&]() -> phpt_tensor * {
+        TensorP out[2];
+        if (!cuda_array_gated(x->t, gate->t, up->t, activation, kept != nullptr, out)) return nullptr;
+        if (kept) *kept = wrap(out[1]);
+        return wrap(out[0]);
+    });
+}
+
+int phpt_gated_backward(phpt_tensor *x, phpt_tensor *gate, phpt_tensor *up, phpt_tensor *kept, phpt_tensor *grad,
+                        int activation, int want_x, int want_weights, phpt_tensor **results)
+{
+    return bounded(-1, [&]() -> int {
+        TensorP out[3];
+        if (!cuda_array_gated_backward(x->t, gate->t, up->t, kept->t, grad->t, activation, want_x != 0, want_weights != 0, out))
+            return -1;
+        for (int i = 0; i < 3; i++) results[i] = wrap(out[i]);
+        return 0;
+    });
+}
+
 static std::vector<TensorP> tensors_of(phpt_tensor **h, int count)
 {
     std::vector<TensorP> out;

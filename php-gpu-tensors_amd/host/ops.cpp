@@ -706,6 +706,8 @@ TensorP native_execute(const NativeSpec &sp, const std::vector<TensorP> &in)
     case NAT_LOGPROBS_BACKWARD: return native_execute_model(sp, in);
     case NAT_ROTARY:
     case NAT_ROTARY_BACKWARD:
+    case NAT_GATED:
+    case NAT_GATED_BACKWARD:
     case NAT_ADAMW:
     case NAT_ADAMW_MOMENTS: return native_execute_block(sp, in);
     default:

@@ -132,6 +132,13 @@ int phpt_rotary(phpt_tensor *q, phpt_tensor *k, phpt_tensor *positions, phpt_rot
  * of q, k, qs and ks */
 int phpt_rotary_backward(phpt_tensor *q, phpt_tensor *k, phpt_tensor *positions, phpt_rotary_plan *plan, phpt_tensor *qs,
                          phpt_tensor *ks, double eps, phpt_tensor *gq, phpt_tensor *gk, phpt_tensor **results);
+/* pt_gated over the last axis of x [.., inner], gate and up [inner, outer];
+ * activation: PT_GATE_*.  kept, where not NULL, gets both products for the
+ * gradient call. */
+phpt_tensor *phpt_gated(phpt_tensor *x, phpt_tensor *gate, phpt_tensor *up, int activation, phpt_tensor **kept);
+/* results[3]: gradients of x (where want_x), gate and up (where want_weights) */
+int phpt_gated_backward(phpt_tensor *x, phpt_tensor *gate, phpt_tensor *up, phpt_tensor *kept, phpt_tensor *grad,
+                        int activation, int want_x, int want_weights, phpt_tensor **results);
 /* pt_adamw over `count` parameters.  states: the moments [blocks, 256] that
  * phpt_adamw_blocks counts, the betas' powers float32 [1] each, with masters
  * (master not 0) float32 [blocks, 256], and with 8 bits int8 [blocks] twice

@@ -205,6 +205,12 @@ bool cuda_array_rotary(const TensorP &q, const TensorP &k, const TensorP &positi
 bool cuda_array_rotary_backward(const TensorP &q, const TensorP &k, const TensorP &positions, const RotaryP &plan,
                                 const TensorP &qs, const TensorP &ks, double eps, const TensorP &gq, const TensorP &gk,
                                 TensorP out[4]);
+// act(x gate) * (x up) over the last axis of x; out: the result and, with
+// keep, both products [2, rows, outer] for the gradient
+bool cuda_array_gated(const TensorP &x, const TensorP &gate, const TensorP &up, int activation, bool keep, TensorP out[2]);
+// out: of x, gate and up (null where not wanted)
+bool cuda_array_gated_backward(const TensorP &x, const TensorP &gate, const TensorP &up, const TensorP &kept,
+                               const TensorP &grad, int activation, bool want_x, bool want_weights, TensorP out[3]);
 // One AdamW step over many tensors; the state's arrays in the order
 // first, second, power1, power2, then with masters master, then with 8-bit
 // moments first's and second's exponents and draws.
@@ -251,7 +257,7 @@ enum NativeKind {
     // operand has written it.
     NAT_BUFFER, NAT_RESULT,
     NAT_ATTENTION, NAT_ATTENTION_BACKWARD, NAT_LAYERNORM_BACKWARD, NAT_LOGPROBS, NAT_LOGPROBS_BACKWARD,
-    NAT_ROTARY, NAT_ROTARY_BACKWARD, NAT_ADAMW, NAT_ADAMW_MOMENTS
+    NAT_ROTARY, NAT_ROTARY_BACKWARD, NAT_GATED, NAT_GATED_BACKWARD, NAT_ADAMW, NAT_ADAMW_MOMENTS
 };
 
 struct NativeSpec {
@@ -265,6 +271,7 @@ struct NativeSpec {
     int axes[kMaxDims] = {0};
     bool has_scale = false, has_bias = false;
     bool causal = false;
+    int activation = 0;
     int top = 0, given = 0;  // given: which optional operands follow (a bit each)
     SequencesP q_seq, k_seq;
     RotaryP rotary;

@@ -81,6 +81,10 @@ class PtRotaryDesc(ctypes.Structure):
                 ("epsilon", ctypes.c_double), ("turns", vp), ("positions", vp), ("position_strides", ctypes.c_size_t * 2)]
 
 
+class PtGatedDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int) for name in ("dtype", "activation", "rows", "inner", "outer")]
+
+
 class PtAdamwTensor(ctypes.Structure):
     _fields_ = [("param", vp), ("grad", vp), ("new_param", vp), ("n", ctypes.c_size_t), ("at", ctypes.c_size_t),
                 ("param_dtype", ctypes.c_int), ("grad_dtype", ctypes.c_int), ("decay", ctypes.c_int)]
@@ -158,6 +162,8 @@ SIGNATURES = {
     "pt_rotary": (ctypes.c_int, [ctypes.POINTER(PtRotaryDesc)] + [ctypes.POINTER(vp)] * 3 + [vp]),
     "pt_rotary_backward": (ctypes.c_int, [ctypes.POINTER(PtRotaryDesc)] + [ctypes.POINTER(vp)] * 3 + [ctypes.c_int]
                            + [ctypes.POINTER(vp)] * 2 + [vp]),
+    "pt_gated": (ctypes.c_int, [ctypes.POINTER(PtGatedDesc)] + [vp] * 6),
+    "pt_gated_backward": (ctypes.c_int, [ctypes.POINTER(PtGatedDesc)] + [vp] * 5 + [ctypes.c_int] + [vp] * 4),
     "pt_adamw": (ctypes.c_int, [ctypes.POINTER(PtAdamwDesc), ctypes.POINTER(PtAdamwTensor), ctypes.c_int, vp]),
     "pt_adamw_moments": (ctypes.c_int, [vp] * 6 + [ctypes.c_size_t, vp]),
     "pt_matmul": (ctypes.c_int, [vp, vp, vp, ctypes.c_int, c_int_p, c_size_p, ctypes.c_int,

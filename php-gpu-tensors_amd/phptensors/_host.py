@@ -57,6 +57,8 @@ SIGNATURES = {
     "phpt_rotary_release": (None, [vp]),
     "phpt_rotary": (ctypes.c_int, [T, T, T, vp, T, T, ctypes.c_double, ctypes.POINTER(T)]),
     "phpt_rotary_backward": (ctypes.c_int, [T, T, T, vp, T, T, ctypes.c_double, T, T, ctypes.POINTER(T)]),
+    "phpt_gated": (T, [T, T, T, ctypes.c_int, ctypes.POINTER(T)]),
+    "phpt_gated_backward": (ctypes.c_int, [T] * 5 + [ctypes.c_int] * 3 + [ctypes.POINTER(T)]),
     "phpt_adamw": (ctypes.c_int, [ctypes.POINTER(T), ctypes.POINTER(T), ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(T),
                                   ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 4 + [T, ctypes.c_double,
                                                                                       ctypes.POINTER(T)]),

@@ -647,6 +647,37 @@ class CudaArray:
                     parts.part(t, name, low=True)
         return out[0] if key is None else (out[0], out[1])
 
+    ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+
+    def gatedProjection(self, gate, up, activation="silu"):
+        """act(self @ gate) * (self @ up): self [.., inner], gate and up
+        [inner, outer], float32, float16 or bfloat16; activation "silu", "gelu"
+        (with the error function), "relu" or "sigmoid".  Both products are
+        taken through the activation in float32 and the result is rounded
+        once.  The gradients have their operands' dtypes; for them both
+        products are kept, rounded to the dtype."""
+        if not isinstance(gate, CudaArray) or not isinstance(up, CudaArray):
+            raise InvalidArgumentException("gatedProjection() expects CudaArray matrices")
+        act = self.ACTIVATIONS.get(activation) if isinstance(activation, str) else None
+        if act is None:
+            raise InvalidArgumentException("gatedProjection() activations are silu, gelu, relu and sigmoid")
+        lib, active = _host.load(), AG.active(self, gate, up)
+        kept = (ctypes.c_void_p * 1)()
+        out = CudaArray._wrap(lib.phpt_gated(self._h, gate._h, up._h, act, kept if active else None), "gatedProjection")
+        if active:
+            products = CudaArray._wrap(kept[0])
+            wanted = AG.needs_grad(self), AG.needs_grad(gate) or AG.needs_grad(up)
+
+            def back(g):
+                if g.getDtype() not in ("float32", self.getDtype()):
+                    g = AG.cast(g, "float32")   # of an operation with a float64 tensor
+                got = (ctypes.c_void_p * 3)()
+                if lib.phpt_gated_backward(self._h, gate._h, up._h, products._h, g._h, act, *map(int, wanted), got):
+                    _host.raise_error("gatedProjection gradient")
+                return [CudaArray._wrap(h) if h else None for h in got]
+            AG.record(out, [self, gate, up], back, "gatedProjection", low=True)
+        return out
+
     def logProbs(self, tokens, top=0):
         """Of each row of scores along the last axis (float32, float16 or
         bfloat16): "logProbs", the log of the softmax at the row's token
