@@ -120,6 +120,21 @@ __device__ __forceinline__ uint16_t float_to_f16(float f)
     return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
+// Two values rounded to the nearest bfloat16 or float16, low | high << 16, by
+// one instruction: float_to_bf16's bits, and float_to_f16's but for a NaN's
+// payload.
+typedef float pt_f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 pt_bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 pt_f16x2 __attribute__((ext_vector_type(2)));
+template <int DT>
+__device__ __forceinline__ uint32_t pack_low(float lo, float hi)
+{
+    static_assert(DT == PT_BFLOAT16 || DT == PT_FLOAT16, "16-bit types");
+    const pt_f32x2 v = {lo, hi};
+    if constexpr (DT == PT_BFLOAT16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pt_bf16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pt_f16x2));
+}
+
 template <int DT> struct DType;
 template <> struct DType<PT_FLOAT32> {
     using S = float; using C = float;

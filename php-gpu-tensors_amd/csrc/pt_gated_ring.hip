@@ -22,19 +22,6 @@
 
 namespace pt {
 
-// Two fp32 values rounded to the 16-bit dtype, packed low | high << 16 (to
-// nearest even).
-typedef float pr_f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 pr_bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 pr_f16x2 __attribute__((ext_vector_type(2)));
-template <int DT>
-__device__ __forceinline__ uint32_t pair_pack(float lo, float hi)
-{
-    const pr_f32x2 v = {lo, hi};
-    if constexpr (DT == PT_BFLOAT16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pr_bf16x2));
-    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pr_f16x2));
-}
-
 constexpr int pair_bases(int stage_bytes, int max_inner)
 {
     int s = 0;
@@ -282,7 +269,7 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
     const int col_l = (lane & 31) & ~1, row_l = (lane >> 5) * 4 + (odd ? 2 : 0);
     typedef uint32_t word __attribute__((aligned(2)));
     auto store4 = [&](void *c, int m, int n, float v0, float v1, float v2, float v3) {
-        const uint32_t p01 = pair_pack<DT>(v0, v1), p23 = pair_pack<DT>(v2, v3);
+        const uint32_t p01 = pack_low<DT>(v0, v1), p23 = pack_low<DT>(v2, v3);
         const uint32_t send = odd ? p01 : p23;
         const uint32_t recv = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)send, 0xB1, 0xF, 0xF, false);
         const uint32_t u = odd ? recv : p01, v = odd ? p23 : recv;

@@ -7,13 +7,15 @@
 // rotated back; dx = dn, or with h = dn w and u = x r
 //   dw = sum dn u,   dx = r (h - u mean(h u)).
 // HBM-bound: a head is read once (with its upstream gradient) and written
-// once.  A unit of work is 2 V elements (V a 16-byte pack where the pairs
-// allow it): V pairs, or 2 V elements that pass; a head takes the power of
-// two of lanes that holds its units, so its sum of squares is a few
-// exchanges inside a wave.  The angles of a block's tokens are computed once
-// into LDS, in double (turns, reduced before they are rounded: positions
-// reach 2^31), while the first heads are on their way, and serve all heads:
-// one cosine and sine per element would cost more than the memory.
+// once.  A lane's unit of work is 2 V elements, V a 16-byte pack: V pairs, or
+// 2 V elements that pass; a head takes the power of two of lanes that holds
+// its units, so its sum of squares is a few exchanges inside a wave.  Waves
+// work on their own: a wave takes one token and walks its heads, the next
+// ones on their way while it turns these.  It computes the token's angles
+// once for all of them, a pair or two a lane, and hands them round through
+// its own part of LDS without a barrier: as turns, reduced in double before
+// they are rounded (positions reach 2^31).  One cosine and sine per element
+// would cost more than the memory.
 #include "pt_common.h"
 
 #include <algorithm>
@@ -21,8 +23,8 @@
 
 namespace pt {
 
-constexpr int kRotThreads = 256;
-constexpr int kRotTable = 256;  // pairs whose cosines and sines a block holds
+constexpr int kRotWaves = 4;
+constexpr int kRotBlocks = 2048;
 
 struct RotSide {
     const void *x;      // null in a backward pass without a norm
@@ -41,290 +43,324 @@ struct RotArgs {
     long long pst[2];           // sequence, token
     unsigned tokens, rows;      // of a sequence, of all
     int size, part, lanes_log2;
-    int group;                  // tokens that a block takes at a time
+    int passes;                 // a wave's turns over 64 >> lanes_log2 heads of a token
     float magnitude, eps;
 };
 
-template <int DT, int V>
-__device__ __forceinline__ void rot_load(const typename DType<DT>::S *p, float *v)
-{
-    using S = typename DType<DT>::S;
-    typedef S vec __attribute__((ext_vector_type(V), aligned(sizeof(S))));
-    if constexpr (V == 1) v[0] = DType<DT>::to_c(*p);
-    else {
-        const vec r = *(const vec *)p;
-#pragma unroll
-        for (int i = 0; i < V; i++) v[i] = DType<DT>::to_c(r[i]);
-    }
-}
-
-template <int DT, int V>
-__device__ __forceinline__ void rot_store(typename DType<DT>::S *p, const float *v)
-{
-    using S = typename DType<DT>::S;
-    typedef S vec __attribute__((ext_vector_type(V), aligned(sizeof(S))));
-    if constexpr (V == 1) *p = DType<DT>::from_c(v[0]);
-    else {
-        vec r;
-#pragma unroll
-        for (int i = 0; i < V; i++) r[i] = DType<DT>::from_c(v[i]);
-        *(vec *)p = r;
-    }
-}
-
-// Unit u of a head: elements at[0] .. +V - 1 and at[1] .. +V - 1, `live` of
-// the 2 V in order that belong to the head, rotated where u < part / 2 / V.
+// Unit u of a head: elements at[0] .. +V - 1 and at[1] .. +V - 1, of which
+// `live` of each belong to it, the first `turned` of V pairs among them.
+// Pairs (2i, 2i + 1): 2 V elements in a row, the end of the turned part
+// inside of one.  Pairs (i, i + part / 2): V in both halves of that part, and
+// units of their own behind it.
 struct RotUnit {
-    int at[2];
-    int live;
-    bool turned;
+    int at[2], live[2], turned;
 };
+
+// V of a kernel: 16 bytes, and 8 in a backward pass in 16 bits, whose values
+// then take 100 registers instead of 160 (8192 tokens of 32 heads of 128: 43
+// against 50 us; the forward pass 36 us with 16 bytes, 43 with 8)
+__host__ __device__ constexpr int rot_width(int dtype, bool back) { return dtype == PT_FLOAT32 || back ? 4 : 8; }
+__host__ __device__ inline int rot_units(int size, int part, bool paired, int v)
+{
+    return paired ? (size + 2 * v - 1) / (2 * v) : (part / 2 + v - 1) / v + (size - part + 2 * v - 1) / (2 * v);
+}
 
 template <int V, bool PAIRED>
 __device__ __forceinline__ RotUnit rot_unit(const RotArgs &a, int u)
 {
-    const int pairs = a.part / 2, units = pairs / V;
+    const int pairs = a.part / 2, units = (pairs + V - 1) / V;
     RotUnit r;
-    r.turned = u < units;
-    r.live = 2 * V;
-    if (r.turned) {
-        r.at[0] = PAIRED ? 2 * V * u : V * u;
-        r.at[1] = PAIRED ? 2 * V * u + V : pairs + V * u;
-    } else {
-        r.at[0] = a.part + (u - units) * 2 * V;
-        r.at[1] = r.at[0] + V;
-        r.live = max(0, min(2 * V, a.size - r.at[0]));
-    }
+    r.turned = max(0, min(V, pairs - u * V));
+    const bool halves = !PAIRED && r.turned;
+    const int base = PAIRED ? 2 * V * u : halves ? V * u : a.part + (u - units) * 2 * V;
+    r.at[0] = base;
+    r.at[1] = halves ? pairs + base : base + V;
+    r.live[0] = halves ? r.turned : max(0, min(V, a.size - base));
+    r.live[1] = halves ? r.turned : max(0, min(V, a.size - base - V));
     return r;
 }
 
+// What a unit's elements are in memory, in whole registers.
+template <int DT, int V> struct RotRaw {
+    static constexpr int N = V * (int)sizeof(typename DType<DT>::S) / 4;
+    typedef unsigned words __attribute__((ext_vector_type(N), aligned(1)));
+    words q[2];
+};
+
+// (16 bytes load and store at any element boundary)
 template <int DT, int V>
-__device__ __forceinline__ void rot_read(const void *base, long long off, const RotUnit &r, float (&v)[2 * V])
+__device__ __forceinline__ void rot_read(const void *base, long long off, const RotUnit &r, RotRaw<DT, V> &raw)
 {
     using S = typename DType<DT>::S;
+    using Words = typename RotRaw<DT, V>::words;
     const S *p = (const S *)base + off;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        if (r.live >= (h + 1) * V) rot_load<DT, V>(p + r.at[h], v + h * V);
-        else
+        if (r.live[h] == V) {
+            raw.q[h] = *(const Words *)(p + r.at[h]);
+        } else {
+            union { Words q; S s[V]; } u;
 #pragma unroll
-            for (int i = 0; i < V; i++) v[h * V + i] = h * V + i < r.live ? DType<DT>::to_c(p[r.at[h] + i]) : 0.0f;
+            for (int i = 0; i < V; i++) u.s[i] = i < r.live[h] ? p[r.at[h] + i] : (S)0;
+            raw.q[h] = u.q;
+        }
     }
 }
-
+template <int DT, int V>
+__device__ __forceinline__ void rot_values(const RotRaw<DT, V> &raw, float (&v)[2 * V])
+{
+    constexpr bool LOW = DT != PT_FLOAT32;
+#pragma unroll
+    for (int i = 0; i < 2 * V; i++) {
+        const unsigned word = raw.q[i / V][LOW ? (i % V) / 2 : i % V];
+        if constexpr (!LOW) v[i] = __uint_as_float(word);
+        else if constexpr (DT == PT_BFLOAT16) v[i] = __uint_as_float(i & 1 ? word & 0xffff0000u : word << 16);
+        else v[i] = f16_to_float((uint16_t)(i & 1 ? word >> 16 : word));
+    }
+}
 template <int DT, int V>
 __device__ __forceinline__ void rot_write(void *base, long long off, const RotUnit &r, const float (&v)[2 * V])
 {
     using S = typename DType<DT>::S;
+    using Words = typename RotRaw<DT, V>::words;
     S *p = (S *)base + off;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        if (r.live >= (h + 1) * V) rot_store<DT, V>(p + r.at[h], v + h * V);
-        else
+        if (r.live[h] == V) {
+            Words q;
+#pragma unroll
+            for (int i = 0; i < RotRaw<DT, V>::N; i++) {
+                if constexpr (DT == PT_FLOAT32) q[i] = __float_as_uint(v[h * V + i]);
+                else q[i] = pack_low<DT>(v[h * V + 2 * i], v[h * V + 2 * i + 1]);
+            }
+            __builtin_nontemporal_store(q, (Words *)(p + r.at[h]));
+        } else
 #pragma unroll
             for (int i = 0; i < V; i++)
-                if (h * V + i < r.live) p[r.at[h] + i] = DType<DT>::from_c(v[h * V + i]);
+                if (i < r.live[h]) p[r.at[h] + i] = DType<DT>::from_c(v[h * V + i]);
     }
 }
 
-// v turned by the angles of the unit's pairs, backwards with sign -1
+// the first n pairs of v turned by their angles, backwards with sign -1
 template <int V, bool PAIRED>
-__device__ __forceinline__ void rot_turn(const float2 *table, int u, float sign, float (&v)[2 * V])
+__device__ __forceinline__ void rot_turn(const float2 (&angle)[V], int n, float sign, float (&v)[2 * V])
 {
+    if (!n) return;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const float2 cs = table[u * V + i];
         const int p = PAIRED ? 2 * i : i, q = PAIRED ? 2 * i + 1 : V + i;
-        const float x = v[p], y = v[q], s = sign * cs.y;
-        v[p] = x * cs.x - y * s;
-        v[q] = x * s + y * cs.x;
+        const float x = v[p], y = v[q], s = sign * angle[i].y;
+        const float a = x * angle[i].x - y * s, b = x * s + y * angle[i].x;
+        v[p] = PAIRED && i >= n ? x : a;  // (in halves what is past the end is not stored)
+        v[q] = PAIRED && i >= n ? y : b;
     }
 }
 
-// the sum over the 2^log2 lanes that share a head
+// the sum over the 2^log2 lanes that share a head (log2 is uniform): up to
+// 16 lanes by DPP (pairs, quads, mirrored halves of a row), without LDS
 __device__ __forceinline__ float rot_sum(float v, int log2)
 {
-    for (int m = 1; m < 1 << log2; m <<= 1) v += __shfl_xor(v, m, PT_WAVE);
+    auto with = [](float x, auto CTRL) {
+        return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(CTRL)::value, 0xF, 0xF, false));
+    };
+    if (log2 > 0) v = with(v, std::integral_constant<int, 0xB1>{});
+    if (log2 > 1) v = with(v, std::integral_constant<int, 0x4E>{});
+    if (log2 > 2) v = with(v, std::integral_constant<int, 0x141>{});
+    if (log2 > 3) v = with(v, std::integral_constant<int, 0x140>{});
+    if (log2 > 4) v += __shfl_xor(v, 16, PT_WAVE);
+    if (log2 > 5) v += __shfl_xor(v, 32, PT_WAVE);
     return v;
 }
 
-// One block takes `group` tokens at a time and all heads of its side
-// (blockIdx.y).  NU units a lane: two where a unit is one pair (heads of up
-// to 256 elements then have 128 units).
-template <int DT, int GDT, int V, bool PAIRED, bool BACK>
-__global__ __launch_bounds__(kRotThreads) void k_rotary(RotArgs a)
+// Forward: the heads of both sides count through.  Backward: blockIdx.y is
+// the side, so that a lane's part of the scale's gradient stays in registers
+// over all the tokens that its wave takes.
+template <int DT, int GDT, bool PAIRED, bool BACK>
+__global__ __launch_bounds__(64 * kRotWaves) void k_rotary(RotArgs a)
 {
-    constexpr int NU = V == 1 ? 2 : 1;
-    __shared__ float2 table[kRotTable];
-    __shared__ float sums[BACK ? kRotThreads * NU * 2 * V : 1];
-    const RotSide &s = a.side[blockIdx.y];
-    const int log2 = a.lanes_log2, lane = threadIdx.x & ((1 << log2) - 1), slot = threadIdx.x >> log2;
-    const int slots = kRotThreads >> log2, pairs = a.part / 2;
-    RotUnit unit[NU];
-    float w[NU][2 * V], dw[NU][2 * V];
-#pragma unroll
-    for (int k = 0; k < NU; k++) {
-        unit[k] = rot_unit<V, PAIRED>(a, lane + (k << log2));
-        if (s.scale) rot_read<DT, V>(s.scale, 0, unit[k], w[k]);
-#pragma unroll
-        for (int i = 0; i < 2 * V; i++) {
-            if (!s.scale) w[k][i] = 1.0f;
-            dw[k][i] = 0.0f;
-        }
-    }
+    constexpr int V = rot_width(DT, BACK);
+    using Raw = RotRaw<DT, V>;
+    __shared__ float2 tables[kRotWaves][128];
+    __shared__ float sums[BACK ? kRotWaves : 1][BACK ? 2 * V : 1][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int log2 = a.lanes_log2, u = lane & ((1 << log2) - 1), slot = lane >> log2, slots = 64 >> log2;
+    const int pairs = a.part / 2;
+    const RotSide &s0 = a.side[BACK ? blockIdx.y : 0], &s1 = a.side[1];
+    const unsigned heads = BACK ? s0.heads : s0.heads + s1.heads;
+    const unsigned units = (heads + slots * a.passes - 1) / (slots * a.passes);  // of a token
+    const RotUnit unit = rot_unit<V, PAIRED>(a, u);
     const float inv_n = 1.0f / (float)a.size;
-    // (blocks times tokens of a group stay below 2^24 here, rows below 2^31)
-    for (unsigned first = blockIdx.x * a.group; first < a.rows; first += gridDim.x * a.group) {
-        const unsigned here = min((unsigned)a.group, a.rows - first);
-        const unsigned items = here * (unsigned)s.heads;
-        float x[NU][2 * V], g[NU][2 * V];
-        long long to = 0;
-        unsigned tok = 0;
-        auto fetch = [&](unsigned item) {
-            tok = item / (unsigned)s.heads;
-            const unsigned head = item - tok * s.heads, row = first + tok, seq = row / a.tokens, t = row - seq * a.tokens;
-            to = ((long long)row * s.heads + head) * a.size;
-            const long long from = seq * s.st[0] + t * s.st[1] + head * s.st[2];
+    float2 *table = tables[wave];
+    // the token and the first head of a wave's turn; rows times units are below 2^48
+    struct Turn {
+        unsigned row, seq, t, first;
+        long long pos;
+    };
+    const unsigned long long total = (unsigned long long)a.rows * units, step = (unsigned long long)gridDim.x * kRotWaves;
+    auto turn_of = [&](unsigned long long at) {
+        Turn n;
+        n.row = units == 1 ? (unsigned)at : (unsigned)(at / units);
+        n.first = (unsigned)(at - (unsigned long long)n.row * units) * a.passes * slots;
+        n.seq = a.tokens == a.rows ? 0 : n.row / a.tokens;
+        n.t = n.row - n.seq * a.tokens;
+        n.pos = a.positions ? (long long)a.positions[n.seq * a.pst[0] + n.t * a.pst[1]] : (long long)n.t;
+        return n;
+    };
+    auto fetch = [&](const Turn &n, unsigned h, Raw &x, RotRaw<GDT, V> &g) {
+        if (h >= heads) return;
+        const bool key = !BACK && h >= (unsigned)s0.heads;
+        const RotSide &s = key ? s1 : s0;
+        const unsigned head = key ? h - s0.heads : h;
+        if (!BACK || s.scale) rot_read<DT, V>(s.x, n.seq * s.st[0] + n.t * s.st[1] + head * s.st[2], unit, x);
+        if constexpr (BACK) rot_read<GDT, V>(s.g, ((long long)n.row * s.heads + head) * a.size, unit, g);
+    };
+    unsigned long long at = (unsigned long long)blockIdx.x * kRotWaves + wave;
+    Raw x, xn, w0, w1;
+    RotRaw<GDT, V> g, gn;
+    Turn now = {}, next = {};
+    if (at < total) {
+        now = turn_of(at);
+        fetch(now, now.first + slot, x, g);
+    }
+    if (s0.scale) rot_read<DT, V>(s0.scale, 0, unit, w0);
+    if (!BACK && s1.scale) rot_read<DT, V>(s1.scale, 0, unit, w1);
+    const double turns0 = a.turns[min(lane, pairs - 1)], turns1 = a.turns[min(lane + 64, pairs - 1)];
+    float dw[2 * V];
 #pragma unroll
-            for (int k = 0; k < NU; k++) {
-                if (!BACK || s.scale) rot_read<DT, V>(s.x, from, unit[k], x[k]);
-                if constexpr (BACK) rot_read<GDT, V>(s.g, to, unit[k], g[k]);
-            }
-        };
-        unsigned item = slot;
-        if (item < items) fetch(item);
-        __syncthreads();  // the table's readers of the group before
-        for (unsigned i = threadIdx.x; i < here * pairs; i += kRotThreads) {
-            const unsigned tk = i / (unsigned)pairs, f = i - tk * pairs;
-            const unsigned row = first + tk, seq = row / a.tokens, t = row - seq * a.tokens;
-            const long long pos = a.positions ? (long long)a.positions[seq * a.pst[0] + t * a.pst[1]] : (long long)t;
-            const double turns = (double)pos * a.turns[f];
-            double sn, cs;
-            sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
-            table[i] = make_float2((float)(cs * a.magnitude), (float)(sn * a.magnitude));
+    for (int i = 0; i < 2 * V; i++) dw[i] = 0.0f;
+    for (; at < total; at += step) {
+        const bool more = at + step < total;
+        if (more) next = turn_of(at + step);
+        for (int f = lane; f < pairs; f += 64) {
+            // the fraction of a turn in two floats: the second corrects the first's cosine and sine
+            double turns = (double)now.pos * (f < 64 ? turns0 : turns1);
+            turns -= rint(turns);
+            const float hi = (float)turns, lo = (float)(turns - (double)hi) * 6.28318531f;
+            float sn, cs;
+            sincospif(2.0f * hi, &sn, &cs);
+            table[f] = make_float2((cs - lo * sn) * a.magnitude, (sn + lo * cs) * a.magnitude);
         }
-        __syncthreads();
-        // (whole groups of lanes enter and leave, so a head's sum has all its lanes)
-        while (item < items) {
-            const float2 *angles = table + tok * pairs;
-            if constexpr (!BACK) {
-                if (s.scale) {
-                    float q = 0.0f;
+        // the table is this wave's own: its LDS accesses stay in order
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        float2 angle[V];
 #pragma unroll
-                    for (int k = 0; k < NU; k++)
+        for (int i = 0; i < V; i++) angle[i] = table[min(u * V + i, pairs - 1)];
+        __builtin_amdgcn_wave_barrier();
+        for (int p = 0; p < a.passes; p++) {
+            const unsigned h = now.first + p * slots + slot;
+            if (p + 1 < a.passes) fetch(now, h + slots, xn, gn);
+            else if (more) fetch(next, next.first + slot, xn, gn);
+            if (h < heads) {  // (whole groups of lanes, so a head's sum has all its lanes)
+                const bool key = !BACK && h >= (unsigned)s0.heads;
+                const RotSide &s = key ? s1 : s0;
+                const unsigned head = key ? h - s0.heads : h;
+                const long long to = ((long long)now.row * s.heads + head) * a.size;
+                float v[2 * V], w[2 * V];
+                rot_values<DT, V>(x, v);
+                if constexpr (!BACK) {
+                    if (s.scale) {
+                        rot_values<DT, V>(key ? w1 : w0, w);
+                        float q = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 2 * V; i++) q = fmaf(x[k][i], x[k][i], q);
-                    const float r = 1.0f / sqrtf(rot_sum(q, log2) * inv_n + a.eps);
+                        for (int i = 0; i < 2 * V; i++) q = fmaf(v[i], v[i], q);
+                        const float r = 1.0f / sqrtf(rot_sum(q, log2) * inv_n + a.eps);
 #pragma unroll
-                    for (int k = 0; k < NU; k++)
-#pragma unroll
-                        for (int i = 0; i < 2 * V; i++) x[k][i] = x[k][i] * r * w[k][i];
-                }
-#pragma unroll
-                for (int k = 0; k < NU; k++) {
-                    if (unit[k].turned) rot_turn<V, PAIRED>(angles, lane + (k << log2), 1.0f, x[k]);
-                    rot_write<DT, V>(s.y, to, unit[k], x[k]);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < NU; k++)
-                    if (unit[k].turned) rot_turn<V, PAIRED>(angles, lane + (k << log2), -1.0f, g[k]);
-                if (s.scale) {
-                    float q = 0.0f, b = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < NU; k++)
+                        for (int i = 0; i < 2 * V; i++) v[i] = v[i] * r * w[i];
+                    }
+                    rot_turn<V, PAIRED>(angle, unit.turned, 1.0f, v);
+                    rot_write<DT, V>(s.y, to, unit, v);
+                } else {
+                    float d[2 * V];
+                    rot_values<GDT, V>(g, d);
+                    rot_turn<V, PAIRED>(angle, unit.turned, -1.0f, d);
+                    if (s.scale) {
+                        rot_values<DT, V>(w0, w);
+                        float q = 0.0f, b = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 2 * V; i++) {
-                            q = fmaf(x[k][i], x[k][i], q);
-                            b = fmaf(g[k][i] * w[k][i], x[k][i], b);
+                            q = fmaf(v[i], v[i], q);
+                            b = fmaf(d[i] * w[i], v[i], b);
                         }
-                    const float r = 1.0f / sqrtf(rot_sum(q, log2) * inv_n + a.eps);
-                    b = rot_sum(b, log2) * inv_n * r;
-#pragma unroll
-                    for (int k = 0; k < NU; k++)
+                        const float r = 1.0f / sqrtf(rot_sum(q, log2) * inv_n + a.eps);
+                        b = rot_sum(b, log2) * inv_n * r;
 #pragma unroll
                         for (int i = 0; i < 2 * V; i++) {
-                            const float u = x[k][i] * r;
-                            dw[k][i] = fmaf(g[k][i], u, dw[k][i]);
-                            g[k][i] = r * (g[k][i] * w[k][i] - u * b);
+                            const float n = v[i] * r;
+                            dw[i] = fmaf(d[i], n, dw[i]);
+                            d[i] = r * (d[i] * w[i] - n * b);
                         }
+                    }
+                    if (s.y) rot_write<DT, V>(s.y, to, unit, d);
                 }
-#pragma unroll
-                for (int k = 0; k < NU; k++)
-                    if (s.y) rot_write<DT, V>(s.y, to, unit[k], g[k]);
             }
-            item += slots;
-            if (item < items) fetch(item);
+            x = xn;
+            if constexpr (BACK) g = gn;
         }
+        now = next;
     }
     if constexpr (BACK) {
-        if (!s.partial) return;
+        if (!s0.partial) return;
+#pragma unroll
+        for (int i = 0; i < 2 * V; i++) {
+            for (int m = 1 << log2; m < 64; m <<= 1) dw[i] += __shfl_xor(dw[i], m, PT_WAVE);
+            sums[wave][i][lane] = dw[i];
+        }
         __syncthreads();
+        if (wave || slot) return;
 #pragma unroll
-        for (int k = 0; k < NU; k++)
-#pragma unroll
-            for (int i = 0; i < 2 * V; i++) sums[(k * 2 * V + i) * kRotThreads + threadIdx.x] = dw[k][i];
-        __syncthreads();
-        if (slot) return;
-#pragma unroll
-        for (int k = 0; k < NU; k++)
-#pragma unroll
-            for (int i = 0; i < 2 * V; i++) {
-                float t = 0.0f;
-                for (int o = 0; o < slots; o++) t += sums[(k * 2 * V + i) * kRotThreads + (o << log2) + lane];
-                if (i < unit[k].live)
-                    s.partial[(long long)blockIdx.x * a.size + unit[k].at[i / V] + i % V] = t;
-            }
+        for (int i = 0; i < 2 * V; i++) {
+            float t = dw[i];
+            for (int o = 1; o < kRotWaves; o++) t += sums[o][i][lane];
+            if (i % V < unit.live[i / V]) s0.partial[(long long)blockIdx.x * a.size + unit.at[i / V] + i % V] = t;
+        }
     }
 }
 
-// The scale's gradient from the blocks' partial rows, in a fixed order: four
-// columns a block of 16 waves, a wave's lanes four columns and 16 rows.
+// The scale's gradient from the blocks' partial rows, in a fixed order: a
+// wave adds four columns, its lanes every 16th row.
 template <int DT>
-__global__ __launch_bounds__(256) void k_rotary_scale(RotArgs a, int parts, void *d0, void *d1)
+__global__ __launch_bounds__(64) void k_rotary_scale(RotArgs a, int parts, void *d0, void *d1)
 {
-    __shared__ float box[64][4];
-    const int c = (int)blockIdx.x * 4 + (threadIdx.x & 3), r0 = threadIdx.x >> 2;
+    const int c = (int)blockIdx.x * 4 + (threadIdx.x & 3);
     void *out = blockIdx.y ? d1 : d0;
     const float *p = a.side[blockIdx.y].partial;
     if (!out) return;  // whole block
     float t = 0.0f;
     if (c < a.size)
-        for (int r = r0; r < parts; r += 64) t += p[(long long)r * a.size + c];
-    box[r0][threadIdx.x & 3] = t;
-    __syncthreads();
-    if (r0 || c >= a.size) return;
-    for (int r = 1; r < 64; r++) t += box[r][threadIdx.x & 3];
-    ((typename DType<DT>::S *)out)[c] = DType<DT>::from_c(t);
-}
-
-template <int DT, int GDT, int V>
-static void launch_rotary(const RotArgs &a, bool interleaved, bool back, dim3 grid, hipStream_t s)
-{
-    if (back) {
-        if (interleaved) k_rotary<DT, GDT, V, true, true><<<grid, kRotThreads, 0, s>>>(a);
-        else k_rotary<DT, GDT, V, false, true><<<grid, kRotThreads, 0, s>>>(a);
-        return;
-    }
-    if constexpr (DT == GDT) {
-        if (interleaved) k_rotary<DT, DT, V, true, false><<<grid, kRotThreads, 0, s>>>(a);
-        else k_rotary<DT, DT, V, false, false><<<grid, kRotThreads, 0, s>>>(a);
-    }
+#pragma unroll 8
+        for (int r = threadIdx.x >> 2; r < parts; r += 16) t += p[(long long)r * a.size + c];
+    for (int m = 4; m < 64; m <<= 1) t += __shfl_xor(t, m, PT_WAVE);
+    if (threadIdx.x < 4 && c < a.size) ((typename DType<DT>::S *)out)[c] = DType<DT>::from_c(t);
 }
 
 template <int DT, int GDT>
-static void launch_rotary_width(RotArgs a, bool interleaved, bool back, unsigned blocks, unsigned sides, hipStream_t s)
+static void launch_rotary(const RotArgs &a, bool interleaved, bool back, dim3 grid, hipStream_t s)
 {
-    constexpr int W = 16 / sizeof(typename DType<DT>::S);  // a pack of 16 bytes
-    const int pairs = a.part / 2;
-    const int v = pairs % W == 0 ? W : pairs % 2 == 0 ? 2 : 1;
-    const int units = pairs / v + (a.size - a.part + 2 * v - 1) / (2 * v);
+    if (back) {
+        if (interleaved) k_rotary<DT, GDT, true, true><<<grid, 64 * kRotWaves, 0, s>>>(a);
+        else k_rotary<DT, GDT, false, true><<<grid, 64 * kRotWaves, 0, s>>>(a);
+        return;
+    }
+    if constexpr (DT == GDT) {
+        if (interleaved) k_rotary<DT, DT, true, false><<<grid, 64 * kRotWaves, 0, s>>>(a);
+        else k_rotary<DT, DT, false, false><<<grid, 64 * kRotWaves, 0, s>>>(a);
+    }
+}
+
+// How the heads go to waves: a wave's passes over a token's heads, as many as
+// leave 8192 waves (two for each slot of the GPU at a register count of 128).
+static unsigned rotary_blocks(RotArgs &a, int dtype, bool paired, bool back, int heads, long long most)
+{
+    const int units = rot_units(a.size, a.part, paired, rot_width(dtype, back));
     a.lanes_log2 = 0;
-    while (a.lanes_log2 < 6 && 1 << a.lanes_log2 < units) a.lanes_log2++;
-    const dim3 grid(blocks, sides);
-    if (v == W) launch_rotary<DT, GDT, W>(a, interleaved, back, grid, s);
-    else if (v == 2) launch_rotary<DT, GDT, 2>(a, interleaved, back, grid, s);
-    else launch_rotary<DT, GDT, 1>(a, interleaved, back, grid, s);
+    while (1 << a.lanes_log2 < units) a.lanes_log2++;  // (at most 64: heads have at most 256 elements)
+    const int all = (heads + (64 >> a.lanes_log2) - 1) >> (6 - a.lanes_log2);
+    a.passes = (int)std::max<long long>(1, std::min<long long>(all, (long long)a.rows * all / 8192));
+    const long long waves = (long long)a.rows * ((all + a.passes - 1) / a.passes);
+    // (in rounds of equal length)
+    const long long blocks = (waves + kRotWaves - 1) / kRotWaves, rounds = (blocks + most - 1) / most;
+    return (unsigned)((blocks + rounds - 1) / rounds);
 }
 
 static pt_status rotary_args(const pt_rotary_desc *d, RotArgs &a)
@@ -359,9 +395,6 @@ static pt_status rotary_args(const pt_rotary_desc *d, RotArgs &a)
         a.side[i].heads = d->heads[i];
         for (int k = 0; k < 3; k++) a.side[i].st[k] = (long long)d->strides[i][k];
     }
-    // tokens of a group: enough pairs for a block's threads, as long as there
-    // is a block for every CU and each of a few turns
-    a.group = std::max(1, std::min({kRotThreads / (d->part / 2), 16, (int)std::min<long long>(rows / 2048, 16)}));
     return PT_OK;
 }
 
@@ -391,10 +424,11 @@ pt_status pt_rotary(const pt_rotary_desc *d, const void *const *x, const void *c
     PT_TRY(ensure_init());
     if (!sides) return PT_OK;
     hipStream_t s = stream_of(stream);
-    const unsigned blocks = (unsigned)std::min<long long>(((long long)a.rows + a.group - 1) / a.group, 1 << 20);
-    if (d->dtype == PT_FLOAT32) launch_rotary_width<PT_FLOAT32, PT_FLOAT32>(a, d->interleaved, false, blocks, sides, s);
-    else if (d->dtype == PT_FLOAT16) launch_rotary_width<PT_FLOAT16, PT_FLOAT16>(a, d->interleaved, false, blocks, sides, s);
-    else launch_rotary_width<PT_BFLOAT16, PT_BFLOAT16>(a, d->interleaved, false, blocks, sides, s);
+    if (sides == 1) a.side[1].heads = 0;
+    const unsigned blocks = rotary_blocks(a, d->dtype, d->interleaved, false, a.side[0].heads + a.side[1].heads, kRotBlocks);
+    if (d->dtype == PT_FLOAT32) launch_rotary<PT_FLOAT32, PT_FLOAT32>(a, d->interleaved, false, blocks, s);
+    else if (d->dtype == PT_FLOAT16) launch_rotary<PT_FLOAT16, PT_FLOAT16>(a, d->interleaved, false, blocks, s);
+    else launch_rotary<PT_BFLOAT16, PT_BFLOAT16>(a, d->interleaved, false, blocks, s);
     return check_hip(hipGetLastError(), "rotary");
 }
 
@@ -433,9 +467,9 @@ pt_status pt_rotary_backward(const pt_rotary_desc *d, const void *const *x, cons
     PT_TRY(ensure_init());
     if (!sides) return PT_OK;
     hipStream_t s = stream_of(stream);
-    long long blocks = ((long long)a.rows + a.group - 1) / a.group;
     // a partial row a block: four blocks a CU walk the tokens
-    blocks = std::min<long long>(blocks, partial ? 1024 : 1 << 20);
+    const unsigned blocks = rotary_blocks(a, d->dtype, d->interleaved, true, std::max(a.side[0].heads, sides > 1 ? a.side[1].heads : 0),
+                                          partial ? kRotBlocks / 2 : kRotBlocks);
     void *scratch = nullptr;
     if (partial) {
         PT_TRY(scratch_alloc(&scratch, (size_t)blocks * 2 * a.size * sizeof(float), s));
@@ -443,19 +477,19 @@ pt_status pt_rotary_backward(const pt_rotary_desc *d, const void *const *x, cons
             if (ds[i]) a.side[i].partial = (float *)scratch + (size_t)i * blocks * a.size;
     }
     const bool same = grad_dtype == d->dtype;
-    if (d->dtype == PT_FLOAT32) launch_rotary_width<PT_FLOAT32, PT_FLOAT32>(a, d->interleaved, true, blocks, sides, s);
+    if (d->dtype == PT_FLOAT32) launch_rotary<PT_FLOAT32, PT_FLOAT32>(a, d->interleaved, true, dim3(blocks, sides), s);
     else if (d->dtype == PT_FLOAT16) {
-        if (same) launch_rotary_width<PT_FLOAT16, PT_FLOAT16>(a, d->interleaved, true, blocks, sides, s);
-        else launch_rotary_width<PT_FLOAT16, PT_FLOAT32>(a, d->interleaved, true, blocks, sides, s);
+        if (same) launch_rotary<PT_FLOAT16, PT_FLOAT16>(a, d->interleaved, true, dim3(blocks, sides), s);
+        else launch_rotary<PT_FLOAT16, PT_FLOAT32>(a, d->interleaved, true, dim3(blocks, sides), s);
     } else {
-        if (same) launch_rotary_width<PT_BFLOAT16, PT_BFLOAT16>(a, d->interleaved, true, blocks, sides, s);
-        else launch_rotary_width<PT_BFLOAT16, PT_FLOAT32>(a, d->interleaved, true, blocks, sides, s);
+        if (same) launch_rotary<PT_BFLOAT16, PT_BFLOAT16>(a, d->interleaved, true, dim3(blocks, sides), s);
+        else launch_rotary<PT_BFLOAT16, PT_FLOAT32>(a, d->interleaved, true, dim3(blocks, sides), s);
     }
     if (partial) {
         const dim3 grid((a.size + 3) / 4, sides);
-        if (d->dtype == PT_FLOAT32) k_rotary_scale<PT_FLOAT32><<<grid, 256, 0, s>>>(a, (int)blocks, ds[0], ds[1]);
-        else if (d->dtype == PT_FLOAT16) k_rotary_scale<PT_FLOAT16><<<grid, 256, 0, s>>>(a, (int)blocks, ds[0], ds[1]);
-        else k_rotary_scale<PT_BFLOAT16><<<grid, 256, 0, s>>>(a, (int)blocks, ds[0], ds[1]);
+        if (d->dtype == PT_FLOAT32) k_rotary_scale<PT_FLOAT32><<<grid, 64, 0, s>>>(a, (int)blocks, ds[0], ds[1]);
+        else if (d->dtype == PT_FLOAT16) k_rotary_scale<PT_FLOAT16><<<grid, 64, 0, s>>>(a, (int)blocks, ds[0], ds[1]);
+        else k_rotary_scale<PT_BFLOAT16><<<grid, 64, 0, s>>>(a, (int)blocks, ds[0], ds[1]);
     }
     const pt_status st = check_hip(hipGetLastError(), "rotary gradient");
     if (scratch) scratch_free(scratch, s);
