@@ -10,7 +10,7 @@
 // one array each, a tensor's from a multiple of 256 elements on; parameters
 // and gradients are the tensors themselves.  A block takes 2048 elements of
 // one tensor, found by bisection of the first blocks in the kernel's
-// arguments; a thread 8 side by side, 16 bytes of a 16-bit tensor.
+// arguments, its waves 256 side by side, twice.
 //
 // Moments in 8 bits: 256 elements share the power of two 2^e that takes the
 // largest of them into [128, 256): a change of scale then leaves values that
@@ -30,7 +30,8 @@
 namespace pt {
 
 constexpr int kAdamTensors = 64;   // a launch: 3.4 KiB of arguments
-constexpr int kAdamBlock = 2048;   // elements
+constexpr int kAdamRounds = 2;     // 256 elements that a wave takes at once
+constexpr int kAdamBlock = 4 * kAdamRounds * 256;  // elements
 
 struct AdamTensor {
     const void *p0, *g;
@@ -56,60 +57,59 @@ struct AdamArgs {
     float b1, one_b1, b2, one_b2, eps, decay, rate_value, decay_value;
 };
 
+// A thread's 4 elements side by side, in 2, 4 or 1 words.
 typedef unsigned ad_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
 typedef unsigned ad_u32x2 __attribute__((ext_vector_type(2), aligned(1)));
 
 template <int DT>
-__device__ __forceinline__ void ad_load8(const void *base, long long i, float (&v)[8])
+__device__ __forceinline__ void ad_load4(const void *base, long long i, float (&v)[4])
 {
-    using S = typename DType<DT>::S;
-    const S *p = (const S *)base + i;
+    if constexpr (DT == PT_FLOAT32) {
+        const ad_u32x4 w = __builtin_nontemporal_load((const ad_u32x4 *)((const float *)base + i));
 #pragma unroll
-    for (int q = 0; q < 8 * (int)sizeof(S) / 16; q++) {
-        union { ad_u32x4 raw; S s[16 / sizeof(S)]; } u;
-        u.raw = __builtin_nontemporal_load((const ad_u32x4 *)(p + q * (16 / sizeof(S))));
+        for (int k = 0; k < 4; k++) v[k] = __uint_as_float(w[k]);
+    } else {
+        const ad_u32x2 w = __builtin_nontemporal_load((const ad_u32x2 *)((const uint16_t *)base + i));
 #pragma unroll
-        for (int k = 0; k < (int)(16 / sizeof(S)); k++) v[q * (16 / sizeof(S)) + k] = DType<DT>::to_c(u.s[k]);
+        for (int k = 0; k < 4; k++) v[k] = DType<DT>::to_c((uint16_t)(w[k / 2] >> (k & 1 ? 16 : 0)));
     }
 }
 
 template <int DT>
-__device__ __forceinline__ void ad_store8(void *base, long long i, const float (&v)[8])
+__device__ __forceinline__ void ad_store4(void *base, long long i, const float (&v)[4])
 {
-    using S = typename DType<DT>::S;
-    S *p = (S *)base + i;
-#pragma unroll
-    for (int q = 0; q < 8 * (int)sizeof(S) / 16; q++) {
-        union { ad_u32x4 raw; S s[16 / sizeof(S)]; } u;
-#pragma unroll
-        for (int k = 0; k < (int)(16 / sizeof(S)); k++) u.s[k] = DType<DT>::from_c(v[q * (16 / sizeof(S)) + k]);
-        __builtin_nontemporal_store(u.raw, (ad_u32x4 *)(p + q * (16 / sizeof(S))));
+    if constexpr (DT == PT_FLOAT32) {
+        const ad_u32x4 w = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        __builtin_nontemporal_store(w, (ad_u32x4 *)((float *)base + i));
+    } else {
+        const ad_u32x2 w = {pack_low<DT>(v[0], v[1]), pack_low<DT>(v[2], v[3])};
+        __builtin_nontemporal_store(w, (ad_u32x2 *)((uint16_t *)base + i));
     }
 }
 
-// `live` of 8 elements from i on, of a tensor of dtype dt (uniform in a block)
+// `live` of 4 elements from i on, of a tensor of dtype dt (uniform in a block)
 template <int DT>
-__device__ __forceinline__ void ad_load_as(const void *base, long long i, int live, float (&v)[8])
+__device__ __forceinline__ void ad_load_as(const void *base, long long i, int live, float (&v)[4])
 {
-    if (live >= 8) return ad_load8<DT>(base, i, v);
+    if (live >= 4) return ad_load4<DT>(base, i, v);
 #pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = k < live ? DType<DT>::to_c(((const typename DType<DT>::S *)base)[i + k]) : 0.0f;
+    for (int k = 0; k < 4; k++) v[k] = k < live ? DType<DT>::to_c(((const typename DType<DT>::S *)base)[i + k]) : 0.0f;
 }
-__device__ __forceinline__ void ad_load(const void *base, int dt, long long i, int live, float (&v)[8])
+__device__ __forceinline__ void ad_load(const void *base, int dt, long long i, int live, float (&v)[4])
 {
     if (dt == PT_FLOAT32) ad_load_as<PT_FLOAT32>(base, i, live, v);
     else if (dt == PT_FLOAT16) ad_load_as<PT_FLOAT16>(base, i, live, v);
     else ad_load_as<PT_BFLOAT16>(base, i, live, v);
 }
 template <int DT>
-__device__ __forceinline__ void ad_store_as(void *base, long long i, int live, const float (&v)[8])
+__device__ __forceinline__ void ad_store_as(void *base, long long i, int live, const float (&v)[4])
 {
-    if (live >= 8) return ad_store8<DT>(base, i, v);
+    if (live >= 4) return ad_store4<DT>(base, i, v);
 #pragma unroll
-    for (int k = 0; k < 8; k++)
+    for (int k = 0; k < 4; k++)
         if (k < live) ((typename DType<DT>::S *)base)[i + k] = DType<DT>::from_c(v[k]);
 }
-__device__ __forceinline__ void ad_store(void *base, int dt, long long i, int live, const float (&v)[8])
+__device__ __forceinline__ void ad_store(void *base, int dt, long long i, int live, const float (&v)[4])
 {
     if (dt == PT_FLOAT32) ad_store_as<PT_FLOAT32>(base, i, live, v);
     else if (dt == PT_FLOAT16) ad_store_as<PT_FLOAT16>(base, i, live, v);
@@ -129,33 +129,24 @@ __device__ __forceinline__ uint32_t ad_mix(uint32_t h)
 // 8-bit values.  A code's bits, moved to a float's exponent and mantissa,
 // are its value times 2^-120 (its exponent bias is 7), below the least
 // normal value too; the block's power of two is one more exact factor.
-__device__ __forceinline__ float ad_power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// (v_ldexp_f32 takes all of it in one instruction, rounding once)
 template <bool ROOT>
-__device__ __forceinline__ float ad_decode(uint32_t code, float scale)
+__device__ __forceinline__ float ad_decode(uint32_t code, int e)
 {
-    const uint32_t bits = ROOT ? code << 19 : (code & 127u) << 20;
-    const float x = __uint_as_float(bits) * 0x1p120f * scale;
-    if constexpr (ROOT) return x * x;
-    else return code & 128u ? -x : x;
+    if constexpr (ROOT) return ldexpf(__uint_as_float(code << 19), 120 + e);
+    else return ldexpf(__uint_as_float((code & 127u) << 20 | (code & 128u) << 24), 120 + e);
 }
 // drawn: 16 bits
 template <bool ROOT>
-__device__ __forceinline__ uint32_t ad_encode(float x, float inverse, uint32_t drawn)
+__device__ __forceinline__ uint32_t ad_encode(float x, int e, uint32_t drawn)
 {
     constexpr int LOW = ROOT ? 19 : 20;
-    const uint32_t size = __float_as_uint(fabsf(x) * inverse * 0x1p-120f);
+    const uint32_t size = __float_as_uint(ldexpf(fabsf(x), -120 - e));
     const uint32_t code = (size + (drawn << (LOW - 16)) + (1u << (LOW - 17))) >> LOW;
     return ROOT ? code : code | (x < 0.0f ? 128u : 0u);
 }
 // exponent of the power of two for a block's largest magnitude
 __device__ __forceinline__ int ad_exponent(float top) { return max((int)(__float_as_uint(top) >> 23) - 127 - 7, -126); }
-// the largest of 32 lanes' values (a block's 256 elements are 8 in each)
-__device__ __forceinline__ float ad_top(float v)
-{
-#pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, PT_WAVE));
-    return v;
-}
 
 template <bool SMALL, bool MASTER>
 __global__ __launch_bounds__(256) void k_adamw(AdamArgs a)
@@ -171,93 +162,120 @@ __global__ __launch_bounds__(256) void k_adamw(AdamArgs a)
     const float c1 = (power1 - 1.0f) * -1.0f, c2 = (power2 - 1.0f) * -1.0f;
     const float rate = a.rate ? a.rate[0] : a.rate_value;
     const float keep = a.rate ? (rate * a.decay - 1.0f) * -1.0f : a.decay_value;
+    // 8 bits: m / c1 / (sqrt(v) / sqrt(c2) + eps) rate
+    const float small_rate = rate / c1, small_root = 1.0f / sqrtf(c2);
     if (blockIdx.x == 0 && threadIdx.x == 0 && a.power1) {
         *a.power1 = power1;
         *a.power2 = power2;
         if (SMALL) *a.draws = (int32_t)((uint32_t)*a.draws0 + 1u);
     }
-    const long long i = (long long)(blockIdx.x - t.first) * kAdamBlock + threadIdx.x * 8;
-    // (the block of 256 that holds the tensor's end is written whole; lanes
-    // past it leave in the 32s that share one)
-    if (i >= ((t.n + 255) & ~255ll)) return;
-    const long long s = t.at + i;
-    const int live = (int)max(0ll, min(8ll, t.n - i));
-    float p[8], g[8], m[8], v[8];
-    if constexpr (MASTER) ad_load8<PT_FLOAT32>(a.master0, s, p);
-    else ad_load(t.p0, t.pdt, i, live, p);
-    ad_load(t.g, t.gdt, i, live, g);
-    float ms = 0.0f, vs = 0.0f;
-    if constexpr (SMALL) {
-        const ad_u32x2 mc = *(const ad_u32x2 *)((const uint8_t *)a.m0 + s), vc = *(const ad_u32x2 *)((const uint8_t *)a.v0 + s);
-        ms = ad_power(a.me0[s >> 8]);
-        vs = ad_power(a.ve0[s >> 8]);
+    // a wave takes 256 elements at a time, an 8-bit block, 4 a lane; it
+    // writes the 256 that hold the tensor's end whole
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const long long i0 = (long long)(blockIdx.x - t.first) * kAdamBlock + wave * (kAdamRounds * 256);
+    const int rounds = (int)min((long long)kAdamRounds, (t.n - i0 + 255) >> 8);  // (may be negative)
+    const uint32_t key = SMALL ? ad_mix((uint32_t)*a.draws0) : 0;
+    float p[kAdamRounds][4], g[kAdamRounds][4], m[kAdamRounds][4], v[kAdamRounds][4];
+    uint32_t mc[kAdamRounds], vc[kAdamRounds];
+    int me[kAdamRounds], ve[kAdamRounds];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            m[k] = ad_decode<false>(mc[k >> 2] >> (8 * (k & 3)) & 255u, ms);
-            v[k] = ad_decode<true>(vc[k >> 2] >> (8 * (k & 3)) & 255u, vs);
+    for (int r = 0; r < kAdamRounds; r++) {
+        if (r >= rounds) break;
+        const long long i = i0 + r * 256 + lane * 4, s = t.at + i;
+        const int live = (int)max(0ll, min(4ll, t.n - i));
+        if constexpr (MASTER) ad_load4<PT_FLOAT32>(a.master0, s, p[r]);
+        else ad_load(t.p0, t.pdt, i, live, p[r]);
+        ad_load(t.g, t.gdt, i, live, g[r]);
+        if constexpr (SMALL) {
+            mc[r] = __builtin_nontemporal_load((const uint32_t *)((const uint8_t *)a.m0 + s));
+            vc[r] = __builtin_nontemporal_load((const uint32_t *)((const uint8_t *)a.v0 + s));
+            me[r] = a.me0[(t.at + i0) / 256 + r];
+            ve[r] = a.ve0[(t.at + i0) / 256 + r];
+        } else {
+            ad_load4<PT_FLOAT32>(a.m0, s, m[r]);
+            ad_load4<PT_FLOAT32>(a.v0, s, v[r]);
         }
-    } else {
-        ad_load8<PT_FLOAT32>(a.m0, s, m);
-        ad_load8<PT_FLOAT32>(a.v0, s, v);
     }
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-        const float mk = m[k] * a.b1 + g[k] * a.one_b1;
-        const float vk = v[k] * a.b2 + (g[k] * g[k]) * a.one_b2;
-        const float step = (mk / c1) / (sqrtf(vk / c2) + a.eps) * rate;
-        const float pk = (t.decay ? p[k] * keep : p[k]) - step;
-        const bool taken = k < live && (SMALL ? fabsf(mk) < 0x1p126f && vk < 0x1p126f : g[k] == g[k]);
-        m[k] = taken ? mk : k < live ? m[k] : 0.0f;
-        v[k] = taken ? vk : k < live ? v[k] : 0.0f;
-        p[k] = taken ? pk : k < live ? p[k] : 0.0f;
-    }
-    if constexpr (MASTER) ad_store8<PT_FLOAT32>(a.master, s, p);
-    ad_store(t.p, t.pdt, i, live, p);
-    if constexpr (SMALL) {
-        float mt = 0.0f, vt = 0.0f;
+    for (int r = 0; r < kAdamRounds; r++) {
+        if (r >= rounds) break;
+        const long long i = i0 + r * 256 + lane * 4, s = t.at + i;
+        const int live = (int)max(0ll, min(4ll, t.n - i));
+        float root[4];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            v[k] = sqrtf(v[k]);
-            mt = fmaxf(mt, fabsf(m[k]));
-            vt = fmaxf(vt, v[k]);
+        for (int k = 0; k < 4; k++) {
+            if constexpr (SMALL) {
+                m[r][k] = ad_decode<false>(mc[r] >> (8 * k) & 255u, me[r]);
+                root[k] = ad_decode<true>(vc[r] >> (8 * k) & 255u, ve[r]);
+                v[r][k] = root[k] * root[k];  // (exact: 10 bits)
+            }
+            const float gk = g[r][k];
+            const float mk = m[r][k] * a.b1 + gk * a.one_b1;
+            const float vk = v[r][k] * a.b2 + (gk * gk) * a.one_b2;
+            float step, new_root = 0.0f;
+            if constexpr (SMALL) {
+                // the root that is held serves the step too, and the divisions
+                // by numbers of the whole call are products: a few ulps of the step
+                new_root = sqrtf(vk);
+                step = mk * small_rate * __builtin_amdgcn_rcpf(new_root * small_root + a.eps);
+            } else {
+                step = (mk / c1) / (sqrtf(vk / c2) + a.eps) * rate;
+            }
+            const float pk = (t.decay ? p[r][k] * keep : p[r][k]) - step;
+            const bool taken = k < live && (SMALL ? fabsf(mk) < 0x1p126f && vk < 0x1p126f : gk == gk);
+            if constexpr (SMALL) root[k] = taken ? new_root : k < live ? root[k] : 0.0f;
+            else v[r][k] = taken ? vk : k < live ? v[r][k] : 0.0f;
+            m[r][k] = taken ? mk : k < live ? m[r][k] : 0.0f;
+            p[r][k] = taken ? pk : k < live ? p[r][k] : 0.0f;
         }
-        const int me = ad_exponent(ad_top(mt)), ve = ad_exponent(ad_top(vt));
-        const float mi = ad_power(-me), vi = ad_power(-ve);
-        const uint32_t key = ad_mix((uint32_t)*a.draws0);
-        ad_u32x2 mc = {0, 0}, vc = {0, 0};
+        if constexpr (MASTER) ad_store4<PT_FLOAT32>(a.master, s, p[r]);
+        ad_store(t.p, t.pdt, i, live, p[r]);
+        if constexpr (SMALL) {
+            float mt = 0.0f, vt = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const uint32_t drawn = ad_mix((uint32_t)(s + k) + key + (uint32_t)(s >> 32) * 0x9E3779B9u);
-            mc[k >> 2] |= ad_encode<false>(m[k], mi, drawn & 0xffffu) << (8 * (k & 3));
-            vc[k >> 2] |= ad_encode<true>(v[k], vi, drawn >> 16) << (8 * (k & 3));
+            for (int k = 0; k < 4; k++) {
+                mt = fmaxf(mt, fabsf(m[r][k]));
+                vt = fmaxf(vt, root[k]);
+            }
+            const int mx = ad_exponent(wave_all(mt, FMax{})), vx = ad_exponent(wave_all(vt, FMax{}));
+            uint32_t mo = 0, vo = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t drawn = ad_mix((uint32_t)(s + k) + key + (uint32_t)(s >> 32) * 0x9E3779B9u);
+                mo |= ad_encode<false>(m[r][k], mx, drawn & 0xffffu) << (8 * k);
+                vo |= ad_encode<true>(root[k], vx, drawn >> 16) << (8 * k);
+            }
+            __builtin_nontemporal_store(mo, (uint32_t *)((uint8_t *)a.m + s));
+            __builtin_nontemporal_store(vo, (uint32_t *)((uint8_t *)a.v + s));
+            if (lane == 0) {
+                a.me[(t.at + i0) / 256 + r] = (int8_t)mx;
+                a.ve[(t.at + i0) / 256 + r] = (int8_t)vx;
+            }
+        } else {
+            ad_store4<PT_FLOAT32>(a.m, s, m[r]);
+            ad_store4<PT_FLOAT32>(a.v, s, v[r]);
         }
-        *(ad_u32x2 *)((uint8_t *)a.m + s) = mc;
-        *(ad_u32x2 *)((uint8_t *)a.v + s) = vc;
-        if ((threadIdx.x & 31) == 0) {
-            a.me[s >> 8] = (int8_t)me;
-            a.ve[s >> 8] = (int8_t)ve;
-        }
-    } else {
-        ad_store8<PT_FLOAT32>(a.m, s, m);
-        ad_store8<PT_FLOAT32>(a.v, s, v);
     }
 }
 
-// float32 values of 8-bit moments; n a multiple of 256
+// float32 values of 8-bit moments; a wave takes a block of 256, 4 a lane
 __global__ __launch_bounds__(256) void k_adamw_moments(const uint8_t *m, const int8_t *me, const uint8_t *v, const int8_t *ve,
-                                                       float *mo, float *vo, long long n)
+                                                       float *mo, float *vo, long long blocks)
 {
-    for (long long s = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; s < n; s += (long long)gridDim.x * 2048) {
-        const ad_u32x2 mc = *(const ad_u32x2 *)(m + s), vc = *(const ad_u32x2 *)(v + s);
-        const float ms = ad_power(me[s >> 8]), vs = ad_power(ve[s >> 8]);
-        float x[8], y[8];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    for (long long b = (long long)blockIdx.x * 4 + wave; b < blocks; b += (long long)gridDim.x * 4) {
+        const long long s = b * 256 + lane * 4;
+        const uint32_t mc = __builtin_nontemporal_load((const uint32_t *)(m + s)), vc = __builtin_nontemporal_load((const uint32_t *)(v + s));
+        const int mx = me[b], vx = ve[b];
+        float x[4], y[4];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            x[k] = ad_decode<false>(mc[k >> 2] >> (8 * (k & 3)) & 255u, ms);
-            y[k] = ad_decode<true>(vc[k >> 2] >> (8 * (k & 3)) & 255u, vs);
+        for (int k = 0; k < 4; k++) {
+            x[k] = ad_decode<false>(mc >> (8 * k) & 255u, mx);
+            const float root = ad_decode<true>(vc >> (8 * k) & 255u, vx);
+            y[k] = root * root;
         }
-        ad_store8<PT_FLOAT32>(mo, s, x);
-        ad_store8<PT_FLOAT32>(vo, s, y);
+        ad_store4<PT_FLOAT32>(mo, s, x);
+        ad_store4<PT_FLOAT32>(vo, s, y);
     }
 }
 
@@ -367,9 +385,9 @@ pt_status pt_adamw_moments(const void *first, const int8_t *first_exponent, cons
         return fail(PT_ERR_INVALID, "8-bit moments miss an operand");
     PT_TRY(ensure_init());
     if (!n) return PT_OK;
-    const unsigned blocks = (unsigned)std::min<size_t>((n + 2047) / 2048, 1 << 20);
+    const unsigned blocks = (unsigned)std::min<size_t>((n / 256 + 3) / 4, 1 << 24);
     k_adamw_moments<<<blocks, 256, 0, stream_of(stream)>>>((const uint8_t *)first, first_exponent, (const uint8_t *)second,
-                                                           second_exponent, first_values, second_values, (long long)n);
+                                                           second_exponent, first_values, second_values, (long long)(n / 256));
     return check_hip(hipGetLastError(), "8-bit moments");
 }
 
