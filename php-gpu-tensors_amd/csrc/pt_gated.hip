@@ -23,20 +23,24 @@ namespace pt {
 // per element), are the B operands of 8 16x16x32 MFMAs, the c-th of which
 // yields each lane's column c; x, 16 rows of it, is the A operand as it
 // lies.  32 bits: each loaded row is the B operand of 4 16x16x4 MFMAs.  So no
-// weight passes through LDS, and the next step's 16 loads are in flight over
-// this step's MFMAs.  The k-steps go to the 8 waves of a block and to S
-// blocks in turn; the waves' sums meet in LDS, in a fixed order, and the
-// blocks' in a second kernel.
+// weight passes through LDS.  One matrix's loads of the next step go into
+// the registers that its products have just left, while the other's are
+// multiplied.  The k-steps go to the 8 waves of a block and to S blocks in
+// turn; the waves' sums meet in LDS, where each wave adds an eighth of the
+// columns in order, and the blocks' in a second kernel.
 constexpr int kFewWaves = 8;
 typedef unsigned gd_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
 
-template <int DT, int MT>
+template <int DT, int MT, int NC>
 __global__ __launch_bounds__(64 * kFewWaves) void k_gated_few(PairArgs g)
 {
     using S = typename GE<DT>::S;
-    constexpr int NC = 16 / sizeof(S);  // columns of a lane
+    constexpr int XV = 16 / sizeof(S);  // elements of x in 16 bytes
+    typedef unsigned words __attribute__((ext_vector_type(NC * sizeof(S) / 4), aligned(1)));
+    constexpr int NW = NC * sizeof(S) / 4;
     constexpr bool LOW = DT != PT_FLOAT32;
-    __shared__ float box[kFewWaves / 2][2 * NC * 4][64];
+    constexpr int SUMS = 2 * NC * 4;    // of a lane and 16 rows
+    __shared__ float box[kFewWaves][SUMS][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kg = lane >> 4, n0 = blockIdx.x * 16 * NC + (lane & 15) * NC, at = min(n0, g.N - NC);
     const S *B[2] = {(const S *)g.b0 + at, (const S *)g.b1 + at};
@@ -52,144 +56,141 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_gated_few(PairArgs g)
 #pragma unroll
             for (int c = 0; c < NC; c++) acc[m][j][c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
+    words w[2][8];
+    gd_u32x4 xv[MT][LOW ? 1 : 2];
     // rows past K: the last one again, taken as zeros below
-    gd_u32x4 w[2][8], xv[MT][LOW ? 1 : 2];
-    auto load = [&](int k0, gd_u32x4 (&w)[2][8], gd_u32x4 (&xv)[MT][LOW ? 1 : 2]) {
+    auto load_w = [&](auto J, int k0) {
+        constexpr int j = decltype(J)::value;
         const int k = k0 + kg * 8;
+        if (k0 + 32 <= g.K) {  // uniform
+            const S *p = B[j] + (long long)k * g.ldb;
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+            for (int i = 0; i < 8; i++) w[j][i] = __builtin_nontemporal_load((const words *)(p + (long long)i * g.ldb));
+        } else {
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                w[j][i] = __builtin_nontemporal_load((const gd_u32x4 *)(B[j] + (long long)min(k + i, g.K - 1) * g.ldb));
+            for (int i = 0; i < 8; i++) w[j][i] = *(const words *)(B[j] + (long long)min(k + i, g.K - 1) * g.ldb);
+        }
+    };
+    auto load_x = [&](int k0) {
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int q = 0; q < (LOW ? 1 : 2); q++) {
-                const int kx = k + q * NC;
-                if (kx + NC <= g.K) xv[m][q] = *(const gd_u32x4 *)(x[m] + kx);
+                const int kx = k0 + kg * 8 + q * XV;
+                if (k0 + 32 <= g.K) xv[m][q] = *(const gd_u32x4 *)(x[m] + kx);  // uniform
                 else {
-                    union { gd_u32x4 raw; S s[NC]; } u;
+                    union { gd_u32x4 raw; S s[XV]; } u;
 #pragma unroll
-                    for (int c = 0; c < NC; c++) u.s[c] = kx + c < g.K ? x[m][kx + c] : (S)0;
+                    for (int c = 0; c < XV; c++) u.s[c] = kx + c < g.K ? x[m][kx + c] : (S)0;
                     xv[m][q] = u.raw;
                 }
             }
     };
-    auto multiply = [&](int k0, gd_u32x4 (&w)[2][8], gd_u32x4 (&xv)[MT][LOW ? 1 : 2]) {
+    auto multiply = [&](auto J, int k0) {
+        constexpr int j = decltype(J)::value;
         if (k0 + 32 > g.K) {  // uniform: what the last step has past K is zeros
             const int k = k0 + kg * 8;
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int i = 0; i < 8; i++)
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) w[j][i][d] = k + i < g.K ? w[j][i][d] : 0u;
+                for (int d = 0; d < NW; d++) w[j][i][d] = k + i < g.K ? w[j][i][d] : 0u;
         }
+        if constexpr (LOW) {
+            using Frag = typename FragT<DT>::type;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            if constexpr (LOW) {
-                using Frag = typename FragT<DT>::type;
+            for (int d = 0; d < NW; d++)
 #pragma unroll
-                for (int d = 0; d < 4; d++)
+                for (int h = 0; h < 2; h++) {
+                    gd_u32x4 col;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        gd_u32x4 col;
+                    for (int i = 0; i < 4; i++)
+                        col[i] = __builtin_amdgcn_perm(w[j][2 * i + 1][d], w[j][2 * i][d], h ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            col[i] = __builtin_amdgcn_perm(w[j][2 * i + 1][d], w[j][2 * i][d], h ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                        for (int m = 0; m < MT; m++) {
-                            floatx4 &to = acc[m][j][2 * d + h];
-                            const Frag fx = __builtin_bit_cast(Frag, xv[m][0]), fw = __builtin_bit_cast(Frag, col);
-                            if constexpr (DT == PT_BFLOAT16) to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fw, to, 0, 0, 0);
-                            else to = __builtin_amdgcn_mfma_f32_16x16x32_f16(fx, fw, to, 0, 0, 0);
-                        }
+                    for (int m = 0; m < MT; m++) {
+                        floatx4 &to = acc[m][j][2 * d + h];
+                        const Frag fx = __builtin_bit_cast(Frag, xv[m][0]), fw = __builtin_bit_cast(Frag, col);
+                        if constexpr (DT == PT_BFLOAT16) to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fw, to, 0, 0, 0);
+                        else to = __builtin_amdgcn_mfma_f32_16x16x32_f16(fx, fw, to, 0, 0, 0);
                     }
-            } else {
+                }
+        } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++)
+            for (int i = 0; i < 8; i++)
 #pragma unroll
-                    for (int m = 0; m < MT; m++)
+                for (int m = 0; m < MT; m++)
 #pragma unroll
-                        for (int c = 0; c < NC; c++)
-                            acc[m][j][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(xv[m][i / 4][i % 4]),
-                                                                                __uint_as_float(w[j][i][c]), acc[m][j][c], 0, 0, 0);
-            }
+                    for (int c = 0; c < NC; c++)
+                        acc[m][j][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(xv[m][i / 4][i % 4]),
+                                                                            __uint_as_float(w[j][i][c]), acc[m][j][c], 0, 0, 0);
         }
     };
     const int step = 32 * kFewWaves * g.split;
     int k0 = 32 * ((int)blockIdx.y * kFewWaves + wave);
     if (k0 < g.K) {
-        load(k0, w, xv);
+        load_w(IC<0>{}, k0);
+        load_x(k0);
+        load_w(IC<1>{}, k0);
         for (;;) {
-            gd_u32x4 wn[2][8], xn[MT][LOW ? 1 : 2];
-            const bool more = k0 + step < g.K;
-            if (more) load(k0 + step, wn, xn);
-            multiply(k0, w, xv);
-            if (!more) break;
-            k0 += step;
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) w[j][i] = wn[j][i];
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int q = 0; q < (LOW ? 1 : 2); q++) xv[m][q] = xn[m][q];
+            const int next = k0 + step;
+            multiply(IC<0>{}, k0);
+            if (next < g.K) load_w(IC<0>{}, next);
+            multiply(IC<1>{}, k0);
+            if (next >= g.K) break;
+            load_x(next);
+            load_w(IC<1>{}, next);
+            k0 = next;
         }
     }
-    // waves w + half add to waves w, half = 4, 2, 1
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-        for (int half = kFewWaves / 2; half; half >>= 1) {
-            __syncthreads();
-            if (wave >= half && wave < 2 * half) {
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int c = 0; c < NC; c++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) box[wave - half][(j * NC + c) * 4 + e][lane] = acc[m][j][c][e];
-            }
-            __syncthreads();
-            if (wave < half) {
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int c = 0; c < NC; c++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) acc[m][j][c][e] += box[wave][(j * NC + c) * 4 + e][lane];
-            }
-        }
-    if (wave || n0 >= g.n_out) return;
-    // lane: rows 4 (l / 16) + e, columns at .. at + NC - 1.  The lane whose
-    // pack was moved back from the end stores what its neighbour stores too.
+    // Each wave adds an eighth of the sums over the waves, in their order, and
+    // stores: SUMS / 8 of them are 4 rows of one column (two in 16 bits) of
+    // the first product or of the second, so waves w and w + 4 hold the same
+    // columns of the two and meet once more.
+    constexpr int MINE = SUMS / kFewWaves;
     const long long plane = (long long)g.M * g.n_out;
-    const int live = min(NC, g.n_out - at);
+    const int live = n0 < g.n_out ? min(NC, g.n_out - at) : 0;
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int m = 0; m < MT; m++) {
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int row = m * 16 + kg * 4 + e;
-            if (row >= g.M) continue;
-            const long long to = (long long)row * g.n_out + at;
+        for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                if (c >= live) continue;
-                const float p = acc[m][0][c][e], q = acc[m][1][c][e];
-                if (g.split > 1) {
-                    float *part = g.parts + (long long)blockIdx.y * 2 * plane + to + c;
-                    part[0] = p;
-                    part[plane] = q;
-                    continue;
-                }
-                if (g.c1) {
-                    store_c<DT>(g.c1, (size_t)(to + c), p);
-                    store_c<DT>(g.c2, (size_t)(to + c), q);
-                }
-                store_c<DT>(g.c0, (size_t)(to + c), gated_act<LOW>(g.act, p) * q);
-            }
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) box[wave][(j * NC + c) * 4 + e][lane] = acc[m][j][c][e];
+        __syncthreads();
+        float sum[MINE];
+#pragma unroll
+        for (int i = 0; i < MINE; i++) {
+            sum[i] = box[0][wave * MINE + i][lane];
+#pragma unroll
+            for (int v = 1; v < kFewWaves; v++) sum[i] += box[v][wave * MINE + i][lane];
         }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MINE; i++) box[0][wave * MINE + i][lane] = sum[i];
+        __syncthreads();
+        // lane: rows 4 (l / 16) + e, columns at .. at + NC - 1.  The lane
+        // whose pack was moved back from the end stores what its neighbour
+        // stores too.
+#pragma unroll
+        for (int i = 0; i < MINE / 2; i++) {
+            const int q = wave * (MINE / 2) + i, c = q / 4, e = q % 4, row = m * 16 + kg * 4 + e;
+            if (row >= g.M || c >= live) continue;
+            const float p = box[0][q][lane], u = box[0][NC * 4 + q][lane];
+            const long long to = (long long)row * g.n_out + at + c;
+            if (g.split > 1) {
+                float *part = g.parts + (long long)blockIdx.y * 2 * plane + to;
+                part[0] = p;
+                part[plane] = u;
+                continue;
+            }
+            if (g.c1) {
+                store_c<DT>(g.c1, (size_t)to, p);
+                store_c<DT>(g.c2, (size_t)to, u);
+            }
+            store_c<DT>(g.c0, (size_t)to, gated_act<LOW>(g.act, p) * u);
+        }
+    }
 }
 
 // ------------------------------------------------- passes over elements
@@ -382,17 +383,29 @@ static pt_status product_f32(const float *a, size_t am, size_t ak, const float *
     return pt_matmul(a, b, c, PT_FLOAT32, sa, ta, 2, sb, tb, 2, sc, 2, stream);
 }
 
-// Blocks that a strip's k-steps are split over: up to a block for every CU.
+// Wide strips, whose k-steps are split over up to a block for every CU; strips
+// of 8-byte packs, without a split, where the split's second kernel (4.5 us)
+// costs more than the CUs that they leave idle: a CU streams 33 GB/s, all of
+// them 5.3 TB/s.  One row of bfloat16, wide against narrow: 4096 x 16384 54
+// and 49 us, 512 x 2048 8.5 and 5.3, 4096 x 4096 19 and 35.
 template <int DT>
 static pt_status launch_few(PairArgs &g, GatedScratch &scratch, hipStream_t s)
 {
-    constexpr int COLS = 16 * GE<DT>::PK;
-    const int strips = (g.n_out + COLS - 1) / COLS, steps = (g.K + 31) / 32;
-    g.split = std::max(1, std::min({256 / strips, steps / kFewWaves, 16}));
+    constexpr int NC = GE<DT>::PK;
+    const int wide = (g.n_out + 16 * NC - 1) / (16 * NC), narrow = (g.n_out + 8 * NC - 1) / (8 * NC), steps = (g.K + 31) / 32;
+    const double bytes = 2.0 * g.K * g.n_out * sizeof(typename GE<DT>::S);
+    g.split = std::max(1, std::min({256 / wide, steps / kFewWaves, 16}));
+    const bool thin = g.split > 1 && bytes / (std::min(narrow, 160) * 33e9) < bytes / 5.3e12 + 4.5e-6;
+    if (thin) g.split = 1;
     if (g.split > 1) PT_TRY(scratch.take((void **)&g.parts, (size_t)g.split * 2 * g.M * g.n_out * sizeof(float)));
-    const dim3 grid(strips, g.split);
-    if (g.M <= 16) k_gated_few<DT, 1><<<grid, 64 * kFewWaves, 0, s>>>(g);
-    else k_gated_few<DT, 2><<<grid, 64 * kFewWaves, 0, s>>>(g);
+    const dim3 grid(thin ? narrow : wide, g.split);
+    if (thin) {
+        if (g.M <= 16) k_gated_few<DT, 1, NC / 2><<<grid, 64 * kFewWaves, 0, s>>>(g);
+        else k_gated_few<DT, 2, NC / 2><<<grid, 64 * kFewWaves, 0, s>>>(g);
+    } else {
+        if (g.M <= 16) k_gated_few<DT, 1, NC><<<grid, 64 * kFewWaves, 0, s>>>(g);
+        else k_gated_few<DT, 2, NC><<<grid, 64 * kFewWaves, 0, s>>>(g);
+    }
     if (g.split > 1) launch_pair_join(g, DT, g.c1 ? GATED_KEPT : GATED_PRODUCT, s);
     return PT_OK;
 }
