@@ -403,15 +403,15 @@ typedef struct {
     int dtype, activation;
     int rows, inner, outer;   /* each at most 2^21 */
 } pt_gated_desc;
-/* kept (may be NULL): [2][rows][outer], both products rounded to the dtype,
- * for the backward call.  Results must not overlap operands, here and in
+/* kept (may be NULL): for the backward call, both products in 24 bits (16-bit
+ * dtypes: 6 rows outer bytes, opaque) or in float32 (8 rows outer bytes).  Results must not overlap operands, here and in
  * the backward call. */
 pt_status pt_gated(const pt_gated_desc *desc, const void *x, const void *gate, const void *up, void *h, void *kept,
                    pt_stream_t stream);
 /* Gradients, contiguous and of the dtype, for the upstream gradient `grad`
  * (contiguous like h, float32 or the dtype): dx, and dgate with dup; dx may
- * be NULL, or dgate and dup both.  In 16 bits the products' gradients are
- * rounded to the dtype for the products that follow.  Results do not depend
+ * be NULL, or dgate and dup both.  In 16 bits the gradients of both
+ * products are rounded to the dtype for the products that follow.  Results do not depend
  * on timing. */
 pt_status pt_gated_backward(const pt_gated_desc *desc, const void *x, const void *gate, const void *up, const void *kept,
                             const void *grad, int grad_dtype, void *dx, void *dgate, void *dup, pt_stream_t stream);

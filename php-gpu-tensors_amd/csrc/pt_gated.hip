@@ -184,25 +184,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_gated_few(PairArgs g)
                 part[plane] = u;
                 continue;
             }
-            if (g.c1) {
-                store_c<DT>(g.c1, (size_t)to, p);
-                store_c<DT>(g.c2, (size_t)to, u);
-            }
+            if (g.c1) gated_keep<DT>(g.c1, plane, to, p, u);
             store_c<DT>(g.c0, (size_t)to, gated_act<LOW>(g.act, p) * u);
         }
     }
 }
 
 // ------------------------------------------------- passes over elements
-// h of fp32 products that lie behind each other.
-__global__ __launch_bounds__(256) void k_gated_product(const float *p, float *h, long long n, int act)
-{
-    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024)
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (i + k < n) h[i + k] = gated_act<false>(act, p[i + k]) * p[n + i + k];
-}
-
 // V elements from p at any element boundary
 template <int DT, int V>
 __device__ __forceinline__ void gd_load(const typename GE<DT>::S *p, int live, float (&v)[V])
@@ -222,6 +210,41 @@ __device__ __forceinline__ void gd_load(const typename GE<DT>::S *p, int live, f
     for (int k = 0; k < V; k++) v[k] = k < live ? DType<DT>::to_c(p[k]) : 0.0f;
 }
 
+// h of fp32 products that lie behind each other; a thread takes 4 elements.
+__global__ __launch_bounds__(256) void k_gated_product(const float *p, float *h, long long n, int act)
+{
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
+        const int live = (int)min(4ll, n - i);
+        float g[4], u[4];
+        gd_load<PT_FLOAT32, 4>(p + i, live, g);
+        gd_load<PT_FLOAT32, 4>(p + n + i, live, u);
+        typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+        float4u v;
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = gated_act<false>(act, g[k]) * u[k];
+        if (live == 4) *(float4u *)(h + i) = v;
+        else
+            for (int k = 0; k < live; k++) h[i + k] = v[k];
+    }
+}
+
+// 8 elements of a product as the gradient keeps it in 24 bits
+__device__ __forceinline__ void gd_load_kept(const void *kept, long long n, int product, long long i, int live, float (&v)[8])
+{
+    const uint16_t *high = (const uint16_t *)((const char *)kept + kept_plane(n, product, false)) + i;
+    const uint8_t *low = (const uint8_t *)kept + kept_plane(n, product, true) + i;
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2), aligned(1)));
+    if (live >= 8) {
+        const gd_u32x4 h = __builtin_nontemporal_load((const gd_u32x4 *)high);
+        const u32x2 l = __builtin_nontemporal_load((const u32x2 *)low);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = kept_value(h[k / 2] >> (k & 1 ? 16 : 0) & 0xffffu, l[k / 4] >> (8 * (k % 4)) & 0xffu);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = k < live ? kept_value(high[k], low[k]) : 0.0f;
+}
+
 // dg and du from the upstream gradient and both products, into rows `pitch`
 // elements apart from d and d + second on, zeros in columns `cols` to
 // `padded` - 1.  A thread takes 8 columns.
@@ -237,8 +260,13 @@ __global__ __launch_bounds__(256) void k_gated_slope(const void *kept, const voi
         const int c = (int)(i - row * packs) * 8, live = min(8, cols - c);
         const long long from = row * cols + c;
         float g[8], u[8], dh[8];
-        gd_load<DT, 8>((const S *)kept + from, live, g);
-        gd_load<DT, 8>((const S *)kept + plane + from, live, u);
+        if constexpr (DT == PT_FLOAT32) {
+            gd_load<DT, 8>((const S *)kept + from, live, g);
+            gd_load<DT, 8>((const S *)kept + plane + from, live, u);
+        } else {
+            gd_load_kept(kept, plane, 0, from, live, g);
+            gd_load_kept(kept, plane, 1, from, live, u);
+        }
         gd_load<GDT, 8>((const typename GE<GDT>::S *)grad + from, live, dh);
         S dg[8], du[8];
 #pragma unroll
@@ -265,20 +293,30 @@ __global__ __launch_bounds__(256) void k_gated_slope(const void *kept, const voi
     }
 }
 
-// two fp32 matrices side by side
-__global__ __launch_bounds__(256) void k_gated_beside(const float *a, const float *b, float *to, int rows, int cols)
+// Two fp32 matrices side by side, or (BACK) apart again.
+template <bool BACK>
+__global__ __launch_bounds__(256) void k_gated_beside(float *a, float *b, float *both, int rows, int cols)
 {
     const long long n = (long long)rows * cols;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
         const long long row = i / cols, at = i + row * cols;
-        to[at] = a[i];
-        to[at + cols] = b[i];
+        if constexpr (BACK) {
+            a[i] = both[at];
+            b[i] = both[at + cols];
+        } else {
+            both[at] = a[i];
+            both[at + cols] = b[i];
+        }
     }
 }
 
-// rows x cols of 16-bit elements into rows of `pitch`, zeros past the end
-__global__ __launch_bounds__(256) void k_gated_pack(const uint16_t *from, uint16_t *to, long long rows, int cols, int pitch)
+// One or two matrices (blockIdx.y) of 16-bit elements into rows of `pitch`,
+// zeros past the end; the second `apart` elements behind the first.
+__global__ __launch_bounds__(256) void k_gated_pack(const uint16_t *from0, const uint16_t *from1, uint16_t *to, long long apart,
+                                                    long long rows, int cols, int pitch)
 {
+    const uint16_t *from = blockIdx.y ? from1 : from0;
+    to += blockIdx.y * apart;
     const int packs = pitch / 8;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * packs; i += (long long)gridDim.x * 256) {
         const long long row = i / packs;
@@ -341,16 +379,21 @@ struct GatedScratch {
         held[count++] = *p;
         return PT_OK;
     }
-    // a 16-bit matrix whose rows start at 16-byte boundaries: itself, or a copy
-    pt_status rows16(const void *from, long long rows, int cols, const void **to, long long *pitch)
+    // 16-bit matrices (b may be null) whose rows start at 16-byte boundaries:
+    // themselves, or copies
+    pt_status rows16(const void *a, const void *b, long long rows, int cols, const void **to_a, const void **to_b, long long *pitch)
     {
         *pitch = round8(cols);
-        *to = from;
-        if (cols % 8 == 0 && ((uintptr_t)from & 15) == 0) return PT_OK;
-        void *p = nullptr;
-        PT_TRY(take(&p, (size_t)rows * *pitch * 2));
-        k_gated_pack<<<grid_for(rows * (*pitch / 8)), 256, 0, s>>>((const uint16_t *)from, (uint16_t *)p, rows, cols, (int)*pitch);
-        *to = p;
+        *to_a = a;
+        if (b) *to_b = b;
+        if (cols % 8 == 0 && (((uintptr_t)a | (uintptr_t)b) & 15) == 0) return PT_OK;
+        uint16_t *p = nullptr;
+        const long long each = rows * *pitch;
+        PT_TRY(take((void **)&p, (size_t)each * (b ? 4 : 2)));
+        k_gated_pack<<<dim3(grid_for(each / 8), b ? 2 : 1), 256, 0, s>>>((const uint16_t *)a, (const uint16_t *)b, p, each, rows,
+                                                                         cols, (int)*pitch);
+        *to_a = p;
+        if (b) *to_b = p + each;
         return PT_OK;
     }
 };
@@ -417,14 +460,12 @@ static pt_status gated_run(const pt_gated_desc *d, const void *x, const void *ga
     GatedScratch scratch(s);
     const int M = d->rows, K = d->inner, F = d->outer;
     const size_t size = dtype_size(d->dtype), n = (size_t)M * F;
-    void *second = kept ? (char *)kept + n * size : nullptr;
     PairArgs g = {};
     g.M = M;
     g.act = d->activation;
     g.n_out = F;
     g.c0 = h;
     g.c1 = kept;
-    g.c2 = second;
     g.a0 = x;
     g.b0 = gate;
     g.b1 = up;
@@ -444,9 +485,8 @@ static pt_status gated_run(const pt_gated_desc *d, const void *x, const void *ga
         k_gated_product<<<grid_for((long long)(n + 3) / 4), 256, 0, s>>>(p, (float *)h, (long long)n, d->activation);
         return PT_OK;
     }
-    PT_TRY(scratch.rows16(x, M, K, &g.a0, &g.lda));
-    PT_TRY(scratch.rows16(gate, K, F, &g.b0, &g.ldb));
-    PT_TRY(scratch.rows16(up, K, F, &g.b1, &g.ldb));
+    PT_TRY(scratch.rows16(x, nullptr, M, K, &g.a0, nullptr, &g.lda));
+    PT_TRY(scratch.rows16(gate, up, K, F, &g.b0, &g.b1, &g.ldb));
     // (of K rounded to 8, A's elements past K are zeros or B's rows past it are out of range)
     g.K = round8(K);
     g.N = (int)g.ldb;
@@ -469,10 +509,18 @@ static pt_status gated_backward_f32(const pt_gated_desc *d, const float *x, cons
                                                                                               d->activation);
     if (dx) {
         PT_TRY(scratch.take((void **)&weights, (size_t)K * 2 * F * sizeof(float)));
-        k_gated_beside<<<grid_for((long long)K * F), 256, 0, s>>>(gate, up, weights, K, F);
+        k_gated_beside<false><<<grid_for((long long)K * F), 256, 0, s>>>((float *)gate, (float *)up, weights, K, F);
         PT_TRY(product_f32(both, 2 * F, 1, weights, 1, 2 * F, dx, M, K, 2 * F, stream));
     }
-    if (dgate) {
+    // both weights' gradients in one product where one alone has fewer tiles
+    // than the GPU has CUs (4096 x 784 x 1024: 149 us with the pass that takes
+    // them apart, 157 one after the other)
+    if (dgate && (long long)((K + 127) / 128) * ((F + 127) / 128) < 256) {
+        float *beside = nullptr;
+        PT_TRY(scratch.take((void **)&beside, (size_t)K * 2 * F * sizeof(float)));
+        PT_TRY(product_f32(x, 1, K, both, 2 * F, 1, beside, K, 2 * F, M, stream));
+        k_gated_beside<true><<<grid_for((long long)K * F), 256, 0, s>>>(dgate, dup, beside, K, F);
+    } else if (dgate) {
         PT_TRY(product_f32(x, 1, K, both, 2 * F, 1, dgate, K, F, M, stream));
         PT_TRY(product_f32(x, 1, K, both + F, 2 * F, 1, dup, K, F, M, stream));
     }
@@ -506,8 +554,7 @@ static pt_status gated_backward_run(const pt_gated_desc *d, const void *x, const
         g.a0 = dg;
         g.a1 = dg + second;
         g.lda = pitch;
-        PT_TRY(scratch.rows16(gate, K, F, &g.b0, &g.ldb));
-        PT_TRY(scratch.rows16(up, K, F, &g.b1, &g.ldb));
+        PT_TRY(scratch.rows16(gate, up, K, F, &g.b0, &g.b1, &g.ldb));
         g.M = M;
         g.N = g.n_out = K;
         g.K = pitch;
@@ -554,7 +601,8 @@ pt_status pt_gated(const pt_gated_desc *d, const void *x, const void *gate, cons
     PT_TRY(ensure_init());
     if (!n) return PT_OK;
     if (!d->inner) {  // empty sums: act(0) 0
-        PT_TRY(zeros(kept, d->dtype, 2 * n, stream));
+        if (d->dtype == PT_FLOAT32) PT_TRY(zeros(kept, PT_FLOAT32, 2 * n, stream));
+        else PT_TRY(zeros(kept, PT_UINT8, 6 * n, stream));
         return zeros(h, d->dtype, n, stream);
     }
     PT_TRY(gated_run(d, x, gate, up, h, kept, stream));

@@ -9,8 +9,8 @@
 // MFMA-bound: both run the ring of the plain whole-line product
 // (pt_gemm_ring.hip): 8 waves in 2 x 4, A in 3 superstages of 64 k (whole
 // 128-byte lines), B in 4 stages of 32 k, one barrier a step, a load to LDS
-// between every few MFMAs, all reads' offsets immediate.  Tiles of 128 rows
-// (TM = 2) serve few rows.  Edges cost nothing inside: rows and columns past
+// between every few MFMAs, all reads' offsets immediate.  Tiles of 192 and 128
+// rows (TM = 3, 2) serve where tiles of 256 leave CUs idle.  Edges cost nothing inside: rows and columns past
 // the end read the last ones again and are not stored; past the
 // contraction's end a lane's offset leaves the buffer's range, for which the
 // buffer unit returns zeros, so what lies there (another row, or nothing) is
@@ -41,9 +41,11 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
     constexpr int NSA = 3, NSB = 4, PERIOD = 12, NS = 2;
     constexpr int SA_ELEMS = BM * 2 * BK;  // superstage: BM rows x 64 k
     constexpr int B_ELEMS = 256 * BK;
-    constexpr int NQA = BM / 128, NQB = 2, PER = NQA + NQB;  // load instructions of a wave and step
+    // load instructions of a wave and step (192 rows: 12 of A, the last one
+    // again by the waves that have none left, so that all wait for as many)
+    constexpr int NQA = (BM + 127) / 128, NQB = 2, PER = NQA + NQB;
     constexpr int GROUP_M = 4;
-    static_assert(TM == 2 || TM == 4, "load split");
+    static_assert(TM >= 2 && TM <= 4, "load split");
     constexpr int SPA = pair_bases(SA_ELEMS * 2, (TM - 1) * 32 * 2 * BK * 2);
     constexpr int SPB = SUM ? pair_bases(B_ELEMS * 2, 32 * BK * 2) : pair_bases(B_ELEMS * 2, (16 + 4) * 128 * 2);
     static_assert(2 * SPA >= NSA && 2 * SPB >= NSB, "two bases cover the rings");
@@ -78,7 +80,7 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
     for (int h = 0; h < 2; h++)
 #pragma unroll
         for (int q4 = 0; q4 < NQA; q4++) {
-            const int row = h * (BM / 2) + (wave * NQA + q4) * 8 + lane / 8, c = (lane % 8) ^ swz_k(row, 8);
+            const int row = h * (BM / 2) + min(wave * NQA + q4, BM / 16 - 1) * 8 + lane / 8, c = (lane % 8) ^ swz_k(row, 8);
             offa[h][q4] = (uint32_t)((long long)(min(m0 + row, g.M - 1) - m0) * g.lda + c * 8) * 2u;
             tail_a[h][q4] = c * 8 < tail ? offa[h][q4] : kPairOut;
         }
@@ -111,7 +113,7 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
             const bool second = SUM && s >= each;
             const int sm = second ? s - each : s;
             buffer_load_lds16(A + ((second ? to_a1 : 0) + (long long)sm * 64), sm == last ? tail_a[h][idx] : offa[h][idx],
-                              (PT_LDS_AS void *)(lds_a + slot * SA_ELEMS + (h * (BM / 2) + (wave * NQA + idx) * 8) * 2 * BK),
+                              (PT_LDS_AS void *)(lds_a + slot * SA_ELEMS + (h * (BM / 2) + min(wave * NQA + idx, BM / 16 - 1) * 8) * 2 * BK),
                               kPairRange);
         } else {
             constexpr int q4 = idx - NQA, slot = (j + 3) % NSB;
@@ -195,6 +197,8 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
         if constexpr (TM == 4)
             asm volatile("s_waitcnt lgkmcnt(0)"
                          : "+v"(fa[0]), "+v"(fa[1]), "+v"(fa[2]), "+v"(fa[3]), "+v"(fb[0]), "+v"(fb[1])::"memory");
+        else if constexpr (TM == 3)
+            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(fa[0]), "+v"(fa[1]), "+v"(fa[2]), "+v"(fb[0]), "+v"(fb[1])::"memory");
         else asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(fa[0]), "+v"(fa[1]), "+v"(fb[0]), "+v"(fb[1])::"memory");
     };
     // the load issued at MFMA Q of slice SL of step kt: A's in slice 0, B's
@@ -244,74 +248,115 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
     ring_wait<0>();  // no load may still target LDS when the workgroup ends
 
     // In a 32 x 32 block lane l holds column l % 32 and rows 8 (e / 4) + 4 (l
-    // / 32) + e % 4.
-    if constexpr (STORE == GATED_PARTS) {
-        const long long plane = (long long)g.M * g.n_out;
-        float *to = g.parts + (long long)blockIdx.y * (SUM ? 1 : 2) * plane;
+    // / 32) + e % 4.  Each wave turns its blocks through its own part of LDS
+    // (the ring is done with it), after which a lane holds 8 columns of a
+    // row and stores 16 bytes.  A row of 40 floats keeps both halves of a
+    // wave's writes, and a quarter's reads, on different banks.
+    ring_barrier();
+    constexpr int ROW = 40;
+    static_assert(NW * 32 * ROW * 4 <= (int)sizeof(lds_a) && NW * 32 * ROW * 4 <= (int)sizeof(lds_b), "turned blocks fit");
+    typedef float lds_float __attribute__((may_alias));
+    typedef float lds_float4 __attribute__((ext_vector_type(4), may_alias));
+    lds_float *box[2] = {(lds_float *)lds_a + wave * 32 * ROW, (lds_float *)lds_b + wave * 32 * ROW};
+    auto turn = [&](const floatx16 &v, lds_float *to) {
 #pragma unroll
-        for (int i = 0; i < TM; i++)
+        for (int e = 0; e < 16; e++) to[(8 * (e / 4) + 4 * (lane >> 5) + e % 4) * ROW + (lane & 31)] = v[e];
+    };
+    auto take = [&](const lds_float *from, int h, float (&v)[8]) {
+        const lds_float4 *p = (const lds_float4 *)(from + (16 * h + lane / 4) * ROW + lane % 4 * 8);
+        const lds_float4 a = p[0], b = p[1];
 #pragma unroll
-            for (int j = 0; j < TN; j++) {
-                const int n = n0 + (SUM ? wn * 64 + j * 32 : wn * 32) + (lane & 31);
-                float *p = to + (SUM ? 0 : j * plane) + n;
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int m = m0 + wm * WTM + i * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-                    if (m < g.M && n < g.n_out) p[(long long)m * g.n_out] = acc[i][j][e];
-                }
-            }
-        return;
-    }
-    // Lane pairs (l, l ^ 1) swap halves, so that each lane stores two
-    // adjacent columns of two rows as 4-byte words: the even lane rows r and
-    // r + 1, the odd lane r + 2 and r + 3.
-    const bool odd = lane & 1;
-    const int col_l = (lane & 31) & ~1, row_l = (lane >> 5) * 4 + (odd ? 2 : 0);
-    typedef uint32_t word __attribute__((aligned(2)));
-    auto store4 = [&](void *c, int m, int n, float v0, float v1, float v2, float v3) {
-        const uint32_t p01 = pack_low<DT>(v0, v1), p23 = pack_low<DT>(v2, v3);
-        const uint32_t send = odd ? p01 : p23;
-        const uint32_t recv = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)send, 0xB1, 0xF, 0xF, false);
-        const uint32_t u = odd ? recv : p01, v = odd ? p23 : recv;
-        const uint32_t w[2] = {(u & 0xffffu) | (v << 16), (u >> 16) | (v & 0xffff0000u)};
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-            if (m + r >= g.M || n >= g.n_out) continue;
-            S *p = (S *)c + (long long)(m + r) * g.n_out + n;
-            if (n + 1 < g.n_out) *(word *)p = w[r];
-            else *p = (S)w[r];
+        for (int k = 0; k < 4; k++) {
+            v[k] = a[k];
+            v[4 + k] = b[k];
         }
     };
+    typedef uint32_t word4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t word2 __attribute__((ext_vector_type(2), aligned(1)));
+    typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+    auto store16 = [&](void *c, long long at, int live, const float (&v)[8]) {
+        word4 w;
 #pragma unroll
-    for (int i = 0; i < TM; i++)
+        for (int k = 0; k < 4; k++) w[k] = pack_low<DT>(v[2 * k], v[2 * k + 1]);
+        if (live >= 8) *(word4 *)((S *)c + at) = w;
+        else
 #pragma unroll
-        for (int e4 = 0; e4 < 4; e4++) {
-            const int m = m0 + wm * WTM + i * 32 + e4 * 8 + row_l;
-            if constexpr (SUM) {
+            for (int k = 0; k < 8; k++)
+                if (k < live) ((S *)c)[at + k] = (S)(w[k / 2] >> (k & 1 ? 16 : 0));
+    };
+    auto store_kept = [&](int product, long long plane, long long at, int live, const float (&v)[8]) {
+        S *high = (S *)((char *)g.c1 + kept_plane(plane, product, false)) + at;
+        uint8_t *low = (uint8_t *)g.c1 + kept_plane(plane, product, true) + at;
+        if (live >= 8) {
+            word4 w;
+            word2 l = {0, 0};
 #pragma unroll
-                for (int j = 0; j < TN; j++) {
-                    const floatx16 &v = acc[i][j];
-                    store4(g.c0, m, n0 + wn * 64 + j * 32 + col_l, v[4 * e4], v[4 * e4 + 1], v[4 * e4 + 2], v[4 * e4 + 3]);
+            for (int k = 0; k < 4; k++) w[k] = kept_high(v[2 * k]) | kept_high(v[2 * k + 1]) << 16;
+#pragma unroll
+            for (int k = 0; k < 8; k++) l[k / 4] |= kept_low(v[k]) << (8 * (k % 4));
+            *(word4 *)high = w;
+            *(word2 *)low = l;
+        } else
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k < live) {
+                    high[k] = (S)kept_high(v[k]);
+                    low[k] = (uint8_t)kept_low(v[k]);
                 }
-            } else {
-                const int n = n0 + wn * 32 + col_l;
-                float p[4], q[4];
+    };
+    const long long plane = (long long)g.M * g.n_out;
+    float *parts = STORE == GATED_PARTS ? g.parts + (long long)blockIdx.y * (SUM ? 1 : 2) * plane : nullptr;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    p[e] = acc[i][0][4 * e4 + e];
-                    q[e] = acc[i][1][4 * e4 + e];
-                }
-                if constexpr (STORE != GATED_PRODUCT) {
-                    store4(g.c1, m, n, p[0], p[1], p[2], p[3]);
-                    store4(g.c2, m, n, q[0], q[1], q[2], q[3]);
-                }
-                if constexpr (STORE != GATED_BOTH) {
+    for (int i = 0; i < TM; i++) {
+        // (a wave's LDS accesses stay in order)
+        turn(acc[i][0], box[0]);
+        turn(acc[i][1], box[1]);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                    for (int e = 0; e < 4; e++) p[e] = gated_act<true>(g.act, p[e]) * q[e];
-                    store4(g.c0, m, n, p[0], p[1], p[2], p[3]);
+        for (int h = 0; h < 2; h++) {
+            float p[8], q[8];
+            take(box[0], h, p);
+            take(box[1], h, q);
+            const int m = m0 + wm * WTM + i * 32 + h * 16 + lane / 4;
+            if (m >= g.M) continue;
+#pragma unroll
+            for (int j = 0; j < (SUM ? 2 : 1); j++) {
+                const int n = n0 + (SUM ? wn * 64 + j * 32 : wn * 32) + lane % 4 * 8;
+                const int live = g.n_out - n;
+                if (live <= 0) continue;
+                const long long at = (long long)m * g.n_out + n;
+                if constexpr (STORE == GATED_PARTS) {
+#pragma unroll
+                    for (int part = 0; part < (SUM ? 1 : 2); part++) {
+                        const float(&v)[8] = SUM ? (j ? q : p) : (part ? q : p);
+                        float *to = parts + part * plane + at;
+                        if (live >= 8) {
+                            *(float4u *)to = float4u{v[0], v[1], v[2], v[3]};
+                            *(float4u *)(to + 4) = float4u{v[4], v[5], v[6], v[7]};
+                        } else
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                                if (k < live) to[k] = v[k];
+                    }
+                } else if constexpr (SUM) {
+                    store16(g.c0, at, live, j ? q : p);
+                } else if constexpr (STORE == GATED_BOTH) {
+                    store16(g.c1, at, live, p);
+                    store16(g.c2, at, live, q);
+                } else {
+                    if constexpr (STORE == GATED_KEPT) {
+                        store_kept(0, plane, at, live, p);
+                        store_kept(1, plane, at, live, q);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; k++) p[k] = gated_act<true>(g.act, p[k]) * q[k];
+                    store16(g.c0, at, live, p);
                 }
             }
         }
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 // Results from the parts of a split contraction, added in order; a thread
@@ -330,23 +375,33 @@ __global__ __launch_bounds__(256) void k_pair_join(PairArgs g)
         if constexpr (SUM) {
             store_c<DT>(g.c0, (size_t)i, p);
         } else {
-            if constexpr (STORE != GATED_PRODUCT) {
+            if constexpr (STORE == GATED_BOTH) {
                 store_c<DT>(g.c1, (size_t)i, p);
                 store_c<DT>(g.c2, (size_t)i, q);
+            } else {
+                if constexpr (STORE == GATED_KEPT) gated_keep<DT>(g.c1, plane, i, p, q);
+                store_c<DT>(g.c0, (size_t)i, gated_act<DT != PT_FLOAT32>(g.act, p) * q);
             }
-            if constexpr (STORE != GATED_BOTH) store_c<DT>(g.c0, (size_t)i, gated_act<DT != PT_FLOAT32>(g.act, p) * q);
         }
     }
 }
 
-// Tiles of 256 rows where they fill the CUs as well as tiles of 128 do (which
-// take 0.55 of their time); fewer tiles than CUs split the contraction, each
-// share at least 4 superstages (256 k).
+// Tiles of 256, 192 or 128 rows, whichever need the least: rounds of 256
+// workgroups at the time that a tile takes (1733 x 1000 x 2731 in float16:
+// T256 us with 256 rows, T192 with 192).  Fewer tiles than CUs split the
+// contraction, each share at least 4 superstages (256 k).
 void pair_plan(PairArgs &g, bool columns, int &tm)
 {
     auto tiles = [&](int rows) { return (long long)((g.M + rows - 1) / rows) * ((g.n_out + (columns ? 127 : 255)) / (columns ? 128 : 256)); };
-    const double wide = (double)((tiles(256) + 255) / 256), narrow = 0.55 * (double)((tiles(128) + 255) / 256);
-    tm = g.M > 128 && wide <= narrow ? 4 : 2;
+    const double time[3] = {0.55, 0.78, 1.0};
+    double best = 0;
+    for (int t = 4; t >= 2; t--) {
+        const double cost = time[t - 2] * (double)((tiles(64 * t) + 255) / 256);
+        if (t == 4 || cost < best) {
+            best = cost;
+            tm = t;
+        }
+    }
     g.tiles_m = (g.M + 64 * tm - 1) / (64 * tm);
     g.tiles_n = (g.n_out + (columns ? 127 : 255)) / (columns ? 128 : 256);
     const int all = (columns ? 1 : 2) * ((g.K + 63) / 64);
@@ -381,11 +436,13 @@ static void launch_pair_store(const PairArgs &g, int tm, hipStream_t s)
     const dim3 grid(g.tiles_m * g.tiles_n, g.split);
     if (g.split > 1) {
         if (tm == 4) k_pair<DT, 4, SUM, GATED_PARTS><<<grid, 512, 0, s>>>(g);
+        else if (tm == 3) k_pair<DT, 3, SUM, GATED_PARTS><<<grid, 512, 0, s>>>(g);
         else k_pair<DT, 2, SUM, GATED_PARTS><<<grid, 512, 0, s>>>(g);
         join_parts<DT, SUM, STORE>(g, s);
         return;
     }
     if (tm == 4) k_pair<DT, 4, SUM, STORE><<<grid, 512, 0, s>>>(g);
+    else if (tm == 3) k_pair<DT, 3, SUM, STORE><<<grid, 512, 0, s>>>(g);
     else k_pair<DT, 2, SUM, STORE><<<grid, 512, 0, s>>>(g);
 }
 

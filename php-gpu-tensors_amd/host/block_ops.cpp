@@ -321,14 +321,14 @@ bool cuda_array_gated(const TensorP &x, const TensorP &gate, const TensorP &up, 
     pt_gated_desc d;
     if (!gated_desc(x, gate, up, activation, d)) return false;
     int shape[kMaxDims];
-    const int nd = gated_shape(*x, *gate, shape), both[3] = {2, d.rows, d.outer};
+    const int nd = gated_shape(*x, *gate, shape), both[3] = {x->dtype == PT_FLOAT32 ? 8 : 6, d.rows, d.outer};
     out[1] = nullptr;
     if (fusion_active()) {
         NativeSpec sp;
         sp.kind = NAT_GATED;
         sp.activation = activation;
         std::vector<TensorP> ins = {x, gate, up};
-        TensorP box = keep ? record_buffer(both, 3, x->dtype) : nullptr;
+        TensorP box = keep ? record_buffer(both, 3, PT_UINT8) : nullptr;
         if (keep && !box) return false;
         if (box) ins.push_back(box);
         out[0] = fusion_record_native(sp, ins, shape, nd, x->dtype);
@@ -337,7 +337,7 @@ bool cuda_array_gated(const TensorP &x, const TensorP &gate, const TensorP &up, 
     }
     if (!guard(x) || !guard(gate) || !guard(up)) return false;
     out[0] = output_tensor(shape, nd, x->dtype);
-    if (out[0] && keep) out[1] = make_empty(both, 3, x->dtype);
+    if (out[0] && keep) out[1] = make_empty(both, 3, PT_UINT8);
     if (!out[0] || (keep && !out[1])) return false;
     return gated_run(x, gate, up, activation, out[0], out[1]);
 }
@@ -365,7 +365,7 @@ bool cuda_array_gated_backward(const TensorP &x, const TensorP &gate, const Tens
     if (!gated_desc(x, gate, up, activation, d)) return false;
     int shape[kMaxDims];
     const int nd = gated_shape(*x, *gate, shape);
-    if (!kept || kept->dtype != x->dtype || kept->ndims != 3 || kept->shape[0] != 2 || kept->shape[1] != d.rows ||
+    if (!kept || kept->dtype != PT_UINT8 || kept->ndims != 3 || kept->shape[0] != (x->dtype == PT_FLOAT32 ? 8 : 6) || kept->shape[1] != d.rows ||
         kept->shape[2] != d.outer) {
         set_invalid("gatedProjection gradients need the forward pass's products");
         return false;

@@ -47,9 +47,9 @@ def reference(x, gate, up, name, dtype, dh=None):
     out = {"h": (a * u, np.abs(a) * u_off + a_off * (np.abs(u) + u_off) + U * np.abs(a * u))}
     if dh is None:
         return out
-    # the gradient takes the products as they are kept, rounded to the type, and rounds dg and du to it
-    low = 0.0 if dtype == "float32" else h
-    gk, uk = g_off * (1 + low) + low * np.abs(g) + tiny, u_off * (1 + low) + low * np.abs(u) + tiny
+    # the gradient takes the products as they are kept, cut to 15 bits behind the first, and rounds dg and du to the type
+    low, cut = (0.0, 0.0) if dtype == "float32" else (h, 2.0 ** -15)
+    gk, uk = g_off * (1 + cut) + cut * np.abs(g), u_off * (1 + cut) + cut * np.abs(u)
     s_off = curve * gk + 32 * U * (1 + np.abs(g)) * (1 + np.abs(slope))
     ak = steep * gk + 16 * U * (np.abs(a) + np.abs(a) * np.abs(g) + steep * np.abs(g))
     if name == "relu":  # a product whose sign is not certain may fall on either side
