@@ -49,6 +49,22 @@ __device__ __forceinline__ float gated_act(int act, float g)
     default: return gated_sigmoid<FAST>(g);
     }
 }
+// p = act(p) q for N of them: one branch, and little code for the
+// instruction cache, which a short kernel finds empty
+template <bool FAST, int N>
+__device__ __forceinline__ void gated_products(int act, float (&p)[N], const float (&q)[N])
+{
+    auto all = [&](auto ACT) {
+#pragma unroll
+        for (int k = 0; k < N; k++) p[k] = gated_act<FAST>(decltype(ACT)::value, p[k]) * q[k];
+    };
+    switch (act) {
+    case PT_GATE_SILU: return all(IC<PT_GATE_SILU>{});
+    case PT_GATE_GELU: return all(IC<PT_GATE_GELU>{});
+    case PT_GATE_RELU: return all(IC<PT_GATE_RELU>{});
+    default: return all(IC<PT_GATE_SIGMOID>{});
+    }
+}
 template <bool FAST>
 __device__ __forceinline__ void gated_slope(int act, float g, float &value, float &slope)
 {

@@ -2,9 +2,9 @@
 //   dg = dh u act'(g),  du = dh act(g)   (g, u: the two products)
 //   dx = dg gate^T + du up^T,  dgate = x^T dg,  dup = x^T du.
 // Forms, by the rows and the type:
-//   16 bits, more than 32 rows: products over a pair of matrices in one
+//   16 bits, more than 64 rows: products over a pair of matrices in one
 //     kernel (pt_gated_ring.hip), bound by the matrix cores.
-//   32 rows or fewer: k_gated_few, bound by the weights' bytes.
+//   64 rows or fewer: k_gated_few, bound by the weights' bytes.
 //   float32, more rows: the framework's fp32 products (94 % of the matrix
 //     cores' rate) and a pass over both results; fusing would save that
 //     pass, 2 % of the time at 4096 inner elements.
@@ -245,54 +245,6 @@ __device__ __forceinline__ void gd_load_kept(const void *kept, long long n, int 
     for (int k = 0; k < 8; k++) v[k] = k < live ? kept_value(high[k], low[k]) : 0.0f;
 }
 
-// dg and du from the upstream gradient and both products, into rows `pitch`
-// elements apart from d and d + second on, zeros in columns `cols` to
-// `padded` - 1.  A thread takes 8 columns.
-template <int DT, int GDT>
-__global__ __launch_bounds__(256) void k_gated_slope(const void *kept, const void *grad, void *d, long long second, int rows,
-                                                     int cols, int padded, int pitch, int act)
-{
-    using S = typename GE<DT>::S;
-    const int packs = (cols + 7) / 8;
-    const long long total = (long long)rows * packs, plane = (long long)rows * cols;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long row = i / packs;
-        const int c = (int)(i - row * packs) * 8, live = min(8, cols - c);
-        const long long from = row * cols + c;
-        float g[8], u[8], dh[8];
-        if constexpr (DT == PT_FLOAT32) {
-            gd_load<DT, 8>((const S *)kept + from, live, g);
-            gd_load<DT, 8>((const S *)kept + plane + from, live, u);
-        } else {
-            gd_load_kept(kept, plane, 0, from, live, g);
-            gd_load_kept(kept, plane, 1, from, live, u);
-        }
-        gd_load<GDT, 8>((const typename GE<GDT>::S *)grad + from, live, dh);
-        S dg[8], du[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            float value, slope;
-            gated_slope<DT != PT_FLOAT32>(act, g[k], value, slope);
-            dg[k] = DType<DT>::from_c(k < live ? dh[k] * u[k] * slope : 0.0f);
-            du[k] = DType<DT>::from_c(k < live ? dh[k] * value : 0.0f);
-        }
-        S *to = (S *)d + row * pitch + c;
-        const int room = min(8, padded - c);
-        if (room == 8) {
-#pragma unroll
-            for (int q = 0; q < 8 / GE<DT>::PK; q++) {
-                *(gd_u32x4 *)(to + q * GE<DT>::PK) = *(gd_u32x4 *)(dg + q * GE<DT>::PK);
-                *(gd_u32x4 *)(to + second + q * GE<DT>::PK) = *(gd_u32x4 *)(du + q * GE<DT>::PK);
-            }
-        } else {
-            for (int k = 0; k < room; k++) {
-                to[k] = dg[k];
-                to[second + k] = du[k];
-            }
-        }
-    }
-}
-
 // Two fp32 matrices side by side, or (BACK) apart again.
 template <bool BACK>
 __global__ __launch_bounds__(256) void k_gated_beside(float *a, float *b, float *both, int rows, int cols)
@@ -331,11 +283,11 @@ __global__ __launch_bounds__(256) void k_gated_pack(const uint16_t *from0, const
 }
 
 // The transpose of rows x cols 16-bit elements, in rows of `pitch` (a
-// multiple of 8, zeros past `rows`): 64 x 64 tiles through LDS.
-__global__ __launch_bounds__(256) void k_gated_transpose(const uint16_t *from, uint16_t *to, int rows, int cols, int pitch)
+// multiple of 8, zeros past `rows`): a 64 x 64 tile through LDS.
+__device__ __forceinline__ void gated_transpose(const uint16_t *from, uint16_t *to, int rows, int cols, int pitch, int r0, int c0,
+                                                uint16_t (&tile)[64][66])
 {
-    __shared__ uint16_t tile[64][66];
-    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, a = threadIdx.x & 7, b = threadIdx.x >> 3;
+    const int a = threadIdx.x & 7, b = threadIdx.x >> 3;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int r = r0 + b + 32 * h, c = c0 + a * 8;
@@ -356,6 +308,70 @@ __global__ __launch_bounds__(256) void k_gated_transpose(const uint16_t *from, u
 #pragma unroll
         for (int k = 0; k < 8; k++) u.s[k] = tile[b + 32 * h][a * 8 + k];
         *(gd_u32x4 *)(to + (long long)c * pitch + r) = u.raw;
+    }
+}
+
+// dg and du from the upstream gradient and both products, into rows `pitch`
+// elements apart from d and d + second on, zeros in columns `cols` to
+// `padded` - 1.  A thread takes 8 columns.  Blocks from `slopes` on transpose
+// x beside it, one 64 x 64 tile each, in one launch less.
+struct SlopeArgs {
+    const void *kept, *grad;
+    void *d;
+    long long second;
+    int rows, cols, padded, pitch, act;
+    unsigned slopes;         // blocks
+    const uint16_t *x;       // [rows][inner]
+    uint16_t *xt;            // [inner][across]
+    int inner, across;
+};
+template <int DT, int GDT>
+__global__ __launch_bounds__(256) void k_gated_slope(SlopeArgs a)
+{
+    using S = typename GE<DT>::S;
+    __shared__ uint16_t tile[64][66];
+    if (blockIdx.x >= a.slopes) {
+        const int t = (int)(blockIdx.x - a.slopes), wide = (a.inner + 63) / 64;
+        gated_transpose(a.x, a.xt, a.rows, a.inner, a.across, t / wide * 64, t % wide * 64, tile);
+        return;
+    }
+    const int packs = (a.cols + 7) / 8;
+    const long long total = (long long)a.rows * packs, plane = (long long)a.rows * a.cols;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)a.slopes * 256) {
+        const long long row = i / packs;
+        const int c = (int)(i - row * packs) * 8, live = min(8, a.cols - c);
+        const long long from = row * a.cols + c;
+        float g[8], u[8], dh[8];
+        if constexpr (DT == PT_FLOAT32) {
+            gd_load<DT, 8>((const S *)a.kept + from, live, g);
+            gd_load<DT, 8>((const S *)a.kept + plane + from, live, u);
+        } else {
+            gd_load_kept(a.kept, plane, 0, from, live, g);
+            gd_load_kept(a.kept, plane, 1, from, live, u);
+        }
+        gd_load<GDT, 8>((const typename GE<GDT>::S *)a.grad + from, live, dh);
+        S dg[8], du[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            float value, slope;
+            gated_slope<DT != PT_FLOAT32>(a.act, g[k], value, slope);
+            dg[k] = DType<DT>::from_c(k < live ? dh[k] * u[k] * slope : 0.0f);
+            du[k] = DType<DT>::from_c(k < live ? dh[k] * value : 0.0f);
+        }
+        S *to = (S *)a.d + row * a.pitch + c;
+        const int room = min(8, a.padded - c);
+        if (room == 8) {
+#pragma unroll
+            for (int q = 0; q < 8 / GE<DT>::PK; q++) {
+                *(gd_u32x4 *)(to + q * GE<DT>::PK) = *(gd_u32x4 *)(dg + q * GE<DT>::PK);
+                *(gd_u32x4 *)(to + a.second + q * GE<DT>::PK) = *(gd_u32x4 *)(du + q * GE<DT>::PK);
+            }
+        } else {
+            for (int k = 0; k < room; k++) {
+                to[k] = dg[k];
+                to[a.second + k] = du[k];
+            }
+        }
     }
 }
 
@@ -435,20 +451,24 @@ template <int DT>
 static pt_status launch_few(PairArgs &g, GatedScratch &scratch, hipStream_t s)
 {
     constexpr int NC = GE<DT>::PK;
+    constexpr bool LOW = DT != PT_FLOAT32;
+    // (16 bits, more than 32 rows: the sums of a wide strip leave no registers)
     const int wide = (g.n_out + 16 * NC - 1) / (16 * NC), narrow = (g.n_out + 8 * NC - 1) / (8 * NC), steps = (g.K + 31) / 32;
+    const bool must = LOW && g.M > 32;
     const double bytes = 2.0 * g.K * g.n_out * sizeof(typename GE<DT>::S);
-    g.split = std::max(1, std::min({256 / wide, steps / kFewWaves, 16}));
-    const bool thin = g.split > 1 && bytes / (std::min(narrow, 160) * 33e9) < bytes / 5.3e12 + 4.5e-6;
-    if (thin) g.split = 1;
+    g.split = std::max(1, std::min({256 / (must ? narrow : wide), steps / kFewWaves, 16}));
+    const bool alone = g.split > 1 && bytes / (std::min(narrow, 160) * 33e9) < bytes / 5.3e12 + 4.5e-6, thin = must || alone;
+    if (alone) g.split = 1;
     if (g.split > 1) PT_TRY(scratch.take((void **)&g.parts, (size_t)g.split * 2 * g.M * g.n_out * sizeof(float)));
     const dim3 grid(thin ? narrow : wide, g.split);
-    if (thin) {
-        if (g.M <= 16) k_gated_few<DT, 1, NC / 2><<<grid, 64 * kFewWaves, 0, s>>>(g);
-        else k_gated_few<DT, 2, NC / 2><<<grid, 64 * kFewWaves, 0, s>>>(g);
-    } else {
-        if (g.M <= 16) k_gated_few<DT, 1, NC><<<grid, 64 * kFewWaves, 0, s>>>(g);
-        else k_gated_few<DT, 2, NC><<<grid, 64 * kFewWaves, 0, s>>>(g);
-    }
+    auto go = [&](auto NCC) {
+        constexpr int N = decltype(NCC)::value;
+        if (g.M <= 16) k_gated_few<DT, 1, N><<<grid, 64 * kFewWaves, 0, s>>>(g);
+        else if ((LOW && N == NC) || g.M <= 32) k_gated_few<DT, 2, N><<<grid, 64 * kFewWaves, 0, s>>>(g);
+        else if constexpr (!LOW || N < NC) k_gated_few<DT, 4, N><<<grid, 64 * kFewWaves, 0, s>>>(g);
+    };
+    if (thin) go(IC<NC / 2>{});
+    else go(IC<NC>{});
     if (g.split > 1) launch_pair_join(g, DT, g.c1 ? GATED_KEPT : GATED_PRODUCT, s);
     return PT_OK;
 }
@@ -473,7 +493,7 @@ static pt_status gated_run(const pt_gated_desc *d, const void *x, const void *ga
     g.ldb = g.N = F;
     g.K = g.kb = K;
     const int pack = (int)(16 / size);
-    if (M <= 32 && F >= pack) {
+    if (M <= 64 && F >= pack) {
         if (d->dtype == PT_FLOAT32) return launch_few<PT_FLOAT32>(g, scratch, s);
         return d->dtype == PT_FLOAT16 ? launch_few<PT_FLOAT16>(g, scratch, s) : launch_few<PT_BFLOAT16>(g, scratch, s);
     }
@@ -505,8 +525,8 @@ static pt_status gated_backward_f32(const pt_gated_desc *d, const float *x, cons
     // dg and du side by side: one product takes both contractions of dx
     float *both = nullptr, *weights = nullptr;
     PT_TRY(scratch.take((void **)&both, (size_t)M * 2 * F * sizeof(float)));
-    k_gated_slope<PT_FLOAT32, PT_FLOAT32><<<grid_for((long long)M * ((F + 7) / 8)), 256, 0, s>>>(kept, grad, both, F, M, F, F, 2 * F,
-                                                                                              d->activation);
+    SlopeArgs a = {kept, grad, both, F, M, F, F, 2 * F, d->activation, grid_for((long long)M * ((F + 7) / 8)), nullptr, nullptr, 0, 0};
+    k_gated_slope<PT_FLOAT32, PT_FLOAT32><<<a.slopes, 256, 0, s>>>(a);
     if (dx) {
         PT_TRY(scratch.take((void **)&weights, (size_t)K * 2 * F * sizeof(float)));
         k_gated_beside<false><<<grid_for((long long)K * F), 256, 0, s>>>((float *)gate, (float *)up, weights, K, F);
@@ -539,14 +559,22 @@ static pt_status gated_backward_run(const pt_gated_desc *d, const void *x, const
     uint16_t *dg = nullptr;
     const long long second = (long long)M * pitch;
     PT_TRY(scratch.take((void **)&dg, (size_t)second * 2 * 2));
-    const unsigned blocks = grid_for((long long)M * (pitch / 8));
+    SlopeArgs a = {kept, grad, dg, second, M, F, pitch, pitch, d->activation, grid_for((long long)M * (pitch / 8)), nullptr, nullptr, 0, 0};
+    unsigned blocks = a.slopes;
+    if (dgate) {
+        a.x = (const uint16_t *)x;
+        a.inner = K;
+        a.across = round8(M);
+        PT_TRY(scratch.take((void **)&a.xt, (size_t)K * a.across * 2));
+        blocks += (unsigned)(((long long)K + 63) / 64 * ((a.across + 63) / 64));
+    }
     const bool same = grad_dtype == d->dtype;
     if (d->dtype == PT_BFLOAT16) {
-        if (same) k_gated_slope<PT_BFLOAT16, PT_BFLOAT16><<<blocks, 256, 0, s>>>(kept, grad, dg, second, M, F, pitch, pitch, d->activation);
-        else k_gated_slope<PT_BFLOAT16, PT_FLOAT32><<<blocks, 256, 0, s>>>(kept, grad, dg, second, M, F, pitch, pitch, d->activation);
+        if (same) k_gated_slope<PT_BFLOAT16, PT_BFLOAT16><<<blocks, 256, 0, s>>>(a);
+        else k_gated_slope<PT_BFLOAT16, PT_FLOAT32><<<blocks, 256, 0, s>>>(a);
     } else {
-        if (same) k_gated_slope<PT_FLOAT16, PT_FLOAT16><<<blocks, 256, 0, s>>>(kept, grad, dg, second, M, F, pitch, pitch, d->activation);
-        else k_gated_slope<PT_FLOAT16, PT_FLOAT32><<<blocks, 256, 0, s>>>(kept, grad, dg, second, M, F, pitch, pitch, d->activation);
+        if (same) k_gated_slope<PT_FLOAT16, PT_FLOAT16><<<blocks, 256, 0, s>>>(a);
+        else k_gated_slope<PT_FLOAT16, PT_FLOAT32><<<blocks, 256, 0, s>>>(a);
     }
     int tm;
     if (dx) {
@@ -565,12 +593,8 @@ static pt_status gated_backward_run(const pt_gated_desc *d, const void *x, const
     }
     if (dgate) {
         PairArgs g = {};
-        const int across = round8(M);
-        uint16_t *xt = nullptr;
-        PT_TRY(scratch.take((void **)&xt, (size_t)K * across * 2));
-        k_gated_transpose<<<dim3((K + 63) / 64, (across + 63) / 64), 256, 0, s>>>((const uint16_t *)x, xt, M, K, across);
-        g.a0 = xt;
-        g.lda = g.K = across;
+        g.a0 = a.xt;
+        g.lda = g.K = a.across;
         g.kb = M;
         g.b0 = dg;
         g.b1 = dg + second;

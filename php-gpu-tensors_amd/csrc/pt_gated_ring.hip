@@ -313,7 +313,7 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
         turn(acc[i][1], box[1]);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < 2; h++) {
             float p[8], q[8];
             take(box[0], h, p);
@@ -349,8 +349,7 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
                         store_kept(0, plane, at, live, p);
                         store_kept(1, plane, at, live, q);
                     }
-#pragma unroll
-                    for (int k = 0; k < 8; k++) p[k] = gated_act<true>(g.act, p[k]) * q[k];
+                    gated_products<true>(g.act, p, q);
                     store16(g.c0, at, live, p);
                 }
             }
@@ -360,61 +359,83 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
 }
 
 // Results from the parts of a split contraction, added in order; a thread
-// takes one element.
+// takes 4 elements and has 4 parts of them on their way.
 template <int DT, bool SUM, int STORE>
 __global__ __launch_bounds__(256) void k_pair_join(PairArgs g)
 {
-    const long long plane = (long long)g.M * g.n_out;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < plane; i += (long long)gridDim.x * 256) {
-        float p = 0.0f, q = 0.0f;
-        for (int k = 0; k < g.split; k++) {
-            const float *from = g.parts + (long long)k * (SUM ? 1 : 2) * plane + i;
-            p += from[0];
-            if (!SUM) q += from[plane];
-        }
-        if constexpr (SUM) {
-            store_c<DT>(g.c0, (size_t)i, p);
+    typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+    const long long plane = (long long)g.M * g.n_out, step = (SUM ? 1 : 2) * plane;
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < plane; i += (long long)gridDim.x * 1024) {
+        float4u p = {0.0f, 0.0f, 0.0f, 0.0f}, q = p;
+        const int live = (int)min(4ll, plane - i);
+        if (live == 4) {
+#pragma unroll 4
+            for (int k = 0; k < g.split; k++) {
+                const float *from = g.parts + k * step + i;
+                p += *(const float4u *)from;
+                if (!SUM) q += *(const float4u *)(from + plane);
+            }
         } else {
-            if constexpr (STORE == GATED_BOTH) {
-                store_c<DT>(g.c1, (size_t)i, p);
-                store_c<DT>(g.c2, (size_t)i, q);
+            for (int k = 0; k < g.split; k++)
+                for (int e = 0; e < live; e++) {
+                    const float *from = g.parts + k * step + i + e;
+                    p[e] += from[0];
+                    if (!SUM) q[e] += from[plane];
+                }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (e >= live) continue;
+            if constexpr (SUM) {
+                store_c<DT>(g.c0, (size_t)(i + e), p[e]);
+            } else if constexpr (STORE == GATED_BOTH) {
+                store_c<DT>(g.c1, (size_t)(i + e), p[e]);
+                store_c<DT>(g.c2, (size_t)(i + e), q[e]);
             } else {
-                if constexpr (STORE == GATED_KEPT) gated_keep<DT>(g.c1, plane, i, p, q);
-                store_c<DT>(g.c0, (size_t)i, gated_act<DT != PT_FLOAT32>(g.act, p) * q);
+                if constexpr (STORE == GATED_KEPT) gated_keep<DT>(g.c1, plane, i + e, p[e], q[e]);
+                store_c<DT>(g.c0, (size_t)(i + e), gated_act<DT != PT_FLOAT32>(g.act, p[e]) * q[e]);
             }
         }
     }
 }
 
-// Tiles of 256, 192 or 128 rows, whichever need the least: rounds of 256
-// workgroups at the time that a tile takes (1733 x 1000 x 2731 in float16:
-// T256 us with 256 rows, T192 with 192).  Fewer tiles than CUs split the
-// contraction, each share at least 4 superstages (256 k).
+// The tile's rows and the split of the contraction that are estimated to take
+// the least time, from what was measured on this GPU: a step of 32 k takes a
+// workgroup of 256, 192 and 128 rows 0.65, 0.58 and 0.5 us where few run, as
+// long as its loads take from HBM, and 0.9, 0.7 and 0.5 us where all CUs run
+// (0.6 at least where one row of tiles shares none of B); HBM gives 5 TB/s; a split writes and reads fp32 parts and joins them in a
+// second kernel, 4 us.
 void pair_plan(PairArgs &g, bool columns, int &tm)
 {
-    auto tiles = [&](int rows) { return (long long)((g.M + rows - 1) / rows) * ((g.n_out + (columns ? 127 : 255)) / (columns ? 128 : 256)); };
-    const double time[3] = {0.55, 0.78, 1.0};
+    const int bn = columns ? 128 : 256, all = (columns ? 1 : 2) * ((g.K + 63) / 64);
+    const long long across = (g.n_out + bn - 1) / bn;
+    const double plane = (columns ? 2.0 : 1.0) * g.M * g.n_out;
+    const double hbm = (2.0 * g.K * g.n_out + (columns ? 1.0 : 2.0) * g.M * g.K) * 2 / 5e6;  // us
     double best = 0;
-    for (int t = 4; t >= 2; t--) {
-        const double cost = time[t - 2] * (double)((tiles(64 * t) + 255) / 256);
-        if (t == 4 || cost < best) {
-            best = cost;
+    g.split = 0;
+    for (int t = 4; t >= 2; t--)
+        for (int parts = 1; parts <= 32; parts *= 2) {
+            const int stages = (all + parts - 1) / parts, split = (all + stages - 1) / stages;
+            if (split > 1 && stages < 2) break;
+            const long long down = (g.M + 64 * t - 1) / (64 * t), groups = down * across * split;
+            const double full = std::min(1.0, (double)groups / 256);
+            const double step = t == 4 ? 0.65 + 0.25 * full : t == 3 ? 0.58 + 0.12 * full : down == 1 ? 0.6 : 0.5;
+            double time = std::max((double)((groups + 255) / 256) * 2 * stages * step, hbm);
+            if (split > 1) time += 4.0 + split * plane * 8 / 5e6;
+            if (g.split && time >= best) continue;
+            best = time;
             tm = t;
+            g.split = split;
+            g.stages = stages;
+            g.tiles_m = (int)down;
         }
-    }
-    g.tiles_m = (g.M + 64 * tm - 1) / (64 * tm);
-    g.tiles_n = (g.n_out + (columns ? 127 : 255)) / (columns ? 128 : 256);
-    const int all = (columns ? 1 : 2) * ((g.K + 63) / 64);
-    const long long t = (long long)g.tiles_m * g.tiles_n;
-    g.split = (int)std::max<long long>(1, std::min<long long>({256 / t, (long long)all / 4, 16}));
-    g.stages = (all + g.split - 1) / g.split;
-    g.split = (all + g.stages - 1) / g.stages;
+    g.tiles_n = (int)across;
 }
 
 template <int DT, bool SUM, int STORE>
 static void join_parts(const PairArgs &g, hipStream_t s)
 {
-    const unsigned blocks = (unsigned)std::min<long long>(((long long)g.M * g.n_out + 255) / 256, 1 << 20);
+    const unsigned blocks = (unsigned)std::min<long long>(((long long)g.M * g.n_out + 1023) / 1024, 1 << 20);
     k_pair_join<DT, SUM, STORE><<<blocks, 256, 0, s>>>(g);
 }
 
