@@ -4,10 +4,12 @@
 // Forms, by the rows and the type:
 //   16 bits, more than 64 rows: products over a pair of matrices in one
 //     kernel (pt_gated_ring.hip), bound by the matrix cores.
-//   64 rows or fewer: k_gated_few, bound by the weights' bytes.
+//   64 rows or fewer (float32: 32, whose matrix instructions are slower):
+//     k_gated_few, bound by the weights' bytes.
 //   float32, more rows: the framework's fp32 products (94 % of the matrix
-//     cores' rate) and a pass over both results; fusing would save that
-//     pass, 2 % of the time at 4096 inner elements.
+//     cores' rate), one for both weights side by side where that is faster,
+//     and a pass over both results; fusing would save that pass, 2 % of the
+//     time at 4096 inner elements.
 #include "pt_gated.h"
 
 #include <algorithm>
@@ -29,6 +31,7 @@ namespace pt {
 // turn; the waves' sums meet in LDS, where each wave adds an eighth of the
 // columns in order, and the blocks' in a second kernel.
 constexpr int kFewWaves = 8;
+constexpr int kFewRows16 = 64, kFewRows32 = 32;  // the most rows
 typedef unsigned gd_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
 
 template <int DT, int MT, int NC>
@@ -210,21 +213,27 @@ __device__ __forceinline__ void gd_load(const typename GE<DT>::S *p, int live, f
     for (int k = 0; k < V; k++) v[k] = k < live ? DType<DT>::to_c(p[k]) : 0.0f;
 }
 
-// h of fp32 products that lie behind each other; a thread takes 4 elements.
-__global__ __launch_bounds__(256) void k_gated_product(const float *p, float *h, long long n, int act)
+// h of fp32 products in rows `pitch` elements apart, the second `second`
+// behind the first; a thread takes 4 columns.
+__global__ __launch_bounds__(256) void k_gated_product(const float *p, float *h, int rows, int cols, int pitch, long long second,
+                                                       int act)
 {
-    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
-        const int live = (int)min(4ll, n - i);
+    const int packs = (cols + 3) / 4;
+    const long long total = (long long)rows * packs;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long row = i / packs;
+        const int c = (int)(i - row * packs) * 4, live = min(4, cols - c);
         float g[4], u[4];
-        gd_load<PT_FLOAT32, 4>(p + i, live, g);
-        gd_load<PT_FLOAT32, 4>(p + n + i, live, u);
+        gd_load<PT_FLOAT32, 4>(p + row * pitch + c, live, g);
+        gd_load<PT_FLOAT32, 4>(p + row * pitch + second + c, live, u);
+        gated_products<false>(act, g, u);
+        float *to = h + row * cols + c;
         typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
-        float4u v;
-#pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = gated_act<false>(act, g[k]) * u[k];
-        if (live == 4) *(float4u *)(h + i) = v;
+        if (live == 4) *(float4u *)to = float4u{g[0], g[1], g[2], g[3]};
         else
-            for (int k = 0; k < live; k++) h[i + k] = v[k];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (k < live) to[k] = g[k];
     }
 }
 
@@ -245,20 +254,33 @@ __device__ __forceinline__ void gd_load_kept(const void *kept, long long n, int 
     for (int k = 0; k < 8; k++) v[k] = k < live ? kept_value(high[k], low[k]) : 0.0f;
 }
 
-// Two fp32 matrices side by side, or (BACK) apart again.
+// Two fp32 matrices [rows][cols] side by side, each in `each` columns (zeros
+// past the end, also in rows up to `down`), or (BACK) apart again.
 template <bool BACK>
-__global__ __launch_bounds__(256) void k_gated_beside(float *a, float *b, float *both, int rows, int cols)
+__global__ __launch_bounds__(256) void k_gated_beside(float *a, float *b, float *both, int rows, int cols, int down, int each)
 {
-    const long long n = (long long)rows * cols;
+    const long long n = (long long)(BACK ? rows : down) * each;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const long long row = i / cols, at = i + row * cols;
+        const long long row = i / each, c = i - row * each, at = i + row * each, from = row * cols + c;
+        const bool live = row < rows && c < cols;
         if constexpr (BACK) {
-            a[i] = both[at];
-            b[i] = both[at + cols];
+            if (live) {
+                a[from] = both[at];
+                b[from] = both[at + each];
+            }
         } else {
-            both[at] = a[i];
-            both[at + cols] = b[i];
+            both[at] = live ? a[from] : 0.0f;
+            both[at + each] = live ? b[from] : 0.0f;
         }
+    }
+}
+
+// fp32 rows of `cols` in rows of `pitch`, zeros past the end
+__global__ __launch_bounds__(256) void k_gated_pitch(const float *from, float *to, long long rows, int cols, int pitch)
+{
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * pitch; i += (long long)gridDim.x * 256) {
+        const long long row = i / pitch, c = i - row * pitch;
+        to[i] = c < cols ? from[row * cols + c] : 0.0f;
     }
 }
 
@@ -320,6 +342,8 @@ struct SlopeArgs {
     void *d;
     long long second;
     int rows, cols, padded, pitch, act;
+    int kept_pitch;          // float32: both products' rows, and where the second one's begin
+    long long kept_second;
     unsigned slopes;         // blocks
     const uint16_t *x;       // [rows][inner]
     uint16_t *xt;            // [inner][across]
@@ -343,8 +367,9 @@ __global__ __launch_bounds__(256) void k_gated_slope(SlopeArgs a)
         const long long from = row * a.cols + c;
         float g[8], u[8], dh[8];
         if constexpr (DT == PT_FLOAT32) {
-            gd_load<DT, 8>((const S *)a.kept + from, live, g);
-            gd_load<DT, 8>((const S *)a.kept + plane + from, live, u);
+            const S *kept = (const S *)a.kept + row * a.kept_pitch + c;
+            gd_load<DT, 8>(kept, live, g);
+            gd_load<DT, 8>(kept + a.kept_second, live, u);
         } else {
             gd_load_kept(a.kept, plane, 0, from, live, g);
             gd_load_kept(a.kept, plane, 1, from, live, u);
@@ -412,6 +437,24 @@ struct GatedScratch {
         if (b) *to_b = p + each;
         return PT_OK;
     }
+    // fp32: two matrices side by side in down x 2 each elements
+    pt_status beside(const float *a, const float *b, int rows, int cols, int down, int each, float **to)
+    {
+        PT_TRY(take((void **)to, (size_t)down * 2 * each * sizeof(float)));
+        k_gated_beside<false><<<grid_for((long long)down * each), 256, 0, s>>>((float *)a, (float *)b, *to, rows, cols, down, each);
+        return PT_OK;
+    }
+    // fp32 rows of `pitch`: themselves where they are, or a copy
+    pt_status rows4(const float *a, long long rows, int cols, int pitch, const float **to)
+    {
+        *to = a;
+        if (cols == pitch) return PT_OK;
+        float *p = nullptr;
+        PT_TRY(take((void **)&p, (size_t)rows * pitch * sizeof(float)));
+        k_gated_pitch<<<grid_for(rows * pitch), 256, 0, s>>>(a, p, rows, cols, pitch);
+        *to = p;
+        return PT_OK;
+    }
 };
 
 static pt_status gated_check(const pt_gated_desc *d)
@@ -442,6 +485,26 @@ static pt_status product_f32(const float *a, size_t am, size_t ak, const float *
     return pt_matmul(a, b, c, PT_FLOAT32, sa, ta, 2, sb, tb, 2, sc, 2, stream);
 }
 
+// fp32, more rows than k_gated_few takes: both weights lie side by side for
+// one product, rather than two, where their rows fill no 16-byte packs (the
+// product then reads whole packs of the copy, and runs the fp32 ring: 2048 x
+// 1000 x 2731 214 us, 299 with two products in place), or where the tiles
+// of one fill the CUs and twice as many take fewer rounds than two products
+// do, which saves more than the copy costs (0.06 us a k against 3.2e-6 a
+// weight: 2048 x 1024 x 2816 209 us, 256 with two).
+struct GatedWide {
+    int inner, outer;  // rounded up to whole packs
+    bool beside;
+    GatedWide(int M, int K, int F) : inner((K + 3) / 4 * 4), outer((F + 3) / 4 * 4)
+    {
+        const long long tiles = (long long)((M + 127) / 128) * ((F + 127) / 128);
+        beside = inner != K || outer != F || (tiles >= 256 && 2 * ((tiles + 255) / 256) > (2 * tiles + 255) / 256 && F < 18750);
+    }
+    // the rows that both products are kept in, and where the second one's begin
+    int pitch(int F) const { return beside ? 2 * outer : F; }
+    long long second(int M, int F) const { return beside ? outer : (long long)M * F; }
+};
+
 // Wide strips, whose k-steps are split over up to a block for every CU; strips
 // of 8-byte packs, without a split, where the split's second kernel (4.5 us)
 // costs more than the CUs that they leave idle: a CU streams 33 GB/s, all of
@@ -464,8 +527,8 @@ static pt_status launch_few(PairArgs &g, GatedScratch &scratch, hipStream_t s)
     auto go = [&](auto NCC) {
         constexpr int N = decltype(NCC)::value;
         if (g.M <= 16) k_gated_few<DT, 1, N><<<grid, 64 * kFewWaves, 0, s>>>(g);
-        else if ((LOW && N == NC) || g.M <= 32) k_gated_few<DT, 2, N><<<grid, 64 * kFewWaves, 0, s>>>(g);
-        else if constexpr (!LOW || N < NC) k_gated_few<DT, 4, N><<<grid, 64 * kFewWaves, 0, s>>>(g);
+        else if (!LOW || N == NC || g.M <= 32) k_gated_few<DT, 2, N><<<grid, 64 * kFewWaves, 0, s>>>(g);
+        else if constexpr (LOW && N < NC) k_gated_few<DT, 4, N><<<grid, 64 * kFewWaves, 0, s>>>(g);
     };
     if (thin) go(IC<NC / 2>{});
     else go(IC<NC>{});
@@ -493,16 +556,26 @@ static pt_status gated_run(const pt_gated_desc *d, const void *x, const void *ga
     g.ldb = g.N = F;
     g.K = g.kb = K;
     const int pack = (int)(16 / size);
-    if (M <= 64 && F >= pack) {
+    if (M <= (d->dtype == PT_FLOAT32 ? kFewRows32 : kFewRows16) && F >= pack) {
         if (d->dtype == PT_FLOAT32) return launch_few<PT_FLOAT32>(g, scratch, s);
         return d->dtype == PT_FLOAT16 ? launch_few<PT_FLOAT16>(g, scratch, s) : launch_few<PT_BFLOAT16>(g, scratch, s);
     }
     if (d->dtype == PT_FLOAT32) {
+        const GatedWide w(M, K, F);
         float *p = (float *)kept;
-        if (!p) PT_TRY(scratch.take((void **)&p, 2 * n * sizeof(float)));
-        PT_TRY(product_f32((const float *)x, K, 1, (const float *)gate, F, 1, p, M, F, K, stream));
-        PT_TRY(product_f32((const float *)x, K, 1, (const float *)up, F, 1, p + n, M, F, K, stream));
-        k_gated_product<<<grid_for((long long)(n + 3) / 4), 256, 0, s>>>(p, (float *)h, (long long)n, d->activation);
+        if (!p) PT_TRY(scratch.take((void **)&p, (size_t)M * 2 * w.outer * sizeof(float)));
+        if (w.beside) {
+            float *weights = nullptr;
+            const float *rows = nullptr;
+            PT_TRY(scratch.beside((const float *)gate, (const float *)up, K, F, w.inner, w.outer, &weights));
+            PT_TRY(scratch.rows4((const float *)x, M, K, w.inner, &rows));
+            PT_TRY(product_f32(rows, w.inner, 1, weights, 2 * (size_t)w.outer, 1, p, M, 2 * w.outer, w.inner, stream));
+        } else {
+            PT_TRY(product_f32((const float *)x, K, 1, (const float *)gate, F, 1, p, M, F, K, stream));
+            PT_TRY(product_f32((const float *)x, K, 1, (const float *)up, F, 1, p + n, M, F, K, stream));
+        }
+        k_gated_product<<<grid_for((long long)M * ((F + 3) / 4)), 256, 0, s>>>(p, (float *)h, M, F, w.pitch(F), w.second(M, F),
+                                                                              d->activation);
         return PT_OK;
     }
     PT_TRY(scratch.rows16(x, nullptr, M, K, &g.a0, nullptr, &g.lda));
@@ -522,27 +595,32 @@ static pt_status gated_backward_f32(const pt_gated_desc *d, const float *x, cons
 {
     hipStream_t s = stream_of(stream);
     const int M = d->rows, K = d->inner, F = d->outer;
+    const GatedWide w(M, K, F);
+    const bool few = M <= kFewRows32 && F >= 4;  // (what k_gated_few kept lies in two planes)
     // dg and du side by side: one product takes both contractions of dx
+    const size_t both_pitch = 2 * (size_t)w.outer;
     float *both = nullptr, *weights = nullptr;
-    PT_TRY(scratch.take((void **)&both, (size_t)M * 2 * F * sizeof(float)));
-    SlopeArgs a = {kept, grad, both, F, M, F, F, 2 * F, d->activation, grid_for((long long)M * ((F + 7) / 8)), nullptr, nullptr, 0, 0};
+    PT_TRY(scratch.take((void **)&both, M * both_pitch * sizeof(float)));
+    SlopeArgs a = {kept, grad, both, w.outer, M, F, w.outer, 2 * w.outer, d->activation, few ? F : w.pitch(F),
+                   few ? (long long)M * F : w.second(M, F), grid_for((long long)M * ((F + 7) / 8)), nullptr, nullptr, 0, 0};
     k_gated_slope<PT_FLOAT32, PT_FLOAT32><<<a.slopes, 256, 0, s>>>(a);
     if (dx) {
-        PT_TRY(scratch.take((void **)&weights, (size_t)K * 2 * F * sizeof(float)));
-        k_gated_beside<false><<<grid_for((long long)K * F), 256, 0, s>>>((float *)gate, (float *)up, weights, K, F);
-        PT_TRY(product_f32(both, 2 * F, 1, weights, 1, 2 * F, dx, M, K, 2 * F, stream));
+        PT_TRY(scratch.beside(gate, up, K, F, K, w.outer, &weights));
+        PT_TRY(product_f32(both, both_pitch, 1, weights, 1, both_pitch, dx, M, K, 2 * w.outer, stream));
     }
-    // both weights' gradients in one product where one alone has fewer tiles
-    // than the GPU has CUs (4096 x 784 x 1024: 149 us with the pass that takes
-    // them apart, 157 one after the other)
-    if (dgate && (long long)((K + 127) / 128) * ((F + 127) / 128) < 256) {
+    // both weights' gradients in one product where rows fill no packs, or
+    // where one alone has fewer tiles than the GPU has CUs (4096 x 784 x
+    // 1024: 149 us with the pass that takes them apart, 157 one after the other)
+    if (dgate && (w.inner != K || w.outer != F || (long long)((K + 127) / 128) * ((F + 127) / 128) < 256)) {
         float *beside = nullptr;
-        PT_TRY(scratch.take((void **)&beside, (size_t)K * 2 * F * sizeof(float)));
-        PT_TRY(product_f32(x, 1, K, both, 2 * F, 1, beside, K, 2 * F, M, stream));
-        k_gated_beside<true><<<grid_for((long long)K * F), 256, 0, s>>>(dgate, dup, beside, K, F);
+        const float *rows = nullptr;
+        PT_TRY(scratch.rows4(x, M, K, w.inner, &rows));
+        PT_TRY(scratch.take((void **)&beside, w.inner * both_pitch * sizeof(float)));
+        PT_TRY(product_f32(rows, 1, w.inner, both, both_pitch, 1, beside, w.inner, 2 * w.outer, M, stream));
+        k_gated_beside<true><<<grid_for((long long)K * w.outer), 256, 0, s>>>(dgate, dup, beside, K, F, K, w.outer);
     } else if (dgate) {
-        PT_TRY(product_f32(x, 1, K, both, 2 * F, 1, dgate, K, F, M, stream));
-        PT_TRY(product_f32(x, 1, K, both + F, 2 * F, 1, dup, K, F, M, stream));
+        PT_TRY(product_f32(x, 1, K, both, both_pitch, 1, dgate, K, F, M, stream));
+        PT_TRY(product_f32(x, 1, K, both + w.outer, both_pitch, 1, dup, K, F, M, stream));
     }
     return PT_OK;
 }
@@ -559,7 +637,7 @@ static pt_status gated_backward_run(const pt_gated_desc *d, const void *x, const
     uint16_t *dg = nullptr;
     const long long second = (long long)M * pitch;
     PT_TRY(scratch.take((void **)&dg, (size_t)second * 2 * 2));
-    SlopeArgs a = {kept, grad, dg, second, M, F, pitch, pitch, d->activation, grid_for((long long)M * (pitch / 8)), nullptr, nullptr, 0, 0};
+    SlopeArgs a = {kept, grad, dg, second, M, F, pitch, pitch, d->activation, 0, 0, grid_for((long long)M * (pitch / 8)), nullptr, nullptr, 0, 0};
     unsigned blocks = a.slopes;
     if (dgate) {
         a.x = (const uint16_t *)x;
@@ -625,7 +703,7 @@ pt_status pt_gated(const pt_gated_desc *d, const void *x, const void *gate, cons
     PT_TRY(ensure_init());
     if (!n) return PT_OK;
     if (!d->inner) {  // empty sums: act(0) 0
-        if (d->dtype == PT_FLOAT32) PT_TRY(zeros(kept, PT_FLOAT32, 2 * n, stream));
+        if (d->dtype == PT_FLOAT32) PT_TRY(zeros(kept, PT_FLOAT32, 2 * (size_t)d->rows * ((d->outer + 3) / 4 * 4), stream));
         else PT_TRY(zeros(kept, PT_UINT8, 6 * n, stream));
         return zeros(h, d->dtype, n, stream);
     }

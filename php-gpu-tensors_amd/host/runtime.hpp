@@ -206,7 +206,7 @@ bool cuda_array_rotary_backward(const TensorP &q, const TensorP &k, const Tensor
                                 const TensorP &qs, const TensorP &ks, double eps, const TensorP &gq, const TensorP &gk,
                                 TensorP out[4]);
 // act(x gate) * (x up) over the last axis of x; out: the result and, with
-// keep, both products for the gradient: uint8 [6 or 8, rows, outer]
+// keep, both products for the gradient: uint8 [bytes, rows, columns]
 bool cuda_array_gated(const TensorP &x, const TensorP &gate, const TensorP &up, int activation, bool keep, TensorP out[2]);
 // out: of x, gate and up (null where not wanted)
 bool cuda_array_gated_backward(const TensorP &x, const TensorP &gate, const TensorP &up, const TensorP &kept,

@@ -82,7 +82,7 @@ def close(got, want, what):
 # rows, inner, outer: single tokens, few rows, tiles that end anywhere, contractions shorter than a stage and split ones
 SHAPES = [(1, 1, 1), (1, 7, 5), (2, 64, 128), (1, 2048, 300), (5, 33, 129), (16, 100, 256), (17, 31, 24), (32, 500, 1000), (33, 64, 128),
           (40, 1, 8), (64, 72, 136), (50, 300, 77), (100, 37, 3), (129, 8, 7), (130, 200, 260), (257, 65, 129), (300, 129, 64), (128, 4096, 128),
-          (513, 96, 640), (70, 2000, 40), (2100, 40, 24)]
+          (513, 96, 640), (70, 2000, 40), (2100, 40, 24), (300, 48, 40), (390, 61, 130)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
