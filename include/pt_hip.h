@@ -434,7 +434,8 @@ pt_status pt_gated_backward(const pt_gated_desc *desc, const void *x, const void
  * bytes, each 256 with a power of two in the exponent arrays: the first
  * moment as sign, 4 bits of exponent, 3 of mantissa, the second moment's root
  * as 4 and 4; both rounded up or down by numbers drawn from `draws`, which
- * every step advances.  An element one of whose new moments is NaN or 2^126
+ * every step advances, but a root whose first moment is not 0 to no less than
+ * the smallest code.  An element one of whose new moments is NaN or 2^126
  * and more then stays as it was.
  *
  * Any new_ address may be the one it is made from, except the powers' and

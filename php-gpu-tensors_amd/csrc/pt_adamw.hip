@@ -19,7 +19,10 @@
 // and 4 bits.  Both are rounded up or down by 16 drawn bits with the
 // probability of the distance: a second moment moves by 0.1 % a step, less
 // than half a step of any 8-bit format, and would never decay if it went to
-// the nearest.  An element one of whose new moments is NaN or 2^126 and more
+// the nearest.  A root whose first moment is not held as zero is not held as
+// zero either, but as the smallest value at least: otherwise an element whose
+// gradients are 1e-6 of its block's largest would now and then step by its
+// first moment over epsilon, hundreds of rates.  An element one of whose new moments is NaN or 2^126 and more
 // stays as it was: it would take its whole block along, or round up past
 // float32.
 #include "pt_common.h"
@@ -242,8 +245,9 @@ __global__ __launch_bounds__(256) void k_adamw(AdamArgs a)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const uint32_t drawn = ad_mix((uint32_t)(s + k) + key + (uint32_t)(s >> 32) * 0x9E3779B9u);
-                mo |= ad_encode<false>(m[r][k], mx, drawn & 0xffffu) << (8 * k);
-                vo |= ad_encode<true>(root[k], vx, drawn >> 16) << (8 * k);
+                const uint32_t code = ad_encode<false>(m[r][k], mx, drawn & 0xffffu);
+                mo |= code << (8 * k);
+                vo |= max(ad_encode<true>(root[k], vx, drawn >> 16), min(code & 127u, 1u)) << (8 * k);
             }
             __builtin_nontemporal_store(mo, (uint32_t *)((uint8_t *)a.m + s));
             __builtin_nontemporal_store(vo, (uint32_t *)((uint8_t *)a.v + s));
@@ -301,6 +305,9 @@ pt_status pt_adamw(const pt_adamw_desc *d, const pt_adamw_tensor *tensors, int c
     if (d->bits == 8 && (!d->first_exponent || !d->second_exponent || !d->new_first_exponent || !d->new_second_exponent ||
                          !d->draws || !d->new_draws))
         return fail(PT_ERR_INVALID, "AdamW misses a state of 8-bit moments");
+    // (every block reads them, one writes them)
+    if (d->new_power1 == d->power1 || d->new_power2 == d->power2 || (d->bits == 8 && d->new_draws == d->draws))
+        return fail(PT_ERR_INVALID, "AdamW's new powers and draws must not take the old ones' place");
     size_t at = 0;
     for (int i = 0; i < count; i++) {
         const pt_adamw_tensor &t = tensors[i];
@@ -336,6 +343,7 @@ pt_status pt_adamw(const pt_adamw_desc *d, const pt_adamw_tensor *tensors, int c
     a.b2 = (float)d->beta2;
     a.one_b2 = (float)(1.0 - d->beta2);
     a.eps = (float)d->epsilon;
+    if (d->bits == 8) a.eps = std::max(a.eps, 0x1p-126f);  // (the reciprocal of less is infinite, of a first moment of 0 too)
     a.decay = (float)d->weight_decay;
     a.rate_value = (float)d->rate_value;
     a.decay_value = (float)(1.0 - d->rate_value * d->weight_decay);

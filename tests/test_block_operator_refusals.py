@@ -89,7 +89,8 @@ def adamw(**change):
     d = _abi.PtAdamwDesc()
     for name, kind in d._fields_:
         setattr(d, name, A if kind is ctypes.c_void_p else 0)
-    for n, v in {**dict(bits=8, beta1=0.9, beta2=0.99, epsilon=1e-8, weight_decay=0.1, rate_value=0.1, rate=0), **change}.items():
+    for n, v in {**dict(bits=8, beta1=0.9, beta2=0.99, epsilon=1e-8, weight_decay=0.1, rate_value=0.1, rate=0,
+                      new_power1=A + 4, new_power2=A + 8, new_draws=A + 12), **change}.items():
         setattr(d, n, v)
     return ctypes.byref(d)
 
@@ -108,7 +109,7 @@ def tensors(*changes):
     dict(weight_decay=-1.0), dict(rate_value=-1.0), dict(rate_value=float("nan")), dict(first=0), dict(second=0), dict(new_first=0),
     dict(new_second=0), dict(power1=0), dict(power2=0), dict(new_power1=0), dict(new_power2=0), dict(master=0), dict(new_master=0),
     dict(first_exponent=0), dict(second_exponent=0), dict(new_first_exponent=0), dict(new_second_exponent=0), dict(draws=0),
-    dict(new_draws=0)], ids=str)
+    dict(new_draws=0), dict(new_power1=A), dict(new_power2=A), dict(new_draws=A)], ids=str)
 def test_adamw_descriptions(change):
     refused(LIB.pt_adamw(adamw(**change), tensors({}), 1, None))
 

@@ -175,7 +175,9 @@ def test_8_bit_moments(scale, dtype):
         codes, exponents = encode(m, False, r[0])
         assert np.array_equal(new["state"]["firstExponent"].toNumpy(), exponents)
         assert np.array_equal(new["state"]["firstMoment"].toNumpy(), codes)
+        held_m = codes & 127
         codes, exponents = encode(np.sqrt(v), True, r[1])
+        codes = np.maximum(codes, np.minimum(held_m, 1))  # (no root of zero under a first moment that is not)
         assert np.array_equal(new["state"]["secondExponent"].toNumpy(), exponents)
         assert np.array_equal(new["state"]["secondMoment"].toNumpy(), codes)
         assert int(new["state"]["draws"].toNumpy()[0]) == -6 + t
@@ -209,6 +211,38 @@ def test_8_bit_rounding_favours_neither_side():
     # the root is kept in the mean, so the square grows by the rounding's variance: below (1 / 16)^2 / 4 of it a step
     # that rounds, which few do; 0.999^100 = 0.905
     assert 0.85 < end / start < 0.96
+
+
+def test_8_bit_steps_of_small_gradients():
+    """A gradient of 1e-7 of its block's largest rounds to zero or to the smallest code, its first moment and its root each
+    for themselves.  A first moment that is held steps by at most 0.92 of its smallest code, 2^-9 / 128 of the block's
+    largest, over a root of at least sqrt(0.999) of its own, 2^-10 / 256 of the largest: 3.7 times the largest element's
+    quotient.  That is 1 but for the codes' roundings, by 1 / 8 and 1 / 16 a step: after 20 steps m is at most 2.6 times
+    what it should be (0.1 sum 1.0125^k / (1 - 0.9^20)), the root 0.3 times (16 / 17)^20.  3.7 * 2.6 / 0.3 = 32 rates; with
+    roots of zero it would be 1e-6 / (0.03 * 1e-7) and more."""
+    n, opt = 256 * 512, Optimizer.adamW(1.0, 0.9, 0.999, 1e-12, 0.0)
+    g = np.full(n, 1e-7, np.float32)
+    g[::256] = 1.0
+    grad, p = CudaArray.fromNumpy(g), CudaArray.zeros([n])
+    state, seen = opt.initFusedState([p], bits=8, seed=11), 0
+    for _ in range(20):
+        new = opt.fusedStep([p], [grad], state)
+        step = (new["parameters"][0] - p).toNumpy()[g < 1]
+        assert np.abs(step).max() < 32
+        p, state = new["parameters"][0], new["state"]
+        m, v = (opt.moments(state)[x].toNumpy().reshape(-1)[g < 1] for x in ("firstMoment", "secondMoment"))
+        assert not ((m != 0) & (v == 0)).any()
+        seen += int((m != 0).sum())
+    assert seen > 0
+
+
+def test_8_bit_without_epsilon():
+    """An element that never had a gradient stays, whatever epsilon is."""
+    p = CudaArray.fromNumpy(np.arange(600, dtype=np.float32))
+    for epsilon in (0.0, 1e-40, 1e-300):
+        opt = Optimizer.adamW(0.01, 0.9, 0.999, epsilon, 0.0)
+        got = opt.fusedStep([p], [CudaArray.zeros([600])], opt.initFusedState([p], bits=8))["parameters"][0]
+        assert same(got.toNumpy(), p.toNumpy())
 
 
 # ------------------------------------------------------------- the calls
