@@ -5,7 +5,8 @@
 //   16 bits, more than 64 rows: products over a pair of matrices in one
 //     kernel (pt_gated_ring.hip), bound by the matrix cores.
 //   64 rows or fewer (float32: 32, whose matrix instructions are slower):
-//     k_gated_few, bound by the weights' bytes.
+//     k_gated_few, bound by the weights' bytes: one row of bfloat16 through
+//     4096 x 16384 twice 42-48 us (5.6-6.4 TB/s).
 //   float32, more rows: the framework's fp32 products (94 % of the matrix
 //     cores' rate), one for both weights side by side where that is faster,
 //     and a pass over both results; fusing would save that pass, 2 % of the
@@ -350,7 +351,8 @@ __device__ __forceinline__ void gated_transpose(const uint16_t *from, uint16_t *
 // dg and du from the upstream gradient and both products, into rows `pitch`
 // elements apart from d and d + second on, zeros in columns `cols` to
 // `padded` - 1.  A thread takes 8 columns.  Blocks from `slopes` on transpose
-// x beside it, one 64 x 64 tile each, in one launch less.
+// x beside it, one 64 x 64 tile each, in one launch less.  HBM-bound: 8192 x
+// 8192 in bfloat16 with a transpose of 8192 x 2048 160-170 us, 5.3 TB/s.
 struct SlopeArgs {
     const void *kept, *grad;
     void *d;

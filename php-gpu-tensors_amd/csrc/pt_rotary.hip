@@ -15,7 +15,12 @@
 // once for all of them, a pair or two a lane, and hands them round through
 // its own part of LDS without a barrier: as turns, reduced in double before
 // they are rounded (positions reach 2^31).  One cosine and sine per element
-// would cost more than the memory.
+// would cost more than the memory.  Blocks with barriers, a head to a group of
+// waves, took twice as long.
+// Measured, bfloat16, 8192 tokens, 32 and 8 heads of 128 with norms: forward
+// 36 us (4.7 TB/s; a large copy 5.0), gradients of the 32 heads 43-45 us (4.5
+// TB/s) and of the 8 17-18 us, each scale's sum 4.8 us; one token for each of
+// 32 texts 4.5 us.
 #include "pt_common.h"
 
 #include <algorithm>
