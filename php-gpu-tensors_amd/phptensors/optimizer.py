@@ -198,11 +198,13 @@ class Optimizer:
     def moments(state):
         """The moments of a state of initFusedState() as float32 values,
         [blocks, 256]: {"firstMoment", "secondMoment"}."""
-        if state.get("bits", 32) == 32:
-            return {n: state[n] for n in ("firstMoment", "secondMoment")}
+        bits, names = state.get("bits", 32), ("firstMoment", "secondMoment", "firstExponent", "secondExponent")
+        if bits not in (32, 8) or any(not isinstance(state.get(n), CudaArray) for n in names[:2 if bits == 32 else 4]):
+            raise InvalidArgumentException("moments() expects a state of initFusedState()")
+        if bits == 32:
+            return {n: state[n] for n in names[:2]}
         got = (ctypes.c_void_p * 2)()
-        if _host.load().phpt_adamw_moments(*(state[n]._h for n in ("firstMoment", "firstExponent", "secondMoment",
-                                                                   "secondExponent")), got):
+        if _host.load().phpt_adamw_moments(*(state[names[i]]._h for i in (0, 2, 1, 3)), got):
             _host.raise_error("moments")
         return dict(zip(("firstMoment", "secondMoment"), map(CudaArray._wrap, got)))
 

@@ -317,6 +317,8 @@ def test_refusals():
            lambda: opt.fusedStep(p, p, dict(s8, draws=CudaArray.zeros([2], "int32"))), lambda: opt.fusedStep(p, p, s, -1.0),
            lambda: opt.fusedStep(p, p, s, float("nan")), lambda: opt.fusedStep(p, p, s, "x"), lambda: opt.fusedStep(p, p, s, CudaArray.zeros([2])),
            lambda: opt.fusedStep(p, p, s, CudaArray.zeros([1], "float64")), lambda: opt.fusedStep(p, p, s, None, [True]),
+           lambda: opt.moments({}), lambda: opt.moments(dict(s8, firstExponent=None)), lambda: opt.moments(dict(s, bits=8)),
+           lambda: opt.moments(dict(s8, bits=4)), lambda: opt.moments(dict(s8, secondExponent=CudaArray.zeros([9], "int8"))),
            lambda: opt.fusedStep(p, p, s, None, [1, 0]), lambda: opt.fusedStep(p, p, dict(s, master=CudaArray.zeros([1, 256])))]
     for i, call in enumerate(bad):
         with pytest.raises(InvalidArgumentException):
