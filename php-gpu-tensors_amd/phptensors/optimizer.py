@@ -126,9 +126,10 @@ class Optimizer:
     @staticmethod
     def _handles(tensors, what):
         tensors = list(tensors)
-        if not all(isinstance(t, CudaArray) for t in tensors):
+        handles = [t._h for t in tensors if isinstance(t, CudaArray)]
+        if len(handles) != len(tensors):
             raise InvalidArgumentException(f"{what} must be CudaArrays")
-        return (ctypes.c_void_p * max(1, len(tensors)))(*(t._h for t in tensors))
+        return (ctypes.c_void_p * max(1, len(handles)))(*handles)
 
     def initFusedState(self, parameters, bits=32, master=False, seed=0):
         """A state for fusedStep(): the moments of all parameters in one
