@@ -296,3 +296,81 @@ def test_two_threads_at_once():
         t.join()
     for s in (1, 2):
         assert all(np.array_equal(p, q) for one, other in zip(want[s], got[s]) for p, q in zip(one, other))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_one_tensor_in_several_places(dtype):
+    """The same queries as keys, the same scale twice, one matrix as gate and up, a parameter listed twice."""
+    rng = np.random.default_rng(8)
+
+    def made(*shape):
+        return CudaArray.fromNumpy(rng.standard_normal(shape).astype(np.float32), dtype)
+    plan, q, s, gq, gk = Rotary(16), made(40, 3, 16), made(16), made(40, 3, 16), made(40, 3, 16)
+
+    def turn(q, k, s, t):
+        for x in (q, k, s, t):
+            x.requiresGrad().zeroGrad()
+        a, b = q.rotary(plan, None, k, s, t)
+        (a * gq + b * gk).sum().backward()
+        return a, b
+    a, b = turn(q, q, s, s)
+    one = [x.grad().toNumpy().astype(np.float64) for x in (q, s)]
+    k, t = q.copy(), s.copy()
+    c, d = turn(q, k, s, t)
+    assert all(np.array_equal(x.toBits(), y.toBits()) for x, y in ((a, c), (b, d)))
+    h = test_gpu_gated.HALF[dtype]
+    for got, x, y in ((one[0], q, k), (one[1], s, t)):
+        x, y = (v.grad().toNumpy().astype(np.float64) for v in (x, y))
+        # the parts are each rounded to the type, and their sum once more
+        assert (np.abs(got - (x + y)) <= 2 * h * (np.abs(x) + np.abs(y)) + 2.0 ** -120).all()
+    x, w, g = made(70, 24), made(24, 40), made(70, 40)
+
+    def project(gate, up):
+        for v in (x, gate, up):
+            v.requiresGrad().zeroGrad()
+        y = x.gatedProjection(gate, up, "gelu")
+        y.backward(g)
+        return y
+    y = project(w, w)
+    both, dx = w.grad().toNumpy().astype(np.float64), x.grad().toBits()
+    u = w.copy()
+    z = project(w, u)
+    p, r = (v.grad().toNumpy().astype(np.float64) for v in (w, u))
+    assert np.array_equal(y.toBits(), z.toBits()) and np.array_equal(dx, x.grad().toBits())
+    assert (np.abs(both - (p + r)) <= 2 * h * (np.abs(p) + np.abs(r)) + 2.0 ** -120).all()
+    opt, grads = Optimizer.adamW(0.1), [made(24, 40), made(24, 40)]
+    w.requiresGrad(False)
+    new = opt.fusedStep([w, w], grads, opt.initFusedState([w, w]))["parameters"]
+    for n, gr in zip(new, grads):
+        assert np.array_equal(n.toBits(), opt.fusedStep([w], [gr], opt.initFusedState([w]))["parameters"][0].toBits())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_broadcast_and_strided_operands(dtype):
+    """Views with steps of zero and others give what their copies do, gradients of broadcast leaves summed."""
+    rng = np.random.default_rng(9)
+
+    def made(*shape):
+        return CudaArray.fromNumpy(rng.standard_normal(shape).astype(np.float32), dtype)
+    plan, at = Rotary(8, interleaved=True), CudaArray.fromNumpy(np.arange(66, dtype=np.int32))
+    for x in (made(33, 1, 12).broadcastTo([33, 5, 12]), made(1, 5, 12).broadcastTo([33, 5, 12]), made(5, 33, 12).swapaxes(0, 1)):
+        for p in (at.slice([0, 66, 2]), at.slice([7, 8]).broadcastTo([33])):
+            assert np.array_equal(x.rotary(plan, p).toBits(), x.copy().rotary(plan, p.copy()).toBits())
+    row, g = made(1, 5, 12), made(33, 5, 12)
+    row.requiresGrad()
+    row.broadcastTo([33, 5, 12]).rotary(plan, at.slice([0, 33])).backward(g)
+    back = row.grad().toNumpy().astype(np.float64)
+    full = row.detach().broadcastTo([33, 5, 12]).copy().requiresGrad()
+    full.rotary(plan, at.slice([0, 33])).backward(g)
+    each = full.grad().toNumpy().astype(np.float64)
+    h = test_gpu_gated.HALF[dtype]
+    # 33 rounded terms, added in float32 and rounded, or added with a rounding each
+    assert (np.abs(back - each.sum(0, keepdims=True)) <= 34 * h * np.abs(each).sum(0, keepdims=True)).all()
+    w, v = made(1, 40).broadcastTo([24, 40]), made(48, 40).slice([0, 48, 2])
+    for rows in (1, 30, 90):
+        for x in (made(1, 24).broadcastTo([rows, 24]), made(24, rows).T, made(rows, 48).slice(":", [0, 48, 2])):
+            assert np.array_equal(x.gatedProjection(w, v).toBits(), x.copy().gatedProjection(w.copy(), v.copy()).toBits())
+    opt = Optimizer.adamW(0.1)
+    state = opt.initFusedState([v], bits=8, master=True)
+    got, want = (opt.fusedStep([p], [g], state)["parameters"][0].toBits() for p, g in ((v, w), (v.copy(), w.copy())))
+    assert np.array_equal(got, want)
