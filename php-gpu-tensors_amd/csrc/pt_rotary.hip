@@ -180,12 +180,14 @@ __device__ __forceinline__ float rot_sum(float v, int log2)
 // Forward: the heads of both sides count through.  Backward: blockIdx.y is
 // the side, so that a lane's part of the scale's gradient stays in registers
 // over all the tokens that its wave takes.
-template <int DT, int GDT, bool PAIRED, bool BACK>
+// MANY: a token's heads fill half of a wave at most, so it takes as many tokens
+// at once as do fill it (`groups`); each lane finds its own token's.
+template <int DT, int GDT, bool PAIRED, bool BACK, bool MANY>
 __global__ __launch_bounds__(64 * kRotWaves) void k_rotary(RotArgs a)
 {
     constexpr int V = rot_width(DT, BACK);
     using Raw = RotRaw<DT, V>;
-    __shared__ float2 tables[kRotWaves][128];
+    __shared__ float2 tables[kRotWaves][MANY ? 64 * V : 128];
     __shared__ float sums[BACK ? kRotWaves : 1][BACK ? 2 * V : 1][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int log2 = a.lanes_log2, u = lane & ((1 << log2) - 1), slot = lane >> log2, slots = 64 >> log2;
@@ -193,6 +195,9 @@ __global__ __launch_bounds__(64 * kRotWaves) void k_rotary(RotArgs a)
     const RotSide &s0 = a.side[BACK ? blockIdx.y : 0], &s1 = a.side[1];
     const unsigned heads = BACK ? s0.heads : s0.heads + s1.heads;
     const unsigned units = (heads + slots * a.passes - 1) / (slots * a.passes);  // of a token
+    // a lane's token of those that a wave takes, and its head on the first pass
+    const unsigned groups = MANY ? slots / heads : 1, group = MANY ? slot / heads : 0;
+    const unsigned head0 = MANY ? (group < groups ? slot - group * heads : heads) : slot;
     const RotUnit unit = rot_unit<V, PAIRED>(a, u);
     const float inv_n = 1.0f / (float)a.size;
     float2 *table = tables[wave];
@@ -201,14 +206,25 @@ __global__ __launch_bounds__(64 * kRotWaves) void k_rotary(RotArgs a)
         unsigned row, seq, t, first;
         long long pos;
     };
-    const unsigned long long total = (unsigned long long)a.rows * units, step = (unsigned long long)gridDim.x * kRotWaves;
+    const unsigned long long total = ((unsigned long long)a.rows + groups - 1) / groups * units;
+    const unsigned long long step = (unsigned long long)gridDim.x * kRotWaves;
+    auto place = [&](unsigned row, Turn &n) {
+        n.row = row;
+        n.seq = a.tokens == a.rows ? 0 : row / a.tokens;
+        n.t = row - n.seq * a.tokens;
+        n.pos = a.positions ? (long long)a.positions[n.seq * a.pst[0] + n.t * a.pst[1]] : (long long)n.t;
+    };
     auto turn_of = [&](unsigned long long at) {
         Turn n;
-        n.row = units == 1 ? (unsigned)at : (unsigned)(at / units);
-        n.first = (unsigned)(at - (unsigned long long)n.row * units) * a.passes * slots;
-        n.seq = a.tokens == a.rows ? 0 : n.row / a.tokens;
-        n.t = n.row - n.seq * a.tokens;
-        n.pos = a.positions ? (long long)a.positions[n.seq * a.pst[0] + n.t * a.pst[1]] : (long long)n.t;
+        const unsigned turn = units == 1 ? (unsigned)at : (unsigned)(at / units);
+        n.first = (unsigned)(at - (unsigned long long)turn * units) * a.passes * slots;
+        if constexpr (MANY) {  // (past the last token: that one again, and no head)
+            const unsigned long long row = (unsigned long long)turn * groups + group;
+            n.first = row < a.rows ? 0 : heads;
+            place((unsigned)min(row, (unsigned long long)a.rows - 1), n);
+        } else {
+            place(turn, n);
+        }
         return n;
     };
     auto fetch = [&](const Turn &n, unsigned h, Raw &x, RotRaw<GDT, V> &g) {
@@ -225,7 +241,7 @@ __global__ __launch_bounds__(64 * kRotWaves) void k_rotary(RotArgs a)
     Turn now = {}, next = {};
     if (at < total) {
         now = turn_of(at);
-        fetch(now, now.first + slot, x, g);
+        fetch(now, now.first + head0, x, g);
     }
     if (s0.scale) rot_read<DT, V>(s0.scale, 0, unit, w0);
     if (!BACK && s1.scale) rot_read<DT, V>(s1.scale, 0, unit, w1);
@@ -236,9 +252,18 @@ __global__ __launch_bounds__(64 * kRotWaves) void k_rotary(RotArgs a)
     for (; at < total; at += step) {
         const bool more = at + step < total;
         if (more) next = turn_of(at + step);
-        for (int f = lane; f < pairs; f += 64) {
+        for (int f = lane; f < (int)groups * pairs; f += 64) {
+            long long pos = now.pos;
+            double each = f < 64 ? turns0 : turns1;
+            if constexpr (MANY) {
+                const int of = f / pairs;
+                Turn n;
+                place((unsigned)min((unsigned long long)(at * groups + of), (unsigned long long)a.rows - 1), n);
+                pos = n.pos;
+                each = a.turns[f - of * pairs];
+            }
             // the fraction of a turn in two floats: the second corrects the first's cosine and sine
-            double turns = (double)now.pos * (f < 64 ? turns0 : turns1);
+            double turns = (double)pos * each;
             turns -= rint(turns);
             const float hi = (float)turns, lo = (float)(turns - (double)hi) * 6.28318531f;
             float sn, cs;
@@ -250,12 +275,12 @@ __global__ __launch_bounds__(64 * kRotWaves) void k_rotary(RotArgs a)
         __builtin_amdgcn_wave_barrier();
         float2 angle[V];
 #pragma unroll
-        for (int i = 0; i < V; i++) angle[i] = table[min(u * V + i, pairs - 1)];
+        for (int i = 0; i < V; i++) angle[i] = table[(MANY ? min(group, groups - 1) * pairs : 0) + min(u * V + i, pairs - 1)];
         __builtin_amdgcn_wave_barrier();
         for (int p = 0; p < a.passes; p++) {
-            const unsigned h = now.first + p * slots + slot;
+            const unsigned h = now.first + p * slots + head0;
             if (p + 1 < a.passes) fetch(now, h + slots, xn, gn);
-            else if (more) fetch(next, next.first + slot, xn, gn);
+            else if (more) fetch(next, next.first + head0, xn, gn);
             if (h < heads) {  // (whole groups of lanes, so a head's sum has all its lanes)
                 const bool key = !BACK && h >= (unsigned)s0.heads;
                 const RotSide &s = key ? s1 : s0;
@@ -339,30 +364,38 @@ __global__ __launch_bounds__(64) void k_rotary_scale(RotArgs a, int parts, void 
     if (threadIdx.x < 4 && c < a.size) ((typename DType<DT>::S *)out)[c] = DType<DT>::from_c(t);
 }
 
-template <int DT, int GDT>
-static void launch_rotary(const RotArgs &a, bool interleaved, bool back, dim3 grid, hipStream_t s)
+template <int DT, int GDT, bool BACK>
+static void launch_rotary_as(const RotArgs &a, bool interleaved, bool many, dim3 grid, hipStream_t s)
 {
-    if (back) {
-        if (interleaved) k_rotary<DT, GDT, true, true><<<grid, 64 * kRotWaves, 0, s>>>(a);
-        else k_rotary<DT, GDT, false, true><<<grid, 64 * kRotWaves, 0, s>>>(a);
-        return;
+    if (many) {
+        if (interleaved) k_rotary<DT, GDT, true, BACK, true><<<grid, 64 * kRotWaves, 0, s>>>(a);
+        else k_rotary<DT, GDT, false, BACK, true><<<grid, 64 * kRotWaves, 0, s>>>(a);
+    } else {
+        if (interleaved) k_rotary<DT, GDT, true, BACK, false><<<grid, 64 * kRotWaves, 0, s>>>(a);
+        else k_rotary<DT, GDT, false, BACK, false><<<grid, 64 * kRotWaves, 0, s>>>(a);
     }
-    if constexpr (DT == GDT) {
-        if (interleaved) k_rotary<DT, DT, true, false><<<grid, 64 * kRotWaves, 0, s>>>(a);
-        else k_rotary<DT, DT, false, false><<<grid, 64 * kRotWaves, 0, s>>>(a);
-    }
+}
+template <int DT, int GDT>
+static void launch_rotary(const RotArgs &a, bool interleaved, bool back, bool many, dim3 grid, hipStream_t s)
+{
+    if (back) return launch_rotary_as<DT, GDT, true>(a, interleaved, many, grid, s);
+    if constexpr (DT == GDT) launch_rotary_as<DT, DT, false>(a, interleaved, many, grid, s);
 }
 
 // How the heads go to waves: a wave's passes over a token's heads, as many as
 // leave 8192 waves (two for each slot of the GPU at a register count of 128).
-static unsigned rotary_blocks(RotArgs &a, int dtype, bool paired, bool back, int heads, long long most)
+// many: several tokens fit a wave, and there are more than the GPU's 1024
+// SIMDs (of a few, the latency of one counts).
+static unsigned rotary_blocks(RotArgs &a, int dtype, bool paired, bool back, int heads, long long most, bool &many)
 {
     const int units = rot_units(a.size, a.part, paired, rot_width(dtype, back));
     a.lanes_log2 = 0;
     while (1 << a.lanes_log2 < units) a.lanes_log2++;  // (at most 64: heads have at most 256 elements)
     const int all = (heads + (64 >> a.lanes_log2) - 1) >> (6 - a.lanes_log2);
     a.passes = (int)std::max<long long>(1, std::min<long long>(all, (long long)a.rows * all / 8192));
-    const long long waves = (long long)a.rows * ((all + a.passes - 1) / a.passes);
+    const int groups = (64 >> a.lanes_log2) / heads;  // (of the side with more heads)
+    many = groups > 1 && a.rows >= 1024;
+    const long long waves = many ? ((long long)a.rows + groups - 1) / groups : (long long)a.rows * ((all + a.passes - 1) / a.passes);
     // (in rounds of equal length)
     const long long blocks = (waves + kRotWaves - 1) / kRotWaves, rounds = (blocks + most - 1) / most;
     return (unsigned)((blocks + rounds - 1) / rounds);
@@ -430,10 +463,11 @@ pt_status pt_rotary(const pt_rotary_desc *d, const void *const *x, const void *c
     if (!sides) return PT_OK;
     hipStream_t s = stream_of(stream);
     if (sides == 1) a.side[1].heads = 0;
-    const unsigned blocks = rotary_blocks(a, d->dtype, d->interleaved, false, a.side[0].heads + a.side[1].heads, kRotBlocks);
-    if (d->dtype == PT_FLOAT32) launch_rotary<PT_FLOAT32, PT_FLOAT32>(a, d->interleaved, false, blocks, s);
-    else if (d->dtype == PT_FLOAT16) launch_rotary<PT_FLOAT16, PT_FLOAT16>(a, d->interleaved, false, blocks, s);
-    else launch_rotary<PT_BFLOAT16, PT_BFLOAT16>(a, d->interleaved, false, blocks, s);
+    bool many;
+    const unsigned blocks = rotary_blocks(a, d->dtype, d->interleaved, false, a.side[0].heads + a.side[1].heads, kRotBlocks, many);
+    if (d->dtype == PT_FLOAT32) launch_rotary<PT_FLOAT32, PT_FLOAT32>(a, d->interleaved, false, many, blocks, s);
+    else if (d->dtype == PT_FLOAT16) launch_rotary<PT_FLOAT16, PT_FLOAT16>(a, d->interleaved, false, many, blocks, s);
+    else launch_rotary<PT_BFLOAT16, PT_BFLOAT16>(a, d->interleaved, false, many, blocks, s);
     return check_hip(hipGetLastError(), "rotary");
 }
 
@@ -473,8 +507,9 @@ pt_status pt_rotary_backward(const pt_rotary_desc *d, const void *const *x, cons
     if (!sides) return PT_OK;
     hipStream_t s = stream_of(stream);
     // a partial row a block: four blocks a CU walk the tokens
+    bool many;
     const unsigned blocks = rotary_blocks(a, d->dtype, d->interleaved, true, std::max(a.side[0].heads, sides > 1 ? a.side[1].heads : 0),
-                                          partial ? kRotBlocks / 2 : kRotBlocks);
+                                          partial ? kRotBlocks / 2 : kRotBlocks, many);
     void *scratch = nullptr;
     if (partial) {
         PT_TRY(scratch_alloc(&scratch, (size_t)blocks * 2 * a.size * sizeof(float), s));
@@ -482,13 +517,13 @@ pt_status pt_rotary_backward(const pt_rotary_desc *d, const void *const *x, cons
             if (ds[i]) a.side[i].partial = (float *)scratch + (size_t)i * blocks * a.size;
     }
     const bool same = grad_dtype == d->dtype;
-    if (d->dtype == PT_FLOAT32) launch_rotary<PT_FLOAT32, PT_FLOAT32>(a, d->interleaved, true, dim3(blocks, sides), s);
+    if (d->dtype == PT_FLOAT32) launch_rotary<PT_FLOAT32, PT_FLOAT32>(a, d->interleaved, true, many, dim3(blocks, sides), s);
     else if (d->dtype == PT_FLOAT16) {
-        if (same) launch_rotary<PT_FLOAT16, PT_FLOAT16>(a, d->interleaved, true, dim3(blocks, sides), s);
-        else launch_rotary<PT_FLOAT16, PT_FLOAT32>(a, d->interleaved, true, dim3(blocks, sides), s);
+        if (same) launch_rotary<PT_FLOAT16, PT_FLOAT16>(a, d->interleaved, true, many, dim3(blocks, sides), s);
+        else launch_rotary<PT_FLOAT16, PT_FLOAT32>(a, d->interleaved, true, many, dim3(blocks, sides), s);
     } else {
-        if (same) launch_rotary<PT_BFLOAT16, PT_BFLOAT16>(a, d->interleaved, true, dim3(blocks, sides), s);
-        else launch_rotary<PT_BFLOAT16, PT_FLOAT32>(a, d->interleaved, true, dim3(blocks, sides), s);
+        if (same) launch_rotary<PT_BFLOAT16, PT_BFLOAT16>(a, d->interleaved, true, many, dim3(blocks, sides), s);
+        else launch_rotary<PT_BFLOAT16, PT_FLOAT32>(a, d->interleaved, true, many, dim3(blocks, sides), s);
     }
     if (partial) {
         const dim3 grid((a.size + 3) / 4, sides);

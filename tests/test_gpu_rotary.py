@@ -216,6 +216,34 @@ def test_rows_past_one_turn_of_the_blocks():
     close(y, want["y"], "y"), close(x.grad(), want["dx"], "dx"), close(s.grad(), want["dw"], "dw")
 
 
+# few heads of many tokens, several of which share a wave: groups of heads that fill it or not, last groups that end inside
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("shape", [((1025,), 1, 1, 2, 2), ((3, 701), 2, 1, 20, 8), ((2, 1100), 1, 1, 64, 64), ((1500,), 3, 1, 7, 6),
+                                   ((1037,), 2, 2, 32, 30), ((2049,), 5, 1, 16, 16), ((1100,), 1, 3, 128, 96)], ids=str)
+def test_tokens_that_share_a_wave(shape, norm, interleaved, dtype):
+    test_both_directions(shape, norm, interleaved, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tokens_together_and_in_parts(dtype):
+    """Many tokens' values and gradients, both sides' in one call, are those of parts of them, which go another way."""
+    plan, n = Rotary(12), 1500
+    q, k, s = values((n, 3, 18), dtype, 1)[0], values((n, 1, 18), dtype, 2)[0], values((18,), dtype, 3, 0.1, 1.0)[0]
+    a, b = values((n, 3, 18), dtype, 4)[0], values((n, 1, 18), dtype, 5)[0]
+
+    def run(lo, hi, at):
+        x, y = (t.slice([lo, hi]).copy().requiresGrad() for t in (q, k))
+        u, v = x.rotary(plan, at, y, s, s, EPS)
+        ((u * a.slice([lo, hi])).sum() + (v * b.slice([lo, hi])).sum()).backward()
+        return [t.toBits() for t in (u, v, x.grad(), y.grad())]
+    whole = run(0, n, None)
+    for lo, hi in ((0, 500), (500, 1000), (1000, n)):
+        part = run(lo, hi, CudaArray.fromNumpy(np.arange(lo, hi, dtype=np.int32)))
+        assert all(np.array_equal(w[lo:hi], p) for w, p in zip(whole, part))
+
+
 def test_no_norm_leaves_what_is_not_finite_in_its_pair():
     x = np.zeros((2, 1, 8), np.float32)
     x[0, 0, 1], x[1, 0, 7] = np.nan, np.inf
