@@ -404,9 +404,8 @@ typedef struct {
     int rows, inner, outer;   /* each at most 2^21 */
 } pt_gated_desc;
 /* kept (may be NULL): for the backward call, both products in 24 bits (16-bit
- * dtypes: 6 rows outer bytes, opaque) or in float32 (8 rows times outer rounded
- * up to 4, in bytes).  Results must not overlap operands, here and in
- * the backward call. */
+ * dtypes: 6 rows outer bytes, opaque) or in float32 (8 rows outer bytes).  Results
+ * must not overlap operands, here and in the backward call. */
 pt_status pt_gated(const pt_gated_desc *desc, const void *x, const void *gate, const void *up, void *h, void *kept,
                    pt_stream_t stream);
 /* Gradients, contiguous and of the dtype, for the upstream gradient `grad`

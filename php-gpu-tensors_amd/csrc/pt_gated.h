@@ -147,7 +147,14 @@ constexpr long long kPairPitch = 1 << 21;  // the most that a row's pitch may be
 void pair_plan(PairArgs &g, bool columns, int &tm);  // tiles, split and stages
 void launch_pair_columns(const PairArgs &g, int dtype, int tm, int store, hipStream_t s);
 void launch_pair_sum(const PairArgs &g, int dtype, int tm, hipStream_t s);
-// the join alone: of few rows' parts, columns form (also float32)
-void launch_pair_join(const PairArgs &g, int dtype, int store, hipStream_t s);
+// the join alone, of parts that were made elsewhere: float32, and few rows in
+// the columns form
+void launch_pair_join(const PairArgs &g, int dtype, bool sum, int store, hipStream_t s);
+
+// The same of fp32 matrices at any pitch (pt_gated_wide.hip): kb is not read,
+// stages are 16 k wide; turned: columns with A [K][M].
+enum { WIDE_COLUMNS = 0, WIDE_TURNED = 1, WIDE_SUM = 2 };
+void wide_plan(PairArgs &g, int form, int &tm);
+void launch_wide(const PairArgs &g, int tm, int form, int store, hipStream_t s);
 
 }  // namespace pt

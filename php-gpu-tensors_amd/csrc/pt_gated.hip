@@ -7,10 +7,8 @@
 //   64 rows or fewer (float32: 32, whose matrix instructions are slower):
 //     k_gated_few, bound by the weights' bytes: one row of bfloat16 through
 //     4096 x 16384 twice 42-48 us (5.6-6.4 TB/s).
-//   float32, more rows: the framework's fp32 products (94 % of the matrix
-//     cores' rate), one for both weights side by side where that is faster,
-//     and a pass over both results; fusing would save that pass, 2 % of the
-//     time at 4096 inner elements.
+//   float32, more rows: the same products in fp32 (pt_gated_wide.hip), and
+//     large gradients by the plain fp32 ring product.
 #include "pt_gated.h"
 
 #include <algorithm>
@@ -214,30 +212,6 @@ __device__ __forceinline__ void gd_load(const typename GE<DT>::S *p, int live, f
     for (int k = 0; k < V; k++) v[k] = k < live ? DType<DT>::to_c(p[k]) : 0.0f;
 }
 
-// h of fp32 products in rows `pitch` elements apart, the second `second`
-// behind the first; a thread takes 4 columns.
-__global__ __launch_bounds__(256) void k_gated_product(const float *p, float *h, int rows, int cols, int pitch, long long second,
-                                                       int act)
-{
-    const int packs = (cols + 3) / 4;
-    const long long total = (long long)rows * packs;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long row = i / packs;
-        const int c = (int)(i - row * packs) * 4, live = min(4, cols - c);
-        float g[4], u[4];
-        gd_load<PT_FLOAT32, 4>(p + row * pitch + c, live, g);
-        gd_load<PT_FLOAT32, 4>(p + row * pitch + second + c, live, u);
-        gated_products<false>(act, g, u);
-        float *to = h + row * cols + c;
-        typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
-        if (live == 4) *(float4u *)to = float4u{g[0], g[1], g[2], g[3]};
-        else
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (k < live) to[k] = g[k];
-    }
-}
-
 // 8 elements of a product as the gradient keeps it in 24 bits
 __device__ __forceinline__ void gd_load_kept(const void *kept, long long n, int product, long long i, int live, float (&v)[8])
 {
@@ -255,38 +229,24 @@ __device__ __forceinline__ void gd_load_kept(const void *kept, long long n, int 
     for (int k = 0; k < 8; k++) v[k] = k < live ? kept_value(high[k], low[k]) : 0.0f;
 }
 
-// Two fp32 matrices [rows][cols] side by side, each in `each` columns (zeros
-// past the end, also in rows up to `down`), or (BACK) apart again.
+// Two fp32 matrices [rows][cols] side by side, or (BACK) apart again, in packs
+// of 4.
 template <bool BACK>
-__global__ __launch_bounds__(256) void k_gated_beside(float *a, float *b, float *both, int rows, int cols, int down, int each)
+__global__ __launch_bounds__(256) void k_gated_beside(float *a, float *b, float *both, int rows, int cols)
 {
-    const long long n = (long long)(BACK ? rows : down) * each;
+    typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+    const int packs = cols / 4;
+    const long long n = (long long)rows * packs;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const long long row = i / each, c = i - row * each, at = i + row * each, from = row * cols + c;
-        const bool live = row < rows && c < cols;
+        const long long row = i / packs, at = row * 2 * cols + (i - row * packs) * 4;
+        float4u *p = (float4u *)a + i, *q = (float4u *)b + i, *r = (float4u *)(both + at), *t = (float4u *)(both + at + cols);
         if constexpr (BACK) {
-            if (live) {
-                a[from] = both[at];
-                b[from] = both[at + each];
-            }
+            *p = *r;
+            *q = *t;
         } else {
-            both[at] = live ? a[from] : 0.0f;
-            both[at + each] = live ? b[from] : 0.0f;
+            *r = *p;
+            *t = *q;
         }
-    }
-}
-
-__global__ __launch_bounds__(256) void k_gated_sum(float *a, const float *b, long long n)
-{
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) a[i] += b[i];
-}
-
-// fp32 rows of `cols` in rows of `pitch`, zeros past the end
-__global__ __launch_bounds__(256) void k_gated_pitch(const float *from, float *to, long long rows, int cols, int pitch)
-{
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * pitch; i += (long long)gridDim.x * 256) {
-        const long long row = i / pitch, c = i - row * pitch;
-        to[i] = c < cols ? from[row * cols + c] : 0.0f;
     }
 }
 
@@ -358,8 +318,6 @@ struct SlopeArgs {
     void *d;
     long long second;
     int rows, cols, padded, pitch, act;
-    int kept_pitch;          // float32: both products' rows, and where the second one's begin
-    long long kept_second;
     unsigned slopes;         // blocks
     const uint16_t *x;       // [rows][inner]
     uint16_t *xt;            // [inner][across]
@@ -383,9 +341,8 @@ __global__ __launch_bounds__(256) void k_gated_slope(SlopeArgs a)
         const long long from = row * a.cols + c;
         float g[8], u[8], dh[8];
         if constexpr (DT == PT_FLOAT32) {
-            const S *kept = (const S *)a.kept + row * a.kept_pitch + c;
-            gd_load<DT, 8>(kept, live, g);
-            gd_load<DT, 8>(kept + a.kept_second, live, u);
+            gd_load<DT, 8>((const S *)a.kept + from, live, g);
+            gd_load<DT, 8>((const S *)a.kept + plane + from, live, u);
         } else {
             gd_load_kept(a.kept, plane, 0, from, live, g);
             gd_load_kept(a.kept, plane, 1, from, live, u);
@@ -466,24 +423,6 @@ struct GatedScratch {
         g.ldb = round8(cols);
         return PT_OK;
     }
-    // fp32: two matrices side by side in down x 2 each elements
-    pt_status beside(const float *a, const float *b, int rows, int cols, int down, int each, float **to)
-    {
-        PT_TRY(take((void **)to, (size_t)down * 2 * each * sizeof(float)));
-        k_gated_beside<false><<<grid_for((long long)down * each), 256, 0, s>>>((float *)a, (float *)b, *to, rows, cols, down, each);
-        return PT_OK;
-    }
-    // fp32 rows of `pitch`: themselves where they are, or a copy
-    pt_status rows4(const float *a, long long rows, int cols, int pitch, const float **to)
-    {
-        *to = a;
-        if (cols == pitch) return PT_OK;
-        float *p = nullptr;
-        PT_TRY(take((void **)&p, (size_t)rows * pitch * sizeof(float)));
-        k_gated_pitch<<<grid_for(rows * pitch), 256, 0, s>>>(a, p, rows, cols, pitch);
-        *to = p;
-        return PT_OK;
-    }
 };
 
 static pt_status gated_check(const pt_gated_desc *d)
@@ -514,25 +453,15 @@ static pt_status product_f32(const float *a, size_t am, size_t ak, const float *
     return pt_matmul(a, b, c, PT_FLOAT32, sa, ta, 2, sb, tb, 2, sc, 2, stream);
 }
 
-// fp32, more rows than k_gated_few takes: both weights lie side by side for
-// one product, rather than two, where their rows fill no 16-byte packs (the
-// product then reads whole packs of the copy, and runs the fp32 ring: 2048 x
-// 1000 x 2731 214 us, 299 with two products in place), or where the tiles
-// of one fill the CUs and twice as many take fewer rounds than two products
-// do, which saves more than the copy costs (0.06 us a k against 3.2e-6 a
-// weight: 2048 x 1024 x 2816 209 us, 256 with two).
-struct GatedWide {
-    int inner, outer;  // rounded up to whole packs
-    bool beside;
-    GatedWide(int M, int K, int F) : inner((K + 3) / 4 * 4), outer((F + 3) / 4 * 4)
-    {
-        const long long tiles = (long long)((M + 127) / 128) * ((F + 127) / 128);
-        beside = inner != K || outer != F || (tiles >= 256 && 2 * ((tiles + 255) / 256) > (2 * tiles + 255) / 256 && F < 18750);
-    }
-    // the rows that both products are kept in, and where the second one's begin
-    int pitch(int F) const { return beside ? 2 * outer : F; }
-    long long second(int M, int F) const { return beside ? outer : (long long)M * F; }
-};
+// A product over a pair of matrices in fp32
+static pt_status run_wide(PairArgs &g, int form, int store, GatedScratch &scratch)
+{
+    int tm;
+    wide_plan(g, form, tm);
+    if (g.split > 1) PT_TRY(scratch.take((void **)&g.parts, (size_t)g.split * (form == WIDE_SUM ? 1 : 2) * g.M * g.n_out * sizeof(float)));
+    launch_wide(g, tm, form, store, scratch.s);
+    return PT_OK;
+}
 
 // Wide strips, whose k-steps are split over up to a block for every CU; strips
 // of 8-byte packs, without a split, where the split's second kernel (4.5 us)
@@ -561,7 +490,7 @@ static pt_status launch_few(PairArgs &g, GatedScratch &scratch, hipStream_t s)
     };
     if (thin) go(IC<NC / 2>{});
     else go(IC<NC>{});
-    if (g.split > 1) launch_pair_join(g, DT, g.c1 ? GATED_KEPT : GATED_PRODUCT, s);
+    if (g.split > 1) launch_pair_join(g, DT, false, g.c1 ? GATED_KEPT : GATED_PRODUCT, s);
     return PT_OK;
 }
 
@@ -589,24 +518,7 @@ static pt_status gated_run(const pt_gated_desc *d, const void *x, const void *ga
         if (d->dtype == PT_FLOAT32) return launch_few<PT_FLOAT32>(g, scratch, s);
         return d->dtype == PT_FLOAT16 ? launch_few<PT_FLOAT16>(g, scratch, s) : launch_few<PT_BFLOAT16>(g, scratch, s);
     }
-    if (d->dtype == PT_FLOAT32) {
-        const GatedWide w(M, K, F);
-        float *p = (float *)kept;
-        if (!p) PT_TRY(scratch.take((void **)&p, (size_t)M * 2 * w.outer * sizeof(float)));
-        if (w.beside) {
-            float *weights = nullptr;
-            const float *rows = nullptr;
-            PT_TRY(scratch.beside((const float *)gate, (const float *)up, K, F, w.inner, w.outer, &weights));
-            PT_TRY(scratch.rows4((const float *)x, M, K, w.inner, &rows));
-            PT_TRY(product_f32(rows, w.inner, 1, weights, 2 * (size_t)w.outer, 1, p, M, 2 * w.outer, w.inner, stream));
-        } else {
-            PT_TRY(product_f32((const float *)x, K, 1, (const float *)gate, F, 1, p, M, F, K, stream));
-            PT_TRY(product_f32((const float *)x, K, 1, (const float *)up, F, 1, p + n, M, F, K, stream));
-        }
-        k_gated_product<<<grid_for((long long)M * ((F + 3) / 4)), 256, 0, s>>>(p, (float *)h, M, F, w.pitch(F), w.second(M, F),
-                                                                              d->activation);
-        return PT_OK;
-    }
+    if (d->dtype == PT_FLOAT32) return run_wide(g, WIDE_COLUMNS, kept ? GATED_KEPT : GATED_PRODUCT, scratch);
     PT_TRY(scratch.rows16(x, M, K, &g.a0, K % 8 || ((uintptr_t)x & 15)));
     PT_TRY(scratch.weights16(gate, up, K, F, g));
     scratch.pack();
@@ -621,45 +533,56 @@ static pt_status gated_run(const pt_gated_desc *d, const void *x, const void *ga
     return PT_OK;
 }
 
+// Large products of whole packs: the plain ring product, whose loads go to LDS
+// by themselves, holds 95-100 % of the matrix cores at its clock where the pair
+// kernel holds 80, which pays for copies of the weights, and of their gradients,
+// side by side: 8192 x 1024 x 1024 both ways 786 us, 919 with the pair
+// kernel, 4096 x 784 x 1024 389 and 414; but 1000 x 768 x 2048 235 and 214.
+static bool gated_ring_f32(int M, int K, int F) { return K % 4 == 0 && F % 4 == 0 && (double)M * K * F > 2.5e9; }
+
 static pt_status gated_backward_f32(const pt_gated_desc *d, const float *x, const float *gate, const float *up, const void *kept,
                                     const void *grad, float *dx, float *dgate, float *dup, GatedScratch &scratch, pt_stream_t stream)
 {
-    hipStream_t s = stream_of(stream);
+    hipStream_t s = scratch.s;
     const int M = d->rows, K = d->inner, F = d->outer;
-    const GatedWide w(M, K, F);
-    const bool few = M <= kFewRows32 && F >= 4;  // (what k_gated_few kept lies in two planes)
-    // dg and du side by side: one product takes both contractions of dx
-    const size_t both_pitch = 2 * (size_t)w.outer;
-    float *both = nullptr, *weights = nullptr;
-    PT_TRY(scratch.take((void **)&both, M * both_pitch * sizeof(float)));
-    SlopeArgs a = {kept, grad, both, w.outer, M, F, w.outer, 2 * w.outer, d->activation, few ? F : w.pitch(F),
-                   few ? (long long)M * F : w.second(M, F), grid_for((long long)M * ((F + 7) / 8)), nullptr, nullptr, 0, 0};
+    const bool ring = gated_ring_f32(M, K, F);
+    // dg and du side by side, where one product takes both contractions of dx
+    const long long pitch = ring ? 2 * F : F, second = ring ? F : ((long long)M * F + 3) / 4 * 4;
+    float *dg = nullptr, *both = nullptr;
+    PT_TRY(scratch.take((void **)&dg, 2 * (ring ? (size_t)M * F : (size_t)second) * sizeof(float)));
+    SlopeArgs a = {kept, grad, dg, second, M, F, F, (int)pitch, d->activation, grid_for((long long)M * ((F + 7) / 8)), nullptr, nullptr, 0, 0};
     k_gated_slope<PT_FLOAT32, PT_FLOAT32><<<a.slopes, 256, 0, s>>>(a);
-    if (dx && (long long)M * 4 < F && F % 4 == 0 && 16.0 * K * F > 1e8) {
-        // few rows: two products and their sum move less than a copy of large
-        // weights (33 x 4096 x 14336 both ways 546 us, 770 with the copy)
-        float *other = nullptr;
-        PT_TRY(scratch.take((void **)&other, (size_t)M * K * sizeof(float)));
-        PT_TRY(product_f32(both, both_pitch, 1, gate, 1, F, dx, M, K, F, stream));
-        PT_TRY(product_f32(both + w.outer, both_pitch, 1, up, 1, F, other, M, K, F, stream));
-        k_gated_sum<<<grid_for((long long)M * K), 256, 0, s>>>(dx, other, (long long)M * K);
+    const unsigned blocks = grid_for((long long)K * F / 4);
+    if (ring) PT_TRY(scratch.take((void **)&both, (size_t)K * 2 * F * sizeof(float)));
+    if (dx && ring) {
+        k_gated_beside<false><<<blocks, 256, 0, s>>>((float *)gate, (float *)up, both, K, F);
+        PT_TRY(product_f32(dg, pitch, 1, both, 1, pitch, dx, M, K, 2 * F, stream));
     } else if (dx) {
-        PT_TRY(scratch.beside(gate, up, K, F, K, w.outer, &weights));
-        PT_TRY(product_f32(both, both_pitch, 1, weights, 1, both_pitch, dx, M, K, 2 * w.outer, stream));
+        PairArgs g = {};
+        g.a0 = dg;
+        g.a1 = dg + second;
+        g.b0 = gate;
+        g.b1 = up;
+        g.lda = g.ldb = g.K = F;
+        g.M = M;
+        g.N = g.n_out = K;
+        g.c0 = dx;
+        PT_TRY(run_wide(g, WIDE_SUM, GATED_PRODUCT, scratch));
     }
-    // both weights' gradients in one product where rows fill no packs, or
-    // where one alone has fewer tiles than the GPU has CUs (4096 x 784 x
-    // 1024: 149 us with the pass that takes them apart, 157 one after the other)
-    if (dgate && (w.inner != K || w.outer != F || (long long)((K + 127) / 128) * ((F + 127) / 128) < 256)) {
-        float *beside = nullptr;
-        const float *rows = nullptr;
-        PT_TRY(scratch.rows4(x, M, K, w.inner, &rows));
-        PT_TRY(scratch.take((void **)&beside, w.inner * both_pitch * sizeof(float)));
-        PT_TRY(product_f32(rows, 1, w.inner, both, both_pitch, 1, beside, w.inner, 2 * w.outer, M, stream));
-        k_gated_beside<true><<<grid_for((long long)K * w.outer), 256, 0, s>>>(dgate, dup, beside, K, F, K, w.outer);
+    if (dgate && ring) {
+        PT_TRY(product_f32(x, 1, K, dg, pitch, 1, both, K, 2 * F, M, stream));
+        k_gated_beside<true><<<blocks, 256, 0, s>>>(dgate, dup, both, K, F);
     } else if (dgate) {
-        PT_TRY(product_f32(x, 1, K, both, both_pitch, 1, dgate, K, F, M, stream));
-        PT_TRY(product_f32(x, 1, K, both + w.outer, both_pitch, 1, dup, K, F, M, stream));
+        PairArgs g = {};
+        g.a0 = x;
+        g.b0 = dg;
+        g.b1 = dg + second;
+        g.lda = g.M = K;
+        g.ldb = g.N = g.n_out = F;
+        g.K = M;
+        g.c1 = dgate;
+        g.c2 = dup;
+        PT_TRY(run_wide(g, WIDE_TURNED, GATED_BOTH, scratch));
     }
     return PT_OK;
 }
@@ -676,7 +599,7 @@ static pt_status gated_backward_run(const pt_gated_desc *d, const void *x, const
     uint16_t *dg = nullptr;
     const long long second = (long long)M * pitch;
     PT_TRY(scratch.take((void **)&dg, (size_t)second * 2 * 2));
-    SlopeArgs a = {kept, grad, dg, second, M, F, pitch, pitch, d->activation, 0, 0, grid_for((long long)M * (pitch / 8)), nullptr, nullptr, 0, 0};
+    SlopeArgs a = {kept, grad, dg, second, M, F, pitch, pitch, d->activation, grid_for((long long)M * (pitch / 8)), nullptr, nullptr, 0, 0};
     unsigned blocks = a.slopes;
     if (dgate) {
         a.x = (const uint16_t *)x;
@@ -743,8 +666,7 @@ pt_status pt_gated(const pt_gated_desc *d, const void *x, const void *gate, cons
     PT_TRY(ensure_init());
     if (!n) return PT_OK;
     if (!d->inner) {  // empty sums: act(0) 0
-        if (d->dtype == PT_FLOAT32) PT_TRY(zeros(kept, PT_FLOAT32, 2 * (size_t)d->rows * ((d->outer + 3) / 4 * 4), stream));
-        else PT_TRY(zeros(kept, PT_UINT8, 6 * n, stream));
+        PT_TRY(zeros(kept, PT_UINT8, (d->dtype == PT_FLOAT32 ? 8 : 6) * n, stream));
         return zeros(h, d->dtype, n, stream);
     }
     PT_TRY(gated_run(d, x, gate, up, h, kept, stream));

@@ -445,16 +445,18 @@ static void join_parts(const PairArgs &g, hipStream_t s)
     k_pair_join<DT, SUM, STORE><<<blocks, 256, 0, s>>>(g);
 }
 
-void launch_pair_join(const PairArgs &g, int dtype, int store, hipStream_t s)
+void launch_pair_join(const PairArgs &g, int dtype, bool sum, int store, hipStream_t s)
 {
     auto go = [&](auto DTC) {
         constexpr int D = decltype(DTC)::value;
         if (store == GATED_PRODUCT) join_parts<D, false, GATED_PRODUCT>(g, s);
         else join_parts<D, false, GATED_KEPT>(g, s);
     };
-    if (dtype == PT_FLOAT32) go(IC<PT_FLOAT32>{});
-    else if (dtype == PT_BFLOAT16) go(IC<PT_BFLOAT16>{});
-    else go(IC<PT_FLOAT16>{});
+    if (dtype == PT_BFLOAT16) go(IC<PT_BFLOAT16>{});
+    else if (dtype == PT_FLOAT16) go(IC<PT_FLOAT16>{});
+    else if (sum) join_parts<PT_FLOAT32, true, GATED_PRODUCT>(g, s);
+    else if (store == GATED_BOTH) join_parts<PT_FLOAT32, false, GATED_BOTH>(g, s);
+    else go(IC<PT_FLOAT32>{});
 }
 
 template <int DT, bool SUM, int STORE>

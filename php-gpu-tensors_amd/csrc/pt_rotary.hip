@@ -181,7 +181,8 @@ __device__ __forceinline__ float rot_sum(float v, int log2)
 // the side, so that a lane's part of the scale's gradient stays in registers
 // over all the tokens that its wave takes.
 // MANY: a token's heads fill half of a wave at most, so it takes as many tokens
-// at once as do fill it (`groups`); each lane finds its own token's.
+// at once as do fill it (`groups`); each lane finds its own token's.  2 heads of
+// 32 in bfloat16 3.5 TB/s instead of 0.6, 8 heads of 32 4.4 instead of 2.2.
 template <int DT, int GDT, bool PAIRED, bool BACK, bool MANY>
 __global__ __launch_bounds__(64 * kRotWaves) void k_rotary(RotArgs a)
 {

@@ -305,9 +305,8 @@ static int gated_shape(const Tensor &x, const Tensor &gate, int *shape)
     return x.ndims;
 }
 
-// what pt_gated keeps of both products: bytes of an element, and of columns
+// what pt_gated keeps of both products, in bytes an element
 static int kept_bytes(const TensorP &x) { return x->dtype == PT_FLOAT32 ? 8 : 6; }
-static int kept_columns(const TensorP &x, int outer) { return x->dtype == PT_FLOAT32 ? (outer + 3) / 4 * 4 : outer; }
 
 static bool gated_run(const TensorP &x, const TensorP &gate, const TensorP &up, int activation, const TensorP &h,
                       const TensorP &kept)
@@ -325,7 +324,7 @@ bool cuda_array_gated(const TensorP &x, const TensorP &gate, const TensorP &up, 
     pt_gated_desc d;
     if (!gated_desc(x, gate, up, activation, d)) return false;
     int shape[kMaxDims];
-    const int nd = gated_shape(*x, *gate, shape), both[3] = {kept_bytes(x), d.rows, kept_columns(x, d.outer)};
+    const int nd = gated_shape(*x, *gate, shape), both[3] = {kept_bytes(x), d.rows, d.outer};
     out[1] = nullptr;
     if (fusion_active()) {
         NativeSpec sp;
@@ -370,7 +369,7 @@ bool cuda_array_gated_backward(const TensorP &x, const TensorP &gate, const Tens
     int shape[kMaxDims];
     const int nd = gated_shape(*x, *gate, shape);
     if (!kept || kept->dtype != PT_UINT8 || kept->ndims != 3 || kept->shape[0] != kept_bytes(x) || kept->shape[1] != d.rows ||
-        kept->shape[2] != kept_columns(x, d.outer)) {
+        kept->shape[2] != d.outer) {
         set_invalid("gatedProjection gradients need the forward pass's products");
         return false;
     }

@@ -14,7 +14,7 @@ BODY = {
                           " values(dx[i], desc->sequences * desc->tokens * desc->heads[i] * desc->size, 3.0f + i, desc->dtype);"
                           " if (dscale) values(dscale[i], desc->size, 5.0f + i, desc->dtype); }",
     "pt_gated": "const size_t n = (size_t)desc->rows * desc->outer; values(h, n, 1.5f, desc->dtype);"
-                " if (kept) memset(kept, 7, desc->dtype == PT_FLOAT32 ? 8 * (size_t)desc->rows * ((desc->outer + 3) / 4 * 4) : 6 * n);",
+                " if (kept) memset(kept, 7, (desc->dtype == PT_FLOAT32 ? 8 : 6) * n);",
     "pt_gated_backward": "const float at = *(const unsigned char *)kept;"
                          " values(dx, (size_t)desc->rows * desc->inner, at + 1.0f, desc->dtype);"
                          " values(dgate, (size_t)desc->inner * desc->outer, at + 2.0f, desc->dtype);"

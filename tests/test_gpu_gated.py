@@ -119,6 +119,12 @@ def test_many_tiles(shape, dtype):
     test_both_directions(shape, dtype)
 
 
+@pytest.mark.parametrize("shape", [(2048, 640, 2048), (2500, 1004, 1000)], ids=str)
+def test_large_float32(shape):
+    """Past 2.5e9 multiplications for a matrix, where the gradients go another way."""
+    test_both_directions(shape, "float32")
+
+
 @pytest.mark.parametrize("name", ACTS)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_activations_over_their_range(name, dtype):
