@@ -385,8 +385,9 @@ static void launch_rotary(const RotArgs &a, bool interleaved, bool back, bool ma
 
 // How the heads go to waves: a wave's passes over a token's heads, as many as
 // leave 8192 waves (two for each slot of the GPU at a register count of 128).
-// many: several tokens fit a wave, and there are more than the GPU's 1024
-// SIMDs (of a few, the latency of one counts).
+// many: several tokens fit a wave, and there are so many of them that it pays
+// (one head of 128 in bfloat16: 2048 tokens 4.6 us alone, 6.4 together; 4096
+// 6.0 and 6.5, 2 heads of 64 6.1 and 5.3; 16384 14 and 7).
 static unsigned rotary_blocks(RotArgs &a, int dtype, bool paired, bool back, int heads, long long most, bool &many)
 {
     const int units = rot_units(a.size, a.part, paired, rot_width(dtype, back));
@@ -395,7 +396,7 @@ static unsigned rotary_blocks(RotArgs &a, int dtype, bool paired, bool back, int
     const int all = (heads + (64 >> a.lanes_log2) - 1) >> (6 - a.lanes_log2);
     a.passes = (int)std::max<long long>(1, std::min<long long>(all, (long long)a.rows * all / 8192));
     const int groups = (64 >> a.lanes_log2) / heads;  // (of the side with more heads)
-    many = groups > 1 && a.rows >= 1024;
+    many = groups > 1 && a.rows >= 4096;
     const long long waves = many ? ((long long)a.rows + groups - 1) / groups : (long long)a.rows * ((all + a.passes - 1) / a.passes);
     // (in rounds of equal length)
     const long long blocks = (waves + kRotWaves - 1) / kRotWaves, rounds = (blocks + most - 1) / most;

@@ -220,8 +220,8 @@ def test_rows_past_one_turn_of_the_blocks():
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("norm", [False, True])
-@pytest.mark.parametrize("shape", [((1025,), 1, 1, 2, 2), ((3, 701), 2, 1, 20, 8), ((2, 1100), 1, 1, 64, 64), ((1500,), 3, 1, 7, 6),
-                                   ((1037,), 2, 2, 32, 30), ((2049,), 5, 1, 16, 16), ((1100,), 1, 3, 128, 96)], ids=str)
+@pytest.mark.parametrize("shape", [((4097,), 1, 1, 2, 2), ((3, 1401), 2, 1, 20, 8), ((2, 2200), 1, 1, 64, 64), ((4500,), 3, 1, 7, 6),
+                                   ((4099,), 2, 2, 32, 30), ((4200,), 5, 1, 16, 16), ((4100,), 1, 3, 128, 96)], ids=str)
 def test_tokens_that_share_a_wave(shape, norm, interleaved, dtype):
     test_both_directions(shape, norm, interleaved, dtype)
 
@@ -229,7 +229,7 @@ def test_tokens_that_share_a_wave(shape, norm, interleaved, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_tokens_together_and_in_parts(dtype):
     """Many tokens' values and gradients, both sides' in one call, are those of parts of them, which go another way."""
-    plan, n = Rotary(12), 1500
+    plan, n = Rotary(12), 4500
     q, k, s = values((n, 3, 18), dtype, 1)[0], values((n, 1, 18), dtype, 2)[0], values((18,), dtype, 3, 0.1, 1.0)[0]
     a, b = values((n, 3, 18), dtype, 4)[0], values((n, 1, 18), dtype, 5)[0]
 
@@ -239,7 +239,7 @@ def test_tokens_together_and_in_parts(dtype):
         ((u * a.slice([lo, hi])).sum() + (v * b.slice([lo, hi])).sum()).backward()
         return [t.toBits() for t in (u, v, x.grad(), y.grad())]
     whole = run(0, n, None)
-    for lo, hi in ((0, 500), (500, 1000), (1000, n)):
+    for lo, hi in ((0, 1500), (1500, 3000), (3000, n)):
         part = run(lo, hi, CudaArray.fromNumpy(np.arange(lo, hi, dtype=np.int32)))
         assert all(np.array_equal(w[lo:hi], p) for w, p in zip(whole, part))
 
