@@ -15,15 +15,16 @@ __device__ __forceinline__ float gated_sigmoid(float g)
     if constexpr (FAST) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f));
     else return 1.0f / (1.0f + expf(-g));
 }
-// The standard normal's distribution and exp(-g^2 / 2).  FAST: erfc(z) = e^(-z^2)
-// t Q(t) with t = 1 / (1 + 0.44 z), Q fitted to the least relative error,
-// 1.9e-7 for z >= 0; so the small values of negative g keep their digits.
+// The standard normal's distribution and exp(-g^2 / 2), by erfc, so that the
+// small values of negative g keep their digits (1 + erf has none left below
+// -6).  FAST: erfc(z) = e^(-z^2) t Q(t) with t = 1 / (1 + 0.44 z), Q fitted to
+// the least relative error, 1.9e-7 for z >= 0.
 template <bool FAST>
 __device__ __forceinline__ float gated_below(float g, float &bell)
 {
     if constexpr (!FAST) {
         bell = expf(-0.5f * g * g);
-        return 0.5f * (1.0f + erff(g * 0.707106781f));
+        return 0.5f * erfcf(g * -0.707106781f);
     } else {
         bell = __builtin_amdgcn_exp2f(g * g * -0.72134752f);
         const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(g), 0.44f * 0.707106781f, 1.0f));
