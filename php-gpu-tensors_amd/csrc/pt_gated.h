@@ -90,7 +90,7 @@ __device__ __forceinline__ void gated_slope(int act, float g, float &value, floa
     default: {
         const float s = gated_sigmoid<FAST>(g);
         value = s;
-        slope = s * (1.0f - s);
+        slope = s * gated_sigmoid<FAST>(-g);  // (1 - s has no digits left where g is large)
     }
     }
 }

@@ -67,7 +67,7 @@ def unit(m, f, dtype, sizes):
 # few rows, and more, which take other kernels
 @pytest.mark.parametrize("rows", [24, 200])
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("name", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("name", ["silu", "gelu", "relu", "sigmoid"])
 def test_activations_keep_their_digits(name, dtype, rows):
     def sizes(rng, shape):
         return rng.uniform(-14, 14, shape)
