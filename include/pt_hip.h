@@ -411,8 +411,10 @@ pt_status pt_gated(const pt_gated_desc *desc, const void *x, const void *gate, c
 /* Gradients, contiguous and of the dtype, for the upstream gradient `grad`
  * (contiguous like h, float32 or the dtype): dx, and dgate with dup; dx may
  * be NULL, or dgate and dup both.  In 16 bits the gradients of both
- * products are rounded to the dtype for the products that follow.  Results do not depend
- * on timing. */
+ * products are rounded to the dtype for the products that follow; in float16
+ * they are multiplied by a power of two for each row (dx) or column (dgate,
+ * dup) around that, so their own size is float32's: only the results have to
+ * fit float16.  Results do not depend on timing. */
 pt_status pt_gated_backward(const pt_gated_desc *desc, const void *x, const void *gate, const void *up, const void *kept,
                             const void *grad, int grad_dtype, void *dx, void *dgate, void *dup, pt_stream_t stream);
 

@@ -123,6 +123,18 @@ __device__ __forceinline__ void gated_keep(void *kept, long long n, long long i,
     }
 }
 
+// float16 gradients: dg and du leave float16's range where their products with
+// the operands do not (an upstream gradient of a mean, a large product), so
+// they are multiplied by powers of two that take the largest of a row (for
+// dx) or of a column (for dgate and dup) into [2^14, 2^15), and the sums are
+// multiplied back in float32.  What is below 2^-29 of that largest one has
+// fewer than float16's digits, within 2^-39 of it.  (bfloat16 has float32's
+// range.)  Shifts past these bounds change no float16 result.
+__device__ __forceinline__ int gated_shift(float top)
+{
+    return top > 0.0f ? min(14 + 127 - (int)(__float_as_uint(top) >> 23), 100) : 0;
+}
+
 // What a pair of products is stored as: act(P0) P1, that and both products as
 // the gradient keeps them (c1), both products (c1, c2), or fp32 parts of a
 // split contraction.
@@ -140,6 +152,8 @@ struct PairArgs {
     int n_out;       // columns that are stored (columns form: N is a multiple of 8)
     void *c0, *c1, *c2;  // results, contiguous
     float *parts;    // [split][1 or 2][M][n_out]
+    const int8_t *shift;  // float16 gradients: the power of two that A's row (sum form, [M]) or B's column (columns form,
+                          // of both matrices, [2][n_out]) was multiplied by
     int act;
     int tiles_m, tiles_n, split, stages;  // stages: 64-wide K stages of a split's share
 };

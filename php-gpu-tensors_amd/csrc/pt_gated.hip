@@ -308,11 +308,37 @@ __device__ __forceinline__ void gated_transpose(const uint16_t *from, uint16_t *
     }
 }
 
-// dg and du from the upstream gradient and both products, into rows `pitch`
-// elements apart from d and d + second on, zeros in columns `cols` to
-// `padded` - 1.  A thread takes 8 columns.  Blocks from `slopes` on transpose
-// x beside it, one 64 x 64 tile each, in one launch less.  HBM-bound: 8192 x
-// 8192 in bfloat16 with a transpose of 8192 x 2048 160-170 us, 5.3 TB/s.
+// dg and du of 8 elements from `from` on, `live` of them, from the upstream
+// gradient and both products; the others are zeros.
+template <int DT, int GDT>
+__device__ __forceinline__ void gd_slopes(const void *kept, const void *grad, int act, long long plane, long long from, int live,
+                                          float (&dg)[8], float (&du)[8])
+{
+    using S = typename GE<DT>::S;
+    float g[8], u[8], dh[8];
+    if constexpr (DT == PT_FLOAT32) {
+        gd_load<DT, 8>((const S *)kept + from, live, g);
+        gd_load<DT, 8>((const S *)kept + plane + from, live, u);
+    } else {
+        gd_load_kept(kept, plane, 0, from, live, g);
+        gd_load_kept(kept, plane, 1, from, live, u);
+    }
+    gd_load<GDT, 8>((const typename GE<GDT>::S *)grad + from, live, dh);
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        float value, slope;
+        gated_slope<DT != PT_FLOAT32>(act, g[k], value, slope);
+        dg[k] = k < live ? dh[k] * u[k] * slope : 0.0f;
+        du[k] = k < live ? dh[k] * value : 0.0f;
+    }
+}
+
+// dg and du into rows `pitch` elements apart from d and d + second on, zeros
+// in columns `cols` to `padded` - 1.  A thread takes 8 columns.  Blocks from
+// `slopes` on transpose x beside it, one 64 x 64 tile each, in one launch
+// less.  HBM-bound: 8192 x 8192 in bfloat16 with a transpose of 8192 x 2048
+// 160-170 us, 5.3 TB/s.  float16: twice, multiplied by the rows' powers of
+// two into d and by the columns' into e (either may be null): 200 us.
 struct SlopeArgs {
     const void *kept, *grad;
     void *d;
@@ -322,6 +348,8 @@ struct SlopeArgs {
     const uint16_t *x;       // [rows][inner]
     uint16_t *xt;            // [inner][across]
     int inner, across;
+    void *e;
+    const int8_t *row_shift, *column_shift;  // [rows], [2][cols] and 8 bytes more
 };
 template <int DT, int GDT>
 __global__ __launch_bounds__(256) void k_gated_slope(SlopeArgs a)
@@ -337,40 +365,154 @@ __global__ __launch_bounds__(256) void k_gated_slope(SlopeArgs a)
     const long long total = (long long)a.rows * packs, plane = (long long)a.rows * a.cols;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)a.slopes * 256) {
         const long long row = i / packs;
-        const int c = (int)(i - row * packs) * 8, live = min(8, a.cols - c);
-        const long long from = row * a.cols + c;
-        float g[8], u[8], dh[8];
-        if constexpr (DT == PT_FLOAT32) {
-            gd_load<DT, 8>((const S *)a.kept + from, live, g);
-            gd_load<DT, 8>((const S *)a.kept + plane + from, live, u);
-        } else {
-            gd_load_kept(a.kept, plane, 0, from, live, g);
-            gd_load_kept(a.kept, plane, 1, from, live, u);
-        }
-        gd_load<GDT, 8>((const typename GE<GDT>::S *)a.grad + from, live, dh);
-        S dg[8], du[8];
+        const int c = (int)(i - row * packs) * 8, live = min(8, a.cols - c), room = min(8, a.padded - c);
+        float dg[8], du[8];
+        gd_slopes<DT, GDT>(a.kept, a.grad, a.act, plane, row * a.cols + c, live, dg, du);
+        auto store = [&](void *d, const float (&p)[8], const float (&q)[8]) {
+            S v[8], w[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            float value, slope;
-            gated_slope<DT != PT_FLOAT32>(a.act, g[k], value, slope);
-            dg[k] = DType<DT>::from_c(k < live ? dh[k] * u[k] * slope : 0.0f);
-            du[k] = DType<DT>::from_c(k < live ? dh[k] * value : 0.0f);
-        }
-        S *to = (S *)a.d + row * a.pitch + c;
-        const int room = min(8, a.padded - c);
-        if (room == 8) {
+            for (int k = 0; k < 8; k++) {
+                v[k] = DType<DT>::from_c(p[k]);
+                w[k] = DType<DT>::from_c(q[k]);
+            }
+            S *to = (S *)d + row * a.pitch + c;
+            if (room == 8) {
 #pragma unroll
-            for (int q = 0; q < 8 / GE<DT>::PK; q++) {
-                *(gd_u32x4 *)(to + q * GE<DT>::PK) = *(gd_u32x4 *)(dg + q * GE<DT>::PK);
-                *(gd_u32x4 *)(to + a.second + q * GE<DT>::PK) = *(gd_u32x4 *)(du + q * GE<DT>::PK);
+                for (int k = 0; k < 8; k += GE<DT>::PK) {
+                    *(gd_u32x4 *)(to + k) = *(gd_u32x4 *)(v + k);
+                    *(gd_u32x4 *)(to + a.second + k) = *(gd_u32x4 *)(w + k);
+                }
+            } else {
+                for (int k = 0; k < room; k++) {
+                    to[k] = v[k];
+                    to[a.second + k] = w[k];
+                }
+            }
+        };
+        if constexpr (DT == PT_FLOAT16) {
+            float p[8], q[8];
+            if (a.d) {
+                const int shift = a.row_shift[row];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    p[k] = ldexpf(dg[k], shift);
+                    q[k] = ldexpf(du[k], shift);
+                }
+                store(a.d, p, q);
+            }
+            if (a.e) {
+                // (past the last column: another shift of a zero)
+                typedef int8_t shifts __attribute__((ext_vector_type(8), aligned(1)));
+                const shifts x = *(const shifts *)(a.column_shift + c), y = *(const shifts *)(a.column_shift + a.cols + c);
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    p[k] = ldexpf(dg[k], x[k]);
+                    q[k] = ldexpf(du[k], y[k]);
+                }
+                store(a.e, p, q);
             }
         } else {
-            for (int k = 0; k < room; k++) {
-                to[k] = dg[k];
-                to[a.second + k] = du[k];
-            }
+            store(a.d, dg, du);
         }
     }
+}
+
+// float16: the largest finite |dg| and |du| of each row and of each column (the
+// two apart), of the rows' and columns' parts that a block takes; the second
+// kernel takes the largest over the parts, in any order the same.  A wave walks
+// `steps` rows, 512 columns of each (fewer columns: as many rows at once as
+// fill it), so a row is reduced over its lanes and a column stays in one.
+// 8192 x 8192: 119-124 us (4.4 TB/s) and 5.
+__device__ __forceinline__ float gd_top(float v, int log2)  // over 2^log2 lanes (uniform), by DPP up to 16
+{
+    auto with = [](float x, auto CTRL) {
+        return fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(CTRL)::value, 0xF, 0xF, false)));
+    };
+    if (log2 == 6) return wave_all(v, FMax{});
+    if (log2 > 0) v = with(v, IC<0xB1>{});
+    if (log2 > 1) v = with(v, IC<0x4E>{});
+    if (log2 > 2) v = with(v, IC<0x141>{});
+    if (log2 > 3) v = with(v, IC<0x140>{});
+    if (log2 > 4) v = fmaxf(v, __shfl_xor(v, 16, PT_WAVE));
+    return v;
+}
+struct RangeArgs {
+    const void *kept, *grad;
+    int rows, cols, act;
+    int lanes_log2, steps;   // lanes of a row; a wave's steps
+    float *row_part;         // [gridDim.x][rows], or null
+    float *column_part;      // [gridDim.y][2][cols], or null
+};
+template <int GDT>
+__global__ __launch_bounds__(256) void k_gated_range(RangeArgs a)
+{
+    __shared__ float box[4][16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lanes = 1 << a.lanes_log2, at_once = 64 >> a.lanes_log2;
+    const int c = (blockIdx.x * lanes + (lane & (lanes - 1))) * 8, live = max(0, min(8, a.cols - c));
+    const long long plane = (long long)a.rows * a.cols;
+    const long long r0 = ((long long)blockIdx.y * 4 + wave) * a.steps * at_once + (lane >> a.lanes_log2);
+    float top[16];
+#pragma unroll
+    for (int k = 0; k < 16; k++) top[k] = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < a.steps; s++) {
+        const long long row = r0 + (long long)s * at_once;
+        const int n = row < a.rows ? live : 0;
+        float dg[8], du[8], most = 0.0f;
+        gd_slopes<PT_FLOAT16, GDT>(a.kept, a.grad, a.act, plane, n ? row * a.cols + c : 0, n, dg, du);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float p = fabsf(dg[k]), q = fabsf(du[k]);
+            top[k] = fmaxf(top[k], p < INFINITY ? p : 0.0f);
+            top[8 + k] = fmaxf(top[8 + k], q < INFINITY ? q : 0.0f);
+            most = fmaxf(most, fmaxf(p < INFINITY ? p : 0.0f, q < INFINITY ? q : 0.0f));
+        }
+        most = gd_top(most, a.lanes_log2);
+        if (a.row_part && !(lane & (lanes - 1)) && row < a.rows) a.row_part[(long long)blockIdx.x * a.rows + row] = most;
+    }
+    if (!a.column_part) return;  // uniform
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        for (int m = lanes; m < 64; m <<= 1) top[k] = fmaxf(top[k], __shfl_xor(top[k], m, PT_WAVE));
+        box[wave][k][lane] = top[k];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * lanes; i += 256) {
+        const int j = i / (8 * lanes), at = i - j * 8 * lanes, column = blockIdx.x * lanes * 8 + at, k = j * 8 + at % 8;
+        if (column >= a.cols) continue;
+        float t = box[0][k][at / 8];
+        for (int w = 1; w < 4; w++) t = fmaxf(t, box[w][k][at / 8]);
+        a.column_part[((long long)blockIdx.y * 2 + j) * a.cols + column] = t;
+    }
+}
+
+// The powers of two from the parts' largest values: items 0 to rows - 1 are
+// rows, the 2 cols behind them columns; a block takes 64, each of its waves
+// every 16th part.
+struct ShiftArgs {
+    const float *row_part, *column_part;
+    int rows, columns;   // 0: none wanted
+    int row_parts, column_parts;
+    int8_t *shift;       // [rows + columns]
+};
+constexpr int kShiftWaves = 16;
+__global__ __launch_bounds__(64 * kShiftWaves) void k_gated_shift(ShiftArgs a)
+{
+    __shared__ float box[kShiftWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long items = (long long)a.rows + a.columns, i = (long long)blockIdx.x * 64 + lane;
+    const bool row = i < a.rows;
+    const float *from = row ? a.row_part + i : a.column_part + (i - a.rows);
+    const int parts = i < items ? (row ? a.row_parts : a.column_parts) : 0, step = row ? a.rows : a.columns;
+    float top = 0.0f;
+#pragma unroll 8
+    for (int k = wave; k < parts; k += kShiftWaves) top = fmaxf(top, from[(long long)k * step]);
+    box[wave][lane] = top;
+    __syncthreads();
+    if (wave || i >= items) return;
+#pragma unroll
+    for (int w = 1; w < kShiftWaves; w++) top = fmaxf(top, box[w][lane]);
+    a.shift[i] = (int8_t)gated_shift(top);
 }
 
 // ------------------------------------------------------------- the calls
@@ -380,7 +522,7 @@ static unsigned grid_for(long long items) { return (unsigned)std::min<long long>
 // Scratch of one call, given back in the stream's order.
 struct GatedScratch {
     hipStream_t s;
-    void *held[8];
+    void *held[10];
     int count = 0;
     explicit GatedScratch(hipStream_t stream) : s(stream) {}
     ~GatedScratch()
@@ -550,7 +692,16 @@ static pt_status gated_backward_f32(const pt_gated_desc *d, const float *x, cons
     const long long pitch = ring ? 2 * F : F, second = ring ? F : ((long long)M * F + 3) / 4 * 4;
     float *dg = nullptr, *both = nullptr;
     PT_TRY(scratch.take((void **)&dg, 2 * (ring ? (size_t)M * F : (size_t)second) * sizeof(float)));
-    SlopeArgs a = {kept, grad, dg, second, M, F, F, (int)pitch, d->activation, grid_for((long long)M * ((F + 7) / 8)), nullptr, nullptr, 0, 0};
+    SlopeArgs a = {};
+    a.kept = kept;
+    a.grad = grad;
+    a.d = dg;
+    a.second = second;
+    a.rows = M;
+    a.cols = a.padded = F;
+    a.pitch = (int)pitch;
+    a.act = d->activation;
+    a.slopes = grid_for((long long)M * ((F + 7) / 8));
     k_gated_slope<PT_FLOAT32, PT_FLOAT32><<<a.slopes, 256, 0, s>>>(a);
     const unsigned blocks = grid_for((long long)K * F / 4);
     if (ring) PT_TRY(scratch.take((void **)&both, (size_t)K * 2 * F * sizeof(float)));
@@ -587,19 +738,69 @@ static pt_status gated_backward_f32(const pt_gated_desc *d, const float *x, cons
     return PT_OK;
 }
 
+// The powers of two of float16 gradients, for dx and for the weights' where
+// wanted.  A wave walks as many rows as leave 2048 blocks, 16 at most, but so
+// many that a column has no more than 256 parts.
+static pt_status gated_shifts(SlopeArgs &s, int grad_dtype, bool rows, bool columns, GatedScratch &scratch)
+{
+    RangeArgs a = {};
+    a.kept = s.kept;
+    a.grad = s.grad;
+    a.rows = s.rows;
+    a.cols = s.cols;
+    a.act = s.act;
+    const int packs = (s.cols + 7) / 8;
+    while (a.lanes_log2 < 6 && 1 << a.lanes_log2 < packs) a.lanes_log2++;
+    const int at_once = 4 * (64 >> a.lanes_log2), chunks = (packs + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
+    const int turns = (s.rows + at_once - 1) / at_once;
+    a.steps = (int)std::max<long long>((turns + 255) / 256, std::min<long long>((long long)turns * chunks / 2048, 16));
+    const int blocks = (turns + a.steps - 1) / a.steps;
+    int8_t *shift = nullptr;
+    const size_t many = (rows ? (size_t)s.rows : 0) + (columns ? 2 * (size_t)s.cols : 0);
+    PT_TRY(scratch.take((void **)&shift, many + 8));
+    const size_t row_parts = rows ? (size_t)chunks * s.rows : 0, column_parts = columns ? (size_t)blocks * 2 * s.cols : 0;
+    float *parts = nullptr;
+    PT_TRY(scratch.take((void **)&parts, (row_parts + column_parts) * sizeof(float)));
+    if (rows) a.row_part = parts;
+    if (columns) a.column_part = parts + row_parts;
+    const dim3 grid(chunks, blocks);
+    if (grad_dtype == PT_FLOAT16) k_gated_range<PT_FLOAT16><<<grid, 256, 0, scratch.s>>>(a);
+    else k_gated_range<PT_FLOAT32><<<grid, 256, 0, scratch.s>>>(a);
+    const ShiftArgs t = {a.row_part, a.column_part, rows ? s.rows : 0, columns ? 2 * s.cols : 0, chunks, blocks, shift};
+    k_gated_shift<<<(unsigned)((many + 63) / 64), 64 * kShiftWaves, 0, scratch.s>>>(t);
+    s.row_shift = shift;
+    s.column_shift = shift + t.rows;
+    return PT_OK;
+}
+
 static pt_status gated_backward_run(const pt_gated_desc *d, const void *x, const void *gate, const void *up, const void *kept,
                                     const void *grad, int grad_dtype, void *dx, void *dgate, void *dup, pt_stream_t stream)
 {
     hipStream_t s = stream_of(stream);
     GatedScratch scratch(s);
     const int M = d->rows, K = d->inner, F = d->outer, pitch = round8(F);
+    const bool half = d->dtype == PT_FLOAT16;
     if (d->dtype == PT_FLOAT32)
         return gated_backward_f32(d, (const float *)x, (const float *)gate, (const float *)up, kept, grad, (float *)dx,
                                   (float *)dgate, (float *)dup, scratch, stream);
-    uint16_t *dg = nullptr;
+    // dg and du for dx, and for the weights' gradients: the same but in float16
+    uint16_t *dg = nullptr, *dw = nullptr;
     const long long second = (long long)M * pitch;
-    PT_TRY(scratch.take((void **)&dg, (size_t)second * 2 * 2));
-    SlopeArgs a = {kept, grad, dg, second, M, F, pitch, pitch, d->activation, grid_for((long long)M * (pitch / 8)), nullptr, nullptr, 0, 0};
+    if (dx || !half) PT_TRY(scratch.take((void **)&dg, (size_t)second * 2 * 2));
+    if (dgate && half) PT_TRY(scratch.take((void **)&dw, (size_t)second * 2 * 2));
+    SlopeArgs a = {};
+    a.kept = kept;
+    a.grad = grad;
+    a.d = dg;
+    a.e = dw;
+    a.second = second;
+    a.rows = M;
+    a.cols = F;
+    a.padded = a.pitch = pitch;
+    a.act = d->activation;
+    a.slopes = grid_for((long long)M * (pitch / 8));
+    if (half) PT_TRY(gated_shifts(a, grad_dtype, dx, dgate, scratch));
+    else dw = dg;
     unsigned blocks = a.slopes;
     if (dgate) {
         a.x = (const uint16_t *)x;
@@ -628,6 +829,7 @@ static pt_status gated_backward_run(const pt_gated_desc *d, const void *x, const
         g.N = g.n_out = K;
         g.K = pitch;
         g.c0 = dx;
+        g.shift = a.row_shift;
         pair_plan(g, false, tm);
         if (g.split > 1) PT_TRY(scratch.take((void **)&g.parts, (size_t)g.split * M * K * sizeof(float)));
         launch_pair_sum(g, d->dtype, tm, s);
@@ -637,13 +839,14 @@ static pt_status gated_backward_run(const pt_gated_desc *d, const void *x, const
         g.a0 = a.xt;
         g.lda = g.K = a.across;
         g.kb = M;
-        g.b0 = dg;
-        g.b1 = dg + second;
+        g.b0 = dw;
+        g.b1 = dw + second;
         g.ldb = g.N = pitch;
         g.n_out = F;
         g.M = K;
         g.c1 = dgate;
         g.c2 = dup;
+        g.shift = a.column_shift;
         pair_plan(g, true, tm);
         if (g.split > 1) PT_TRY(scratch.take((void **)&g.parts, (size_t)g.split * 2 * K * F * sizeof(float)));
         launch_pair_columns(g, d->dtype, tm, GATED_BOTH, s);

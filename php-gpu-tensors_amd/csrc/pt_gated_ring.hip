@@ -312,6 +312,16 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
     };
     const long long plane = (long long)g.M * g.n_out;
     float *parts = STORE == GATED_PARTS ? g.parts + (long long)blockIdx.y * (SUM ? 1 : 2) * plane : nullptr;
+    // float16 gradients: multiplied back
+    constexpr bool SHIFTED = DT == PT_FLOAT16 && (SUM ? STORE != GATED_PARTS : STORE == GATED_BOTH);
+    int back[2][8];
+    if constexpr (SHIFTED && !SUM)
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int n = min(n0 + wn * 32 + lane % 4 * 8 + k, g.n_out - 1);
+            back[0][k] = -g.shift[n];
+            back[1][k] = -g.shift[g.n_out + n];
+        }
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         // (a wave's LDS accesses stay in order)
@@ -326,6 +336,14 @@ __global__ __launch_bounds__(512, 1) void k_pair(PairArgs g)
             take(box[1], h, q);
             const int m = m0 + wm * WTM + i * 32 + h * 16 + lane / 4;
             if (m >= g.M) continue;
+            if constexpr (SHIFTED) {
+                const int row = SUM ? -g.shift[m] : 0;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    p[k] = ldexpf(p[k], SUM ? row : back[0][k]);
+                    q[k] = ldexpf(q[k], SUM ? row : back[1][k]);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < (SUM ? 2 : 1); j++) {
                 const int n = n0 + (SUM ? wn * 64 + j * 32 : wn * 32) + lane % 4 * 8;
@@ -388,6 +406,17 @@ __global__ __launch_bounds__(256) void k_pair_join(PairArgs g)
                     p[e] += from[0];
                     if (!SUM) q[e] += from[plane];
                 }
+        }
+        if constexpr (DT == PT_FLOAT16 && (SUM || STORE == GATED_BOTH)) {
+            long long row = i / g.n_out;
+            int column = (int)(i - row * g.n_out);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (e >= live) continue;
+                p[e] = ldexpf(p[e], -g.shift[SUM ? row : column]);
+                if (!SUM) q[e] = ldexpf(q[e], -g.shift[g.n_out + column]);
+                if (++column == g.n_out) column = 0, row++;
+            }
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {

@@ -655,7 +655,8 @@ class CudaArray:
         (with the error function), "relu" or "sigmoid".  Both products are
         taken through the activation in float32 and the result is rounded
         once.  The gradients have their operands' dtypes; for them both
-        products are kept, in 24 bits for 16-bit operands."""
+        products are kept, in 24 bits for 16-bit operands.  In float16 only the
+        gradients themselves have to fit the type, not those of the products."""
         if not isinstance(gate, CudaArray) or not isinstance(up, CudaArray):
             raise InvalidArgumentException("gatedProjection() expects CudaArray matrices")
         act = self.ACTIVATIONS.get(activation) if isinstance(activation, str) else None

@@ -1,10 +1,12 @@
-"""CudaArray.gatedProjection and its gradients where values are small: the activations and their slopes relative to
-themselves, element by element.  U: half a step of float32, HALF: of the operands' type."""
+"""CudaArray.gatedProjection and its gradients where values are small or large: the activations and their slopes relative
+to themselves, element by element, and float16 gradients whose inner values leave float16's range.  U: half a step of
+float32, HALF: of the operands' type."""
 import math
 
 import numpy as np
 import pytest
 
+import test_gpu_gated
 from phptensors import CudaArray
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +82,113 @@ def test_activations_keep_their_digits(name, dtype, rows):
     for got, (want, off) in ((gate, (s * u, (s_off + 2 * U * np.abs(s)) * u)), (up, (v, v_off + U * np.abs(v)))):
         # dg and du are rounded to the type once, and the sum of that one term again, which leaves it
         within(got.grad(), want, off, dtype, "gradient")
+
+
+# ------------------------------------------- float16: gradients of both products past float16's range
+# The gradients are linear in the upstream one, so rows (and columns) of that which are scaled by powers of two scale the
+# exact rows of dx (columns of dgate and dup) and all of their bounds, those of test_gpu_gated.reference for upstream
+# gradients of order 1.  Its 2^-25 for each of dg and du stays far above what they are held with: 2^-39 of their row's or
+# column's largest, which is below 2^7 here.
+# rows, inner, outer: few and more, odd widths, several chunks of columns, split contractions of both, tall and narrow
+RANGED = [(24, 64, 40), (300, 40, 77), (5, 48, 1203), (24, 64, 8000), (2100, 40, 24), (70001, 8, 9), (1, 9, 3)]
+
+
+def ranged(shape, x_scale=1.0, w_scale=1.0, up_scale=1.0):
+    """(arrays, float64 values) of x, gate and up in float16, and upstream values of order 1."""
+    m, k, f = shape
+    rng = np.random.default_rng(11)
+    made = [CudaArray.fromNumpy((rng.standard_normal(s) * c).astype(np.float32), "float16").requiresGrad()
+            for s, c in (((m, k), x_scale), ((k, f), w_scale * k ** -0.5), ((k, f), w_scale * up_scale * k ** -0.5))]
+    return made, [t.toNumpy().astype(np.float64).reshape(t.getShape()) for t in made], \
+        rng.standard_normal((m, f)).astype(np.float32).astype(np.float64)
+
+
+def gradients(made, dh, dtype="float32"):
+    for t in made:
+        t.zeroGrad()
+    h = made[0].gatedProjection(made[1], made[2], "silu")
+    g = CudaArray.fromNumpy(np.asarray(dh, np.float32), dtype)
+    if dtype == "float16":
+        h.backward(g)
+    else:
+        (h * g).sum().backward()
+    return [t.grad() for t in made]
+
+
+def ranged_close(got, want, scales, what):
+    for t, n, c in zip(got, ("dx", "dgate", "dup"), scales):
+        if c is not None:
+            assert t.getDtype() == "float16"
+            within(t, want[n][0] * c, want[n][1] * c, "float16", (what, n))
+
+
+# (past 65504 only the results that float16 holds)
+@pytest.mark.parametrize("power,x_scale,wanted", [(-27, 2.0 ** 9, (1, 1, 1)), (-27, 2.0 ** -12, (1, 1, 1)), (-40, 2.0 ** 12, (1, 1, 1)),
+                                                  (15, 2.0 ** -9, (0, 1, 1)), (15, 2.0 ** 9, (1, 0, 0))])
+@pytest.mark.parametrize("shape", RANGED, ids=str)
+def test_float16_upstream_gradients_of_any_size(shape, power, x_scale, wanted):
+    made, values, dh = ranged(shape, x_scale, 1 / x_scale)
+    got = gradients(made, dh * 2.0 ** power)
+    want = test_gpu_gated.reference(*values, "silu", "float16", dh)
+    ranged_close(got, want, [2.0 ** power if w else None for w in wanted], "scaled")
+
+
+@pytest.mark.parametrize("shape", RANGED, ids=str)
+def test_float16_rows_and_columns_of_their_own_size(shape):
+    """Small rows keep dx, and small columns dgate and dup, beside large ones; some have no gradient at all."""
+    m, _, f = shape
+    rng = np.random.default_rng(12)
+    for axis, n, x_scale in ((0, m, 2.0 ** -8), (1, f, 2.0 ** 3)):
+        made, values, dh = ranged(shape, x_scale, 1 / x_scale)
+        c = 2.0 ** rng.integers(-24, 2, n).astype(np.float64)
+        c[rng.random(n) < 0.1] = 0.0
+        c = c[:, None] if axis == 0 else c[None, :]
+        got = gradients(made, dh * c)
+        want = test_gpu_gated.reference(*values, "silu", "float16", dh)
+        ranged_close(got, want, (c, None, None) if axis == 0 else (None, c, c), axis)
+        # each gradient alone is what it is among all
+        for i, t in enumerate(made):
+            for o in made:
+                o.requiresGrad(o is t)
+            alone = gradients(made, dh * c)[i]
+            assert np.array_equal(alone.toBits(), got[i].toBits())
+        for o in made:
+            o.requiresGrad()
+
+
+@pytest.mark.parametrize("shape", RANGED[:5], ids=str)
+@pytest.mark.parametrize("value", [np.inf, np.nan, 1e30, -3e38])
+def test_one_float16_outlier_stays_in_its_row_and_column(shape, value):
+    m, _, f = shape
+    made, values, dh = ranged(shape)
+    want = test_gpu_gated.reference(*values, "silu", "float16", dh)
+    row, column = m // 2, f - 2
+    dh[row, column] = value
+    dx, *dw = gradients(made, dh)
+    rows, columns = np.arange(m) != row, np.arange(f) != column
+    for t, n, keep in ((dx, "dx", np.s_[rows]), (dw[0], "dgate", np.s_[:, columns]), (dw[1], "dup", np.s_[:, columns])):
+        v = t.toNumpy().reshape(t.getShape()).astype(np.float32)
+        if v[keep].size:
+            within(CudaArray.fromNumpy(np.ascontiguousarray(v[keep]), "float16"), want[n][0][keep], want[n][1][keep], "float16", n)
+        # (a float32 product with 3e38 may end before infinity, its share of a float16 result does not)
+        assert not np.isfinite(v[~rows] if n == "dx" else v[:, ~columns]).any()
+
+
+def test_float16_products_of_large_values():
+    """dg past 65504 from float16 operands and upstream gradients, dx and dgate within it."""
+    for shape in ((24, 64, 16), (300, 64, 16)):
+        made, values, dh = ranged(shape, 2.0 ** -6, 2.0 ** -3, 2.0 ** 14)
+        dh = (dh * 2.0 ** 11).astype(np.float16).astype(np.float64)
+        want = test_gpu_gated.reference(*values, "silu", "float16", dh)
+        x, gate, up = values
+        g, u = x @ gate, x @ up
+        assert (np.abs(dh * u) * 0.5).max() > 70000 and max(np.abs(want[n][0]).max() for n in ("dx", "dgate", "dup")) < 60000
+        ranged_close(gradients(made, dh, "float16"), want, (1, 1, 1), shape)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_no_upstream_gradient(dtype):
+    for m in (3, 100):
+        x, a, b = (CudaArray.ones(s, dtype).requiresGrad() for s in ((m, 24), (24, 33), (24, 33)))
+        x.gatedProjection(a, b).backward(CudaArray.zeros([m, 33], dtype))
+        assert not any(t.grad().toNumpy().any() for t in (x, a, b))
