@@ -39,6 +39,8 @@ namespace pt {
 constexpr int kAdamTensors = 64;   // a launch: 3.4 KiB of arguments
 constexpr int kAdamRounds = 2;     // 256 elements that a wave takes at once
 constexpr int kAdamBlock = 4 * kAdamRounds * 256;  // elements
+constexpr long long kAdamMost = (1 << 24) - 1;     // blocks of a launch: below 2^32 threads, of which HIP drops the rest
+constexpr long long kAdamPart = 1ll << 31;         // elements of a tensor that a launch's table takes as one
 
 struct AdamTensor {
     const void *p0, *g;
@@ -374,18 +376,21 @@ pt_status pt_adamw(const pt_adamw_desc *d, const pt_adamw_tensor *tensors, int c
     bool launched = false;
     for (int i = 0; i < count; i++) {
         const pt_adamw_tensor &t = tensors[i];
-        if (!t.n) continue;
-        const long long more = ((long long)t.n + kAdamBlock - 1) / kAdamBlock;
-        if (a.count == kAdamTensors || blocks + more > 0x7fffffff) {
-            launch((unsigned)blocks);
-            a.count = 0;
-            blocks = 0;
-            launched = true;
+        for (long long from = 0; from < (long long)t.n; from += kAdamPart) {
+            const long long n = std::min((long long)t.n - from, kAdamPart), more = (n + kAdamBlock - 1) / kAdamBlock;
+            if (a.count == kAdamTensors || blocks + more > kAdamMost) {
+                launch((unsigned)blocks);
+                a.count = 0;
+                blocks = 0;
+                launched = true;
+            }
+            auto part = [&](const void *base, int dtype) { return base ? (const char *)base + from * (long long)dtype_size(dtype) : nullptr; };
+            AdamTensor &to = a.t[a.count++];
+            to = {part(t.param, t.param_dtype), part(t.grad, t.grad_dtype), (void *)part(t.new_param, t.param_dtype), n,
+                  (long long)t.at + from, (unsigned)blocks, (uint8_t)t.param_dtype, (uint8_t)t.grad_dtype,
+                  (uint8_t)(t.decay && d->weight_decay > 0.0)};
+            blocks += more;
         }
-        AdamTensor &to = a.t[a.count++];
-        to = {t.param, t.grad, t.new_param, (long long)t.n, (long long)t.at, (unsigned)blocks, (uint8_t)t.param_dtype,
-              (uint8_t)t.grad_dtype, (uint8_t)(t.decay && d->weight_decay > 0.0)};
-        blocks += more;
     }
     if (!blocks && !launched) {
         // no element: the powers go on all the same

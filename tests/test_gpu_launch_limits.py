@@ -1,0 +1,54 @@
+"""AdamW over many tensors of more elements than one launch holds (2^32 threads: 2^35 elements), through the C entry: 150
+GB of the card's 288."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from phptensors import _abi
+from test_gpu_block_sizes import big, end
+
+pytestmark = pytest.mark.gpu
+
+
+def download(pointer, like):
+    out = np.empty_like(like)
+    _abi.check(_abi.load().pt_memcpy_d2h(out.ctypes.data, pointer, out.nbytes, None))
+    return out
+
+
+def test_adamw():
+    """Sixteen tensors of 2^31 elements and one of 700 in 8 bits, moments in place.  All read the same old values and
+    gradients, zeros but for 700 at the end, so each one's last elements step as those alone do."""
+    lib, rng, last, each, many = _abi.load(), np.random.default_rng(3), 700, 2 ** 31, 16
+    p, g = (rng.standard_normal(last).astype(np.float16) for _ in range(2))
+    old, grad = big(each * 2, p), big(each * 2, g)
+
+    def run(sizes):
+        total = sum(-(-n // 256) * 256 for n in sizes)
+        new, m, v = big(sum(sizes) * 2), big(total), big(total)
+        e = [big(total // 256) for _ in range(2)]
+        numbers, draws = _abi.to_device(np.ones(4, np.float32)), _abi.to_device(np.array([7, 0], np.int32))
+        d, t, at, ends = _abi.PtAdamwDesc(), (_abi.PtAdamwTensor * len(sizes))(), 0, []
+        for i, n in enumerate(sizes):
+            skip = (each - n) * 2
+            t[i] = _abi.PtAdamwTensor(old.ptr + skip, grad.ptr + skip, new.ptr + sum(sizes[:i]) * 2, n, at, _abi.FLOAT16,
+                                      _abi.FLOAT16, 1)
+            at += -(-n // 256) * 256
+            ends.append(new.ptr + sum(sizes[:i + 1]) * 2 - p.nbytes)
+        for name, x in dict(bits=8, beta1=0.9, beta2=0.99, epsilon=1e-8, weight_decay=0.1, rate_value=0.1, first=m.ptr,
+                            second=v.ptr, new_first=m.ptr, new_second=v.ptr, power1=numbers.ptr, power2=numbers.ptr + 4,
+                            new_power1=numbers.ptr + 8, new_power2=numbers.ptr + 12, first_exponent=e[0].ptr,
+                            second_exponent=e[1].ptr, new_first_exponent=e[0].ptr, new_second_exponent=e[1].ptr, draws=draws.ptr,
+                            new_draws=draws.ptr + 4).items():
+            setattr(d, name, x)
+        _abi.check(lib.pt_adamw(ctypes.byref(d), t, len(sizes), None))
+        moments = end(m, np.empty(768, np.uint8))
+        return [download(x, p) for x in ends], moments, download(numbers.ptr, np.empty(4, np.float32)), download(
+            draws.ptr, np.empty(2, np.int32))
+    (want,), _, numbers, _ = run([last])
+    got, moments, powers, draws = run([each] * many + [last])
+    assert not np.array_equal(want, p) and all(np.array_equal(x, want) for x in got)
+    assert np.array_equal(powers, numbers) and draws[1] == 8
+    assert (moments[:last] != 0).mean() > 0.9 and not moments[last:].any()
+
