@@ -276,7 +276,7 @@ __global__ __launch_bounds__(256) void k_adamw(AdamArgs a)
     }
 }
 
-// float32 values of 8-bit moments; a wave takes a block of 256, 4 a lane
+// float32 values of 8-bit moments; a wave takes blocks of 256, 4 elements a lane
 __global__ __launch_bounds__(256) void k_adamw_moments(const uint8_t *m, const int8_t *me, const uint8_t *v, const int8_t *ve,
                                                        float *mo, float *vo, long long blocks)
 {
@@ -410,7 +410,7 @@ pt_status pt_adamw_moments(const void *first, const int8_t *first_exponent, cons
         return fail(PT_ERR_INVALID, "8-bit moments miss an operand");
     PT_TRY(ensure_init());
     if (!n) return PT_OK;
-    const unsigned blocks = (unsigned)std::min<size_t>((n / 256 + 3) / 4, 1 << 24);
+    const unsigned blocks = (unsigned)std::min<size_t>((n / 256 + 3) / 4, kAdamMost);
     k_adamw_moments<<<blocks, 256, 0, stream_of(stream)>>>((const uint8_t *)first, first_exponent, (const uint8_t *)second,
                                                            second_exponent, first_values, second_values, (long long)(n / 256));
     return check_hip(hipGetLastError(), "8-bit moments");

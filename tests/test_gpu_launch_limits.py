@@ -1,5 +1,5 @@
-"""AdamW over many tensors of more elements than one launch holds (2^32 threads: 2^35 elements), through the C entry: 150
-GB of the card's 288."""
+"""AdamW over many tensors, and 8-bit moments, of more elements than one launch holds (2^32 threads: 2^35 and 2^34 of
+them), through the C entries: 150 and 155 GB of the card's 288."""
 import ctypes
 
 import numpy as np
@@ -52,3 +52,21 @@ def test_adamw():
     assert np.array_equal(powers, numbers) and draws[1] == 8
     assert (moments[:last] != 0).mean() > 0.9 and not moments[last:].any()
 
+
+def test_moments():
+    lib, n = _abi.load(), 2 ** 34 + 512
+    tail = np.random.default_rng(4).integers(0, 256, 512).astype(np.uint8)
+    code, exponent = big(n, tail), big(n // 256, np.array([3, -5], np.int8))
+    out = [_abi.DeviceBuffer(n * 4) for _ in range(2)]
+    for b in out:
+        _abi.check(lib.pt_memset(b.ptr, 0xFF, n * 4, None))
+
+    def run(code, exponent, values, n):
+        _abi.check(lib.pt_adamw_moments(code, exponent, code, exponent, *values, n, None))
+    run(code.ptr, exponent.ptr, [b.ptr for b in out], n)
+    few = [_abi.DeviceBuffer(512 * 4) for _ in range(2)]
+    run(code.ptr + n - 512, exponent.ptr + n // 256 - 2, [b.ptr for b in few], 512)
+    for a, b in zip(out, few):
+        assert np.array_equal(end(a, np.empty(512, np.float32)), download(b.ptr, np.empty(512, np.float32)))
+        for at in (0, n // 2, n - 1536):
+            assert not download(a.ptr + at * 4, np.empty(1024, np.float32)).any()
