@@ -1,5 +1,5 @@
-// One AdamW step over many tensors in one launch (a few hundred tensors: a
-// launch a hundred), for gfx950.  Per element, in this order and without
+// One AdamW step over many tensors in one launch (more than 64: a launch for
+// each 64), for gfx950.  Per element, in this order and without
 // contraction, as the composed step's operations round:
 //   m = m0 b1 + g (1 - b1),  v = v0 b2 + (g g) (1 - b2)
 //   p = p0 (1 - rate decay) - (m / c1) / (sqrt(v / c2) + eps) rate
@@ -36,7 +36,7 @@
 
 namespace pt {
 
-constexpr int kAdamTensors = 64;   // a launch: 3.4 KiB of arguments
+constexpr int kAdamTensors = 64;   // of a launch, in its arguments
 constexpr int kAdamRounds = 2;     // 256 elements that a wave takes at once
 constexpr int kAdamBlock = 4 * kAdamRounds * 256;  // elements
 constexpr long long kAdamMost = (1 << 24) - 1;     // blocks of a launch: below 2^32 threads, of which HIP drops the rest
@@ -65,6 +65,7 @@ struct AdamArgs {
     float *power1, *power2;   // written by the first launch, else null
     float b1, one_b1, b2, one_b2, eps, decay, rate_value, decay_value;
 };
+static_assert(sizeof(AdamArgs) <= 4096, "a kernel's arguments hold the table");
 
 // A thread's 4 elements side by side, in 2, 4 or 1 words.
 typedef unsigned ad_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
