@@ -675,12 +675,14 @@ static pt_status gated_run(const pt_gated_desc *d, const void *x, const void *ga
     return PT_OK;
 }
 
-// Large products of whole packs: the plain ring product, whose loads go to LDS
-// by themselves, holds 95-100 % of the matrix cores at its clock where the pair
-// kernel holds 80, which pays for copies of the weights, and of their gradients,
-// side by side: 8192 x 1024 x 1024 both ways 786 us, 919 with the pair
-// kernel, 4096 x 784 x 1024 389 and 414; but 1000 x 768 x 2048 235 and 214.
-static bool gated_ring_f32(int M, int K, int F) { return K % 4 == 0 && F % 4 == 0 && (double)M * K * F > 2.5e9; }
+// Large products of whole packs and of 512 rows or more: the plain ring
+// product, whose loads go to LDS by themselves, holds 95-100 % of the matrix
+// cores at its clock where the pair kernel holds 80, which pays for copies of
+// the weights, and of their gradients, side by side: both ways 8192 x 1024 x
+// 1024 801 us, 934 with the pair kernel, 4096 x 784 x 1024 383 and 415; but 1000 x 768 x
+// 2048 223 and 216, and of 4096 x 14336 64 rows 893 and 529, 256 1741 and 1588,
+// 512 2958 and 2996.
+static bool gated_ring_f32(int M, int K, int F) { return K % 4 == 0 && F % 4 == 0 && M >= 512 && (double)M * K * F > 2.5e9; }
 
 static pt_status gated_backward_f32(const pt_gated_desc *d, const float *x, const float *gate, const float *up, const void *kept,
                                     const void *grad, float *dx, float *dgate, float *dup, GatedScratch &scratch, pt_stream_t stream)

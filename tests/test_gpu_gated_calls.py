@@ -20,6 +20,13 @@ def test_split_contractions_of_few_rows(shape, dtype):
     test_gpu_gated.test_both_directions(shape, dtype)
 
 
+@pytest.mark.parametrize("shape", [(96, 1000, 27000), (511, 1200, 5600), (512, 1200, 5600)], ids=str)
+def test_large_float32_weights(shape):
+    """Past 2.5e9 multiplications for a matrix with few rows, and on both sides of the rows where the gradients go another
+    way."""
+    test_gpu_gated.test_both_directions(shape, "float32")
+
+
 @pytest.mark.parametrize("dtype", test_gpu_gated.DTYPES)
 @pytest.mark.parametrize("shape", [(1, 64, 40), (20, 72, 136), (40, 64, 128), (80, 64, 128), (150, 65, 77), (2048, 640, 2048)], ids=str)
 def test_any_address(shape, dtype):
