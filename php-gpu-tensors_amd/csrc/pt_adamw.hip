@@ -39,8 +39,8 @@ namespace pt {
 constexpr int kAdamTensors = 64;   // of a launch, in its arguments
 constexpr int kAdamRounds = 2;     // 256 elements that a wave takes at once
 constexpr int kAdamBlock = 4 * kAdamRounds * 256;  // elements
-constexpr long long kAdamMost = (1 << 24) - 1;     // blocks of a launch: below 2^32 threads, of which HIP drops the rest
-constexpr long long kAdamPart = 1ll << 31;         // elements of a tensor that a launch's table takes as one
+constexpr long long kAdamMost = kLaunchThreads / 256;  // blocks of a launch
+constexpr long long kAdamPart = 1ll << 31;             // elements of a tensor that a launch's table takes as one
 
 struct AdamTensor {
     const void *p0, *g;
@@ -411,7 +411,7 @@ pt_status pt_adamw_moments(const void *first, const int8_t *first_exponent, cons
         return fail(PT_ERR_INVALID, "8-bit moments miss an operand");
     PT_TRY(ensure_init());
     if (!n) return PT_OK;
-    const unsigned blocks = (unsigned)std::min<size_t>((n / 256 + 3) / 4, kAdamMost);
+    const unsigned blocks = launch_blocks((n / 256 + 3) / 4);
     k_adamw_moments<<<blocks, 256, 0, stream_of(stream)>>>((const uint8_t *)first, first_exponent, (const uint8_t *)second,
                                                            second_exponent, first_values, second_values, (long long)(n / 256));
     return check_hip(hipGetLastError(), "8-bit moments");

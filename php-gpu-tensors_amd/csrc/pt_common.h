@@ -224,6 +224,16 @@ __device__ __forceinline__ T wave_all(T v, F f)
     return f(f(a, b), f(c, d));
 }
 
+// A launch counts its threads in 32 bits: HIP drops what is above without an
+// error, so no launch has more.
+constexpr long long kLaunchThreads = 0xffffffffll;
+// the blocks of a kernel that walks on over what one launch does not hold
+inline unsigned launch_blocks(size_t blocks, int threads = 256)
+{
+    const size_t most = (size_t)(kLaunchThreads / threads);
+    return (unsigned)(blocks < most ? blocks : most);
+}
+
 struct FAdd { template <typename T> __device__ T operator()(T a, T b) const { return a + b; } };
 struct FMax { __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
               __device__ double operator()(double a, double b) const { return fmax(a, b); } };

@@ -645,11 +645,12 @@ static unsigned grid_for(long long n, int per_thread = 1)
 {
     // one thread per work item: a full grid streams HBM faster on gfx950
     // than a capped grid-stride loop; the loops cover grids above the limit
-    long long blocks = (n + 256LL * per_thread - 1) / (256LL * per_thread);
-    if (blocks > 0x7fffffffLL) blocks = 0x7fffffffLL;
-    if (blocks < 1) blocks = 1;
-    return (unsigned)blocks;
+    const long long blocks = (n + 256LL * per_thread - 1) / (256LL * per_thread);
+    return launch_blocks((size_t)(blocks < 1 ? 1 : blocks));
 }
+// the kernels over packs take one each and do not walk: what fills more than a
+// launch goes element by element
+static bool packs_fit(long long n, int per_thread) { return n <= kLaunchThreads / 256 * 256 * per_thread; }
 
 static bool valid_binary_op(int op)
 {
@@ -779,7 +780,7 @@ static pt_status binary_impl(const void *a, int dta, const size_t *sa, size_t of
     const char *pb = scalar ? nullptr : (const char *)b + offb * dtype_size(dtb);
     Opnd oa, ob;
     bool vec = vec_float(dta) && (dto == dta || dto == PT_FLOAT32) && (scalar || dtb == dta) &&
-               as_opnd(s, s.sa, pa, oa);
+               packs_fit(s.total, 16 / (int)dtype_size(dta)) && as_opnd(s, s.sa, pa, oa);
     if (vec && scalar) ob = Opnd{nullptr, OPND_IMM, 0u, (float)scalar_as_double(scalar)};
     else vec = vec && as_opnd(s, s.sb, pb, ob);
     if (vec) {
@@ -882,7 +883,7 @@ pt_status pt_unary(const void *input, int dtype, const size_t *strides, size_t o
     hipStream_t st_ = stream_of(stream);
     const char *px = (const char *)input + offset * dtype_size(dtype);
     Opnd ox;
-    if (vec_float(dtype) && as_opnd(s, s.sa, px, ox)) {
+    if (vec_float(dtype) && packs_fit(s.total, 16 / (int)dtype_size(dtype)) && as_opnd(s, s.sa, px, ox)) {
         const size_t total = (size_t)s.total;
         const bool nt = dtype == PT_FLOAT32 &&
                         streams(total * dtype_size(dtype) * 2, 1, {ox.mode == OPND_FLAT ? px : nullptr, out});
@@ -947,7 +948,8 @@ pt_status pt_cast(const void *input, int dtype_in, const size_t *strides, size_t
     }
     Opnd ox;
     EwShape32 s32;
-    if (vec_float(dtype_in) && vec_float(dtype_out) && dtype_in != dtype_out && as_opnd(s, s.sa, px, ox)) {
+    if (vec_float(dtype_in) && vec_float(dtype_out) && dtype_in != dtype_out && packs_fit(s.total, 8) &&
+        as_opnd(s, s.sa, px, ox)) {
         const size_t total = (size_t)s.total;
         with_vec_dtype(dtype_in, [&](auto I) {
             with_vec_dtype(dtype_out, [&](auto O) {
@@ -980,7 +982,7 @@ pt_status pt_where(const void *cond, int dtype_cond, const size_t *strides_cond,
     Opnd oc, ox, oy;
     EwShape32 s32;
     const int csz = (int)dtype_size(dtype_cond), esz = (int)dtype_size(dtype_xy);
-    if (csz <= 4 && (esz == 2 || esz == 4) && as_opnd(s, s.sc, cond, oc) && as_opnd(s, s.sa, x, ox) &&
+    if (csz <= 4 && (esz == 2 || esz == 4) && packs_fit(s.total, 16 / esz) && as_opnd(s, s.sc, cond, oc) && as_opnd(s, s.sa, x, ox) &&
         as_opnd(s, s.sb, y, oy)) {
         const size_t total = (size_t)s.total;
         // a floating condition holds unless it is +0 or -0; integers and bool unless they are 0

@@ -664,6 +664,8 @@ pt_status pt_launch(pt_function_t function, unsigned grid_x, unsigned block_x,
                     void **params, pt_stream_t stream)
 {
     if (!grid_x) return PT_OK;
+    if (block_x > kLaunchThreads / grid_x)
+        return fail(PT_ERR_INVALID, "a launch of %u blocks of %u threads has 2^32 threads or more", grid_x, block_x);
     return check_hip(hipModuleLaunchKernel((hipFunction_t)function, grid_x, 1, 1, block_x, 1, 1,
                                            0, stream_of(stream), params, nullptr),
                      "hipModuleLaunchKernel");

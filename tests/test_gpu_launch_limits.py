@@ -1,11 +1,11 @@
-"""AdamW over many tensors, and 8-bit moments, of more elements than one launch holds (2^32 threads: 2^35 and 2^34 of
-them), through the C entries: 150 and 155 GB of the card's 288."""
+"""Calls of more than one launch holds, which counts its threads in 32 bits: AdamW over many tensors and 8-bit moments
+(through the C entries), elementwise operations, reductions, rows, products, plans.  Up to 155 GB of the card's 288."""
 import ctypes
 
 import numpy as np
 import pytest
 
-from phptensors import _abi
+from phptensors import CudaArray, Fusion, _abi
 from test_gpu_block_sizes import big, end
 
 pytestmark = pytest.mark.gpu
@@ -70,3 +70,31 @@ def test_moments():
         assert np.array_equal(end(a, np.empty(512, np.float32)), download(b.ptr, np.empty(512, np.float32)))
         for at in (0, n // 2, n - 1536):
             assert not download(a.ptr + at * 4, np.empty(1024, np.float32)).any()
+
+
+# Tensors of one value: a tensor's first, middle and last rows.  No two results that follow each other are alike, so
+# memory that is used again holds nothing that passes.
+def same(t, want):
+    n = t.getShape()[0]
+    for at in (0, n // 2, n - 3):
+        x = t.slice([at, at + 3]).toNumpy()
+        assert np.array_equal(x, np.broadcast_to(np.asarray(want, x.dtype), x.shape)), (at, want)
+
+
+@pytest.mark.parametrize("rows", [2 ** 16, 2 ** 16 + 1])
+def test_elements(rows):
+    """A thread for each of 2^32 elements, and of more."""
+    x = CudaArray.full([rows, 2 ** 16], 3, "uint8")
+    same(x, 3)
+    same(x + x, 6)
+    same(x.astype("int16"), 3)
+    same(CudaArray.where(x, CudaArray.full([1], 9, "uint8"), CudaArray.full([1], 1, "uint8")), 9)
+
+
+@pytest.mark.parametrize("dtype,rows", [("float32", 2 ** 17 + 1), ("bfloat16", 2 ** 18 + 1)])
+def test_packs(dtype, rows):
+    """A thread for each 16 bytes."""
+    x = CudaArray.full([rows, 2 ** 17], 1.5, dtype)
+    same(x, 1.5)
+    same(x * 2.0, 3.0)
+    same(x.neg(), -1.5)
