@@ -2214,8 +2214,18 @@ static bool launch_rows_dt(int rop, const void *x, size_t rows, int n, size_t ld
     return false;
 }
 
-static bool launch_rows(int dt, int rop, const void *x, size_t rows, int n, size_t ld, void *out,
-                        int out_dt, int correction, int take_sqrt, hipStream_t s)
+// The rows of one launch, f(first, count): a row takes up to 512 threads.
+// More rows go in equal parts, whole groups of 4, so that all take the same
+// kernel.
+template <typename F> static void row_launches(size_t rows, F f)
+{
+    constexpr size_t most = (size_t)(kLaunchThreads / 512) / 4 * 4;
+    const size_t parts = (rows + most - 1) / most, each = parts ? (rows + 4 * parts - 1) / (4 * parts) * 4 : 0;
+    for (size_t from = 0; from < rows; from += each) f(from, rows - from < each ? rows - from : each);
+}
+
+static bool launch_row_part(int dt, int rop, const void *x, size_t rows, int n, size_t ld, void *out,
+                            int out_dt, int correction, int take_sqrt, hipStream_t s)
 {
     switch (dt) {
     case PT_FLOAT32: return launch_rows_dt<PT_FLOAT32>(rop, x, rows, n, ld, out, out_dt, correction, take_sqrt, s);
@@ -2224,6 +2234,17 @@ static bool launch_rows(int dt, int rop, const void *x, size_t rows, int n, size
     case PT_FLOAT16: return launch_rows_dt<PT_FLOAT16>(rop, x, rows, n, ld, out, out_dt, correction, take_sqrt, s);
     default: return false;
     }
+}
+
+static bool launch_rows(int dt, int rop, const void *x, size_t rows, int n, size_t ld, void *out,
+                        int out_dt, int correction, int take_sqrt, hipStream_t s)
+{
+    bool taken = true;
+    row_launches(rows, [&](size_t from, size_t count) {
+        taken = taken && launch_row_part(dt, rop, (const char *)x + from * ld * dtype_size(dt), count, n, ld,
+                                         (char *)out + from * dtype_size(out_dt), out_dt, correction, take_sqrt, s);
+    });
+    return taken;
 }
 
 static int result_dtype(int dtype, int rop)
@@ -2600,7 +2621,7 @@ static void launch_layernorm_nch(const void *x, size_t rows, int n, CT eps, cons
 }
 
 template <int DT, int PDT, typename CT>
-static void launch_layernorm_rows(const void *x, size_t rows, int n, CT eps, const void *g,
+static void launch_layernorm_part(const void *x, size_t rows, int n, CT eps, const void *g,
                                   const void *b, CT *y, hipStream_t s)
 {
     constexpr int V = RT<DT>::V;
@@ -2628,22 +2649,31 @@ static void launch_layernorm_rows(const void *x, size_t rows, int n, CT eps, con
     k_row_layernorm_stream<DT, CT, PDT><<<(unsigned)rows, 256, 0, s>>>(x, n, eps, g, b, y);
 }
 
+template <int DT, int PDT, typename CT>
+static void launch_layernorm_rows(const void *x, size_t rows, int n, CT eps, const void *g,
+                                  const void *b, CT *y, hipStream_t s)
+{
+    row_launches(rows, [&](size_t from, size_t count) {
+        launch_layernorm_part<DT, PDT, CT>((const char *)x + from * n * dtype_size(DT), count, n, eps, g, b, y + from * n, s);
+    });
+}
+
 // Strided -> contiguous permuted copy used to move the softmax axis last.
 __global__ void k_permute_copy(const void *__restrict__ x, void *__restrict__ y, int esz,
                                GenParams p, size_t total)
 {
-    size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= total) return;
-    size_t rem = i, off = p.base;
-    for (int d = p.ndims - 1; d >= 0; d--) {
-        off += (rem % (size_t)p.shape[d]) * p.strides[d];
-        rem /= (size_t)p.shape[d];
-    }
-    switch (esz) {
-    case 1: ((uint8_t *)y)[i] = ((const uint8_t *)x)[off]; break;
-    case 2: ((uint16_t *)y)[i] = ((const uint16_t *)x)[off]; break;
-    case 4: ((uint32_t *)y)[i] = ((const uint32_t *)x)[off]; break;
-    default: ((uint64_t *)y)[i] = ((const uint64_t *)x)[off]; break;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
+        size_t rem = i, off = p.base;
+        for (int d = p.ndims - 1; d >= 0; d--) {
+            off += (rem % (size_t)p.shape[d]) * p.strides[d];
+            rem /= (size_t)p.shape[d];
+        }
+        switch (esz) {
+        case 1: ((uint8_t *)y)[i] = ((const uint8_t *)x)[off]; break;
+        case 2: ((uint16_t *)y)[i] = ((const uint16_t *)x)[off]; break;
+        case 4: ((uint32_t *)y)[i] = ((const uint32_t *)x)[off]; break;
+        default: ((uint64_t *)y)[i] = ((const uint64_t *)x)[off]; break;
+        }
     }
 }
 
@@ -2782,12 +2812,16 @@ pt_status pt_softmax(const void *input, void *output, int input_dtype, int outpu
         }
     }
     if (n > 0) {
-        switch (input_dtype) {
-        case PT_FLOAT32: launch_softmax_rows<PT_FLOAT32, float>(src, rows, n, ld, (float *)dst, s); break;
-        case PT_BFLOAT16: launch_softmax_rows<PT_BFLOAT16, float>(src, rows, n, ld, (float *)dst, s); break;
-        case PT_FLOAT16: launch_softmax_rows<PT_FLOAT16, float>(src, rows, n, ld, (float *)dst, s); break;
-        case PT_FLOAT64: launch_softmax_rows<PT_FLOAT64, double>(src, rows, n, ld, (double *)dst, s); break;
-        }
+        row_launches(rows, [&](size_t from, size_t count) {
+            const char *x = (const char *)src + from * ld * dtype_size(input_dtype);
+            char *y = (char *)dst + from * (size_t)n * dtype_size(output_dtype);
+            switch (input_dtype) {
+            case PT_FLOAT32: launch_softmax_rows<PT_FLOAT32, float>(x, count, n, ld, (float *)y, s); break;
+            case PT_BFLOAT16: launch_softmax_rows<PT_BFLOAT16, float>(x, count, n, ld, (float *)y, s); break;
+            case PT_FLOAT16: launch_softmax_rows<PT_FLOAT16, float>(x, count, n, ld, (float *)y, s); break;
+            case PT_FLOAT64: launch_softmax_rows<PT_FLOAT64, double>(x, count, n, ld, (double *)y, s); break;
+            }
+        });
     }
     hipError_t err = hipGetLastError();
     if (err == hipSuccess && tmp_out) {

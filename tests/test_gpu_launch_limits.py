@@ -98,3 +98,32 @@ def test_packs(dtype, rows):
     same(x, 1.5)
     same(x * 2.0, 3.0)
     same(x.neg(), -1.5)
+
+
+# Tensors that repeat 1021 rows: every row's result is that of the row alone.
+def repeated(shape, dtype, seed=1):
+    base = np.random.default_rng(seed).integers(-8, 9, (1021, *shape[1:])).astype(np.int32 if dtype == "int32" else np.float32)
+    return CudaArray.fromNumpy(np.resize(base, shape), dtype), CudaArray.fromNumpy(base, dtype)
+
+
+def repeats(many, few, what):
+    a, b = many.toBits(), few.toBits()
+    assert np.array_equal(a, np.resize(b, a.shape)), what
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_rows(dtype):
+    """A wave for each of more than 2^26 rows."""
+    x, y = repeated((2 ** 26 + 64, 4), dtype)
+    for name in ("sum", "mean", "max", "min", "prod", "argMax", "argMin", "var", "softmax"):
+        repeats(getattr(x, name)(-1), getattr(y, name)(-1), name)
+    repeats(x.layerNorm([1], 1e-3), y.layerNorm([1], 1e-3), "layerNorm")
+
+
+def test_long_rows():
+    """512 threads for each of more than 2^23 rows."""
+    x = CudaArray.full([2 ** 23 + 64, 1028], 0.5)
+    same(x.sum(-1), 514.0)
+    same(x.max(-1), 0.5)
+    few = CudaArray.full([1, 1028], 0.5).softmax(-1).toNumpy()[0, 0]
+    same(x.softmax(-1), few)
