@@ -1475,6 +1475,7 @@ struct GenParams {
     int out_dt;
     int correction;
     int take_sqrt;
+    size_t first;      // output of a launch's first workgroup (k_strided_reduce)
 };
 
 __device__ void gen_finish(const GenAcc &a, const GenParams &p, void *out, size_t o)
@@ -1557,7 +1558,7 @@ __global__ __launch_bounds__(128) void k_strided_reduce(const void *__restrict__
                                                         GenParams p)
 {
     __shared__ GenAcc lds[128];
-    const size_t o = blockIdx.x;
+    const size_t o = p.first + blockIdx.x;
     if (o >= p.outputs) return;
     GenAcc a;
     gen_init(a, op, dt);
@@ -2024,11 +2025,11 @@ __global__ __launch_bounds__(256) void k_global_final(const GenAcc *__restrict__
 // Fill used for empty-axis identities (sum 0, prod 1, mean NaN).
 __global__ void k_fill_identity(void *out, int out_dt, size_t n, double value)
 {
-    size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= n) return;
-    if (out_dt == PT_FLOAT32) ((float *)out)[i] = (float)value;
-    else if (out_dt == PT_FLOAT64) ((double *)out)[i] = value;
-    else store_bits_dt(out, out_dt, i, (uint64_t)(int64_t)value);
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
+        if (out_dt == PT_FLOAT32) ((float *)out)[i] = (float)value;
+        else if (out_dt == PT_FLOAT64) ((double *)out)[i] = value;
+        else store_bits_dt(out, out_dt, i, (uint64_t)(int64_t)value);
+    }
 }
 
 // ================================================================== host
@@ -2308,6 +2309,11 @@ static pt_status launch_cols_t(const void *x, size_t outer, size_t n, size_t inn
     constexpr bool VAR16 = OP == R_VAR && sizeof(typename RT<DT>::S) == 2;
     const bool wide = vec_blocks * splits * outer >= 512;
     const int width = !vec ? 1 : packed ? (OP == R_VAR && splits == 1 && !wide ? W : V) : wide && !VAR16 ? V : W;
+    // (more columns than a launch holds, and so no slices: another kernel's)
+    if ((inner + 64 * width - 1) / (64 * width) > (size_t)(kLaunchThreads / 256)) {
+        scratch_free(partial, s);
+        return -1;
+    }
     auto go = [&](auto N, auto T) {
         constexpr int C = decltype(N)::value;
         const dim3 grid((unsigned)((inner + 64 * C - 1) / (64 * C)), (unsigned)splits, (unsigned)outer);
@@ -2409,7 +2415,7 @@ static pt_status reduce_driver(const void *input, void *output, int dtype, int r
         if (rop == R_ARGMAX || rop == R_ARGMIN)
             return fail(PT_ERR_INVALID, "Arg reduction has no identity for an empty axis");
         double ident = (rop == R_PROD || rop == R_ALL) ? 1.0 : (rop == R_MEAN ? NAN : 0.0);
-        k_fill_identity<<<(unsigned)((outputs + 255) / 256), 256, 0, s>>>(output, out_dt, outputs, ident);
+        k_fill_identity<<<launch_blocks((outputs + 255) / 256), 256, 0, s>>>(output, out_dt, outputs, ident);
         PT_LAUNCH_CHECK("reduction identity fill");
         return PT_OK;
     }
@@ -2506,8 +2512,8 @@ static pt_status reduce_driver(const void *input, void *output, int dtype, int r
             counters().column_reduce_calls++;
             return PT_OK;
         }
-        if (outer <= 65535) {
-            dim3 grid((unsigned)((inner + 63) / 64), (unsigned)outer);
+        if (outer <= 65535 && col_blocks <= (size_t)(kLaunchThreads / 256)) {
+            dim3 grid((unsigned)col_blocks, (unsigned)outer);
             k_column_reduce<<<grid, 256, 0, s>>>(xb, output, rop, dtype,
                                                  outer, count, inner, p);
             PT_LAUNCH_CHECK("column reduction");
@@ -2517,7 +2523,8 @@ static pt_status reduce_driver(const void *input, void *output, int dtype, int r
     }
     if (outputs > 0x7fffffffu)
         return fail(PT_ERR_INVALID, "reduction: too many outputs");
-    k_strided_reduce<<<(unsigned)outputs, 128, 0, s>>>(input, output, rop, dtype, p);
+    for (; p.first < outputs; p.first += launch_blocks(outputs, 128))
+        k_strided_reduce<<<launch_blocks(outputs - p.first, 128), 128, 0, s>>>(input, output, rop, dtype, p);
     PT_LAUNCH_CHECK("strided reduction");
     counters().strided_reduce_calls++;
     return PT_OK;
@@ -2688,7 +2695,7 @@ static pt_status permute_copy(const void *x, void *y, int esz, const int *shape,
     }
     size_t total = numel(shape, ndims);
     if (!total) return PT_OK;
-    k_permute_copy<<<(unsigned)((total + 255) / 256), 256, 0, s>>>(x, y, esz, p, total);
+    k_permute_copy<<<launch_blocks((total + 255) / 256), 256, 0, s>>>(x, y, esz, p, total);
     PT_LAUNCH_CHECK("permute copy");
     return PT_OK;
 }

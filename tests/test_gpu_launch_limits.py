@@ -127,3 +127,33 @@ def test_long_rows():
     same(x.max(-1), 0.5)
     few = CudaArray.full([1, 1028], 0.5).softmax(-1).toNumpy()[0, 0]
     same(x.softmax(-1), few)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "int32"])
+def test_strided_reductions(dtype):
+    """128 threads for each of more than 2^25 results."""
+    x, y = repeated((2 ** 25 + 64, 3, 2), dtype)
+    for name in ("sum", "max"):
+        repeats(getattr(x, name)(1), getattr(y, name)(1), name)
+    repeats(x.swapaxes(1, 2).sum(-1), y.swapaxes(1, 2).sum(-1), "swapped")
+    repeats(x.sum(-1), y.sum(-1), "last")
+
+
+def test_empty_axes():
+    same(CudaArray.zeros([2 ** 16 + 1, 0, 2 ** 16]).prod(1), 1.0)
+
+
+def test_columns():
+    """64 columns of bytes to a workgroup, 512 of bfloat16."""
+    x = CudaArray.full([2, 2 ** 30 + 1], 3, "uint8")
+    got = x.sum(0)
+    same(got, 6)
+    del x, got
+    x = CudaArray.full([2, 2 ** 16 + 1, 2 ** 16], 1.0, "bfloat16")
+    same(x.sum(0), 2.0)
+
+
+def test_softmax_of_another_axis():
+    """An element to a thread, moved there and back."""
+    x = CudaArray.full([2 ** 11 + 1, 2, 2 ** 20], 1.0, "bfloat16")
+    same(x.softmax(1), 0.5)
