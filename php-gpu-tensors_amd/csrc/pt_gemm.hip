@@ -973,8 +973,7 @@ static void launch_dt(GemmArgs g, int tile, bool a_kc, bool b_kc, bool check, hi
 
 __global__ void k_zero_fill(uint8_t *p, size_t n)
 {
-    size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) p[i] = 0;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) p[i] = 0;
 }
 
 static int g_precision = 0;
@@ -1105,11 +1104,32 @@ pt_status pt_matmul(const void *a, const void *b, void *c, int dtype,
     if (g.K == 0) {
         // empty inner product: zeros (host_array_math.phpt:84-85)
         size_t bytes = (size_t)batch * g.M * g.N * dtype_size(dtype);
-        k_zero_fill<<<(unsigned)((bytes + 255) / 256), 256, 0, s>>>((uint8_t *)c, bytes);
+        k_zero_fill<<<launch_blocks((bytes + 255) / 256), 256, 0, s>>>((uint8_t *)c, bytes);
         PT_LAUNCH_CHECK("matmul zero fill");
         return PT_OK;
     }
     if (batch > 65535LL * 65535LL) return fail(PT_ERR_INVALID, "matmul batch too large");
+    // Batches of more than 2^23 tiles of 64 x 64 (512 threads at most) may not
+    // fit a launch: the outermost axis goes in halves.
+    if (batch > 1 && (long long)((g.M + 63) / 64) * ((g.N + 63) / 64) > kLaunchThreads / 512 / batch) {
+        int d = 0;
+        while (shape_c[d] == 1) d++;
+        int sa[PT_MAX_DIMS], sb[PT_MAX_DIMS], sc[PT_MAX_DIMS];
+        std::copy(shape_a, shape_a + nd_a, sa);
+        std::copy(shape_b, shape_b + nd_b, sb);
+        std::copy(shape_c, shape_c + nd_c, sc);
+        const int ia = d - (nd_c - nd_a), ib = d - (nd_c - nd_b), half = shape_c[d] / 2;
+        const bool along_a = ia >= 0 && sa[ia] != 1, along_b = ib >= 0 && sb[ib] != 1;
+        const size_t es = dtype_size(dtype), plane = (size_t)g.M * g.N * (size_t)(batch / shape_c[d]);
+        for (int first = 0; first < shape_c[d]; first += sc[d]) {
+            sc[d] = first ? shape_c[d] - half : half;
+            if (along_a) sa[ia] = sc[d];
+            if (along_b) sb[ib] = sc[d];
+            PT_TRY(pt_matmul((const char *)a + (along_a ? first * strides_a[ia] * es : 0), (const char *)b + (along_b ? first * strides_b[ib] * es : 0),
+                             (char *)c + first * plane * es, dtype, sa, strides_a, nd_a, sb, strides_b, nd_b, sc, nd_c, stream));
+        }
+        return PT_OK;
+    }
     g.a = a;
     g.b = b;
     g.c = c;
@@ -1191,7 +1211,7 @@ pt_status pt_matmul(const void *a, const void *b, void *c, int dtype,
         for (int d = 0; d < g.nbd; d++)
             if (g.bsa[d] % 8 || g.bsb[d] % 8) ok = false;
         long long tiles = (long long)(g.M / 256) * (g.N / bn) * batch;
-        if (ok && tiles <= 0x7fffffffLL) {
+        if (ok && tiles <= kLaunchThreads / 512) {
             g.tiles_m = g.M / 256;
             g.tiles_n = g.N / bn;
             g.remap = tiles % 8 == 0;
@@ -1217,7 +1237,7 @@ pt_status pt_matmul(const void *a, const void *b, void *c, int dtype,
         for (int d = 0; d < g.nbd; d++)
             if (g.bsa[d] % 8 || g.bsb[d] % 8) direct = false;
         long long tiles = (long long)(g.M / 256) * (g.N / 256) * batch;
-        if (direct && tiles <= 0x7fffffffLL) {
+        if (direct && tiles <= kLaunchThreads / 512) {
             g.tiles_m = g.M / 256;
             g.tiles_n = g.N / 256;
             g.remap = tiles % 8 == 0;
@@ -1287,7 +1307,7 @@ pt_status pt_matmul(const void *a, const void *b, void *c, int dtype,
     }
     long long total_tiles = (long long)((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn) * batch;
     g.remap = total_tiles % 8 == 0;
-    if (total_tiles > 0x7fffffffLL) return fail(PT_ERR_INVALID, "matmul grid too large");
+    if (total_tiles > kLaunchThreads / 512) return fail(PT_ERR_INVALID, "matmul grid too large");
     // split-K when the tiles cannot give every CU a workgroup and K is
     // long: about 512 workgroups of K chunks (each at least 4 K steps)
     // write fp32 partials, then one ordered sum per output element

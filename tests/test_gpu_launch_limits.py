@@ -157,3 +157,25 @@ def test_softmax_of_another_axis():
     """An element to a thread, moved there and back."""
     x = CudaArray.full([2 ** 11 + 1, 2, 2 ** 20], 1.0, "bfloat16")
     same(x.softmax(1), 0.5)
+
+
+@pytest.mark.parametrize("lead", [(2 ** 24 + 8,), (4099, 1, 4097)], ids=str)
+@pytest.mark.parametrize("shared", ["left", "right"])
+def test_small_products(lead, shared):
+    """A tile for each of more than 2^24 products, one factor common to all."""
+    n = int(np.prod(lead))
+    x, y = repeated((n, 2, 2), "float32")
+    w = CudaArray.fromNumpy(np.array([[1, 2], [-3, 4]], np.float32))
+    a, b = (w.matmul(x.reshape([*lead, 2, 2])), w.matmul(y)) if shared == "left" else (x.reshape([*lead, 2, 2]).matmul(w), y.matmul(w))
+    assert a.getShape() == [*lead, 2, 2]
+    repeats(a.reshape([n, 2, 2]), b, shared)
+
+
+def test_small_products_of_pairs():
+    x, y = repeated((2 ** 24 + 8, 2, 3), "bfloat16")
+    u, v = repeated((2 ** 24 + 8, 3, 2), "bfloat16", 2)
+    repeats(x.matmul(u), y.matmul(v), "pairs")
+
+
+def test_empty_products():
+    same(CudaArray.zeros([2 ** 16 + 1, 0], "float16").matmul(CudaArray.zeros([0, 2 ** 16], "float16")), 0.0)
