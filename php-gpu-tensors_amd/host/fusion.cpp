@@ -1654,6 +1654,9 @@ static const void *leaf_ptr(const Plan &p, const std::vector<TensorP> &vals, int
     return v->data();
 }
 
+// A launch counts its threads in 32 bits; HIP drops what is above.
+constexpr size_t kLaunchThreads = 0xffffffff;
+
 static bool launch_kernel(Plan &p, Kernel &k, std::vector<TensorP> &vals)
 {
     std::vector<void *> ptrs;
@@ -1673,10 +1676,10 @@ static bool launch_kernel(Plan &p, Kernel &k, std::vector<TensorP> &vals)
     for (void *&ptr : ptrs) params.push_back(&ptr);
     size_t work = vec_ok ? k.total / 4 : k.total;
     // one thread per work item: a full grid streams HBM faster on gfx950
-    // than a capped grid-stride loop (the loop remains for grids above the
-    // hardware limit)
+    // than a capped grid-stride loop (the loop remains for what a launch of
+    // fewer than 2^32 threads does not hold)
     size_t blocks = (work + 255) / 256;
-    if (blocks > 0x7fffffffu) blocks = 0x7fffffffu;
+    if (blocks > kLaunchThreads / 256) blocks = kLaunchThreads / 256;
     return check_status(pt_launch(vec_ok ? k.fn_vec : k.fn_scalar, (unsigned)blocks, 256, params.data(),
                                   nullptr),
                         "Fusion kernel launch failed");
@@ -1725,10 +1728,12 @@ static bool run_step(Plan &p, const Step &st, std::vector<TensorP> &vals)
 
 // The chain's kernel: one 64-thread workgroup per row.  A reduction whose
 // chunked order was assumed needs its rows 16-byte aligned, as the native
-// kernel does to read them in chunks; otherwise `launched` stays false.
+// kernel does to read them in chunks; otherwise `launched` stays false, as
+// for rows that one launch does not hold.
 static bool launch_chain(Plan &p, RowChain &ch, std::vector<TensorP> &vals, bool &launched)
 {
     launched = false;
+    if ((size_t)ch.rows > kLaunchThreads / 64) return true;
     std::vector<void *> ptrs;
     for (size_t j = 0; j < ch.members.size(); j++) {
         const Step &st = p.steps[ch.members[j]];

@@ -179,3 +179,18 @@ def test_small_products_of_pairs():
 
 def test_empty_products():
     same(CudaArray.zeros([2 ** 16 + 1, 0], "float16").matmul(CudaArray.zeros([0, 2 ** 16], "float16")), 0.0)
+
+
+def test_plan_of_elements():
+    x = CudaArray.full([2 ** 16, 2 ** 16], 3, "int32")
+    plan = Fusion.compile(lambda t: [t * t + t], [x])
+    same(plan.run(x)[0], 12)
+
+
+def test_plan_of_rows():
+    """Reductions and what follows them, a workgroup for each of more than 2^26 rows."""
+    x, y = repeated((2 ** 26 + 64, 4), "float32")
+
+    def body(t):
+        return [(t - t.max(-1).reshape([-1, 1])).exp().sum(-1) * 0.5]
+    repeats(Fusion.compile(body, [x]).run(x)[0], body(y)[0], "plan")
