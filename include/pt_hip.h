@@ -640,7 +640,8 @@ pt_status pt_rtc_compile(const char *source, const char *program_name,
 pt_status pt_module_function(pt_module_t module, const char *name, pt_function_t *function);
 pt_status pt_module_unload(pt_module_t module);
 /* Replaces cuLaunchKernel (fusion_execute.c): params is the kernel
- * argument array as for hipModuleLaunchKernel. */
+ * argument array as for hipModuleLaunchKernel.  Refuses 2^32 threads and
+ * more, of which HIP would keep the low 32 bits. */
 pt_status pt_launch(pt_function_t function, unsigned grid_x, unsigned block_x,
                     void **params, pt_stream_t stream);
 

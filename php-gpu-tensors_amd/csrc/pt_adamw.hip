@@ -5,10 +5,10 @@
 //   p = p0 (1 - rate decay) - (m / c1) / (sqrt(v / c2) + eps) rate
 // with c = 1 - b^t; an element whose gradient is NaN stays as it was.
 // HBM-bound: everything is read once and written once.  134 M elements,
-// bfloat16 with float32 masters: 652 us, 5.75 TB/s (a large copy 5.0).  With
-// moments in 8 bits and no masters 409 us for a third of the bytes: 100 vector
-// instructions an element, of which the exact root and the drawn numbers are
-// half, take longer than HBM.
+// bfloat16 with float32 masters: 626-664 us, 5.7-6.0 TB/s (a large copy 5.0).
+// With moments in 8 bits and no masters 382-419 us for a third of the bytes:
+// 100 vector instructions an element, of which the exact root and the drawn
+// numbers are half, take longer than HBM.
 //
 // The moments (and float32 masters of 16-bit parameters) of all tensors lie in
 // one array each, a tensor's from a multiple of 256 elements on; parameters
