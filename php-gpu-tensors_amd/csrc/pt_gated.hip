@@ -417,13 +417,8 @@ __global__ __launch_bounds__(256) void k_gated_slope(SlopeArgs a)
     }
 }
 
-// float16: the largest finite |dg| and |du| of each row and of each column (the
-// two apart), of the rows' and columns' parts that a block takes; the second
-// kernel takes the largest over the parts, in any order the same.  A wave walks
-// `steps` rows, 512 columns of each (fewer columns: as many rows at once as
-// fill it), so a row is reduced over its lanes and a column stays in one.
-// 8192 x 8192: 119-124 us (4.4 TB/s) and 5.
-__device__ __forceinline__ float gd_top(float v, int log2)  // over 2^log2 lanes (uniform), by DPP up to 16
+// the largest over the 2^log2 lanes that share a row (log2 is uniform), by DPP up to 16
+__device__ __forceinline__ float gd_top(float v, int log2)
 {
     auto with = [](float x, auto CTRL) {
         return fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(CTRL)::value, 0xF, 0xF, false)));
@@ -436,6 +431,13 @@ __device__ __forceinline__ float gd_top(float v, int log2)  // over 2^log2 lanes
     if (log2 > 4) v = fmaxf(v, __shfl_xor(v, 16, PT_WAVE));
     return v;
 }
+
+// float16: the largest finite |dg| and |du| of each row and of each column (the
+// two apart), of the rows' and columns' parts that a block takes; the second
+// kernel takes the largest over the parts, in any order the same.  A wave walks
+// `steps` rows, 512 columns of each (fewer columns: as many rows at once as
+// fill it), so a row is reduced over its lanes and a column stays in one.
+// 8192 x 8192: 119-124 us (4.4 TB/s) and 5.
 struct RangeArgs {
     const void *kept, *grad;
     int rows, cols, act;
